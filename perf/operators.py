@@ -252,7 +252,7 @@ def run(st):
         return {"q": q, "k": k}
     if op == "append":
         q = native.paged_append(st["k"], st["v"], st["k_cache"], st["v_cache"], st["table"], st["cu_q"],
-                                st["kv_lens"], max_q_len=st["max_q"], q=st["q"], rope=st["rope"],
+                                st["kv_lens"], q=st["q"], rope=st["rope"],
                                 q_weight=st.get("q_weight"), k_weight=st.get("k_weight"), eps=EPS,
                                 interleaved=st["case"]["interleaved"])
         return {"q": q, "k_cache": st["k_cache"], "v_cache": st["v_cache"]}
