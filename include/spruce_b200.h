@@ -36,6 +36,9 @@ extern "C" {
 /* Bits kernels OR into the optional device status word (uint32). */
 #define SPRUCE_STATUS_TIMEOUT 1u   /* a bounded pipeline wait ran out       */
 #define SPRUCE_STATUS_EMPTY_ROW 2u /* a selected_blocks row had no block    */
+#define SPRUCE_STATUS_BAD_PAGE 4u  /* a page id outside the cache was needed */
+#define SPRUCE_STATUS_BAD_LENGTH 8u    /* a sequence length or offset outside its bounds */
+#define SPRUCE_STATUS_BAD_POSITION 16u /* a position outside the rotation table */
 
 #define SPRUCE_DTYPE_F32 0
 #define SPRUCE_DTYPE_BF16 1
@@ -406,6 +409,83 @@ SPRUCE_API int spruce_kv_summary_table(const void *key, const int64_t key_stride
                                        float *keys, float *values, float *counts, float *log_counts,
                                        int64_t *range_starts, int64_t *range_ends, void *workspace,
                                        int64_t workspace_bytes, void *stream);
+
+/*
+ * The serving operators around the sparse-prefill layer; the reference takes
+ * post-RoPE Q/K from its model and leaves decode to SDPA
+ * (kernels/sparse_prefill.py:63-65), so they have no counterpart there.
+ *
+ * Head norms and rotary positions of q [B, Hq, T, D] and k [B, Hkv, T, D]
+ * (element strides, unit last) into q_out / k_out (same shapes, by strides; the
+ * output may be the input itself), in fp32 with one rounding at the store:
+ *   y = x * rsqrt(mean(x^2) + eps) * weight     (weight fp32 [D]; NULL: no norm)
+ *   pairs (a, b) of the first rd dims -> (a cos - b sin, b cos + a sin),
+ * pairs (i, i + rd/2), or (2i, 2i + 1) when interleaved, angles from row
+ * `position` of rope [table_rows, rd] fp32 (cos of the rd/2 angles, then sin).
+ * positions int64 by element strides (b, t), or NULL: token t is at position t.
+ * A position outside the table takes the nearest row and raises
+ * SPRUCE_STATUS_BAD_POSITION in *status (optional).  D and rd even, rd <= D <=
+ * 256; rows that are not 16-byte aligned take scalar loads.
+ */
+SPRUCE_API int spruce_qk_norm_rope(const void *q, const int64_t q_strides[4], const void *k,
+                                   const int64_t k_strides[4], int dtype, int64_t B, int64_t Hq, int64_t Hkv,
+                                   int64_t T, int64_t D, const float *rope, int64_t table_rows, int64_t rd,
+                                   int32_t interleaved, const int64_t *positions, const int64_t pos_strides[2],
+                                   const float *q_weight, const float *k_weight, float eps, void *q_out,
+                                   const int64_t q_out_strides[4], void *k_out, const int64_t k_out_strides[4],
+                                   uint32_t *status, void *stream);
+
+/*
+ * Append new keys and values to a paged cache, the norm and rotation of
+ * spruce_qk_norm_rope applied on the way (to q as well, when it is given).
+ * q [N, Hq, D], k / v [N, Hkv, D] are the packed new tokens of S sequences:
+ * sequence s has tokens [cu_q[s], cu_q[s+1]) and holds kv_lens[s] tokens after
+ * this call, so its token i lands at cache position kv_lens[s] - q_len + i:
+ * page block_table[s][position / page_size], row position % page_size of
+ * k_cache / v_cache [num_pages, Hkv, page_size, D] (element strides page, head,
+ * row; unit last).  The same position picks the rotation's angles unless
+ * `positions` [N] gives them.  rd = 0: no rotation.  q_out [N, Hq, D] (NULL with
+ * q) may be q.  Strides of packed tensors are (token, head).  A token whose
+ * position lies outside its table row, or whose page id lies outside the cache,
+ * is not written and raises SPRUCE_STATUS_BAD_LENGTH / _BAD_PAGE; tokens past
+ * cu_q[S] are left out.
+ */
+SPRUCE_API int spruce_paged_append(const void *q, const int64_t q_strides[2], const void *k,
+                                   const int64_t k_strides[2], const void *v, const int64_t v_strides[2], int dtype,
+                                   int64_t N, int64_t Hq, int64_t Hkv, int64_t D, const float *rope,
+                                   int64_t table_rows, int64_t rd, int32_t interleaved, const int64_t *positions,
+                                   const float *q_weight, const float *k_weight, float eps, void *q_out,
+                                   const int64_t q_out_strides[2], void *k_cache, const int64_t kc_strides[3],
+                                   void *v_cache, const int64_t vc_strides[3], int64_t num_pages, int64_t page_size,
+                                   const int32_t *block_table, int64_t table_stride, int64_t max_pages,
+                                   const int32_t *cu_q, const int32_t *kv_lens, int64_t S, uint32_t *status,
+                                   void *stream);
+
+/*
+ * Causal GQA attention of new tokens over a paged cache: sequence s's query i
+ * (packed as above, already in the cache) sees positions 0 .. kv_lens[s] -
+ * q_len + i.  From single tokens to prefill chunks, of any mix of lengths; a
+ * query that sees nothing (an empty sequence) yields zeros, rows past cu_q[S]
+ * are not written.  Cache rows at or past kv_lens[s] never reach an output,
+ * whatever they hold.  max_q_len and max_kv_len bound q_len and kv_lens (they
+ * size the launch); a longer sequence is cut to them and raises
+ * SPRUCE_STATUS_BAD_LENGTH, a page id outside the cache reads zeros and raises
+ * SPRUCE_STATUS_BAD_PAGE.  D in {64, 128}, page_size a multiple of 16, every
+ * row 16-byte aligned.  bf16 / fp16 run tensor-core kernels, fp32 a CUDA-core
+ * kernel.  workspace (spruce_paged_attention_workspace_bytes, -1 for an invalid
+ * shape; 256-byte aligned)
+ * holds the parts of sequences that several CTAs share; a call uses it alone.
+ */
+SPRUCE_API int64_t spruce_paged_attention_workspace_bytes(int64_t Hq, int64_t Hkv, int64_t D, int64_t max_q_len,
+                                                          int dtype);
+SPRUCE_API int spruce_paged_attention(const void *q, const int64_t q_strides[2], const void *k_cache,
+                                      const int64_t kc_strides[3], const void *v_cache, const int64_t vc_strides[3],
+                                      int dtype, int64_t N, int64_t Hq, int64_t Hkv, int64_t D, int64_t num_pages,
+                                      int64_t page_size, const int32_t *block_table, int64_t table_stride,
+                                      int64_t max_pages, const int32_t *cu_q, const int32_t *kv_lens, int64_t S,
+                                      int64_t max_q_len, int64_t max_kv_len, float scale, void *out,
+                                      const int64_t out_strides[2], void *workspace, int64_t workspace_bytes,
+                                      uint32_t *status, void *stream);
 
 #ifdef __cplusplus
 }

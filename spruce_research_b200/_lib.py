@@ -22,6 +22,9 @@ ERR_WORKSPACE = 4
 
 STATUS_TIMEOUT = 1
 STATUS_EMPTY_ROW = 2
+STATUS_BAD_PAGE = 4
+STATUS_BAD_LENGTH = 8
+STATUS_BAD_POSITION = 16
 
 DTYPE_CODE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
@@ -73,6 +76,13 @@ SIGNATURES = {
                                           _I64, _I64, _F, _I64, _I64, _P, _P], _INT),
     "spruce_sparse_attention_fwd_scatter": ([_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _INT, _I64, _I64, _I64,
                                              _I64, _I64, _I64, _F, _I64, _I64, _P, ctypes.c_int32, _P, _P], _INT),
+    "spruce_qk_norm_rope": ([_P, _P, _P, _P, _INT, _I64, _I64, _I64, _I64, _I64, _P, _I64, _I64, _INT, _P, _P, _P,
+                             _P, _F, _P, _P, _P, _P, _P, _P], _INT),
+    "spruce_paged_append": ([_P, _P, _P, _P, _P, _P, _INT, _I64, _I64, _I64, _I64, _P, _I64, _I64, _INT, _P, _P, _P,
+                             _F, _P, _P, _P, _P, _P, _P, _I64, _I64, _P, _I64, _I64, _P, _P, _I64, _P, _P], _INT),
+    "spruce_paged_attention_workspace_bytes": ([_I64, _I64, _I64, _I64, _INT], _I64),
+    "spruce_paged_attention": ([_P, _P, _P, _P, _P, _P, _INT, _I64, _I64, _I64, _I64, _I64, _I64, _P, _I64, _I64, _P,
+                                _P, _I64, _I64, _I64, _F, _P, _P, _P, _I64, _P, _P], _INT),
 }
 
 _lib = None

@@ -754,4 +754,176 @@ int spruce_kv_summary_table(const void* key, const int64_t key_strides[4], const
   return cuda_status(e, "summary table launch");
 }
 
+// Checks shared by the operators that rotate: norms, table and rotary width.
+static int check_rope(int64_t D, const float* rope, int64_t table_rows, int64_t rd) {
+  if (D < 2 || D > 256 || D % 2) return fail(SPRUCE_ERR_UNSUPPORTED, "head_dim must be even and at most 256, got %lld", (long long)D);
+  if (rd < 0 || rd > D || rd % 2)
+    return fail(SPRUCE_ERR_INVALID, "rotary width must be even and at most head_dim, got %lld of %lld", (long long)rd, (long long)D);
+  if (rd > 0 && (rope == nullptr || table_rows < 1)) return fail(SPRUCE_ERR_INVALID, "the rotation table is empty");
+  return SPRUCE_OK;
+}
+
+int spruce_qk_norm_rope(const void* q, const int64_t q_strides[4], const void* k, const int64_t k_strides[4],
+                        int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t T, int64_t D, const float* rope,
+                        int64_t table_rows, int64_t rd, int32_t interleaved, const int64_t* positions,
+                        const int64_t pos_strides[2], const float* q_weight, const float* k_weight, float eps,
+                        void* q_out, const int64_t q_out_strides[4], void* k_out, const int64_t k_out_strides[4],
+                        uint32_t* status, void* stream) {
+  if (!valid_dtype(dtype)) return fail(SPRUCE_ERR_INVALID, "unsupported dtype code %d", dtype);
+  if (B < 0 || Hq < 1 || Hkv < 1 || T < 0 || Hq > 65535 || Hkv > 65535) return fail(SPRUCE_ERR_INVALID, "bad shape");
+  if (int rc = check_rope(D, rope, table_rows, rd)) return rc;
+  if (B == 0 || T == 0) return SPRUCE_OK;
+  if (B > INT32_MAX || T > INT32_MAX || B * T > INT64_MAX / (Hq + Hkv) / 32)
+    return fail(SPRUCE_ERR_UNSUPPORTED, "shape too large");
+  if (q == nullptr || k == nullptr || q_out == nullptr || k_out == nullptr) return fail(SPRUCE_ERR_INVALID, "null pointer");
+  if (q_strides[3] != 1 || k_strides[3] != 1 || q_out_strides[3] != 1 || k_out_strides[3] != 1)
+    return fail(SPRUCE_ERR_UNSUPPORTED, "q, k and their outputs need a unit last stride");
+  spruce::RowsArgs a{};
+  a.q = {q, q_strides[0], q_strides[1], q_strides[2], q_out, q_out_strides[0], q_out_strides[1], q_out_strides[2], q_weight};
+  a.k = {k, k_strides[0], k_strides[1], k_strides[2], k_out, k_out_strides[0], k_out_strides[1], k_out_strides[2], k_weight};
+  a.B = (int)B;
+  a.T = (int)T;
+  a.Hq = (int)Hq;
+  a.Hkv = (int)Hkv;
+  a.D = (int)D;
+  a.rd = (int)rd;
+  a.interleaved = interleaved != 0;
+  a.eps = eps;
+  a.rope = rope;
+  a.table_rows = table_rows;
+  a.positions = positions;
+  if (positions != nullptr) {
+    a.pos_sb = pos_strides[0];
+    a.pos_st = pos_strides[1];
+  }
+  a.status = status;
+  return cuda_status(spruce::launch_norm_rope(a, dtype, as_stream(stream)), "norm and rotation launch");
+}
+
+// The paged cache's shape and metadata, shared by the append and the attention.
+static int check_paged(int dtype, int64_t N, int64_t Hq, int64_t Hkv, int64_t num_pages, int64_t page_size,
+                       const int32_t* block_table, int64_t max_pages, const int32_t* cu_q, const int32_t* kv_lens,
+                       int64_t S) {
+  if (!valid_dtype(dtype)) return fail(SPRUCE_ERR_INVALID, "unsupported dtype code %d", dtype);
+  if (N < 0 || S < 0 || Hkv < 1 || Hq < 0 || Hq > 65535 || Hkv > 65535 || num_pages < 0 || max_pages < 0)
+    return fail(SPRUCE_ERR_INVALID, "bad shape");
+  if (page_size < 16 || page_size % 16)
+    return fail(SPRUCE_ERR_UNSUPPORTED, "page_size must be a multiple of 16, got %lld", (long long)page_size);
+  if (N >= INT32_MAX || S >= INT32_MAX || max_pages > INT32_MAX || page_size > INT32_MAX || num_pages > INT32_MAX)
+    return fail(SPRUCE_ERR_UNSUPPORTED, "shape too large");
+  if (N > 0 && S > 0 && (cu_q == nullptr || kv_lens == nullptr || (block_table == nullptr && max_pages > 0)))
+    return fail(SPRUCE_ERR_INVALID, "cu_q, kv_lens or block_table is NULL");
+  return SPRUCE_OK;
+}
+
+int spruce_paged_append(const void* q, const int64_t q_strides[2], const void* k, const int64_t k_strides[2],
+                        const void* v, const int64_t v_strides[2], int dtype, int64_t N, int64_t Hq, int64_t Hkv,
+                        int64_t D, const float* rope, int64_t table_rows, int64_t rd, int32_t interleaved,
+                        const int64_t* positions, const float* q_weight, const float* k_weight, float eps, void* q_out,
+                        const int64_t q_out_strides[2], void* k_cache, const int64_t kc_strides[3], void* v_cache,
+                        const int64_t vc_strides[3], int64_t num_pages, int64_t page_size, const int32_t* block_table,
+                        int64_t table_stride, int64_t max_pages, const int32_t* cu_q, const int32_t* kv_lens,
+                        int64_t S, uint32_t* status, void* stream) {
+  if (int rc = check_paged(dtype, N, Hq, Hkv, num_pages, page_size, block_table, max_pages, cu_q, kv_lens, S)) return rc;
+  if (int rc = check_rope(D, rope, table_rows, rd)) return rc;
+  if (N == 0 || S == 0) return SPRUCE_OK;
+  if (k == nullptr || v == nullptr || k_cache == nullptr || v_cache == nullptr || (q != nullptr && q_out == nullptr))
+    return fail(SPRUCE_ERR_INVALID, "null pointer");
+  spruce::RowsArgs a{};
+  if (q != nullptr) {
+    a.q = {q, 0, q_strides[1], q_strides[0], q_out, 0, q_out_strides[1], q_out_strides[0], q_weight};
+    a.Hq = (int)Hq;
+  }
+  a.k = {k, 0, k_strides[1], k_strides[0], k_cache, kc_strides[0], kc_strides[1], kc_strides[2], k_weight};
+  a.v = {v, 0, v_strides[1], v_strides[0], v_cache, vc_strides[0], vc_strides[1], vc_strides[2], nullptr};
+  a.B = 1;
+  a.T = (int)N;
+  a.Hkv = (int)Hkv;
+  a.D = (int)D;
+  a.rd = (int)rd;
+  a.interleaved = interleaved != 0;
+  a.eps = eps;
+  a.rope = rope;
+  a.table_rows = table_rows;
+  a.positions = positions;
+  a.pos_st = 1;
+  a.cu_q = cu_q;
+  a.kv_lens = kv_lens;
+  a.block_table = block_table;
+  a.table_stride = table_stride;
+  a.S = (int)S;
+  a.max_pages = (int)max_pages;
+  a.page_size = (int)page_size;
+  a.num_pages = num_pages;
+  a.status = status;
+  return cuda_status(spruce::launch_norm_rope(a, dtype, as_stream(stream)), "paged append launch");
+}
+
+int64_t spruce_paged_attention_workspace_bytes(int64_t Hq, int64_t Hkv, int64_t D, int64_t max_q_len, int dtype) {
+  if (!valid_dtype(dtype) || Hkv < 1 || Hq < 1 || Hq % Hkv || (D != 64 && D != 128) || max_q_len < 0 ||
+      max_q_len > INT32_MAX / Hq)
+    return -1;
+  return spruce::paged_workspace_bytes(Hq, Hkv, D, max_q_len, dtype);
+}
+
+int spruce_paged_attention(const void* q, const int64_t q_strides[2], const void* k_cache,
+                           const int64_t kc_strides[3], const void* v_cache, const int64_t vc_strides[3], int dtype,
+                           int64_t N, int64_t Hq, int64_t Hkv, int64_t D, int64_t num_pages, int64_t page_size,
+                           const int32_t* block_table, int64_t table_stride, int64_t max_pages, const int32_t* cu_q,
+                           const int32_t* kv_lens, int64_t S, int64_t max_q_len, int64_t max_kv_len, float scale,
+                           void* out, const int64_t out_strides[2], void* workspace, int64_t workspace_bytes,
+                           uint32_t* status, void* stream) {
+  if (int rc = check_paged(dtype, N, Hq, Hkv, num_pages, page_size, block_table, max_pages, cu_q, kv_lens, S)) return rc;
+  if (Hq < 1 || Hq % Hkv)
+    return fail(SPRUCE_ERR_INVALID, "query heads (%lld) must be divisible by KV heads (%lld)", (long long)Hq, (long long)Hkv);
+  if (D != 64 && D != 128) return fail(SPRUCE_ERR_UNSUPPORTED, "paged attention needs head_dim 64 or 128, got %lld", (long long)D);
+  if (max_q_len < 0 || max_kv_len < 0) return fail(SPRUCE_ERR_INVALID, "max_q_len and max_kv_len must not be negative");
+  if (max_q_len > INT32_MAX / Hq || max_kv_len > INT32_MAX) return fail(SPRUCE_ERR_UNSUPPORTED, "sequence too long");
+  if (N == 0 || S == 0 || max_q_len == 0) return SPRUCE_OK;
+  if (q == nullptr || out == nullptr || ((k_cache == nullptr || v_cache == nullptr) && num_pages > 0))
+    return fail(SPRUCE_ERR_INVALID, "null pointer");
+  const int64_t vn = 16 / elem_size(dtype);
+  bool ok = aligned16(q) && aligned16(out) && aligned16(k_cache) && aligned16(v_cache);
+  for (int i = 0; i < 2; ++i) ok = ok && q_strides[i] % vn == 0 && out_strides[i] % vn == 0;
+  for (int i = 0; i < 3; ++i) ok = ok && kc_strides[i] % vn == 0 && vc_strides[i] % vn == 0;
+  if (!ok) return fail(SPRUCE_ERR_UNSUPPORTED, "q, out and the cache need 16-byte aligned rows");
+  const int64_t need = spruce_paged_attention_workspace_bytes(Hq, Hkv, D, max_q_len, dtype);
+  if (workspace == nullptr || workspace_bytes < need)
+    return fail(SPRUCE_ERR_WORKSPACE, "paged attention workspace needs %lld bytes, got %lld", (long long)need,
+                (long long)workspace_bytes);
+  if (reinterpret_cast<uintptr_t>(workspace) & 255u) return fail(SPRUCE_ERR_UNSUPPORTED, "workspace must be 256-byte aligned");
+  spruce::PagedArgs a{};
+  a.q = q;
+  a.qn = q_strides[0];
+  a.qh = q_strides[1];
+  a.kc = k_cache;
+  a.vc = v_cache;
+  for (int i = 0; i < 3; ++i) {
+    a.ks[i] = kc_strides[i];
+    a.vs[i] = vc_strides[i];
+  }
+  a.block_table = block_table;
+  a.table_stride = table_stride;
+  a.cu_q = cu_q;
+  a.kv_lens = kv_lens;
+  a.out = out;
+  a.on = out_strides[0];
+  a.oh = out_strides[1];
+  a.S = (int)S;
+  a.N = (int)N;
+  a.Hq = (int)Hq;
+  a.Hkv = (int)Hkv;
+  a.D = (int)D;
+  a.page_size = (int)page_size;
+  a.max_pages = num_pages > 0 ? (int)max_pages : 0;
+  a.max_q = (int)max_q_len;
+  a.max_kv = (int)max_kv_len;
+  a.num_pages = num_pages;
+  a.scale = scale;
+  a.workspace = workspace;
+  a.workspace_bytes = workspace_bytes;
+  a.status = status;
+  return cuda_status(spruce::launch_paged_attention(a, dtype, as_stream(stream)), "paged attention launch");
+}
+
 }  // extern "C"

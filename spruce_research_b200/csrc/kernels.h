@@ -140,6 +140,57 @@ int attn_pair_max_kw(int D);
 // The pair kernel's FMA-pipe polynomial exp2 and the MUFU exp2 over n values (self-check).
 cudaError_t launch_exp2_probe(const float* x, float* poly, float* mufu, int64_t n, cudaStream_t stream);
 
+// Head norms and rotary positions, dense or into a paged cache (rope.cu).
+struct Rows {
+  const void* x;            // [B, H, T, D], element strides (unit last); nullptr: none
+  int64_t sb, sh, st;
+  void* out;                // dense: by (b, h, t); cache rows: by (page, head, row of the page)
+  int64_t ob, oh, ot;
+  const float* weight;      // head norm [D], or nullptr
+};
+struct RowsArgs {
+  Rows q, k, v;             // v only on the way into a cache
+  int B, T, Hq, Hkv, D, rd;
+  bool interleaved;
+  float eps;
+  const float* rope;        // [table_rows, rd] cos | sin
+  int64_t table_rows;
+  const int64_t* positions; // by strides (b, t), or nullptr: t, or the token's place in its sequence
+  int64_t pos_sb, pos_st;
+  // Into a cache (cu_q != nullptr): packed tokens (B = 1) of S sequences.
+  const int32_t* cu_q;
+  const int32_t* kv_lens;
+  const int32_t* block_table;
+  int64_t table_stride;
+  int S, max_pages, page_size;
+  int64_t num_pages;
+  uint32_t* status;
+};
+cudaError_t launch_norm_rope(const RowsArgs& a, int dtype, cudaStream_t stream);
+
+// Causal GQA attention of packed new tokens over a paged K/V cache (paged_*.cu).
+struct PagedArgs {
+  const void* q;              // [N, Hq, D]
+  int64_t qn, qh;
+  const void* kc;             // [num_pages, Hkv, page_size, D]
+  const void* vc;
+  int64_t ks[3], vs[3];       // element strides: page, head, row
+  const int32_t* block_table; // [S, max_pages]
+  int64_t table_stride;
+  const int32_t* cu_q;        // [S + 1]
+  const int32_t* kv_lens;     // [S]
+  void* out;                  // [N, Hq, D]
+  int64_t on, oh;
+  int S, N, Hq, Hkv, D, page_size, max_pages, max_q, max_kv;
+  int64_t num_pages;
+  float scale;
+  void* workspace;
+  int64_t workspace_bytes;
+  uint32_t* status;
+};
+int64_t paged_workspace_bytes(int64_t Hq, int64_t Hkv, int64_t D, int64_t max_q, int dtype);
+cudaError_t launch_paged_attention(const PagedArgs& a, int dtype, cudaStream_t stream);
+
 // K/V summary table of the residual tree (summaries.cu).
 struct KvSummaryArgs {
   const void* key;            // [B, H, T, D] strided, unit last stride

@@ -1,0 +1,281 @@
+// Attention of new tokens over a paged K/V cache: the CUDA-core kernel, the join of split units, and the choice of
+// kernel.  The work's split is in paged_common.cuh.
+//
+// For a query row q at position i: o = sum_j p_j v_j / sum_j p_j, p_j = 2^(q.k_j scale log2(e) - m), j <= i, over
+// key tiles in one pass with the running maximum m and sum.  Rows that see nothing are zero.  Cache rows at or past
+// the sequence's length are never loaded.
+//
+// A CTA of 256 threads holds R query rows and TK keys in shared memory as fp32; a thread forms TR x TC scores, then
+// TR rows x D / NC output dims.
+#include <algorithm>
+#include <climits>
+
+#include "paged_common.cuh"
+
+namespace spruce {
+
+template <typename T, int D, int R, int TK, int TR, int TC>
+__global__ void __launch_bounds__(256) paged_attn_simt_kernel(const PagedParams p) {
+  constexpr int NC = TK / TC;       // threads along the keys, and along D
+  constexpr int KP = D + 4;         // padded rows: float4 reads of adjacent keys hit distinct banks
+  constexpr int DV = D / NC;
+  constexpr int VN = 16 / sizeof(T);
+  static_assert((R / TR) * NC == 256 && NC <= 32, "256 threads");
+  extern __shared__ float fsm[];
+  float* Qs = fsm;                  // [R][D]
+  float* Ks = Qs + R * D;           // [TK][KP]
+  float* Vs = Ks + TK * KP;         // [TK][D]
+  float* Ps = Vs + TK * D;          // [R][TK + 1]
+  __shared__ int64_t scratch[33];
+
+  const int tid = threadIdx.x;
+  const int rg = tid / NC, cg = tid % NC;
+  PagedWalk<R, TK> walk;
+  const bool any = paged_run<R, TK, 256>(p, walk, scratch);
+  int4 mine = make_int4(0, 0, 0, 0);
+  PagedPiece x;
+  while (any && walk.next(p, x)) {
+    const int rows = min(R, x.q.qlen * p.rep - x.qt * R);
+    __syncthreads();
+    for (int e = tid; e < R * (D / VN); e += 256) {
+      const int r = e / (D / VN), d = e % (D / VN) * VN;
+      alignas(16) T v[VN] = {};
+      if (r < rows) {
+        int64_t tok;
+        int head;
+        paged_row(p, x, x.qt * R + r, tok, head);
+        *reinterpret_cast<uint4*>(v) =
+            *reinterpret_cast<const uint4*>(static_cast<const T*>(p.a.q) + tok * p.a.qn + head * p.a.qh + d);
+      }
+#pragma unroll
+      for (int i = 0; i < VN; ++i) Qs[r * D + d + i] = Elem<T>::to_f(v[i]);
+    }
+    float o[TR][DV], m[TR], l[TR];
+    int seen[TR];  // keys the row sees
+#pragma unroll
+    for (int i = 0; i < TR; ++i) {
+      m[i] = -INFINITY;
+      l[i] = 0.0f;
+      const int r = x.qt * R + rg * TR + i;
+      seen[i] = min(x.q.first + r / p.rep + 1, x.keys);
+#pragma unroll
+      for (int d = 0; d < DV; ++d) o[i][d] = 0.0f;
+    }
+    const int32_t* table = p.a.block_table + x.s * p.a.table_stride;
+    for (int t = x.t0; t < x.t1 && x.keys > 0; ++t) {
+      __syncthreads();
+      for (int e = tid; e < TK * (D / VN); e += 256) {
+        const int r = e / (D / VN), d = e % (D / VN) * VN;
+        const int key = t * TK + r;
+        alignas(16) T kk[VN] = {}, vv[VN] = {};
+        if (key < x.keys) {
+          const int pi = key / p.a.page_size;
+          const int64_t page = paged_page(p, table, pi);
+          const int64_t row = key - pi * p.a.page_size;
+          if (page >= 0) {
+            *reinterpret_cast<uint4*>(kk) = *reinterpret_cast<const uint4*>(
+                static_cast<const T*>(p.a.kc) + page * p.a.ks[0] + x.g * p.a.ks[1] + row * p.a.ks[2] + d);
+            *reinterpret_cast<uint4*>(vv) = *reinterpret_cast<const uint4*>(
+                static_cast<const T*>(p.a.vc) + page * p.a.vs[0] + x.g * p.a.vs[1] + row * p.a.vs[2] + d);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < VN; ++i) {
+          Ks[r * KP + d + i] = Elem<T>::to_f(kk[i]);
+          Vs[r * D + d + i] = Elem<T>::to_f(vv[i]);
+        }
+      }
+      __syncthreads();
+      float s[TR][TC];
+#pragma unroll
+      for (int i = 0; i < TR; ++i)
+#pragma unroll
+        for (int j = 0; j < TC; ++j) s[i][j] = 0.0f;
+#pragma unroll 4
+      for (int d = 0; d < D; d += 4) {
+        float4 qv[TR], kv[TC];
+#pragma unroll
+        for (int i = 0; i < TR; ++i) qv[i] = *reinterpret_cast<const float4*>(Qs + (rg * TR + i) * D + d);
+#pragma unroll
+        for (int j = 0; j < TC; ++j) kv[j] = *reinterpret_cast<const float4*>(Ks + (cg + j * NC) * KP + d);
+#pragma unroll
+        for (int i = 0; i < TR; ++i)
+#pragma unroll
+          for (int j = 0; j < TC; ++j)
+            s[i][j] = fmaf(qv[i].x, kv[j].x,
+                           fmaf(qv[i].y, kv[j].y, fmaf(qv[i].z, kv[j].z, fmaf(qv[i].w, kv[j].w, s[i][j]))));
+      }
+#pragma unroll
+      for (int i = 0; i < TR; ++i) {
+        float mx = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < TC; ++j) {
+          s[i][j] = t * TK + cg + j * NC < seen[i] ? s[i][j] * p.scale_log2 : -INFINITY;
+          mx = fmaxf(mx, s[i][j]);
+        }
+#pragma unroll
+        for (int off = NC / 2; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+        const float m_new = fmaxf(m[i], mx);
+        const float ref = m_new == -INFINITY ? 0.0f : m_new;
+        const float alpha = exp2f(m[i] - ref);  // 0 while the row has seen nothing
+        float sum = 0.0f;
+#pragma unroll
+        for (int j = 0; j < TC; ++j) {
+          const float e = exp2f(s[i][j] - ref);
+          Ps[(rg * TR + i) * (TK + 1) + cg + j * NC] = e;
+          sum += e;
+        }
+#pragma unroll
+        for (int off = NC / 2; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+        l[i] = l[i] * alpha + sum;
+        m[i] = m_new;
+#pragma unroll
+        for (int d = 0; d < DV; ++d) o[i][d] *= alpha;
+      }
+      __syncwarp();  // a row's probabilities are written and read by the same NC lanes
+#pragma unroll 4
+      for (int j = 0; j < TK; ++j) {
+        float pr[TR];
+#pragma unroll
+        for (int i = 0; i < TR; ++i) pr[i] = Ps[(rg * TR + i) * (TK + 1) + j];
+#pragma unroll
+        for (int d = 0; d < DV; ++d) {
+          const float v = Vs[j * D + cg * DV + d];
+#pragma unroll
+          for (int i = 0; i < TR; ++i) o[i][d] = fmaf(pr[i], v, o[i][d]);
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < TR; ++i) {
+      const int r = rg * TR + i;
+      if (r >= rows) continue;
+      if (x.slot < 0) {
+        int64_t tok;
+        int head;
+        paged_row(p, x, x.qt * R + r, tok, head);
+        T* dst = static_cast<T*>(p.a.out) + tok * p.a.on + head * p.a.oh + cg * DV;
+        const float inv = l[i] > 0.0f ? 1.0f / l[i] : 0.0f;
+#pragma unroll
+        for (int d = 0; d < DV; ++d) dst[d] = Elem<T>::from_f(o[i][d] * inv);
+      } else {
+        const int64_t at = (int64_t)(2 * blockIdx.x + x.slot) * R + r;
+        if (cg == 0) p.part_ml[at] = make_float2(m[i], l[i]);
+#pragma unroll
+        for (int d = 0; d < DV; ++d) p.part_o[at * D + cg * DV + d] = o[i][d];
+      }
+    }
+    if (x.parts > 0) mine = make_int4(x.s, x.qt, x.g, x.parts | x.slot << 30);
+  }
+  if (tid == 0) p.desc[blockIdx.x] = mine;
+}
+
+// One warp a row of a split unit: the parts' rows weighted by 2^(m_i - max), in the order of the keys.
+template <typename T>
+__global__ void __launch_bounds__(128) paged_join_kernel(const PagedParams p, int R) {
+  const int4 d = p.desc[blockIdx.x];
+  const int parts = d.w & 0x3fffffff;
+  const int r = blockIdx.y * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (parts == 0) return;
+  PagedPiece x;
+  x.q = paged_seq(p, d.x);
+  x.s = d.x;
+  x.g = d.z;
+  if (r >= min(R, x.q.qlen * p.rep - d.y * R)) return;
+  const int D = p.a.D;
+  auto at = [&](int i) { return (int64_t)(2 * (blockIdx.x + i) + (i == 0 ? (d.w >> 30) & 1 : 0)) * R + r; };
+  float top = -INFINITY;
+  for (int i = lane; i < parts; i += 32) top = fmaxf(top, p.part_ml[at(i)].x);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  const float ref = top == -INFINITY ? 0.0f : top;
+  float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f}, l = 0.0f;
+  const int dims = D / 32;  // 2 or 4 adjacent dims a lane
+  for (int i = 0; i < parts; ++i) {
+    const float2 ml = p.part_ml[at(i)];
+    const float w = exp2f(ml.x - ref);
+    l = fmaf(ml.y, w, l);
+    const float* o = p.part_o + at(i) * D + lane * dims;
+    if (dims == 4) {
+      const float4 v = *reinterpret_cast<const float4*>(o);
+      acc[0] = fmaf(v.x, w, acc[0]);
+      acc[1] = fmaf(v.y, w, acc[1]);
+      acc[2] = fmaf(v.z, w, acc[2]);
+      acc[3] = fmaf(v.w, w, acc[3]);
+    } else {
+      const float2 v = *reinterpret_cast<const float2*>(o);
+      acc[0] = fmaf(v.x, w, acc[0]);
+      acc[1] = fmaf(v.y, w, acc[1]);
+    }
+  }
+  int64_t tok;
+  int head;
+  paged_row(p, x, d.y * R + r, tok, head);
+  T* dst = static_cast<T*>(p.a.out) + tok * p.a.on + head * p.a.oh + lane * dims;
+  const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+  for (int i = 0; i < dims; ++i) dst[i] = Elem<T>::from_f(acc[i] * inv);
+}
+
+template <typename T>
+cudaError_t launch_paged_join(const PagedParams& p, int R, int G, cudaStream_t stream) {
+  paged_join_kernel<T><<<dim3(G, (R + 3) / 4), 128, 0, stream>>>(p, R);
+  return cudaGetLastError();
+}
+template cudaError_t launch_paged_join<float>(const PagedParams&, int, int, cudaStream_t);
+template cudaError_t launch_paged_join<__nv_bfloat16>(const PagedParams&, int, int, cudaStream_t);
+template cudaError_t launch_paged_join<__half>(const PagedParams&, int, int, cudaStream_t);
+
+constexpr int kMaxSms = 160;
+
+static int sm_count() {
+  static int n = 0;
+  if (n == 0) {
+    int dev = 0, v = 0;
+    if (cudaGetDevice(&dev) == cudaSuccess &&
+        cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess && v > 0)
+      n = std::min(v, kMaxSms);
+  }
+  return n > 0 ? n : 148;
+}
+
+// CTAs worth launching: all resident ones, or fewer where the tiles cannot be more.
+static int grid_for(const PagedArgs& a, int R, int TK, int resident) {
+  const int64_t rt = ((int64_t)a.max_q * (a.Hq / a.Hkv) + R - 1) / R;
+  const int64_t kt = std::max<int64_t>(1, ((int64_t)a.max_kv + TK - 1) / TK);
+  const __int128 tiles = (__int128)a.S * rt * kt * a.Hkv;
+  return tiles < resident ? static_cast<int>(tiles) : resident;
+}
+
+template <typename T, int D, int R, int TK, int TR, int TC>
+static cudaError_t launch_simt(const PagedArgs& a, cudaStream_t stream) {
+  constexpr int kPerSm = 2;
+  const size_t smem = sizeof(float) * (R * D + TK * (D + 4) + TK * D + R * (TK + 1));
+  auto kern = paged_attn_simt_kernel<T, D, R, TK, TR, TC>;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e != cudaSuccess) return e;
+  const int G = grid_for(a, R, TK, sm_count() * kPerSm);
+  const PagedParams p = paged_params(a, R, G, 1);
+  kern<<<G, 256, smem, stream>>>(p);
+  e = cudaGetLastError();
+  return e != cudaSuccess ? e : launch_paged_join<T>(p, R, G, stream);
+}
+
+template <typename T>
+static cudaError_t launch_simt_dtype(const PagedArgs& a, cudaStream_t stream) {
+  const bool few = (int64_t)a.max_q * (a.Hq / a.Hkv) <= 16;
+  if (a.D == 128)
+    return few ? launch_simt<T, 128, 16, 64, 2, 2>(a, stream) : launch_simt<T, 128, 64, 32, 4, 2>(a, stream);
+  return few ? launch_simt<T, 64, 16, 64, 2, 2>(a, stream) : launch_simt<T, 64, 64, 32, 4, 2>(a, stream);
+}
+
+int64_t paged_workspace_bytes(int64_t Hq, int64_t Hkv, int64_t D, int64_t max_q, int dtype) {
+  return paged_params_bytes(64, kMaxSms * 2, D);
+}
+
+cudaError_t launch_paged_attention(const PagedArgs& a, int dtype, cudaStream_t stream) {
+  if (dtype == SPRUCE_DTYPE_F32) return launch_simt_dtype<float>(a, stream);
+  if (dtype == SPRUCE_DTYPE_BF16) return launch_simt_dtype<__nv_bfloat16>(a, stream);
+  return launch_simt_dtype<__half>(a, stream);
+}
+
+}  // namespace spruce
