@@ -470,7 +470,7 @@ SPRUCE_API int spruce_paged_append(const void *q, const int64_t q_strides[2], co
  * whatever they hold.  max_q_len and max_kv_len bound q_len and kv_lens (they
  * size the launch); a longer sequence is cut to them and raises
  * SPRUCE_STATUS_BAD_LENGTH, a page id outside the cache reads zeros and raises
- * SPRUCE_STATUS_BAD_PAGE.  D in {64, 128}, page_size a multiple of 16, every
+ * SPRUCE_STATUS_BAD_PAGE.  scale >= 0, D in {64, 128}, page_size a multiple of 16, every
  * row 16-byte aligned.  bf16 / fp16 run tensor-core kernels, fp32 a CUDA-core
  * kernel.  workspace (spruce_paged_attention_workspace_bytes, -1 for an invalid
  * shape; 256-byte aligned)

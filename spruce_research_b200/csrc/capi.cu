@@ -879,6 +879,7 @@ int spruce_paged_attention(const void* q, const int64_t q_strides[2], const void
   if (D != 64 && D != 128) return fail(SPRUCE_ERR_UNSUPPORTED, "paged attention needs head_dim 64 or 128, got %lld", (long long)D);
   if (max_q_len < 0 || max_kv_len < 0) return fail(SPRUCE_ERR_INVALID, "max_q_len and max_kv_len must not be negative");
   if (max_q_len > INT32_MAX / Hq || max_kv_len > INT32_MAX) return fail(SPRUCE_ERR_UNSUPPORTED, "sequence too long");
+  if (!(scale >= 0.0f && scale <= 3.0e38f)) return fail(SPRUCE_ERR_INVALID, "scale must be finite and not negative, got %g", scale);
   if (N == 0 || S == 0 || max_q_len == 0) return SPRUCE_OK;
   if (q == nullptr || out == nullptr || ((k_cache == nullptr || v_cache == nullptr) && num_pages > 0))
     return fail(SPRUCE_ERR_INVALID, "null pointer");

@@ -268,11 +268,17 @@ static cudaError_t launch_simt_dtype(const PagedArgs& a, cudaStream_t stream) {
   return few ? launch_simt<T, 64, 16, 64, 2, 2>(a, stream) : launch_simt<T, 64, 64, 32, 4, 2>(a, stream);
 }
 
+static bool use_chunk(const PagedArgs& a, int dtype) {
+  return dtype != SPRUCE_DTYPE_F32 && a.num_pages > 0 && (int64_t)a.max_q * (a.Hq / a.Hkv) > 64;
+}
+
 int64_t paged_workspace_bytes(int64_t Hq, int64_t Hkv, int64_t D, int64_t max_q, int dtype) {
-  return paged_params_bytes(64, kMaxSms * 2, D);
+  return std::max(paged_params_bytes(64, kMaxSms * 2, D), paged_params_bytes(kPagedChunkRows, kMaxSms, D));
 }
 
 cudaError_t launch_paged_attention(const PagedArgs& a, int dtype, cudaStream_t stream) {
+  if (use_chunk(a, dtype))
+    return launch_paged_chunk(a, dtype, grid_for(a, kPagedChunkRows, kPagedChunkKeys, sm_count()), stream);
   if (dtype == SPRUCE_DTYPE_F32) return launch_simt_dtype<float>(a, stream);
   if (dtype == SPRUCE_DTYPE_BF16) return launch_simt_dtype<__nv_bfloat16>(a, stream);
   return launch_simt_dtype<__half>(a, stream);

@@ -1,0 +1,508 @@
+// Attention of chunks of new tokens over a paged K/V cache on the tcgen05 tensor cores (bf16 / fp16).
+//
+// The mathematics, the split of the work and its join are those of paged_common.cuh and paged_attn.cu.  A unit has R = 256
+// query rows -- two M = 128 tiles of (token, head of the group) rows, so a group of 7 heads fills its tiles as well as one of
+// 8 -- and its keys come in tiles of 128:
+//   S_t = Q_t K^T   M128 N128 K16, D / 16 MMAs      O_t += P_t V   M128 N = D K16, 8 MMAs.
+// A CTA per SM walks its run of key tiles, from unit to unit, with the loads running ahead across the units' border.
+//
+// Warps: 0-3 softmax and epilogue of tile 0 (thread = row = TMEM lane), 4-7 of tile 1, 8 loads K and V, 9 issues the MMAs
+// and owns TMEM.  The softmax warps also bring in their own Q rows (once a unit).  O_0 O_1 S_0 S_1 fill TMEM's columns; P_t
+// is written over the first half of S_t.  One thread issues QK_0(j) PV_1(j-1) QK_1(j) PV_0(j) ..., in whose order they
+// execute, so QK_t(j+1) overwrites P_t(j) after PV_t(j) has read it, and while one tile's softmax runs the tensor core
+// works for the other.  P is announced in halves of 64 keys, so PV starts on the first while the second is
+// exponentiated.  O is rescaled only when the running maximum grew by more than 8 (log2 units): P stays below
+// 2^8, which both 16-bit types hold, and O / l is exact for any reference.  P is rounded to the input type (the MMA's
+// operand); the sum l is of the unrounded fp32 values.
+//
+// Pages: one TMA box of a page's rows (or of 128 of them, or of its largest power-of-two divisor) lands as rows of the
+// 128-byte-swizzled tile.  Boxes past the sequence's end take a page index past the cache, which reads zeros; the rows of
+// the last page past the end may hold anything, so the loader clears them in V (their scores are masked by selection)
+// before the MMA issuer may read the tile.
+//
+// Every wait is bounded (common.cuh).
+#include <algorithm>
+
+#include "attn_common.cuh"
+#include "paged_common.cuh"
+
+namespace spruce {
+
+constexpr int kChunkThreads = 320;
+constexpr int kChunkLoader = 8;
+constexpr int kChunkMma = 9;
+constexpr int kChunkRows = kPagedChunkRows;
+constexpr int kChunkKeys = kPagedChunkKeys;
+
+template <int D>
+struct ChunkLayout {
+  static constexpr int STAGES = D == 128 ? 2 : 4;
+  static constexpr int NP = D / 64;           // 128-byte panels along the head dim
+  static constexpr int PANEL = 128 * 128;     // 128 rows x 128 B
+  static constexpr int TILE = NP * PANEL;
+  static constexpr int OFF_Q = 0;
+  static constexpr int OFF_K = 2 * TILE;
+  static constexpr int OFF_V = OFF_K + STAGES * TILE;
+  static constexpr int OFF_BAR = OFF_V + STAGES * TILE;
+  // q_full[2], k_full[S], v_full[S], kv_empty[S], v_tail, s_full[2], p_full[2][2], o_done[2], drain
+  static constexpr int NBAR = 2 + 3 * STAGES + 1 + 2 + 4 + 2 + 1;
+  static constexpr int OFF_MISC = OFF_BAR + NBAR * 8;
+  static constexpr int OFF_SCAN = (OFF_MISC + 16 + 15) / 16 * 16;
+  static constexpr int BYTES = 1024 + OFF_SCAN + 33 * 8;
+  static constexpr int COL_S = 2 * D;         // S_t (and P_t) at COL_S + 128 t
+};
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kChunkThreads, 1)
+    paged_chunk_sm100_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv,
+                             const PagedParams p, int box) {
+  using L = ChunkLayout<D>;
+  constexpr int STAGES = L::STAGES;
+  using Walk = PagedWalk<kChunkRows, kChunkKeys>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  uint32_t* const status = p.a.status;
+
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::OFF_BAR);
+  uint64_t* q_full = bars;                // [tile]: its Q rows are in shared memory (128 arrivals)
+  uint64_t* k_full = q_full + 2;
+  uint64_t* v_full = k_full + STAGES;
+  uint64_t* kv_empty = v_full + STAGES;
+  uint64_t* v_tail = kv_empty + STAGES;   // the loader's own: a V tile whose tail it clears has landed
+  uint64_t* s_full = v_tail + 1;          // [tile]: S_t(j) written
+  uint64_t* p_full = s_full + 2;          // [tile * 2 + half]: that half of P_t(j) written (128 arrivals)
+  uint64_t* o_done = p_full + 4;          // [tile]: the piece's last PV_t complete
+  uint64_t* drain = o_done + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::OFF_MISC);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::OFF_MISC + 4);
+  int64_t* scan = reinterpret_cast<int64_t*>(smem + L::OFF_SCAN);
+
+  if (warp == kChunkLoader) {
+    if (lane == 0) {
+      *abort_flag = 0;
+      for (int s = 0; s < STAGES; ++s) {
+        mbar_init(&k_full[s], 1);
+        mbar_init(&v_full[s], 1);
+        mbar_init(&kv_empty[s], 1);
+      }
+      for (int t = 0; t < 2; ++t) {
+        mbar_init(&q_full[t], 128);
+        mbar_init(&s_full[t], 1);
+        mbar_init(&p_full[2 * t], 128);
+        mbar_init(&p_full[2 * t + 1], 128);
+        mbar_init(&o_done[t], 1);
+      }
+      mbar_init(v_tail, 1);
+      mbar_init(drain, 1);
+      fence_barrier_init();
+      prefetch_tmap(&tmk);
+      prefetch_tmap(&tmv);
+    }
+    __syncwarp();
+  } else if (warp == kChunkMma) {
+    tmem_alloc(tmem_slot, 512u);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  Walk walk;
+  const bool any = paged_run<kChunkRows, kChunkKeys, kChunkThreads>(p, walk, scan);
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  if (!any) walk.left = 0;
+  PagedPiece x;
+
+  if (warp == kChunkLoader) {
+    // ------------------------------------------------------------ K and V
+    const int boxes = kChunkKeys / box * L::NP;  // per tile and tensor; at most 16
+    const int pp = lane % L::NP, row0 = lane / L::NP * box;
+    const bool mine = lane < boxes;
+    int j = 0;         // tiles loaded by this CTA
+    uint32_t tails = 0;
+    bool ok = true;
+    while (ok && walk.next(p, x)) {
+      if (x.keys == 0) continue;
+      const int32_t* table = p.a.block_table + x.s * p.a.table_stride;
+      auto page_of = [&](int t, int& row) {  // this lane's box of tile t
+        const int key = t * kChunkKeys + row0;
+        if (!mine || t >= x.t1 || key >= x.keys) return static_cast<int>(p.a.num_pages);
+        const int pi = key / p.a.page_size;
+        row = key - pi * p.a.page_size;
+        const int page = paged_page(p, table, pi);
+        return page < 0 ? static_cast<int>(p.a.num_pages) : page;
+      };
+      int row = 0, page = page_of(x.t0, row);
+      for (int t = x.t0; t < x.t1; ++t, ++j) {
+        const int st = j % STAGES;
+        if (j >= STAGES && !__all_sync(0xffffffffu, mbar_wait(&kv_empty[st], ((j / STAGES) - 1) & 1, status, abort_flag))) {
+          ok = false;
+          break;
+        }
+        uint8_t* ks = smem + L::OFF_K + st * L::TILE;
+        uint8_t* vs = smem + L::OFF_V + st * L::TILE;
+        const int valid = x.keys - t * kChunkKeys;       // keys of this tile that exist
+        const bool tail = valid < kChunkKeys && valid % box != 0;
+        if (lane == 0) {
+          mbar_arrive_expect_tx(&k_full[st], L::TILE);
+          mbar_arrive_expect_tx(tail ? v_tail : &v_full[st], L::TILE);
+        }
+        __syncwarp();
+        if (mine) {
+          tma_load_4d(ks + pp * L::PANEL + row0 * 128, &tmk, &k_full[st], pp * 64, row, x.g, page);
+          tma_load_4d(vs + pp * L::PANEL + row0 * 128, &tmv, tail ? v_tail : &v_full[st], pp * 64, row, x.g, page);
+        }
+        row = 0;
+        page = page_of(t + 1, row);  // its latency passes behind the wait for the next stage
+        if (tail) {
+          ok = __all_sync(0xffffffffu, mbar_wait(v_tail, tails & 1, status, abort_flag));
+          ++tails;
+          // Rows past the end, to the end of their box (whole 16-byte chunks: any swizzle).
+          const int end = min(kChunkKeys, (valid / box + 1) * box);
+          for (int e = lane; e < (end - valid) * 8 * L::NP; e += 32) {
+            const int panel = e / ((end - valid) * 8), c = e % ((end - valid) * 8);
+            *reinterpret_cast<uint4*>(vs + panel * L::PANEL + (valid + c / 8) * 128 + c % 8 * 16) = make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&v_full[st]);
+          if (!ok) break;
+        }
+      }
+    }
+    // No copy may be in flight when the CTA exits.
+    for (int i = max(0, j - STAGES); i < j; ++i) {
+      mbar_wait(&k_full[i % STAGES], (i / STAGES) & 1, status, nullptr);
+      mbar_wait(&v_full[i % STAGES], (i / STAGES) & 1, status, nullptr);
+    }
+    __syncwarp();
+  } else if (warp == kChunkMma) {
+    // ------------------------------------------------------------ MMA issuer
+    const bool leader = elect_one();
+    constexpr uint32_t fmt = UmmaFormat<T>::value;
+    constexpr uint32_t idesc_qk = idesc_f16(fmt, 0, 0, 128, 128);
+    constexpr uint32_t idesc_pv = idesc_f16(fmt, 0, 1, D, 128);
+    const uint64_t dq0 = smem_desc(smem_u32(smem + L::OFF_Q), 16, 1024);
+    const uint64_t dk0 = smem_desc(smem_u32(smem + L::OFF_K), 16, 1024);
+    const uint64_t dv0 = smem_desc(smem_u32(smem + L::OFF_V), L::PANEL, 1024);
+    auto commit = [&](uint64_t* bar) {
+      if (leader) umma_commit(bar);
+      __syncwarp();
+    };
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+      return __all_sync(0xffffffffu, mbar_wait(bar, parity, status, abort_flag));
+    };
+    auto issue_qk = [&](int t, int st) {
+      const uint32_t d = tmem + L::COL_S + 128 * t;
+      const uint64_t qa = dq0 + (uint64_t)((t * L::TILE) >> 4);
+      const uint64_t kb = dk0 + (uint64_t)((st * L::TILE) >> 4);
+#pragma unroll
+      for (int ks = 0; ks < D / 16; ++ks) {
+        const uint32_t off = ((ks >> 2) * L::PANEL + (ks & 3) * 32) >> 4;
+        if (leader) umma_f16_ss(d, qa + off, kb + off, idesc_qk, ks > 0 ? 1u : 0u);
+        __syncwarp();
+      }
+      commit(&s_full[t]);
+    };
+    uint32_t np_[2] = {0, 0};  // PVs issued for each tile
+    auto pv = [&](int t, int st, bool first) {
+      for (int h = 0; h < 2; ++h) {
+        if (!wait(&p_full[2 * t + h], np_[t] & 1)) return false;
+        tc_fence_after();
+        const uint32_t a = tmem + L::COL_S + 128 * t;
+        const uint64_t vb = dv0 + (uint64_t)((st * L::TILE) >> 4);
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) {
+          const int ks = 4 * h + kk;
+          if (leader)
+            umma_f16_ts(tmem + t * D, a + ks * 8, vb + (uint64_t)((ks * 2048) >> 4), idesc_pv,
+                        (!first || ks > 0) ? 1u : 0u);
+          __syncwarp();
+        }
+      }
+      ++np_[t];
+      return true;
+    };
+    int j = 0;
+    uint32_t pieces[2] = {0, 0};
+    bool ok = true;
+    while (ok && walk.next(p, x)) {
+      const int rows = min(kChunkRows, x.q.qlen * p.rep - x.qt * kChunkRows);
+      const bool two = rows > 128;
+      if (x.keys == 0) continue;
+      ok = wait(&q_full[0], pieces[0]++ & 1) && (!two || wait(&q_full[1], pieces[1]++ & 1));
+      const int n = x.t1 - x.t0;
+      for (int i = 0; ok && i <= n; ++i) {
+        const int st = (j + i) % STAGES;
+        const int sp = (j + i + STAGES - 1) % STAGES;  // stage of tile i - 1
+        const uint32_t ph = ((j + i) / STAGES) & 1;
+        if (i < n) {
+          if (!(ok = wait(&k_full[st], ph))) break;
+          tc_fence_after();
+          issue_qk(0, st);
+        }
+        if (i > 0 && two) {
+          if (!(ok = pv(1, sp, i == 1))) break;
+          if (i == n) commit(&o_done[1]);
+        }
+        if (i > 0) commit(&kv_empty[sp]);  // every MMA reading that stage is issued before this
+        if (i == n) break;
+        if (two) issue_qk(1, st);
+        if (!(ok = wait(&v_full[st], ph) && pv(0, st, i == 0))) break;
+        if (i == n - 1) commit(&o_done[0]);
+      }
+      j += n;
+    }
+    commit(drain);  // no MMA may be in flight when TMEM is released
+    mbar_wait(drain, 0, status, nullptr);
+    __syncwarp();
+  } else {
+    // ------------------------------------------------------------ softmax + epilogue
+    const int t = warp >> 2;
+    const int row = (warp & 3) * 32 + lane;  // TMEM lane == tile row
+    const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t tO = tmem + lane_off + t * D;
+    const uint32_t tS = tmem + lane_off + L::COL_S + 128 * t;
+    const float sl2 = p.scale_log2;
+    int4 mine = make_int4(0, 0, 0, 0);
+    uint32_t sj = 0, pieces = 0;  // tiles and pieces of this M-tile so far
+    bool ok = true;
+    while (ok && walk.next(p, x)) {
+      if (x.parts > 0) mine = make_int4(x.s, x.qt, x.g, x.parts | x.slot << 30);
+      const int rows = min(128, x.q.qlen * p.rep - x.qt * kChunkRows - t * 128);
+      if (rows <= 0) continue;
+      const int r0 = x.qt * kChunkRows + t * 128;  // the tile's first row in the sequence
+      const int n = x.keys == 0 ? 0 : x.t1 - x.t0;
+      if (n > 0) {
+        // This warp's 32 rows of Q into the swizzled layout (rows past the end: zeros).
+        constexpr int CH = D / 8;  // 16-byte chunks of a row
+        uint8_t* qs = smem + L::OFF_Q + t * L::TILE;
+#pragma unroll 4
+        for (int e = lane; e < 32 * CH; e += 32) {
+          const int r = (warp & 3) * 32 + e / CH, c = e % CH;
+          uint4 v = make_uint4(0, 0, 0, 0);
+          if (r < rows) {
+            int64_t tok;
+            int head;
+            paged_row(p, x, r0 + r, tok, head);
+            v = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.a.q) + tok * p.a.qn + head * p.a.qh + c * 8);
+          }
+          *reinterpret_cast<uint4*>(qs + (c >> 3) * L::PANEL + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v;
+        }
+        fence_proxy_async_smem();
+        mbar_arrive(&q_full[t]);
+      }
+      const int seen = min(x.q.first + (r0 + row) / p.rep + 1, x.keys);  // keys this row sees
+      float m_used = -INFINITY;  // reference max (log2 units) the exponentials use
+      float l = 0.0f;
+      for (int j = 0; j < n; ++j, ++sj) {
+        ok = __all_sync(0xffffffffu, mbar_wait(&s_full[t], sj & 1, status, abort_flag));
+        if (!ok) break;
+        tc_fence_after();
+        float s[4][32];  // s[q][c] = column 32q + c
+#pragma unroll
+        for (int q = 0; q < 4; ++q) tmem_ld32(tS + 32 * q, s[q]);
+        tmem_wait_ld();
+        const int lim = seen - (x.t0 + j) * kChunkKeys;  // columns below it are seen
+        const bool masked = __any_sync(0xffffffffu, lim < kChunkKeys);
+        if (masked) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+#pragma unroll
+            for (int c = 0; c < 32; ++c)
+              if (32 * q + c >= lim) s[q][c] = -INFINITY;
+        }
+        float mx8[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          float a = fmax3(s[0][u], s[0][u + 8], s[0][u + 16]);
+          a = fmax3(a, s[0][u + 24], s[1][u]);
+          a = fmax3(a, s[1][u + 8], s[1][u + 16]);
+          a = fmax3(a, s[1][u + 24], s[2][u]);
+          a = fmax3(a, s[2][u + 8], s[2][u + 16]);
+          a = fmax3(a, s[2][u + 24], s[3][u]);
+          a = fmax3(a, s[3][u + 8], s[3][u + 16]);
+          mx8[u] = fmaxf(a, s[3][u + 24]);
+        }
+        const float mx = fmaxf(fmax3(mx8[0], mx8[1], mx8[2]), fmax3(mx8[3], mx8[4], fmax3(mx8[5], mx8[6], mx8[7])));
+        const float m_new = fmaxf(m_used, mx == -INFINITY ? -INFINITY : mx * sl2);
+        const bool rescale = (j == 0) || (m_new > m_used + 8.0f);
+        const float alpha = (j > 0 && rescale) ? fast_exp2(m_used - m_new) : 1.0f;
+        if (rescale) m_used = m_new;
+        const float neg_ref = (m_used == -INFINITY) ? 0.0f : -m_used;
+        uint64_t sum2[2] = {f2_pack(0.0f, 0.0f), f2_pack(0.0f, 0.0f)};
+        const uint64_t sl2x2 = f2_pack(sl2, sl2), nref2 = f2_pack(neg_ref, neg_ref);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          uint32_t pk[16];
+          if (!masked) {
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {
+              float x0, x1, e0, e1;
+              f2_unpack(f2_fma(f2_pack(s[q][2 * k], s[q][2 * k + 1]), sl2x2, nref2), x0, x1);
+              if ((k & 7) == 7) {
+                poly_exp2_x2(x0, x1, e0, e1);
+              } else {
+                e0 = fast_exp2(x0);
+                e1 = fast_exp2(x1);
+              }
+              sum2[k & 1] = f2_add(sum2[k & 1], f2_pack(e0, e1));
+              pk[k] = Pack2<T>::pack(e0, e1);
+            }
+          } else {
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {
+              float x0, x1;
+              f2_unpack(f2_fma(f2_pack(s[q][2 * k], s[q][2 * k + 1]), sl2x2, nref2), x0, x1);
+              const float e0 = fast_exp2(x0);
+              const float e1 = fast_exp2(x1);
+              sum2[k & 1] = f2_add(sum2[k & 1], f2_pack(e0, e1));
+              pk[k] = Pack2<T>::pack(e0, e1);
+            }
+          }
+          tmem_st16u(tS + 16 * q, pk);
+          if (q == 1) {
+            // First half of P written: rescale O (PV_t(j-1) is complete, PV_t(j) not
+            // yet issued), then let the issuer start PV over these 64 keys.
+            if (j > 0 && __any_sync(0xffffffffu, rescale)) {
+#pragma unroll 1
+              for (int cc = 0; cc < D / 32; ++cc) {
+                float o[32];
+                tmem_ld32(tO + cc * 32, o);
+                tmem_wait_ld();
+#pragma unroll
+                for (int e = 0; e < 32; ++e) o[e] *= alpha;
+                tmem_st32(tO + cc * 32, o);
+              }
+            }
+            tmem_wait_st();
+            tc_fence_before();
+            mbar_arrive(&p_full[2 * t]);
+          }
+        }
+        float part[4];
+        f2_unpack(sum2[0], part[0], part[1]);
+        f2_unpack(sum2[1], part[2], part[3]);
+        l = l * alpha + ((part[0] + part[1]) + (part[2] + part[3]));
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(&p_full[2 * t + 1]);
+      }
+      if (!ok) break;
+      if (n > 0) {
+        ok = __all_sync(0xffffffffu, mbar_wait(&o_done[t], pieces & 1, status, abort_flag));
+        ++pieces;
+        if (!ok) break;
+        tc_fence_after();
+      }
+      const bool whole = x.slot < 0;
+      const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+      T* dst = nullptr;
+      float* part_o = nullptr;
+      if (row < rows) {
+        if (whole) {
+          int64_t tok;
+          int head;
+          paged_row(p, x, r0 + row, tok, head);
+          dst = static_cast<T*>(p.a.out) + tok * p.a.on + head * p.a.oh;
+        } else {
+          const int64_t at = (int64_t)(2 * blockIdx.x + x.slot) * kChunkRows + t * 128 + row;
+          p.part_ml[at] = make_float2(m_used, l);
+          part_o = p.part_o + at * D;
+        }
+      }
+#pragma unroll 1
+      for (int cc = 0; cc < D / 32; ++cc) {
+        float o[32];
+        if (n > 0) {
+          tmem_ld32(tO + cc * 32, o);
+          tmem_wait_ld();
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = 0.0f;
+        }
+        if (dst != nullptr) {
+#pragma unroll
+          for (int v4 = 0; v4 < 4; ++v4) {
+            uint4 v;
+            v.x = Pack2<T>::pack(o[v4 * 8 + 0] * inv, o[v4 * 8 + 1] * inv);
+            v.y = Pack2<T>::pack(o[v4 * 8 + 2] * inv, o[v4 * 8 + 3] * inv);
+            v.z = Pack2<T>::pack(o[v4 * 8 + 4] * inv, o[v4 * 8 + 5] * inv);
+            v.w = Pack2<T>::pack(o[v4 * 8 + 6] * inv, o[v4 * 8 + 7] * inv);
+            *reinterpret_cast<uint4*>(dst + cc * 32 + v4 * 8) = v;
+          }
+        } else if (part_o != nullptr) {
+#pragma unroll
+          for (int v4 = 0; v4 < 8; ++v4)
+            *reinterpret_cast<float4*>(part_o + cc * 32 + v4 * 4) =
+                make_float4(o[v4 * 4], o[v4 * 4 + 1], o[v4 * 4 + 2], o[v4 * 4 + 3]);
+        }
+      }
+      tc_fence_before();  // O and S are read before the next piece's MMAs, which wait for its Q
+    }
+    if (threadIdx.x == 0) p.desc[blockIdx.x] = mine;
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kChunkMma) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512u);
+  }
+}
+
+// Tensor map of a cache [pages, Hkv, page_size, D]: boxes of 64 dims x `box` rows of one head's page.
+static bool cache_map(CUtensorMap* m, const void* base, CUtensorMapDataType dt, const PagedArgs& a, const int64_t* s,
+                      int box) {
+  EncodeTiledFn fn = encode_fn();
+  if (fn == nullptr) return false;
+  const cuuint64_t dims[4] = {(cuuint64_t)a.D, (cuuint64_t)a.page_size, (cuuint64_t)a.Hkv, (cuuint64_t)a.num_pages};
+  // A dimension of one element never steps: any valid stride will do.
+  const cuuint64_t row = (cuuint64_t)a.D * 2;
+  const cuuint64_t strides[3] = {(cuuint64_t)s[2] * 2, a.Hkv > 1 ? (cuuint64_t)s[1] * 2 : row,
+                                 a.num_pages > 1 ? (cuuint64_t)s[0] * 2 : row};
+  const cuuint32_t b[4] = {64, (cuuint32_t)box, 1, 1};
+  const cuuint32_t estr[4] = {1, 1, 1, 1};
+  return fn(m, dt, 4, const_cast<void*>(base), dims, strides, b, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Rows of a TMA box: a page's, where they divide the tile; else the largest power of two that divides them.
+int paged_box(int page_size, int tile) {
+  int box = 16;
+  while (box < tile && page_size % (2 * box) == 0) box *= 2;
+  return box;
+}
+
+bool paged_cache_maps(const PagedArgs& a, int dtype, int box, CUtensorMap* mk, CUtensorMap* mv) {
+  const CUtensorMapDataType dt =
+      dtype == SPRUCE_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  return cache_map(mk, a.kc, dt, a, a.ks, box) && cache_map(mv, a.vc, dt, a, a.vs, box);
+}
+
+template <typename T, int D>
+static cudaError_t launch_chunk(const PagedArgs& a, int dtype, int G, cudaStream_t stream) {
+  using L = ChunkLayout<D>;
+  CUtensorMap mk, mv;
+  const int box = paged_box(a.page_size, kChunkKeys);
+  if (!paged_cache_maps(a, dtype, box, &mk, &mv)) return cudaErrorInvalidValue;
+  auto kern = paged_chunk_sm100_kernel<T, D>;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::BYTES);
+  if (e != cudaSuccess) return e;
+  const PagedParams p = paged_params(a, kChunkRows, G, 1);
+  kern<<<G, kChunkThreads, L::BYTES, stream>>>(mk, mv, p, box);
+  e = cudaGetLastError();
+  return e != cudaSuccess ? e : launch_paged_join<T>(p, kChunkRows, G, stream);
+}
+
+cudaError_t launch_paged_chunk(const PagedArgs& a, int dtype, int G, cudaStream_t stream) {
+  if (dtype == SPRUCE_DTYPE_BF16)
+    return a.D == 128 ? launch_chunk<__nv_bfloat16, 128>(a, dtype, G, stream)
+                      : launch_chunk<__nv_bfloat16, 64>(a, dtype, G, stream);
+  return a.D == 128 ? launch_chunk<__half, 128>(a, dtype, G, stream) : launch_chunk<__half, 64>(a, dtype, G, stream);
+}
+
+}  // namespace spruce

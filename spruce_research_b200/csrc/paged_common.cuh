@@ -209,6 +209,10 @@ __device__ __forceinline__ int paged_page(const PagedParams& p, const int32_t* t
   return -1;
 }
 
+// Tensor-core attention of chunks (paged_chunk_sm100.cu), on G CTAs.
+constexpr int kPagedChunkRows = 256, kPagedChunkKeys = 128;
+cudaError_t launch_paged_chunk(const PagedArgs& a, int dtype, int G, cudaStream_t stream);
+
 // Joins the parts of split units (paged_attn.cu).
 template <typename T>
 cudaError_t launch_paged_join(const PagedParams& p, int R, int G, cudaStream_t stream);
@@ -228,7 +232,8 @@ inline PagedParams paged_params(const PagedArgs& a, int R, int G, int min_tiles)
   p.part_ml = reinterpret_cast<float2*>(ws);
   ws += (int64_t)2 * G * R * 8;
   p.part_o = reinterpret_cast<float*>(ws);
-  p.scale_log2 = a.scale * 1.4426950408889634f;
+  // Not 0: a masked score (-inf) times 0 is not a number.  1e-30 makes every finite score 0 as well.
+  p.scale_log2 = a.scale > 0.0f ? a.scale * 1.4426950408889634f : 1e-30f;
   return p;
 }
 inline int64_t paged_params_bytes(int R, int G, int64_t D) {
