@@ -22,7 +22,7 @@ CSRC = os.path.join(PKG, "csrc")
 LIB = os.path.join(PKG, "libspruce_b200.so")
 SOURCES = ["pool.cu", "select.cu", "tree.cu", "attn_sm100.cu", "attn_pair_sm100.cu", "attn_f32.cu",
            "summaries.cu", "residual.cu", "rope.cu", "paged_attn.cu",
-           "paged_chunk_sm100.cu", "capi.cu"]
+           "paged_chunk_sm100.cu", "paged_rows_sm100.cu", "capi.cu"]
 HEADERS = ["common.cuh", "kernels.h", "attn_common.cuh", "paged_common.cuh"]
 
 NVCC_FLAGS = [

@@ -881,7 +881,8 @@ int spruce_paged_attention(const void* q, const int64_t q_strides[2], const void
   if (max_q_len > INT32_MAX / Hq || max_kv_len > INT32_MAX) return fail(SPRUCE_ERR_UNSUPPORTED, "sequence too long");
   if (!(scale >= 0.0f && scale <= 3.0e38f)) return fail(SPRUCE_ERR_INVALID, "scale must be finite and not negative, got %g", scale);
   if (N == 0 || S == 0 || max_q_len == 0) return SPRUCE_OK;
-  if (q == nullptr || out == nullptr || ((k_cache == nullptr || v_cache == nullptr) && num_pages > 0))
+  if (num_pages < 1) return fail(SPRUCE_ERR_INVALID, "the cache has no pages");
+  if (q == nullptr || out == nullptr || k_cache == nullptr || v_cache == nullptr)
     return fail(SPRUCE_ERR_INVALID, "null pointer");
   const int64_t vn = 16 / elem_size(dtype);
   bool ok = aligned16(q) && aligned16(out) && aligned16(k_cache) && aligned16(v_cache);
@@ -916,7 +917,7 @@ int spruce_paged_attention(const void* q, const int64_t q_strides[2], const void
   a.Hkv = (int)Hkv;
   a.D = (int)D;
   a.page_size = (int)page_size;
-  a.max_pages = num_pages > 0 ? (int)max_pages : 0;
+  a.max_pages = (int)max_pages;
   a.max_q = (int)max_q_len;
   a.max_kv = (int)max_kv_len;
   a.num_pages = num_pages;

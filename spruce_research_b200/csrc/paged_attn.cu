@@ -1,5 +1,5 @@
-// Attention of new tokens over a paged K/V cache: the CUDA-core kernel, the join of split units, and the choice of
-// kernel.  The work's split is in paged_common.cuh.
+// Attention of new tokens over a paged K/V cache: the fp32 CUDA-core kernel, the join of split units, and the
+// choice of kernel.  The work's split is in paged_common.cuh.
 //
 // For a query row q at position i: o = sum_j p_j v_j / sum_j p_j, p_j = 2^(q.k_j scale log2(e) - m), j <= i, over
 // key tiles in one pass with the running maximum m and sum.  Rows that see nothing are zero.  Cache rows at or past
@@ -14,12 +14,12 @@
 
 namespace spruce {
 
-template <typename T, int D, int R, int TK, int TR, int TC>
-__global__ void __launch_bounds__(256) paged_attn_simt_kernel(const PagedParams p) {
+template <int D, int R, int TK, int TR, int TC>
+__global__ void __launch_bounds__(256) paged_attn_f32_kernel(const PagedParams p) {
   constexpr int NC = TK / TC;       // threads along the keys, and along D
   constexpr int KP = D + 4;         // padded rows: float4 reads of adjacent keys hit distinct banks
   constexpr int DV = D / NC;
-  constexpr int VN = 16 / sizeof(T);
+  constexpr int VN = 4;             // floats of a 16-byte load
   static_assert((R / TR) * NC == 256 && NC <= 32, "256 threads");
   extern __shared__ float fsm[];
   float* Qs = fsm;                  // [R][D]
@@ -39,16 +39,14 @@ __global__ void __launch_bounds__(256) paged_attn_simt_kernel(const PagedParams 
     __syncthreads();
     for (int e = tid; e < R * (D / VN); e += 256) {
       const int r = e / (D / VN), d = e % (D / VN) * VN;
-      alignas(16) T v[VN] = {};
+      float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
       if (r < rows) {
         int64_t tok;
         int head;
         paged_row(p, x, x.qt * R + r, tok, head);
-        *reinterpret_cast<uint4*>(v) =
-            *reinterpret_cast<const uint4*>(static_cast<const T*>(p.a.q) + tok * p.a.qn + head * p.a.qh + d);
+        v = *reinterpret_cast<const float4*>(static_cast<const float*>(p.a.q) + tok * p.a.qn + head * p.a.qh + d);
       }
-#pragma unroll
-      for (int i = 0; i < VN; ++i) Qs[r * D + d + i] = Elem<T>::to_f(v[i]);
+      *reinterpret_cast<float4*>(Qs + r * D + d) = v;
     }
     float o[TR][DV], m[TR], l[TR];
     int seen[TR];  // keys the row sees
@@ -67,23 +65,20 @@ __global__ void __launch_bounds__(256) paged_attn_simt_kernel(const PagedParams 
       for (int e = tid; e < TK * (D / VN); e += 256) {
         const int r = e / (D / VN), d = e % (D / VN) * VN;
         const int key = t * TK + r;
-        alignas(16) T kk[VN] = {}, vv[VN] = {};
+        float4 kk = make_float4(0.0f, 0.0f, 0.0f, 0.0f), vv = kk;
         if (key < x.keys) {
           const int pi = key / p.a.page_size;
           const int64_t page = paged_page(p, table, pi);
           const int64_t row = key - pi * p.a.page_size;
           if (page >= 0) {
-            *reinterpret_cast<uint4*>(kk) = *reinterpret_cast<const uint4*>(
-                static_cast<const T*>(p.a.kc) + page * p.a.ks[0] + x.g * p.a.ks[1] + row * p.a.ks[2] + d);
-            *reinterpret_cast<uint4*>(vv) = *reinterpret_cast<const uint4*>(
-                static_cast<const T*>(p.a.vc) + page * p.a.vs[0] + x.g * p.a.vs[1] + row * p.a.vs[2] + d);
+            kk = *reinterpret_cast<const float4*>(static_cast<const float*>(p.a.kc) + page * p.a.ks[0] +
+                                                  x.g * p.a.ks[1] + row * p.a.ks[2] + d);
+            vv = *reinterpret_cast<const float4*>(static_cast<const float*>(p.a.vc) + page * p.a.vs[0] +
+                                                  x.g * p.a.vs[1] + row * p.a.vs[2] + d);
           }
         }
-#pragma unroll
-        for (int i = 0; i < VN; ++i) {
-          Ks[r * KP + d + i] = Elem<T>::to_f(kk[i]);
-          Vs[r * D + d + i] = Elem<T>::to_f(vv[i]);
-        }
+        *reinterpret_cast<float4*>(Ks + r * KP + d) = kk;
+        *reinterpret_cast<float4*>(Vs + r * D + d) = vv;
       }
       __syncthreads();
       float s[TR][TC];
@@ -154,10 +149,10 @@ __global__ void __launch_bounds__(256) paged_attn_simt_kernel(const PagedParams 
         int64_t tok;
         int head;
         paged_row(p, x, x.qt * R + r, tok, head);
-        T* dst = static_cast<T*>(p.a.out) + tok * p.a.on + head * p.a.oh + cg * DV;
+        float* dst = static_cast<float*>(p.a.out) + tok * p.a.on + head * p.a.oh + cg * DV;
         const float inv = l[i] > 0.0f ? 1.0f / l[i] : 0.0f;
 #pragma unroll
-        for (int d = 0; d < DV; ++d) dst[d] = Elem<T>::from_f(o[i][d] * inv);
+        for (int d = 0; d < DV; ++d) dst[d] = o[i][d] * inv;
       } else {
         const int64_t at = (int64_t)(2 * blockIdx.x + x.slot) * R + r;
         if (cg == 0) p.part_ml[at] = make_float2(m[i], l[i]);
@@ -246,42 +241,42 @@ static int grid_for(const PagedArgs& a, int R, int TK, int resident) {
   return tiles < resident ? static_cast<int>(tiles) : resident;
 }
 
-template <typename T, int D, int R, int TK, int TR, int TC>
-static cudaError_t launch_simt(const PagedArgs& a, cudaStream_t stream) {
-  constexpr int kPerSm = 2;
+constexpr int kF32Rows = 64, kF32PerSm = 2;
+
+template <int D, int R, int TK, int TR, int TC>
+static cudaError_t launch_f32(const PagedArgs& a, cudaStream_t stream) {
   const size_t smem = sizeof(float) * (R * D + TK * (D + 4) + TK * D + R * (TK + 1));
-  auto kern = paged_attn_simt_kernel<T, D, R, TK, TR, TC>;
+  auto kern = paged_attn_f32_kernel<D, R, TK, TR, TC>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return e;
-  const int G = grid_for(a, R, TK, sm_count() * kPerSm);
+  const int G = grid_for(a, R, TK, sm_count() * kF32PerSm);
   const PagedParams p = paged_params(a, R, G, 1);
   kern<<<G, 256, smem, stream>>>(p);
   e = cudaGetLastError();
-  return e != cudaSuccess ? e : launch_paged_join<T>(p, R, G, stream);
+  return e != cudaSuccess ? e : launch_paged_join<float>(p, R, G, stream);
 }
 
-template <typename T>
-static cudaError_t launch_simt_dtype(const PagedArgs& a, cudaStream_t stream) {
+static cudaError_t launch_paged_f32(const PagedArgs& a, cudaStream_t stream) {
   const bool few = (int64_t)a.max_q * (a.Hq / a.Hkv) <= 16;
-  if (a.D == 128)
-    return few ? launch_simt<T, 128, 16, 64, 2, 2>(a, stream) : launch_simt<T, 128, 64, 32, 4, 2>(a, stream);
-  return few ? launch_simt<T, 64, 16, 64, 2, 2>(a, stream) : launch_simt<T, 64, 64, 32, 4, 2>(a, stream);
-}
-
-static bool use_chunk(const PagedArgs& a, int dtype) {
-  return dtype != SPRUCE_DTYPE_F32 && a.num_pages > 0 && (int64_t)a.max_q * (a.Hq / a.Hkv) > 64;
+  if (a.D == 128) return few ? launch_f32<128, 16, 64, 2, 2>(a, stream) : launch_f32<128, kF32Rows, 32, 4, 2>(a, stream);
+  return few ? launch_f32<64, 16, 64, 2, 2>(a, stream) : launch_f32<64, kF32Rows, 32, 4, 2>(a, stream);
 }
 
 int64_t paged_workspace_bytes(int64_t Hq, int64_t Hkv, int64_t D, int64_t max_q, int dtype) {
-  return std::max(paged_params_bytes(64, kMaxSms * 2, D), paged_params_bytes(kPagedChunkRows, kMaxSms, D));
+  if (dtype == SPRUCE_DTYPE_F32) return paged_params_bytes(kF32Rows, kMaxSms * kF32PerSm, D);
+  if (max_q * (Hq / Hkv) <= kPagedRowsMax) return paged_params_bytes(kPagedRowsMax, kMaxSms * kPagedRowsPerSm, D);
+  return paged_params_bytes(kPagedChunkRows, kMaxSms, D);
 }
 
 cudaError_t launch_paged_attention(const PagedArgs& a, int dtype, cudaStream_t stream) {
-  if (use_chunk(a, dtype))
-    return launch_paged_chunk(a, dtype, grid_for(a, kPagedChunkRows, kPagedChunkKeys, sm_count()), stream);
-  if (dtype == SPRUCE_DTYPE_F32) return launch_simt_dtype<float>(a, stream);
-  if (dtype == SPRUCE_DTYPE_BF16) return launch_simt_dtype<__nv_bfloat16>(a, stream);
-  return launch_simt_dtype<__half>(a, stream);
+  if (dtype == SPRUCE_DTYPE_F32) return launch_paged_f32(a, stream);
+  const int64_t rows = (int64_t)a.max_q * (a.Hq / a.Hkv);
+  if (rows <= kPagedRowsMax) {
+    const int tiles = rows <= 16 ? 1 : (rows <= 32 ? 2 : 4);
+    return launch_paged_rows(a, dtype, tiles, grid_for(a, 16 * tiles, kPagedRowsKeys, sm_count() * kPagedRowsPerSm),
+                             stream);
+  }
+  return launch_paged_chunk(a, dtype, grid_for(a, kPagedChunkRows, kPagedChunkKeys, sm_count()), stream);
 }
 
 }  // namespace spruce

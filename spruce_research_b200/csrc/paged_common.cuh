@@ -213,6 +213,13 @@ __device__ __forceinline__ int paged_page(const PagedParams& p, const int32_t* t
 constexpr int kPagedChunkRows = 256, kPagedChunkKeys = 128;
 cudaError_t launch_paged_chunk(const PagedArgs& a, int dtype, int G, cudaStream_t stream);
 
+// Warp-MMA attention of at most 64 query rows a unit, in 1, 2 or 4 tiles of 16 (paged_rows_sm100.cu).
+constexpr int kPagedRowsMax = 64, kPagedRowsKeys = 64, kPagedRowsPerSm = 2;
+cudaError_t launch_paged_rows(const PagedArgs& a, int dtype, int tiles, int G, cudaStream_t stream);
+// The cache's tensor maps, and the rows of a box of them, for key tiles of `tile` (paged_chunk_sm100.cu).
+bool paged_cache_maps(const PagedArgs& a, int dtype, int box, CUtensorMap* mk, CUtensorMap* mv);
+int paged_box(int page_size, int tile);
+
 // Joins the parts of split units (paged_attn.cu).
 template <typename T>
 cudaError_t launch_paged_join(const PagedParams& p, int R, int G, cudaStream_t stream);
@@ -223,8 +230,9 @@ inline PagedParams paged_params(const PagedArgs& a, int R, int G, int min_tiles)
   p.a = a;
   p.rep = a.Hq / a.Hkv;
   p.row_tiles = static_cast<int>(((int64_t)a.max_q * p.rep + R - 1) / R);
-  p.kv_cap = static_cast<int>(a.max_kv < (int64_t)a.max_pages * a.page_size ? (int64_t)a.max_kv
-                                                                             : (int64_t)a.max_pages * a.page_size);
+  int64_t cap = (int64_t)a.max_pages * a.page_size;
+  cap = cap < a.max_kv ? cap : a.max_kv;
+  p.kv_cap = static_cast<int>(cap < (1 << 30) ? cap : 1 << 30);  // key indices stay ints with room for a tile more
   p.min_tiles = min_tiles;
   uint8_t* ws = static_cast<uint8_t*>(a.workspace);
   p.desc = reinterpret_cast<int4*>(ws);

@@ -92,13 +92,13 @@ def test_entry_points_refuse_before_device_work():
             _lib.check(rope(**kw))
 
     def attend(D=64, Hq=4, Hkv=2, page=16, N=1, S=1, max_q=1, max_kv=16, cu=16, q=16, kc=s3, ws=256, ws_bytes=1 << 30,
-               scale=0.1):
-        return L.spruce_paged_attention(q, s2, 16, kc, 16, s3, 1, N, Hq, Hkv, D, 4, page, 16, 2, 2, cu, 16, S, max_q,
+               scale=0.1, pages=4):
+        return L.spruce_paged_attention(q, s2, 16, kc, 16, s3, 1, N, Hq, Hkv, D, pages, page, 16, 2, 2, cu, 16, S, max_q,
                                         max_kv, scale, 16, s2, ws, ws_bytes, None, None)
 
     for kw, text in ((dict(D=96), "head_dim 64 or 128"), (dict(Hq=5), "divisible"), (dict(page=24), "page_size"),
                      (dict(page=8), "page_size"), (dict(N=-1), "bad shape"), (dict(max_q=-1), "negative"),
-                     (dict(max_q=1 << 30), "too long"), (dict(scale=-1.0), "scale"), (dict(scale=float("nan")), "scale"),
+                     (dict(max_q=1 << 30), "too long"), (dict(pages=0), "no pages"), (dict(scale=-1.0), "scale"), (dict(scale=float("nan")), "scale"),
                      (dict(scale=float("inf")), "scale"), (dict(cu=None), "NULL"), (dict(q=None), "null"),
                      (dict(q=8), "16-byte aligned"), (dict(kc=_lib.int64s(64, 60, 64)), "16-byte aligned"),
                      (dict(ws=128), "256-byte")):
