@@ -411,7 +411,9 @@ SPRUCE_API int spruce_kv_summary_table(const void *key, const int64_t key_stride
                                        int64_t workspace_bytes, void *stream);
 
 /*
- * The serving operators around the sparse-prefill layer; the reference takes
+ * The serving operators around the sparse-prefill layer, each called once or
+ * twice a layer and token: their arguments come in one struct (every field 8
+ * bytes wide), which a foreign caller packs in one go.  The reference takes
  * post-RoPE Q/K from its model and leaves decode to SDPA
  * (kernels/sparse_prefill.py:63-65), so they have no counterpart there.
  *
@@ -427,13 +429,19 @@ SPRUCE_API int spruce_kv_summary_table(const void *key, const int64_t key_stride
  * SPRUCE_STATUS_BAD_POSITION in *status (optional).  D and rd even, rd <= D <=
  * 256; rows that are not 16-byte aligned take scalar loads.
  */
-SPRUCE_API int spruce_qk_norm_rope(const void *q, const int64_t q_strides[4], const void *k,
-                                   const int64_t k_strides[4], int dtype, int64_t B, int64_t Hq, int64_t Hkv,
-                                   int64_t T, int64_t D, const float *rope, int64_t table_rows, int64_t rd,
-                                   int32_t interleaved, const int64_t *positions, const int64_t pos_strides[2],
-                                   const float *q_weight, const float *k_weight, float eps, void *q_out,
-                                   const int64_t q_out_strides[4], void *k_out, const int64_t k_out_strides[4],
-                                   uint32_t *status, void *stream);
+typedef struct {
+  const void *q, *k;
+  void *q_out, *k_out;
+  const float *rope;
+  const int64_t *positions;
+  const float *q_weight, *k_weight;
+  uint32_t *status;
+  void *stream;
+  int64_t q_strides[4], k_strides[4], q_out_strides[4], k_out_strides[4], pos_strides[2];
+  int64_t dtype, B, Hq, Hkv, T, D, table_rows, rd, interleaved;
+  double eps;
+} spruce_qk_norm_rope_args;
+SPRUCE_API int spruce_qk_norm_rope(const spruce_qk_norm_rope_args *args);
 
 /*
  * Append new keys and values to a paged cache, the norm and rotation of
@@ -450,16 +458,20 @@ SPRUCE_API int spruce_qk_norm_rope(const void *q, const int64_t q_strides[4], co
  * is not written and raises SPRUCE_STATUS_BAD_LENGTH / _BAD_PAGE; tokens past
  * cu_q[S] are left out.
  */
-SPRUCE_API int spruce_paged_append(const void *q, const int64_t q_strides[2], const void *k,
-                                   const int64_t k_strides[2], const void *v, const int64_t v_strides[2], int dtype,
-                                   int64_t N, int64_t Hq, int64_t Hkv, int64_t D, const float *rope,
-                                   int64_t table_rows, int64_t rd, int32_t interleaved, const int64_t *positions,
-                                   const float *q_weight, const float *k_weight, float eps, void *q_out,
-                                   const int64_t q_out_strides[2], void *k_cache, const int64_t kc_strides[3],
-                                   void *v_cache, const int64_t vc_strides[3], int64_t num_pages, int64_t page_size,
-                                   const int32_t *block_table, int64_t table_stride, int64_t max_pages,
-                                   const int32_t *cu_q, const int32_t *kv_lens, int64_t S, uint32_t *status,
-                                   void *stream);
+typedef struct {
+  const void *q, *k, *v;
+  void *q_out, *k_cache, *v_cache;
+  const float *rope;
+  const int64_t *positions;
+  const float *q_weight, *k_weight;
+  const int32_t *block_table, *cu_q, *kv_lens;
+  uint32_t *status;
+  void *stream;
+  int64_t q_strides[2], k_strides[2], v_strides[2], q_out_strides[2], kc_strides[3], vc_strides[3];
+  int64_t dtype, N, S, Hq, Hkv, D, num_pages, page_size, table_stride, max_pages, table_rows, rd, interleaved;
+  double eps;
+} spruce_paged_append_args;
+SPRUCE_API int spruce_paged_append(const spruce_paged_append_args *args);
 
 /*
  * Causal GQA attention of new tokens over a paged cache: sequence s's query i
@@ -478,14 +490,19 @@ SPRUCE_API int spruce_paged_append(const void *q, const int64_t q_strides[2], co
  */
 SPRUCE_API int64_t spruce_paged_attention_workspace_bytes(int64_t Hq, int64_t Hkv, int64_t D, int64_t max_q_len,
                                                           int dtype);
-SPRUCE_API int spruce_paged_attention(const void *q, const int64_t q_strides[2], const void *k_cache,
-                                      const int64_t kc_strides[3], const void *v_cache, const int64_t vc_strides[3],
-                                      int dtype, int64_t N, int64_t Hq, int64_t Hkv, int64_t D, int64_t num_pages,
-                                      int64_t page_size, const int32_t *block_table, int64_t table_stride,
-                                      int64_t max_pages, const int32_t *cu_q, const int32_t *kv_lens, int64_t S,
-                                      int64_t max_q_len, int64_t max_kv_len, float scale, void *out,
-                                      const int64_t out_strides[2], void *workspace, int64_t workspace_bytes,
-                                      uint32_t *status, void *stream);
+typedef struct {
+  const void *q, *k_cache, *v_cache;
+  void *out;
+  const int32_t *block_table, *cu_q, *kv_lens;
+  void *workspace;
+  uint32_t *status;
+  void *stream;
+  int64_t q_strides[2], kc_strides[3], vc_strides[3], out_strides[2];
+  int64_t dtype, N, S, Hq, Hkv, D, num_pages, page_size, table_stride, max_pages, max_q_len, max_kv_len,
+      workspace_bytes;
+  double scale;
+} spruce_paged_attention_args;
+SPRUCE_API int spruce_paged_attention(const spruce_paged_attention_args *args);
 
 #ifdef __cplusplus
 }

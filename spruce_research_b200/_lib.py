@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 
 import torch
 
@@ -76,14 +77,16 @@ SIGNATURES = {
                                           _I64, _I64, _F, _I64, _I64, _P, _P], _INT),
     "spruce_sparse_attention_fwd_scatter": ([_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _INT, _I64, _I64, _I64,
                                              _I64, _I64, _I64, _F, _I64, _I64, _P, ctypes.c_int32, _P, _P], _INT),
-    "spruce_qk_norm_rope": ([_P, _P, _P, _P, _INT, _I64, _I64, _I64, _I64, _I64, _P, _I64, _I64, _INT, _P, _P, _P,
-                             _P, _F, _P, _P, _P, _P, _P, _P], _INT),
-    "spruce_paged_append": ([_P, _P, _P, _P, _P, _P, _INT, _I64, _I64, _I64, _I64, _P, _I64, _I64, _INT, _P, _P, _P,
-                             _F, _P, _P, _P, _P, _P, _P, _I64, _I64, _P, _I64, _I64, _P, _P, _I64, _P, _P], _INT),
+    "spruce_qk_norm_rope": ([_P], _INT),
+    "spruce_paged_append": ([_P], _INT),
     "spruce_paged_attention_workspace_bytes": ([_I64, _I64, _I64, _I64, _INT], _I64),
-    "spruce_paged_attention": ([_P, _P, _P, _P, _P, _P, _INT, _I64, _I64, _I64, _I64, _I64, _I64, _P, _I64, _I64, _P,
-                                _P, _I64, _I64, _I64, _F, _P, _P, _P, _I64, _P, _P], _INT),
+    "spruce_paged_attention": ([_P], _INT),
 }
+
+# The argument structs of the serving operators: 8-byte pointers and integers, a double at the end.
+QK_NORM_ROPE_ARGS = struct.Struct("=37qd")
+PAGED_APPEND_ARGS = struct.Struct("=42qd")
+PAGED_ATTENTION_ARGS = struct.Struct("=33qd")
 
 _lib = None
 
@@ -137,6 +140,11 @@ def int64s(*vals):
 
 def stream_of(t: torch.Tensor) -> int:
     return torch.cuda.current_stream(t.device).cuda_stream
+
+
+def stream_on(device: int) -> int:
+    """Handle of the device's current stream, without the Stream object (1.3 us) around it."""
+    return torch._C._cuda_getCurrentRawStream(device)
 
 
 def require_cuda(*tensors: torch.Tensor, what: str = "the SPRUCE B200 kernels") -> None:

@@ -763,100 +763,99 @@ static int check_rope(int64_t D, const float* rope, int64_t table_rows, int64_t 
   return SPRUCE_OK;
 }
 
-int spruce_qk_norm_rope(const void* q, const int64_t q_strides[4], const void* k, const int64_t k_strides[4],
-                        int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t T, int64_t D, const float* rope,
-                        int64_t table_rows, int64_t rd, int32_t interleaved, const int64_t* positions,
-                        const int64_t pos_strides[2], const float* q_weight, const float* k_weight, float eps,
-                        void* q_out, const int64_t q_out_strides[4], void* k_out, const int64_t k_out_strides[4],
-                        uint32_t* status, void* stream) {
-  if (!valid_dtype(dtype)) return fail(SPRUCE_ERR_INVALID, "unsupported dtype code %d", dtype);
-  if (B < 0 || Hq < 1 || Hkv < 1 || T < 0 || Hq > 65535 || Hkv > 65535) return fail(SPRUCE_ERR_INVALID, "bad shape");
-  if (int rc = check_rope(D, rope, table_rows, rd)) return rc;
-  if (B == 0 || T == 0) return SPRUCE_OK;
-  if (B > INT32_MAX || T > INT32_MAX || B * T > INT64_MAX / (Hq + Hkv) / 32)
+int spruce_qk_norm_rope(const spruce_qk_norm_rope_args* args) {
+  const spruce_qk_norm_rope_args& x = *args;
+  if (x.dtype != (int)x.dtype || !valid_dtype((int)x.dtype))
+    return fail(SPRUCE_ERR_INVALID, "unsupported dtype code %lld", (long long)x.dtype);
+  if (x.B < 0 || x.Hq < 1 || x.Hkv < 1 || x.T < 0 || x.Hq > 65535 || x.Hkv > 65535)
+    return fail(SPRUCE_ERR_INVALID, "bad shape");
+  if (int rc = check_rope(x.D, x.rope, x.table_rows, x.rd)) return rc;
+  if (x.B == 0 || x.T == 0) return SPRUCE_OK;
+  if (x.B > INT32_MAX || x.T > INT32_MAX || x.B * x.T > INT32_MAX)
     return fail(SPRUCE_ERR_UNSUPPORTED, "shape too large");
-  if (q == nullptr || k == nullptr || q_out == nullptr || k_out == nullptr) return fail(SPRUCE_ERR_INVALID, "null pointer");
-  if (q_strides[3] != 1 || k_strides[3] != 1 || q_out_strides[3] != 1 || k_out_strides[3] != 1)
+  if (x.q == nullptr || x.k == nullptr || x.q_out == nullptr || x.k_out == nullptr)
+    return fail(SPRUCE_ERR_INVALID, "null pointer");
+  if (x.q_strides[3] != 1 || x.k_strides[3] != 1 || x.q_out_strides[3] != 1 || x.k_out_strides[3] != 1)
     return fail(SPRUCE_ERR_UNSUPPORTED, "q, k and their outputs need a unit last stride");
   spruce::RowsArgs a{};
-  a.q = {q, q_strides[0], q_strides[1], q_strides[2], q_out, q_out_strides[0], q_out_strides[1], q_out_strides[2], q_weight};
-  a.k = {k, k_strides[0], k_strides[1], k_strides[2], k_out, k_out_strides[0], k_out_strides[1], k_out_strides[2], k_weight};
-  a.B = (int)B;
-  a.T = (int)T;
-  a.Hq = (int)Hq;
-  a.Hkv = (int)Hkv;
-  a.D = (int)D;
-  a.rd = (int)rd;
-  a.interleaved = interleaved != 0;
-  a.eps = eps;
-  a.rope = rope;
-  a.table_rows = table_rows;
-  a.positions = positions;
-  if (positions != nullptr) {
-    a.pos_sb = pos_strides[0];
-    a.pos_st = pos_strides[1];
-  }
-  a.status = status;
-  return cuda_status(spruce::launch_norm_rope(a, dtype, as_stream(stream)), "norm and rotation launch");
+  a.q = {x.q, x.q_strides[0], x.q_strides[1], x.q_strides[2],
+         x.q_out, x.q_out_strides[0], x.q_out_strides[1], x.q_out_strides[2], x.q_weight};
+  a.k = {x.k, x.k_strides[0], x.k_strides[1], x.k_strides[2],
+         x.k_out, x.k_out_strides[0], x.k_out_strides[1], x.k_out_strides[2], x.k_weight};
+  a.B = (int)x.B;
+  a.T = (int)x.T;
+  a.Hq = (int)x.Hq;
+  a.Hkv = (int)x.Hkv;
+  a.D = (int)x.D;
+  a.rd = (int)x.rd;
+  a.interleaved = x.interleaved != 0;
+  a.eps = (float)x.eps;
+  a.rope = x.rope;
+  a.table_rows = x.table_rows;
+  a.positions = x.positions;
+  a.pos_sb = x.pos_strides[0];
+  a.pos_st = x.pos_strides[1];
+  a.status = x.status;
+  return cuda_status(spruce::launch_norm_rope(a, (int)x.dtype, as_stream(x.stream)), "norm and rotation launch");
 }
 
 // The paged cache's shape and metadata, shared by the append and the attention.
-static int check_paged(int dtype, int64_t N, int64_t Hq, int64_t Hkv, int64_t num_pages, int64_t page_size,
-                       const int32_t* block_table, int64_t max_pages, const int32_t* cu_q, const int32_t* kv_lens,
-                       int64_t S) {
-  if (!valid_dtype(dtype)) return fail(SPRUCE_ERR_INVALID, "unsupported dtype code %d", dtype);
-  if (N < 0 || S < 0 || Hkv < 1 || Hq < 0 || Hq > 65535 || Hkv > 65535 || num_pages < 0 || max_pages < 0)
+extern "C++" {
+template <typename Args>
+static int check_paged(const Args& x) {
+  if (x.dtype != (int)x.dtype || !valid_dtype((int)x.dtype))
+    return fail(SPRUCE_ERR_INVALID, "unsupported dtype code %lld", (long long)x.dtype);
+  if (x.N < 0 || x.S < 0 || x.Hkv < 1 || x.Hq < 0 || x.Hq > 65535 || x.Hkv > 65535 || x.num_pages < 0 || x.max_pages < 0)
     return fail(SPRUCE_ERR_INVALID, "bad shape");
-  if (page_size < 16 || page_size % 16)
-    return fail(SPRUCE_ERR_UNSUPPORTED, "page_size must be a multiple of 16, got %lld", (long long)page_size);
-  if (N >= INT32_MAX || S >= INT32_MAX || max_pages > INT32_MAX || page_size > INT32_MAX || num_pages > INT32_MAX)
+  if (x.page_size < 16 || x.page_size % 16)
+    return fail(SPRUCE_ERR_UNSUPPORTED, "page_size must be a multiple of 16, got %lld", (long long)x.page_size);
+  if (x.N >= INT32_MAX || x.S >= INT32_MAX || x.max_pages > INT32_MAX || x.page_size > INT32_MAX ||
+      x.num_pages > INT32_MAX)
     return fail(SPRUCE_ERR_UNSUPPORTED, "shape too large");
-  if (N > 0 && S > 0 && (cu_q == nullptr || kv_lens == nullptr || (block_table == nullptr && max_pages > 0)))
+  if (x.N > 0 && x.S > 0 &&
+      (x.cu_q == nullptr || x.kv_lens == nullptr || (x.block_table == nullptr && x.max_pages > 0)))
     return fail(SPRUCE_ERR_INVALID, "cu_q, kv_lens or block_table is NULL");
   return SPRUCE_OK;
 }
+}
 
-int spruce_paged_append(const void* q, const int64_t q_strides[2], const void* k, const int64_t k_strides[2],
-                        const void* v, const int64_t v_strides[2], int dtype, int64_t N, int64_t Hq, int64_t Hkv,
-                        int64_t D, const float* rope, int64_t table_rows, int64_t rd, int32_t interleaved,
-                        const int64_t* positions, const float* q_weight, const float* k_weight, float eps, void* q_out,
-                        const int64_t q_out_strides[2], void* k_cache, const int64_t kc_strides[3], void* v_cache,
-                        const int64_t vc_strides[3], int64_t num_pages, int64_t page_size, const int32_t* block_table,
-                        int64_t table_stride, int64_t max_pages, const int32_t* cu_q, const int32_t* kv_lens,
-                        int64_t S, uint32_t* status, void* stream) {
-  if (int rc = check_paged(dtype, N, Hq, Hkv, num_pages, page_size, block_table, max_pages, cu_q, kv_lens, S)) return rc;
-  if (int rc = check_rope(D, rope, table_rows, rd)) return rc;
-  if (N == 0 || S == 0) return SPRUCE_OK;
-  if (k == nullptr || v == nullptr || k_cache == nullptr || v_cache == nullptr || (q != nullptr && q_out == nullptr))
+int spruce_paged_append(const spruce_paged_append_args* args) {
+  const spruce_paged_append_args& x = *args;
+  if (int rc = check_paged(x)) return rc;
+  if (int rc = check_rope(x.D, x.rope, x.table_rows, x.rd)) return rc;
+  if (x.N == 0 || x.S == 0) return SPRUCE_OK;
+  if (x.k == nullptr || x.v == nullptr || x.k_cache == nullptr || x.v_cache == nullptr ||
+      (x.q != nullptr && x.q_out == nullptr))
     return fail(SPRUCE_ERR_INVALID, "null pointer");
   spruce::RowsArgs a{};
-  if (q != nullptr) {
-    a.q = {q, 0, q_strides[1], q_strides[0], q_out, 0, q_out_strides[1], q_out_strides[0], q_weight};
-    a.Hq = (int)Hq;
+  if (x.q != nullptr) {
+    a.q = {x.q, 0, x.q_strides[1], x.q_strides[0], x.q_out, 0, x.q_out_strides[1], x.q_out_strides[0], x.q_weight};
+    a.Hq = (int)x.Hq;
   }
-  a.k = {k, 0, k_strides[1], k_strides[0], k_cache, kc_strides[0], kc_strides[1], kc_strides[2], k_weight};
-  a.v = {v, 0, v_strides[1], v_strides[0], v_cache, vc_strides[0], vc_strides[1], vc_strides[2], nullptr};
+  a.k = {x.k, 0, x.k_strides[1], x.k_strides[0],
+         x.k_cache, x.kc_strides[0], x.kc_strides[1], x.kc_strides[2], x.k_weight};
+  a.v = {x.v, 0, x.v_strides[1], x.v_strides[0], x.v_cache, x.vc_strides[0], x.vc_strides[1], x.vc_strides[2], nullptr};
   a.B = 1;
-  a.T = (int)N;
-  a.Hkv = (int)Hkv;
-  a.D = (int)D;
-  a.rd = (int)rd;
-  a.interleaved = interleaved != 0;
-  a.eps = eps;
-  a.rope = rope;
-  a.table_rows = table_rows;
-  a.positions = positions;
+  a.T = (int)x.N;
+  a.Hkv = (int)x.Hkv;
+  a.D = (int)x.D;
+  a.rd = (int)x.rd;
+  a.interleaved = x.interleaved != 0;
+  a.eps = (float)x.eps;
+  a.rope = x.rope;
+  a.table_rows = x.table_rows;
+  a.positions = x.positions;
   a.pos_st = 1;
-  a.cu_q = cu_q;
-  a.kv_lens = kv_lens;
-  a.block_table = block_table;
-  a.table_stride = table_stride;
-  a.S = (int)S;
-  a.max_pages = (int)max_pages;
-  a.page_size = (int)page_size;
-  a.num_pages = num_pages;
-  a.status = status;
-  return cuda_status(spruce::launch_norm_rope(a, dtype, as_stream(stream)), "paged append launch");
+  a.cu_q = x.cu_q;
+  a.kv_lens = x.kv_lens;
+  a.block_table = x.block_table;
+  a.table_stride = x.table_stride;
+  a.S = (int)x.S;
+  a.max_pages = (int)x.max_pages;
+  a.page_size = (int)x.page_size;
+  a.num_pages = x.num_pages;
+  a.status = x.status;
+  return cuda_status(spruce::launch_norm_rope(a, (int)x.dtype, as_stream(x.stream)), "paged append launch");
 }
 
 int64_t spruce_paged_attention_workspace_bytes(int64_t Hq, int64_t Hkv, int64_t D, int64_t max_q_len, int dtype) {
@@ -866,66 +865,67 @@ int64_t spruce_paged_attention_workspace_bytes(int64_t Hq, int64_t Hkv, int64_t 
   return spruce::paged_workspace_bytes(Hq, Hkv, D, max_q_len, dtype);
 }
 
-int spruce_paged_attention(const void* q, const int64_t q_strides[2], const void* k_cache,
-                           const int64_t kc_strides[3], const void* v_cache, const int64_t vc_strides[3], int dtype,
-                           int64_t N, int64_t Hq, int64_t Hkv, int64_t D, int64_t num_pages, int64_t page_size,
-                           const int32_t* block_table, int64_t table_stride, int64_t max_pages, const int32_t* cu_q,
-                           const int32_t* kv_lens, int64_t S, int64_t max_q_len, int64_t max_kv_len, float scale,
-                           void* out, const int64_t out_strides[2], void* workspace, int64_t workspace_bytes,
-                           uint32_t* status, void* stream) {
-  if (int rc = check_paged(dtype, N, Hq, Hkv, num_pages, page_size, block_table, max_pages, cu_q, kv_lens, S)) return rc;
-  if (Hq < 1 || Hq % Hkv)
-    return fail(SPRUCE_ERR_INVALID, "query heads (%lld) must be divisible by KV heads (%lld)", (long long)Hq, (long long)Hkv);
-  if (D != 64 && D != 128) return fail(SPRUCE_ERR_UNSUPPORTED, "paged attention needs head_dim 64 or 128, got %lld", (long long)D);
-  if (max_q_len < 0 || max_kv_len < 0) return fail(SPRUCE_ERR_INVALID, "max_q_len and max_kv_len must not be negative");
-  if (max_q_len > INT32_MAX / Hq || max_kv_len > INT32_MAX) return fail(SPRUCE_ERR_UNSUPPORTED, "sequence too long");
-  if (!(scale >= 0.0f && scale <= 3.0e38f)) return fail(SPRUCE_ERR_INVALID, "scale must be finite and not negative, got %g", scale);
-  if (N == 0 || S == 0 || max_q_len == 0) return SPRUCE_OK;
-  if (num_pages < 1) return fail(SPRUCE_ERR_INVALID, "the cache has no pages");
-  if (q == nullptr || out == nullptr || k_cache == nullptr || v_cache == nullptr)
+int spruce_paged_attention(const spruce_paged_attention_args* args) {
+  const spruce_paged_attention_args& x = *args;
+  if (int rc = check_paged(x)) return rc;
+  if (x.Hq < 1 || x.Hq % x.Hkv)
+    return fail(SPRUCE_ERR_INVALID, "query heads (%lld) must be divisible by KV heads (%lld)", (long long)x.Hq,
+                (long long)x.Hkv);
+  if (x.D != 64 && x.D != 128)
+    return fail(SPRUCE_ERR_UNSUPPORTED, "paged attention needs head_dim 64 or 128, got %lld", (long long)x.D);
+  if (x.max_q_len < 0 || x.max_kv_len < 0)
+    return fail(SPRUCE_ERR_INVALID, "max_q_len and max_kv_len must not be negative");
+  if (x.max_q_len > INT32_MAX / x.Hq || x.max_kv_len > INT32_MAX)
+    return fail(SPRUCE_ERR_UNSUPPORTED, "sequence too long");
+  const float scale = (float)x.scale;
+  if (!(scale >= 0.0f && scale <= 3.0e38f))
+    return fail(SPRUCE_ERR_INVALID, "scale must be finite and not negative, got %g", x.scale);
+  if (x.N == 0 || x.S == 0 || x.max_q_len == 0) return SPRUCE_OK;
+  if (x.num_pages < 1) return fail(SPRUCE_ERR_INVALID, "the cache has no pages");
+  if (x.q == nullptr || x.out == nullptr || x.k_cache == nullptr || x.v_cache == nullptr)
     return fail(SPRUCE_ERR_INVALID, "null pointer");
-  const int64_t vn = 16 / elem_size(dtype);
-  bool ok = aligned16(q) && aligned16(out) && aligned16(k_cache) && aligned16(v_cache);
-  for (int i = 0; i < 2; ++i) ok = ok && q_strides[i] % vn == 0 && out_strides[i] % vn == 0;
-  for (int i = 0; i < 3; ++i) ok = ok && kc_strides[i] % vn == 0 && vc_strides[i] % vn == 0;
+  const int64_t vn = 16 / elem_size((int)x.dtype);
+  bool ok = aligned16(x.q) && aligned16(x.out) && aligned16(x.k_cache) && aligned16(x.v_cache);
+  for (int i = 0; i < 2; ++i) ok = ok && x.q_strides[i] % vn == 0 && x.out_strides[i] % vn == 0;
+  for (int i = 0; i < 3; ++i) ok = ok && x.kc_strides[i] % vn == 0 && x.vc_strides[i] % vn == 0;
   if (!ok) return fail(SPRUCE_ERR_UNSUPPORTED, "q, out and the cache need 16-byte aligned rows");
-  const int64_t need = spruce_paged_attention_workspace_bytes(Hq, Hkv, D, max_q_len, dtype);
-  if (workspace == nullptr || workspace_bytes < need)
+  const int64_t need = spruce::paged_workspace_bytes(x.Hq, x.Hkv, x.D, x.max_q_len, (int)x.dtype);
+  if (x.workspace == nullptr || x.workspace_bytes < need)
     return fail(SPRUCE_ERR_WORKSPACE, "paged attention workspace needs %lld bytes, got %lld", (long long)need,
-                (long long)workspace_bytes);
-  if (reinterpret_cast<uintptr_t>(workspace) & 255u) return fail(SPRUCE_ERR_UNSUPPORTED, "workspace must be 256-byte aligned");
+                (long long)x.workspace_bytes);
+  if (reinterpret_cast<uintptr_t>(x.workspace) & 255u)
+    return fail(SPRUCE_ERR_UNSUPPORTED, "workspace must be 256-byte aligned");
   spruce::PagedArgs a{};
-  a.q = q;
-  a.qn = q_strides[0];
-  a.qh = q_strides[1];
-  a.kc = k_cache;
-  a.vc = v_cache;
+  a.q = x.q;
+  a.qn = x.q_strides[0];
+  a.qh = x.q_strides[1];
+  a.kc = x.k_cache;
+  a.vc = x.v_cache;
   for (int i = 0; i < 3; ++i) {
-    a.ks[i] = kc_strides[i];
-    a.vs[i] = vc_strides[i];
+    a.ks[i] = x.kc_strides[i];
+    a.vs[i] = x.vc_strides[i];
   }
-  a.block_table = block_table;
-  a.table_stride = table_stride;
-  a.cu_q = cu_q;
-  a.kv_lens = kv_lens;
-  a.out = out;
-  a.on = out_strides[0];
-  a.oh = out_strides[1];
-  a.S = (int)S;
-  a.N = (int)N;
-  a.Hq = (int)Hq;
-  a.Hkv = (int)Hkv;
-  a.D = (int)D;
-  a.page_size = (int)page_size;
-  a.max_pages = (int)max_pages;
-  a.max_q = (int)max_q_len;
-  a.max_kv = (int)max_kv_len;
-  a.num_pages = num_pages;
+  a.block_table = x.block_table;
+  a.table_stride = x.table_stride;
+  a.cu_q = x.cu_q;
+  a.kv_lens = x.kv_lens;
+  a.out = x.out;
+  a.on = x.out_strides[0];
+  a.oh = x.out_strides[1];
+  a.S = (int)x.S;
+  a.N = (int)x.N;
+  a.Hq = (int)x.Hq;
+  a.Hkv = (int)x.Hkv;
+  a.D = (int)x.D;
+  a.page_size = (int)x.page_size;
+  a.max_pages = (int)x.max_pages;
+  a.max_q = (int)x.max_q_len;
+  a.max_kv = (int)x.max_kv_len;
+  a.num_pages = x.num_pages;
   a.scale = scale;
-  a.workspace = workspace;
-  a.workspace_bytes = workspace_bytes;
-  a.status = status;
-  return cuda_status(spruce::launch_paged_attention(a, dtype, as_stream(stream)), "paged attention launch");
+  a.workspace = x.workspace;
+  a.status = x.status;
+  return cuda_status(spruce::launch_paged_attention(a, (int)x.dtype, as_stream(x.stream)), "paged attention launch");
 }
 
 }  // extern "C"

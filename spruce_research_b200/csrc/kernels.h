@@ -185,7 +185,6 @@ struct PagedArgs {
   int64_t num_pages;
   float scale;
   void* workspace;
-  int64_t workspace_bytes;
   uint32_t* status;
 };
 int64_t paged_workspace_bytes(int64_t Hq, int64_t Hkv, int64_t D, int64_t max_q, int dtype);

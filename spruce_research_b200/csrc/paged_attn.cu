@@ -10,9 +10,21 @@
 #include <algorithm>
 #include <climits>
 
+#include "attn_common.cuh"
 #include "paged_common.cuh"
 
 namespace spruce {
+
+static int sm_count() {
+  static int n = 0;
+  if (n == 0) {
+    int dev = 0, v = 0;
+    if (cudaGetDevice(&dev) == cudaSuccess &&
+        cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess && v > 0)
+      n = std::min(v, kMaxSms);
+  }
+  return n > 0 ? n : 148;
+}
 
 template <int D, int R, int TK, int TR, int TC>
 __global__ void __launch_bounds__(256) paged_attn_f32_kernel(const PagedParams p) {
@@ -160,78 +172,175 @@ __global__ void __launch_bounds__(256) paged_attn_f32_kernel(const PagedParams p
         for (int d = 0; d < DV; ++d) p.part_o[at * D + cg * DV + d] = o[i][d];
       }
     }
-    if (x.parts > 0) mine = make_int4(x.s, x.qt, x.g, x.parts | x.slot << 30);
+    if (x.parts > 0) mine = paged_desc(x, rows);
   }
   if (tid == 0) p.desc[blockIdx.x] = mine;
 }
 
-// One warp a row of a split unit: the parts' rows weighted by 2^(m_i - max), in the order of the keys.
+// Joins the parts of split units: a row is the parts' rows weighted by 2^(m_i - max), taken in the order of the keys.
+//
+// Every CTA reads the (at most 2 G) descriptions and deals the split units out as jobs: eight rows, a warp each,
+// where a unit has few parts, else one row whose parts the eight warps share.  The launch is programmatic: its
+// CTAs start while the attention's last ones run, and wait before they read.
+constexpr int kJoinThreads = 256, kJoinWarps = kJoinThreads / 32, kJoinPerSm = 4;
+
 template <typename T>
-__global__ void __launch_bounds__(128) paged_join_kernel(const PagedParams p, int R) {
-  const int4 d = p.desc[blockIdx.x];
-  const int parts = d.w & 0x3fffffff;
-  const int r = blockIdx.y * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  if (parts == 0) return;
-  PagedPiece x;
-  x.q = paged_seq(p, d.x);
-  x.s = d.x;
-  x.g = d.z;
-  if (r >= min(R, x.q.qlen * p.rep - d.y * R)) return;
-  const int D = p.a.D;
-  auto at = [&](int i) { return (int64_t)(2 * (blockIdx.x + i) + (i == 0 ? (d.w >> 30) & 1 : 0)) * R + r; };
-  float top = -INFINITY;
-  for (int i = lane; i < parts; i += 32) top = fmaxf(top, p.part_ml[at(i)].x);
+__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PagedParams p, int R, int G) {
+  static_assert(kPagedMaxRuns <= 2 * kJoinThreads, "two descriptions a thread");
+  __shared__ int4 desc[kPagedMaxRuns];
+  __shared__ int first[kPagedMaxRuns + 1];  // jobs before each unit
+  __shared__ int sums[kJoinWarps], job_s;
+  __shared__ float l_s[kJoinWarps], o_s[kJoinWarps][128];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int D = p.a.D, dims = D / 32;  // 2 or 4 adjacent dims a lane
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+
+  // Jobs of each unit, summed.
+  int n[2] = {0, 0};
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  const float ref = top == -INFINITY ? 0.0f : top;
-  float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f}, l = 0.0f;
-  const int dims = D / 32;  // 2 or 4 adjacent dims a lane
-  for (int i = 0; i < parts; ++i) {
-    const float2 ml = p.part_ml[at(i)];
-    const float w = exp2f(ml.x - ref);
-    l = fmaf(ml.y, w, l);
-    const float* o = p.part_o + at(i) * D + lane * dims;
-    if (dims == 4) {
-      const float4 v = *reinterpret_cast<const float4*>(o);
-      acc[0] = fmaf(v.x, w, acc[0]);
-      acc[1] = fmaf(v.y, w, acc[1]);
-      acc[2] = fmaf(v.z, w, acc[2]);
-      acc[3] = fmaf(v.w, w, acc[3]);
-    } else {
-      const float2 v = *reinterpret_cast<const float2*>(o);
-      acc[0] = fmaf(v.x, w, acc[0]);
-      acc[1] = fmaf(v.y, w, acc[1]);
+  for (int u = 0; u < 2; ++u)
+    if (2 * tid + u < G) {
+      const int4 d = p.desc[2 * tid + u];
+      desc[2 * tid + u] = d;
+      const int parts = paged_desc_parts(d.w), rows = paged_desc_rows(d.w);
+      n[u] = parts == 0 ? 0 : (parts <= kJoinWarps ? (rows + kJoinWarps - 1) / kJoinWarps : rows);
     }
+  int inc = n[0] + n[1];
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= o) inc += y;
   }
-  int64_t tok;
-  int head;
-  paged_row(p, x, d.y * R + r, tok, head);
-  T* dst = static_cast<T*>(p.a.out) + tok * p.a.on + head * p.a.oh + lane * dims;
-  const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-  for (int i = 0; i < dims; ++i) dst[i] = Elem<T>::from_f(acc[i] * inv);
+  if (lane == 31) sums[warp] = inc;
+  __syncthreads();
+  int jobs = 0, before = inc - n[0] - n[1];
+#pragma unroll
+  for (int w = 0; w < kJoinWarps; ++w) {
+    before += w < warp ? sums[w] : 0;
+    jobs += sums[w];
+  }
+  if (2 * tid < G) first[2 * tid] = before;
+  if (2 * tid + 1 < G) first[2 * tid + 1] = before + n[0];
+  if (tid == 0) first[G] = jobs;
+  __syncthreads();
+
+  for (int job = blockIdx.x; job < jobs; job += gridDim.x) {
+    for (int c = tid; c < G; c += kJoinThreads)
+      if (first[c] <= job && job < first[c + 1]) job_s = c;
+    __syncthreads();
+    const int c = job_s;
+    const int4 d = desc[c];
+    const int parts = paged_desc_parts(d.w), rows = paged_desc_rows(d.w);
+    const bool few = parts <= kJoinWarps;
+    const int r = few ? (job - first[c]) * kJoinWarps + warp : job - first[c];
+    const int step = few ? 1 : kJoinWarps, start = few ? 0 : warp;
+    float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f}, l = 0.0f;
+    if (r < rows) {
+      // Part i > 0 begins its run (slot 0); part 0 has the described slot.
+      auto at = [&](int i) { return (int64_t)(2 * (c + i) + (i == 0 ? paged_desc_slot(d.w) : 0)) * R + r; };
+      constexpr int U = 4;  // parts whose loads are in flight together
+      float2 ml[U];
+      float v[U][4];
+      auto load = [&](int i0) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int i = i0 + u * step;
+          const bool in = i < parts;
+          const int64_t row = at(in ? i : 0);
+          ml[u] = in ? p.part_ml[row] : make_float2(-INFINITY, 0.0f);
+          const float* o = p.part_o + row * D + lane * dims;
+          v[u][2] = v[u][3] = 0.0f;
+          if (dims == 4) {
+            const float4 y = *reinterpret_cast<const float4*>(o);
+            v[u][0] = y.x;
+            v[u][1] = y.y;
+            v[u][2] = y.z;
+            v[u][3] = y.w;
+          } else {
+            const float2 y = *reinterpret_cast<const float2*>(o);
+            v[u][0] = y.x;
+            v[u][1] = y.y;
+          }
+        }
+      };
+      load(start);
+      float top = -INFINITY;
+      for (int i = lane; i < parts; i += 32) top = fmaxf(top, p.part_ml[at(i)].x);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      const float ref = top == -INFINITY ? 0.0f : top;
+      for (int i0 = start; i0 < parts; i0 += U * step) {
+        if (i0 > start) load(i0);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          if (i0 + u * step >= parts) break;  // a repeated first part is not added
+          const float w = exp2f(ml[u].x - ref);
+          l = fmaf(ml[u].y, w, l);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) acc[k] = fmaf(v[u][k], w, acc[k]);
+        }
+      }
+    }
+    if (!few) {  // the warps' sums share one maximum: add them in order
+      if (lane == 0) l_s[warp] = l;
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (k < dims) o_s[warp][lane * dims + k] = acc[k];
+      __syncthreads();
+      if (warp == 0) {
+        l = 0.0f;
+        acc[0] = acc[1] = acc[2] = acc[3] = 0.0f;
+        for (int w = 0; w < kJoinWarps; ++w) {
+          l += l_s[w];
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (k < dims) acc[k] += o_s[w][lane * dims + k];
+        }
+      }
+    }
+    if (r < rows && (few || warp == 0)) {
+      PagedPiece x;
+      x.q.q0 = d.x;
+      x.g = d.z;
+      int64_t tok;
+      int head;
+      paged_row(p, x, d.y * R + r, tok, head);
+      T* dst = static_cast<T*>(p.a.out) + tok * p.a.on + head * p.a.oh + lane * dims;
+      const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+      if constexpr (sizeof(T) == 4) {
+        if (dims == 4)
+          *reinterpret_cast<float4*>(dst) = make_float4(acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv);
+        else
+          *reinterpret_cast<float2*>(dst) = make_float2(acc[0] * inv, acc[1] * inv);
+      } else {
+        const uint32_t lo = Pack2<T>::pack(acc[0] * inv, acc[1] * inv);
+        if (dims == 4)
+          *reinterpret_cast<uint2*>(dst) = make_uint2(lo, Pack2<T>::pack(acc[2] * inv, acc[3] * inv));
+        else
+          *reinterpret_cast<uint32_t*>(dst) = lo;
+      }
+    }
+    __syncthreads();
+  }
 }
 
 template <typename T>
-cudaError_t launch_paged_join(const PagedParams& p, int R, int G, cudaStream_t stream) {
-  paged_join_kernel<T><<<dim3(G, (R + 3) / 4), 128, 0, stream>>>(p, R);
-  return cudaGetLastError();
+cudaError_t launch_paged_join(const PagedParams& p, int R, int G, int TK, cudaStream_t stream) {
+  if (p.a.max_kv <= TK) return cudaSuccess;  // one key tile a unit: none is split
+  cudaLaunchConfig_t cfg{};
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = dim3(kJoinPerSm * sm_count());
+  cfg.blockDim = dim3(kJoinThreads);
+  cfg.stream = stream;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, paged_join_kernel<T>, p, R, G);
 }
-template cudaError_t launch_paged_join<float>(const PagedParams&, int, int, cudaStream_t);
-template cudaError_t launch_paged_join<__nv_bfloat16>(const PagedParams&, int, int, cudaStream_t);
-template cudaError_t launch_paged_join<__half>(const PagedParams&, int, int, cudaStream_t);
-
-constexpr int kMaxSms = 160;
-
-static int sm_count() {
-  static int n = 0;
-  if (n == 0) {
-    int dev = 0, v = 0;
-    if (cudaGetDevice(&dev) == cudaSuccess &&
-        cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess && v > 0)
-      n = std::min(v, kMaxSms);
-  }
-  return n > 0 ? n : 148;
-}
+template cudaError_t launch_paged_join<float>(const PagedParams&, int, int, int, cudaStream_t);
+template cudaError_t launch_paged_join<__nv_bfloat16>(const PagedParams&, int, int, int, cudaStream_t);
+template cudaError_t launch_paged_join<__half>(const PagedParams&, int, int, int, cudaStream_t);
 
 // CTAs worth launching: all resident ones, or fewer where the tiles cannot be more.
 static int grid_for(const PagedArgs& a, int R, int TK, int resident) {
@@ -247,13 +356,14 @@ template <int D, int R, int TK, int TR, int TC>
 static cudaError_t launch_f32(const PagedArgs& a, cudaStream_t stream) {
   const size_t smem = sizeof(float) * (R * D + TK * (D + 4) + TK * D + R * (TK + 1));
   auto kern = paged_attn_f32_kernel<D, R, TK, TR, TC>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  static std::atomic<uint64_t> done{0};
+  cudaError_t e = allow_smem(reinterpret_cast<const void*>(kern), (int)smem, done);
   if (e != cudaSuccess) return e;
   const int G = grid_for(a, R, TK, sm_count() * kF32PerSm);
   const PagedParams p = paged_params(a, R, G, 1);
   kern<<<G, 256, smem, stream>>>(p);
   e = cudaGetLastError();
-  return e != cudaSuccess ? e : launch_paged_join<float>(p, R, G, stream);
+  return e != cudaSuccess ? e : launch_paged_join<float>(p, R, G, TK, stream);
 }
 
 static cudaError_t launch_paged_f32(const PagedArgs& a, cudaStream_t stream) {

@@ -107,6 +107,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     tmem_relinquish();
   }
   tc_fence_before();
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the join may take its place; it waits for our end
   Walk walk;
   const bool any = paged_run<kChunkRows, kChunkKeys, kChunkThreads>(p, walk, scan);
   __syncthreads();
@@ -270,7 +271,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     uint32_t sj = 0, pieces = 0;  // tiles and pieces of this M-tile so far
     bool ok = true;
     while (ok && walk.next(p, x)) {
-      if (x.parts > 0) mine = make_int4(x.s, x.qt, x.g, x.parts | x.slot << 30);
+      if (x.parts > 0) mine = paged_desc(x, min(kChunkRows, x.q.qlen * p.rep - x.qt * kChunkRows));
       const int rows = min(128, x.q.qlen * p.rep - x.qt * kChunkRows - t * 128);
       if (rows <= 0) continue;
       const int r0 = x.qt * kChunkRows + t * 128;  // the tile's first row in the sequence
@@ -490,12 +491,13 @@ static cudaError_t launch_chunk(const PagedArgs& a, int dtype, int G, cudaStream
   const int box = paged_box(a.page_size, kChunkKeys);
   if (!paged_cache_maps(a, dtype, box, &mk, &mv)) return cudaErrorInvalidValue;
   auto kern = paged_chunk_sm100_kernel<T, D>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::BYTES);
+  static std::atomic<uint64_t> done{0};
+  cudaError_t e = allow_smem(reinterpret_cast<const void*>(kern), L::BYTES, done);
   if (e != cudaSuccess) return e;
   const PagedParams p = paged_params(a, kChunkRows, G, 1);
   kern<<<G, kChunkThreads, L::BYTES, stream>>>(mk, mv, p, box);
   e = cudaGetLastError();
-  return e != cudaSuccess ? e : launch_paged_join<T>(p, kChunkRows, G, stream);
+  return e != cudaSuccess ? e : launch_paged_join<T>(p, kChunkRows, G, kChunkKeys, stream);
 }
 
 cudaError_t launch_paged_chunk(const PagedArgs& a, int dtype, int G, cudaStream_t stream) {

@@ -12,6 +12,8 @@
 // kernel joins the parts in the order of the keys, so results do not depend on timing.
 #pragma once
 
+#include <atomic>
+
 #include "common.cuh"
 #include "kernels.h"
 
@@ -22,7 +24,7 @@ struct PagedParams {
   int rep, row_tiles;     // Hq / Hkv; row tiles of the longest sequence allowed
   int kv_cap;             // keys a sequence may hold: min(max_kv, max_pages * page_size)
   int min_tiles;          // shortest run
-  int4* desc;             // [G] split unit whose first part is the run's last: {s, qt, g, parts | slot << 30}
+  int4* desc;             // [G] split unit whose first part is the run's last: {first token, qt, g, parts | slot << 12 | rows << 16}
   float2* part_ml;        // [2 G][R] softmax maximum (log2 units) and sum
   float* part_o;          // [2 G][R][D]
   float scale_log2;
@@ -64,6 +66,15 @@ struct PagedPiece {
   int slot;         // of the partial result; -1: the whole unit
   int parts;        // > 0: the first part of a unit that this many runs share
 };
+
+constexpr int kMaxSms = 160, kPagedMaxRuns = 2 * kMaxSms;
+static_assert(kPagedMaxRuns < 1 << 12, "parts of a unit fit their field");
+__device__ __forceinline__ int4 paged_desc(const PagedPiece& x, int rows) {
+  return make_int4(x.q.q0, x.qt, x.g, x.parts | x.slot << 12 | rows << 16);
+}
+__device__ __forceinline__ int paged_desc_parts(int w) { return w & 0xfff; }
+__device__ __forceinline__ int paged_desc_slot(int w) { return (w >> 12) & 1; }
+__device__ __forceinline__ int paged_desc_rows(int w) { return w >> 16; }
 
 // Walks a run's pieces; every thread that calls next() with the same walker sees the same ones.
 template <int R, int TK>
@@ -209,6 +220,19 @@ __device__ __forceinline__ int paged_page(const PagedParams& p, const int32_t* t
   return -1;
 }
 
+// Opts a kernel into `bytes` of dynamic shared memory, once a device (`done` is the kernel's own mask of devices).
+inline cudaError_t allow_smem(const void* kern, int bytes, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess || dev < 0 || dev > 63 || (done.load() >> dev & 1)) {
+    if (e == cudaSuccess && dev > 63) e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    return e;
+  }
+  e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) done.fetch_or(uint64_t(1) << dev);
+  return e;
+}
+
 // Tensor-core attention of chunks (paged_chunk_sm100.cu), on G CTAs.
 constexpr int kPagedChunkRows = 256, kPagedChunkKeys = 128;
 cudaError_t launch_paged_chunk(const PagedArgs& a, int dtype, int G, cudaStream_t stream);
@@ -222,7 +246,7 @@ int paged_box(int page_size, int tile);
 
 // Joins the parts of split units (paged_attn.cu).
 template <typename T>
-cudaError_t launch_paged_join(const PagedParams& p, int R, int G, cudaStream_t stream);
+cudaError_t launch_paged_join(const PagedParams& p, int R, int G, int TK, cudaStream_t stream);
 
 // Parameters of a launch with R-row tiles on at most G CTAs, its workspace carved up.
 inline PagedParams paged_params(const PagedArgs& a, int R, int G, int min_tiles) {

@@ -88,6 +88,7 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
     prefetch_tmap(&tmk);
     prefetch_tmap(&tmv);
   }
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the join may take its place; it waits for our end
   Walk walk;
   const bool any = paged_run<R, kRowsKeys, kRowsThreads>(p, walk, scan);
   __syncthreads();
@@ -149,8 +150,8 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
   int j = 0;
   bool ok = true;
   while (walk.next(p, x)) {  // after a wait that ran out the warps still meet at the joins' barriers
-    if (x.parts > 0) mine = make_int4(x.s, x.qt, x.g, x.parts | x.slot << 30);
     const int rows = min(R, x.q.qlen * p.rep - x.qt * R);
+    if (x.parts > 0) mine = paged_desc(x, rows);
     uint32_t q[D / 16][4];
     int seen[2];  // keys that this thread's two rows see
 #pragma unroll
@@ -335,12 +336,13 @@ static cudaError_t launch_rows(const PagedArgs& a, int dtype, int G, cudaStream_
   const int box = paged_box(a.page_size, kRowsKeys);
   if (!paged_cache_maps(a, dtype, box, &mk, &mv)) return cudaErrorInvalidValue;
   auto kern = paged_rows_sm100_kernel<T, D, MT>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::BYTES);
+  static std::atomic<uint64_t> done{0};
+  cudaError_t e = allow_smem(reinterpret_cast<const void*>(kern), L::BYTES, done);
   if (e != cudaSuccess) return e;
   const PagedParams p = paged_params(a, 16 * MT, G, 1);
   kern<<<G, kRowsThreads, L::BYTES, stream>>>(mk, mv, p, box);
   e = cudaGetLastError();
-  return e != cudaSuccess ? e : launch_paged_join<T>(p, 16 * MT, G, stream);
+  return e != cudaSuccess ? e : launch_paged_join<T>(p, 16 * MT, G, kRowsKeys, stream);
 }
 
 template <typename T, int D>

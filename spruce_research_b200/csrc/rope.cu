@@ -11,262 +11,377 @@
 //
 // Layout: a row is held by LPR lanes (8 at D = 128 in 16 bits), each with two 16-byte vectors that hold whole pairs
 // (half: one vector of each half; interleaved: adjacent vectors), so a rotation needs no exchange and the norm three
-// shuffles.  A lane group takes HC heads of one token: the angles are loaded once for them and 2 HC loads are in flight
-// per lane.  Shapes, strides or bases that 16-byte vectors do not fit take the same kernel with one element a load.
-#include <algorithm>
-
-#include "common.cuh"
-#include "kernels.h"
+// shuffles.  A lane group takes up to four heads of one token: the angles are loaded once for them, and their vectors
+// are brought in by cp.async, 16 KB a CTA and 128 KB an SM in flight, which registers could not hold.
+#include "attn_common.cuh"
 
 namespace spruce {
 
-constexpr int kRowThreads = 256;
+constexpr int kRowThreads = 128;
 constexpr int kHeadsPerGroup = 4;
+constexpr int kRowCtasPerSm = 8;
 
-template <typename T, int VN>
-struct RowVec {
-  T e[VN];
-  __device__ __forceinline__ void load(const T* p) {
-    if constexpr (VN * sizeof(T) == 16)
-      *reinterpret_cast<uint4*>(e) = *reinterpret_cast<const uint4*>(p);  // not __ldg: the output may be the input
-    else
-      for (int i = 0; i < VN; ++i) e[i] = p[i];
+__device__ __forceinline__ uint64_t unpack2(uint32_t v, __nv_bfloat16) {
+  return f2_pack(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
+}
+__device__ __forceinline__ uint64_t unpack2(uint32_t v, __half) {
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&v));
+  return f2_pack(f.x, f.y);
+}
+// A 16-byte vector to and from packed fp32 pairs.
+template <typename T, int NP>
+__device__ __forceinline__ void unpack16(const uint4& v, uint64_t (&x)[NP]) {
+  if constexpr (sizeof(T) == 4) {
+    x[0] = f2_pack(__uint_as_float(v.x), __uint_as_float(v.y));
+    x[1] = f2_pack(__uint_as_float(v.z), __uint_as_float(v.w));
+  } else {
+    x[0] = unpack2(v.x, T());
+    x[1] = unpack2(v.y, T());
+    x[2] = unpack2(v.z, T());
+    x[3] = unpack2(v.w, T());
   }
-  __device__ __forceinline__ void store(T* p) const {
-    if constexpr (VN * sizeof(T) == 16)
-      *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(e);
-    else
-      for (int i = 0; i < VN; ++i) p[i] = e[i];
+}
+template <typename T, int NP>
+__device__ __forceinline__ uint4 pack16(const uint64_t (&x)[NP]) {
+  float f[2 * NP];
+#pragma unroll
+  for (int i = 0; i < NP; ++i) f2_unpack(x[i], f[2 * i], f[2 * i + 1]);
+  if constexpr (sizeof(T) == 4)
+    return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+  else
+    return make_uint4(Pack2<T>::pack(f[0], f[1]), Pack2<T>::pack(f[2], f[3]), Pack2<T>::pack(f[4], f[5]),
+                      Pack2<T>::pack(f[6], f[7]));
+}
+__device__ __forceinline__ void load_pairs(const float* p, uint64_t& a, uint64_t& b) {
+  const float4 v = __ldg(reinterpret_cast<const float4*>(p));
+  a = f2_pack(v.x, v.y);
+  b = f2_pack(v.z, v.w);
+}
+
+__device__ __forceinline__ uint64_t load_pair(const float* p) {
+  const float2 v = __ldg(reinterpret_cast<const float2*>(p));
+  return f2_pack(v.x, v.y);
+}
+
+__device__ __forceinline__ void copy16(uint4* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+// Until at most n of this thread's latest copy groups are under way (n a constant after unrolling).
+__device__ __forceinline__ void wait_copies(int n) {
+  switch (n) {
+    case 0: asm volatile("cp.async.wait_group 0;" ::: "memory"); break;
+    case 1: asm volatile("cp.async.wait_group 1;" ::: "memory"); break;
+    case 2: asm volatile("cp.async.wait_group 2;" ::: "memory"); break;
+    default: asm volatile("cp.async.wait_group 3;" ::: "memory"); break;
   }
+}
+
+// Interleaved pairs: x[e] holds (a, b) of one pair, its angle is number first + e of cs / sn.
+template <int NP>
+__device__ __forceinline__ void turn_pairs(uint64_t (&x)[NP], const uint64_t (&cs)[NP], const uint64_t (&sn)[NP], int first) {
+#pragma unroll
+  for (int e = 0; e < NP; ++e) {
+    const int i = first + e;
+    float c0, c1, s0, s1, u, v;
+    f2_unpack(cs[i / 2], c0, c1);
+    f2_unpack(sn[i / 2], s0, s1);
+    f2_unpack(x[e], u, v);
+    const float c = i & 1 ? c1 : c0, s = i & 1 ? s1 : s0;
+    x[e] = f2_pack(u * c - v * s, v * c + u * s);
+  }
+}
+
+// Where a token's rotation and cache rows are.
+struct TokenPlace {
+  const float* angles;  // its row of the table
+  int64_t page;
+  int slot;
+  bool write, cached;   // the token is one of a sequence's; its cache row exists
 };
 
-// Largest s with cu[s] <= n, for 0 <= n < cu[S] (cu non-decreasing).
-__device__ __forceinline__ int seq_of_token(const int32_t* cu, int S, int n) {
-  if (n < S && cu[n] == n && cu[n + 1] == n + 1) return n;  // single-token sequences
-  int lo = 0, hi = S;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (cu[mid] <= n) lo = mid;
-    else hi = mid;
-  }
-  return lo;
-}
-
-template <typename T, int VN, int ITERS, bool APPEND>
-__global__ void __launch_bounds__(kRowThreads) norm_rope_kernel(const RowsArgs a, int lpr, int chunks) {
-  constexpr int HC = kHeadsPerGroup;
-  alignas(16) RowVec<T, VN> va[HC][ITERS], vb[HC][ITERS];
-  const int l = threadIdx.x & (lpr - 1);
-  const int64_t group = (int64_t)blockIdx.x * (kRowThreads / lpr) + threadIdx.x / lpr;
-  const int64_t tokens = (int64_t)a.B * a.T;
-  const bool live = group < tokens * chunks;
-  const int64_t n = live ? group / chunks : 0;
-  const int h0 = live ? static_cast<int>(group % chunks) * HC : 0;
-  const int heads = a.Hq + (APPEND ? 2 : 1) * a.Hkv;  // query rows, key rows, (value rows)
-  const int64_t b = n / a.T, t = n % a.T;
-  const int items = a.D / (2 * VN);
-
-  // Where the token's rotation and cache rows are.
-  int64_t pos = t, page = 0;
-  int slot = 0;
-  bool write = live, cached = live;
+template <bool APPEND>
+__device__ __forceinline__ TokenPlace place_token(const RowsArgs& a, bool live, int n, int b, int t) {
+  TokenPlace w{nullptr, 0, 0, live, live};
+  int64_t pos = t;
   if constexpr (APPEND) {
-    cached = write = live && n < a.cu_q[a.S];
-    if (write) {
-      const int s = seq_of_token(a.cu_q, a.S, static_cast<int>(n));
-      pos = (int64_t)a.kv_lens[s] - (a.cu_q[s + 1] - n);
-      const int64_t pi = pos >= 0 ? pos / a.page_size : -1;
-      cached = pi >= 0 && pi < a.max_pages;
-      if (!cached) raise_status(a.status, SPRUCE_STATUS_BAD_LENGTH);
-      if (cached) {
-        page = a.block_table[(int64_t)s * a.table_stride + pi];
-        cached = page >= 0 && page < a.num_pages;
-        if (!cached) raise_status(a.status, SPRUCE_STATUS_BAD_PAGE);
-        slot = static_cast<int>(pos - pi * a.page_size);
+    if (live) {
+      // A sequence of one token most often: s == n.  These loads do not wait for one another.
+      const int end = a.cu_q[a.S];
+      int s = min(n, a.S - 1);
+      int first = a.cu_q[s], next = a.cu_q[s + 1], kv = a.kv_lens[s];
+      w.write = n < end;
+      if (w.write && (first > n || next <= n)) {
+        int lo = 0, hi = a.S;  // the largest s with cu_q[s] <= n
+        while (hi - lo > 1) {
+          const int mid = (lo + hi) >> 1;
+          if (a.cu_q[mid] <= n) lo = mid;
+          else hi = mid;
+        }
+        s = lo;
+        next = a.cu_q[s + 1];
+        kv = a.kv_lens[s];
+      }
+      pos = (int64_t)kv - next + n;
+      const int p = pos >= 0 && pos < 0x7fffffff ? static_cast<int>(pos) : -1;
+      const int pi = p >= 0 ? p / a.page_size : a.max_pages;
+      w.cached = w.write && pi < a.max_pages;
+      if (w.write && !w.cached) raise_status(a.status, SPRUCE_STATUS_BAD_LENGTH);
+      if (w.cached) {
+        w.page = a.block_table[(int64_t)s * a.table_stride + pi];
+        w.cached = w.page >= 0 && w.page < a.num_pages;
+        if (!w.cached) raise_status(a.status, SPRUCE_STATUS_BAD_PAGE);
+        w.slot = p - pi * a.page_size;
       }
     }
   }
-  const float* angles = nullptr;
   if (a.rd > 0) {
-    if (a.positions != nullptr && write) pos = a.positions[b * a.pos_sb + t * a.pos_st];
-    if (write && (pos < 0 || pos >= a.table_rows)) raise_status(a.status, SPRUCE_STATUS_BAD_POSITION);
+    if (a.positions != nullptr && w.write) pos = a.positions[b * a.pos_sb + t * a.pos_st];
+    if (w.write && (pos < 0 || pos >= a.table_rows)) raise_status(a.status, SPRUCE_STATUS_BAD_POSITION);
     pos = pos < 0 ? 0 : (pos < a.table_rows ? pos : a.table_rows - 1);
-    angles = a.rope + pos * a.rd;
+    w.angles = a.rope + pos * a.rd;
   }
+  return w;
+}
 
-  // Vector offsets of this lane's pairs, and their angles.
-  int oa[ITERS], ob[ITERS];
-  bool in[ITERS], rot[ITERS];
-  float cs[ITERS][VN], sn[ITERS][VN];
-#pragma unroll
-  for (int it = 0; it < ITERS; ++it) {
-    const int item = l + it * lpr;
-    const int nrot = a.rd / (2 * VN);
-    in[it] = item < items;
-    rot[it] = item < nrot;
-    if (a.interleaved || !rot[it]) {
-      oa[it] = 2 * item * VN;
-      ob[it] = oa[it] + VN;
-    } else {
-      oa[it] = item * VN;
-      ob[it] = a.rd / 2 + item * VN;
-    }
-    if (in[it] && rot[it]) {
-      const float* c = angles + item * VN;
-      const float* s = c + a.rd / 2;
-      if constexpr (VN % 4 == 0) {
-#pragma unroll
-        for (int e = 0; e < VN; e += 4) {
-          *reinterpret_cast<float4*>(&cs[it][e]) = __ldg(reinterpret_cast<const float4*>(c + e));
-          *reinterpret_cast<float4*>(&sn[it][e]) = __ldg(reinterpret_cast<const float4*>(s + e));
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < VN; ++e) {
-          cs[it][e] = c[e];
-          sn[it][e] = s[e];
-        }
-      }
-    }
-  }
+// The tensor a head belongs to, and its number there.
+__device__ __forceinline__ const Rows& rows_of(const RowsArgs& a, int h, int& hh) {
+  hh = h < a.Hq ? h : (h < a.Hq + a.Hkv ? h - a.Hq : h - a.Hq - a.Hkv);
+  return h < a.Hq ? a.q : (h < a.Hq + a.Hkv ? a.k : a.v);
+}
 
-  // All loads of the group's heads first.
-  const T* src[HC];
+// 16-byte vectors.  Bound by instruction issue before HBM unless the arithmetic is packed: fp32 pairs throughout.
+template <typename T, bool APPEND>
+__global__ void __launch_bounds__(kRowThreads, kRowCtasPerSm)
+    norm_rope_kernel(const RowsArgs a, int lpr, int hc, int chunks) {
+  constexpr int HC = kHeadsPerGroup, VN = 16 / sizeof(T), NP = VN / 2;
+  __shared__ uint4 stage[HC * 2][kRowThreads];  // a thread's own vectors: no barrier
+  const int l = threadIdx.x & (lpr - 1);
+  const unsigned block = blockIdx.x / chunks;
+  const int h0 = static_cast<int>(blockIdx.x - block * chunks) * hc;
+  const int64_t n = (int64_t)block * (kRowThreads / lpr) + threadIdx.x / lpr;
+  const int heads = a.Hq + (APPEND ? 2 : 1) * a.Hkv;  // query rows, key rows, (value rows)
+  const int rows = min(hc, heads - h0);
+  const bool live = n < (int64_t)a.B * a.T;
+  const int b = a.B == 1 ? 0 : static_cast<int>(n / a.T), t = static_cast<int>(n - (int64_t)b * a.T);
+  const int items = a.D / (2 * VN), nrot = a.rd / (2 * VN);
+  // This lane's two vectors.  Half pairs: the same place in each half of the rotated dims (or of the rest).  Interleaved:
+  // of each half of the head, as a pair lies in one vector.  Adjacent lanes take adjacent vectors either way.
+  const bool in = live && l < items;
+  const bool rot = a.interleaved ? l * VN < a.rd : l < nrot;
+  const int oa = a.interleaved || rot ? l * VN : a.rd + (l - nrot) * VN;
+  const int ob = a.interleaved ? a.D / 2 + oa : (rot ? a.rd / 2 : (a.D - a.rd) / 2) + oa;
+  const bool rot_b = a.interleaved ? ob < a.rd : rot;
+
+  // The rows first: where they go and how they turn takes dependent loads of its own.
 #pragma unroll
   for (int i = 0; i < HC; ++i) {
-    const int h = h0 + i;
-    const bool isq = h < a.Hq, isk = h < a.Hq + a.Hkv;
-    const Rows& r = isq ? a.q : (isk ? a.k : a.v);
-    const int hh = isq ? h : (isk ? h - a.Hq : h - a.Hq - a.Hkv);
-    src[i] = write && h < heads ? static_cast<const T*>(r.x) + b * r.sb + hh * r.sh + t * r.st : nullptr;
-#pragma unroll
-    for (int it = 0; it < ITERS; ++it)
-      if (src[i] != nullptr && in[it]) {
-        va[i][it].load(src[i] + oa[it]);
-        vb[i][it].load(src[i] + ob[it]);
-      }
+    if (in && i < rows) {
+      int hh;
+      const Rows& r = rows_of(a, h0 + i, hh);
+      const T* src = static_cast<const T*>(r.x) + b * r.sb + hh * r.sh + t * r.st;
+      copy16(&stage[2 * i][threadIdx.x], src + oa);
+      copy16(&stage[2 * i + 1][threadIdx.x], src + ob);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
   }
+  const TokenPlace w = place_token<APPEND>(a, live, static_cast<int>(n), b, t);
+  // cos and sin of the pairs (half), or of vector a's pairs and then vector b's (interleaved).
+  uint64_t cs[NP], sn[NP];
+  if constexpr (NP == 4) {
+    if (rot && in) {
+      const float* c = w.angles + (a.interleaved ? oa / 2 : oa);
+      load_pairs(c, cs[0], cs[1]);
+      load_pairs(c + a.rd / 2, sn[0], sn[1]);
+    }
+    if (rot_b && in) {
+      const float* c = w.angles + (a.interleaved ? ob / 2 : oa + 4);
+      load_pairs(c, cs[2], cs[3]);
+      load_pairs(c + a.rd / 2, sn[2], sn[3]);
+    }
+  } else if (in) {
+    if (a.interleaved) {
+      if (rot) {
+        cs[0] = load_pair(w.angles + oa / 2);
+        sn[0] = load_pair(w.angles + a.rd / 2 + oa / 2);
+      }
+      if (rot_b) {
+        cs[1] = load_pair(w.angles + ob / 2);
+        sn[1] = load_pair(w.angles + a.rd / 2 + ob / 2);
+      }
+    } else if (rot) {
+      load_pairs(w.angles + oa, cs[0], cs[1]);
+      load_pairs(w.angles + a.rd / 2 + oa, sn[0], sn[1]);
+    }
+  }
+  const bool norm = a.q.weight != nullptr || a.k.weight != nullptr;
 
 #pragma unroll
   for (int i = 0; i < HC; ++i) {
+    wait_copies(HC - 1 - i);
+    if (i >= rows) break;  // of the whole CTA
+    int hh;
     const int h = h0 + i;
-    const bool isq = h < a.Hq, isk = !isq && h < a.Hq + a.Hkv;
-    const Rows& r = isq ? a.q : (isk ? a.k : a.v);
-    const int hh = isq ? h : (isk ? h - a.Hq : h - a.Hq - a.Hkv);
-    const float* w = isq ? a.q.weight : (isk ? a.k.weight : nullptr);
-    // The norm's shuffles are executed by every lane; a row's lanes are adjacent.
-    float inv = 1.0f;
-    if (a.q.weight != nullptr || a.k.weight != nullptr) {
-      float ss = 0.0f;
-      if (src[i] != nullptr) {
-#pragma unroll
-        for (int it = 0; it < ITERS; ++it)
-          if (in[it]) {
-#pragma unroll
-            for (int e = 0; e < VN; ++e) {
-              const float x = Elem<T>::to_f(va[i][it].e[e]), y = Elem<T>::to_f(vb[i][it].e[e]);
-              ss = fmaf(x, x, fmaf(y, y, ss));
-            }
-          }
-      }
-      for (int o = lpr >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-      inv = rsqrtf(ss / static_cast<float>(a.D) + a.eps);
+    const Rows& r = rows_of(a, h, hh);
+    const bool isq = h < a.Hq, isv = h >= a.Hq + a.Hkv;
+    uint4 ra = make_uint4(0, 0, 0, 0), rb = ra;
+    if (in) {
+      ra = stage[2 * i][threadIdx.x];
+      rb = stage[2 * i + 1][threadIdx.x];
     }
-    if (src[i] == nullptr) continue;
-    T* dst;
-    if (APPEND && !isq) {
-      if (!cached) continue;
-      dst = static_cast<T*>(r.out) + page * r.ob + hh * r.oh + slot * r.ot;
-    } else {
-      dst = static_cast<T*>(r.out) + b * r.ob + hh * r.oh + t * r.ot;
-    }
+    if (!isv) {
+      uint64_t x[NP], y[NP];
+      unpack16<T>(ra, x);
+      unpack16<T>(rb, y);
+      if (norm) {  // the shuffles are executed by every lane; a row's lanes are adjacent
+        uint64_t s2 = f2_mul(x[0], x[0]);
 #pragma unroll
-    for (int it = 0; it < ITERS; ++it) {
-      if (!in[it]) continue;
-      if (isq || isk) {
-        float x[VN], y[VN];
+        for (int e = 1; e < NP; ++e) s2 = f2_fma(x[e], x[e], s2);
 #pragma unroll
-        for (int e = 0; e < VN; ++e) {
-          x[e] = Elem<T>::to_f(va[i][it].e[e]);
-          y[e] = Elem<T>::to_f(vb[i][it].e[e]);
-        }
-        if (w != nullptr) {
+        for (int e = 0; e < NP; ++e) s2 = f2_fma(y[e], y[e], s2);
+        float s0, s1;
+        f2_unpack(s2, s0, s1);
+        float ss = s0 + s1;
+        for (int o = lpr >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        const float inv = rsqrtf(ss / static_cast<float>(a.D) + a.eps);
+        if (r.weight != nullptr && in) {
+          const uint64_t inv2 = f2_pack(inv, inv);
 #pragma unroll
-          for (int e = 0; e < VN; ++e) {
-            x[e] *= inv * w[oa[it] + e];
-            y[e] *= inv * w[ob[it] + e];
+          for (int e = 0; e < NP; e += 2) {
+            uint64_t w0, w1;
+            load_pairs(r.weight + oa + 2 * e, w0, w1);
+            x[e] = f2_mul(x[e], f2_mul(w0, inv2));
+            x[e + 1] = f2_mul(x[e + 1], f2_mul(w1, inv2));
+            load_pairs(r.weight + ob + 2 * e, w0, w1);
+            y[e] = f2_mul(y[e], f2_mul(w0, inv2));
+            y[e + 1] = f2_mul(y[e + 1], f2_mul(w1, inv2));
           }
-        }
-        if (rot[it]) {
-          if (VN > 1 && a.interleaved) {
-#pragma unroll
-            for (int e = 0; e + 1 < VN; e += 2) {
-              const float c0 = cs[it][e / 2], s0 = sn[it][e / 2];
-              const float c1 = cs[it][VN / 2 + e / 2], s1 = sn[it][VN / 2 + e / 2];
-              const float x0 = x[e], x1 = x[e + 1], y0 = y[e], y1 = y[e + 1];
-              x[e] = x0 * c0 - x1 * s0;
-              x[e + 1] = x1 * c0 + x0 * s0;
-              y[e] = y0 * c1 - y1 * s1;
-              y[e + 1] = y1 * c1 + y0 * s1;
-            }
-          } else {
-#pragma unroll
-            for (int e = 0; e < VN; ++e) {
-              const float x0 = x[e], y0 = y[e];
-              x[e] = x0 * cs[it][e] - y0 * sn[it][e];
-              y[e] = y0 * cs[it][e] + x0 * sn[it][e];
-            }
-          }
-        }
-#pragma unroll
-        for (int e = 0; e < VN; ++e) {
-          va[i][it].e[e] = Elem<T>::from_f(x[e]);
-          vb[i][it].e[e] = Elem<T>::from_f(y[e]);
         }
       }
-      va[i][it].store(dst + oa[it]);
-      vb[i][it].store(dst + ob[it]);
+      if (rot) {
+        if (a.interleaved) {
+          // Angle i of cs is pair i of vector a, or pair i - NP of vector b.
+          turn_pairs(x, cs, sn, 0);
+          if (rot_b) turn_pairs(y, cs, sn, NP);
+        } else {
+#pragma unroll
+          for (int e = 0; e < NP; ++e) {
+            const uint64_t u = x[e], v = y[e];
+            x[e] = f2_sub(f2_mul(u, cs[e]), f2_mul(v, sn[e]));
+            y[e] = f2_fma(u, sn[e], f2_mul(v, cs[e]));
+          }
+        }
+      }
+      ra = pack16<T>(x);
+      rb = pack16<T>(y);
     }
+    if (!in || !w.write || (APPEND && !isq && !w.cached)) continue;
+    T* dst = static_cast<T*>(r.out) +
+             (APPEND && !isq ? w.page * r.ob + hh * r.oh + w.slot * r.ot : b * r.ob + hh * r.oh + t * r.ot);
+    *reinterpret_cast<uint4*>(dst + oa) = ra;
+    *reinterpret_cast<uint4*>(dst + ob) = rb;
   }
 }
 
-template <typename T, int VN, int ITERS, bool APPEND>
-static cudaError_t launch_rows_typed(const RowsArgs& a, cudaStream_t stream) {
-  const int items = a.D / (2 * VN);
-  int lpr = 1;
-  while (lpr < items && lpr < 32) lpr *= 2;
+// Rows that 16-byte vectors do not fit: a warp a row, one element a load; pairs l, l + 32, ... of at most 128.
+template <typename T, bool APPEND>
+__global__ void __launch_bounds__(kRowThreads) norm_rope_scalar_kernel(const RowsArgs a) {
+  const int lane = threadIdx.x & 31;
   const int heads = a.Hq + (APPEND ? 2 : 1) * a.Hkv;
-  const int chunks = (heads + kHeadsPerGroup - 1) / kHeadsPerGroup;
-  const int64_t groups = (int64_t)a.B * a.T * chunks;
+  const int64_t row = (int64_t)blockIdx.x * (kRowThreads / 32) + (threadIdx.x >> 5);
+  const int64_t n = row / heads;
+  const int h = static_cast<int>(row - n * heads);
+  if (n >= (int64_t)a.B * a.T) return;
+  const int b = static_cast<int>(n / a.T), t = static_cast<int>(n - (int64_t)b * a.T);
+  const TokenPlace w = place_token<APPEND>(a, true, static_cast<int>(n), b, t);
+  int hh;
+  const Rows& r = rows_of(a, h, hh);
+  const bool isq = h < a.Hq, isv = h >= a.Hq + a.Hkv;
+  if (!w.write || (APPEND && !isq && !w.cached)) return;
+  const T* src = static_cast<const T*>(r.x) + b * r.sb + hh * r.sh + t * r.st;
+  T* dst = static_cast<T*>(r.out) +
+           (APPEND && !isq ? w.page * r.ob + hh * r.oh + w.slot * r.ot : b * r.ob + hh * r.oh + t * r.ot);
+  const int pairs = a.D / 2, nrot = isv ? 0 : a.rd / 2;
+  T x[4], y[4];
+  float ss = 0.0f;
+#pragma unroll
+  for (int it = 0; it < 4; ++it) {
+    const int p = lane + 32 * it;
+    if (p >= pairs) continue;
+    const bool half = p < nrot && !a.interleaved;
+    x[it] = src[half ? p : 2 * p];
+    y[it] = src[half ? p + nrot : 2 * p + 1];
+    const float u = Elem<T>::to_f(x[it]), v = Elem<T>::to_f(y[it]);
+    ss = fmaf(u, u, fmaf(v, v, ss));
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+  const float inv = rsqrtf(ss / static_cast<float>(a.D) + a.eps);
+#pragma unroll
+  for (int it = 0; it < 4; ++it) {
+    const int p = lane + 32 * it;
+    if (p >= pairs) continue;
+    const bool half = p < nrot && !a.interleaved;
+    const int oa = half ? p : 2 * p, ob = half ? p + nrot : 2 * p + 1;
+    if (isv) {
+      dst[oa] = x[it];
+      dst[ob] = y[it];
+      continue;
+    }
+    float u = Elem<T>::to_f(x[it]), v = Elem<T>::to_f(y[it]);
+    if (r.weight != nullptr) {
+      u *= inv * r.weight[oa];
+      v *= inv * r.weight[ob];
+    }
+    if (p < nrot) {
+      const float c = w.angles[p], s = w.angles[nrot + p], u0 = u;
+      u = u0 * c - v * s;
+      v = v * c + u0 * s;
+    }
+    dst[oa] = Elem<T>::from_f(u);
+    dst[ob] = Elem<T>::from_f(v);
+  }
+}
+
+template <typename T, bool APPEND>
+static cudaError_t launch_rows_typed(const RowsArgs& a, bool vec, cudaStream_t stream) {
+  const int heads = a.Hq + (APPEND ? 2 : 1) * a.Hkv;
+  const int64_t tokens = (int64_t)a.B * a.T;
+  if (!vec) {
+    const int64_t ctas = (tokens * heads + kRowThreads / 32 - 1) / (kRowThreads / 32);
+    if (ctas > 0x7fffffff) return cudaErrorInvalidValue;
+    norm_rope_scalar_kernel<T, APPEND><<<(unsigned)ctas, kRowThreads, 0, stream>>>(a);
+    return cudaGetLastError();
+  }
+  const int items = a.D / (32 / (int)sizeof(T));
+  int lpr = 1;
+  while (lpr < items) lpr *= 2;
   const int per = kRowThreads / lpr;
-  const int64_t ctas = (groups + per - 1) / per;
-  if (ctas > 0x7fffffff) return cudaErrorInvalidValue;
-  norm_rope_kernel<T, VN, ITERS, APPEND><<<(unsigned)ctas, kRowThreads, 0, stream>>>(a, lpr, chunks);
+  const int64_t blocks = (tokens + per - 1) / per;
+  // Four rows a group keep enough bytes in flight; where that leaves SMs without work, one.
+  int hc = kHeadsPerGroup;
+  if (blocks * ((heads + hc - 1) / hc) < 2 * 148) hc = 1;
+  const int chunks = (heads + hc - 1) / hc;
+  if (blocks * chunks > 0x7fffffff) return cudaErrorInvalidValue;
+  norm_rope_kernel<T, APPEND><<<(unsigned)(blocks * chunks), kRowThreads, 0, stream>>>(a, lpr, hc, chunks);
   return cudaGetLastError();
 }
 
-template <typename T>
-static cudaError_t launch_rows_dtype(const RowsArgs& a, bool vec, cudaStream_t stream) {
-  constexpr int V = 16 / sizeof(T);
-  if (a.cu_q != nullptr)
-    return vec ? launch_rows_typed<T, V, 1, true>(a, stream) : launch_rows_typed<T, 1, 4, true>(a, stream);
-  return vec ? launch_rows_typed<T, V, 1, false>(a, stream) : launch_rows_typed<T, 1, 4, false>(a, stream);
-}
-
 cudaError_t launch_norm_rope(const RowsArgs& a, int dtype, cudaStream_t stream) {
-  const int es = dtype == SPRUCE_DTYPE_F32 ? 4 : 2;
-  const int V = 16 / es;
+  const int V = dtype == SPRUCE_DTYPE_F32 ? 4 : 8;
   // 16-byte vectors: pairs that fill them, and bases and strides that keep every one aligned.
-  bool vec = a.D % (2 * V) == 0 && a.rd % (2 * V) == 0 && (reinterpret_cast<uintptr_t>(a.rope) & 15) == 0;
+  auto at16 = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; };
   auto fits = [&](const Rows& r) {
-    return r.x == nullptr || ((reinterpret_cast<uintptr_t>(r.x) & 15) == 0 && (reinterpret_cast<uintptr_t>(r.out) & 15) == 0 &&
-                              r.sb % V == 0 && r.sh % V == 0 && r.st % V == 0 && r.ob % V == 0 && r.oh % V == 0 &&
-                              r.ot % V == 0);
+    return r.x == nullptr || (at16(r.x) && at16(r.out) && at16(r.weight) && r.sb % V == 0 && r.sh % V == 0 &&
+                              r.st % V == 0 && r.ob % V == 0 && r.oh % V == 0 && r.ot % V == 0);
   };
-  vec = vec && fits(a.q) && fits(a.k) && fits(a.v);
-  if (dtype == SPRUCE_DTYPE_F32) return launch_rows_dtype<float>(a, vec, stream);
-  if (dtype == SPRUCE_DTYPE_BF16) return launch_rows_dtype<__nv_bfloat16>(a, vec, stream);
-  return launch_rows_dtype<__half>(a, vec, stream);
+  const bool vec = a.D % (2 * V) == 0 && a.rd % (2 * V) == 0 && at16(a.rope) && fits(a.q) && fits(a.k) && fits(a.v);
+  const bool append = a.cu_q != nullptr;
+  if (dtype == SPRUCE_DTYPE_F32)
+    return append ? launch_rows_typed<float, true>(a, vec, stream) : launch_rows_typed<float, false>(a, vec, stream);
+  if (dtype == SPRUCE_DTYPE_BF16)
+    return append ? launch_rows_typed<__nv_bfloat16, true>(a, vec, stream)
+                  : launch_rows_typed<__nv_bfloat16, false>(a, vec, stream);
+  return append ? launch_rows_typed<__half, true>(a, vec, stream) : launch_rows_typed<__half, false>(a, vec, stream);
 }
 
 }  // namespace spruce

@@ -9,6 +9,7 @@ layers over these.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 
 import torch
@@ -450,32 +451,35 @@ def tree_topk(scores: torch.Tensor, valid: torch.Tensor, cand: torch.Tensor, k: 
     return out
 
 
+def _device_of(*tensors: torch.Tensor | None) -> int:
+    """The one CUDA device of these tensors (None: an argument that was left out)."""
+    device = tensors[0].get_device()
+    for t in tensors:
+        if t is not None and t.get_device() != device or device < 0:
+            _lib.require_cuda(*(t for t in tensors if t is not None))
+            raise ValueError(f"tensors on {tensors[0].device} and {t.device}")
+    return device
+
+
+def _ptr(t: torch.Tensor | None) -> int:
+    return 0 if t is None else t.data_ptr()
+
+
 def _head_weight(w: torch.Tensor | None, D: int, name: str) -> torch.Tensor | None:
     if w is None:
         return None
-    _lib.require_cuda(w)
     if tuple(w.shape) != (D,):
         raise ValueError(f"{name} must be [{D}], got {tuple(w.shape)}")
+    if w.dtype == torch.float32 and w.is_contiguous():
+        return w
     return w.detach().float().contiguous()
 
 
-def _rope_table(rope: torch.Tensor, D: int) -> torch.Tensor:
-    _lib.require_cuda(rope)
+def _check_rope(rope: torch.Tensor, D: int) -> None:
     if rope.dim() != 2 or rope.dtype != torch.float32 or not rope.is_contiguous():
         raise ValueError("the rotation table must be contiguous float32 [positions, rotary width]")
     if rope.shape[1] > D or rope.shape[1] % 2:
         raise ValueError(f"rotary width {rope.shape[1]} must be even and at most head_dim {D}")
-    return rope
-
-
-def _ptr(t: torch.Tensor | None):
-    return None if t is None else t.data_ptr()
-
-
-def _same_device(first: torch.Tensor, *rest) -> None:
-    for t in rest:
-        if t is not None and t.device != first.device:
-            raise ValueError(f"tensors on {first.device} and {t.device}")
 
 
 def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, rope: torch.Tensor, positions: torch.Tensor | None = None, *,
@@ -489,60 +493,63 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, rope: torch.Tensor, positions
     token-major tensors viewed as [B, H, T, D] (the layout the selector and the attention take), or
     ``q_out`` / ``k_out``, which may be q and k themselves.
     """
-    _lib.require_cuda(q, k)
+    device = _device_of(q, k, rope, positions, q_weight, k_weight, q_out, k_out, status)
     B, Hq, T, D = q.shape
-    if q.dtype != k.dtype:
+    dtype = q.dtype
+    if dtype != k.dtype:
         raise ValueError("q and k must share a dtype")
     if k.dim() != 4 or k.shape[0] != B or k.shape[2:] != q.shape[2:]:
         raise ValueError(f"k must be [{B}, Hkv, {T}, {D}], got {tuple(k.shape)}")
     Hkv = k.shape[1]
-    rope = _rope_table(rope, D)
+    _check_rope(rope, D)
     q_weight, k_weight = _head_weight(q_weight, D, "q_weight"), _head_weight(k_weight, D, "k_weight")
+    pos_strides = (0, 0)
     if positions is not None:
-        _lib.require_cuda(positions)
-        if positions.dim() not in (1, 2) or positions.shape != q.shape[2:3] and tuple(positions.shape) != (B, T):
+        if tuple(positions.shape) not in ((T,), (B, T)):
             raise ValueError(f"positions must be [{T}] or [{B}, {T}], got {tuple(positions.shape)}")
         if positions.is_floating_point():
             raise ValueError("positions must be integers")
         positions = positions.to(torch.int64).expand(B, T)
+        pos_strides = positions.stride()
     elif T > rope.shape[0]:
         raise ValueError(f"{T} tokens need a rotation table of as many positions, got {rope.shape[0]}")
-    q = q if q.stride(-1) == 1 else q.contiguous()
-    k = k if k.stride(-1) == 1 else k.contiguous()
+    q = q if q.stride(3) == 1 else q.contiguous()
+    k = k if k.stride(3) == 1 else k.contiguous()
     if q_out is None:
-        q_out = torch.empty((B, T, Hq, D), device=q.device, dtype=q.dtype).transpose(1, 2)
+        q_out = q.new_empty_strided((B, Hq, T, D), (T * Hq * D, D, Hq * D, 1))
+    elif q_out.shape != q.shape or q_out.dtype != dtype or q_out.stride(3) != 1:
+        raise ValueError(f"an output must be {dtype} {tuple(q.shape)} with a unit last stride")
     if k_out is None:
-        k_out = torch.empty((B, T, Hkv, D), device=q.device, dtype=q.dtype).transpose(1, 2)
-    for x, y in ((q, q_out), (k, k_out)):
-        if y.shape != x.shape or y.dtype != x.dtype or y.stride(-1) != 1:
-            raise ValueError(f"an output must be {x.dtype} {tuple(x.shape)} with a unit last stride")
-    _same_device(q, k, rope, positions, q_weight, k_weight, q_out, k_out, status)
-    _lib.check(_lib.load().spruce_qk_norm_rope(
-        q.data_ptr(), _lib.strides(q), k.data_ptr(), _lib.strides(k), _dt(q), B, Hq, Hkv, T, D, rope.data_ptr(),
-        rope.shape[0], rope.shape[1], int(interleaved), _ptr(positions),
-        None if positions is None else _lib.strides(positions, 2), _ptr(q_weight), _ptr(k_weight), float(eps),
-        q_out.data_ptr(), _lib.strides(q_out), k_out.data_ptr(), _lib.strides(k_out), _ptr(status),
-        _lib.stream_of(q)))
+        k_out = q.new_empty_strided((B, Hkv, T, D), (T * Hkv * D, D, Hkv * D, 1))
+    elif k_out.shape != k.shape or k_out.dtype != dtype or k_out.stride(3) != 1:
+        raise ValueError(f"an output must be {dtype} {tuple(k.shape)} with a unit last stride")
+    args = _lib.QK_NORM_ROPE_ARGS.pack(
+        q.data_ptr(), k.data_ptr(), q_out.data_ptr(), k_out.data_ptr(), rope.data_ptr(), _ptr(positions),
+        _ptr(q_weight), _ptr(k_weight), _ptr(status), _lib.stream_on(device), *q.stride(), *k.stride(),
+        *q_out.stride(), *k_out.stride(), *pos_strides, _dt(q), B, Hq, Hkv, T, D, *rope.shape, interleaved, eps)
+    _lib.check(_lib.load().spruce_qk_norm_rope(args))
     return q_out, k_out
 
 
 def _paged_shapes(k_cache, v_cache, block_table, cu_q, kv_lens, dtype):
-    """(num_pages, Hkv, page_size, D, S) of a paged cache and its metadata, checked."""
-    if k_cache.dim() != 4 or v_cache.shape != k_cache.shape:
+    """(num_pages, Hkv, page_size, D, S, (table stride, table width)) of a paged cache and its metadata, checked."""
+    shape = k_cache.shape
+    if len(shape) != 4 or v_cache.shape != shape:
         raise ValueError("the caches must be [pages, Hkv, page_size, D] of one shape")
     if k_cache.dtype != dtype or v_cache.dtype != dtype:
         raise ValueError("the caches must have the new tokens' dtype")
     if k_cache.stride(3) != 1 or v_cache.stride(3) != 1:
         raise ValueError("the caches need a unit last stride")
-    S = kv_lens.shape[0]
     if not (block_table.dtype == cu_q.dtype == kv_lens.dtype == torch.int32):
         raise ValueError("block_table, cu_q and kv_lens must be int32")
-    if block_table.dim() != 2 or block_table.shape[0] != S or kv_lens.dim() != 1 or tuple(cu_q.shape) != (S + 1,):
+    table, (S, *more) = block_table.shape, kv_lens.shape
+    if more or len(table) != 2 or table[0] != S or cu_q.shape != (S + 1,):
         raise ValueError(f"expected block_table [S, pages], cu_q [S + 1] and kv_lens [S], got "
-                         f"{tuple(block_table.shape)}, {tuple(cu_q.shape)}, {tuple(kv_lens.shape)}")
-    if block_table.stride(1) != 1 and block_table.shape[1] > 1 or not (cu_q.is_contiguous() and kv_lens.is_contiguous()):
+                         f"{tuple(table)}, {tuple(cu_q.shape)}, {tuple(kv_lens.shape)}")
+    step, unit = block_table.stride()
+    if unit != 1 and table[1] > 1 or not (cu_q.is_contiguous() and kv_lens.is_contiguous()):
         raise ValueError("block_table needs a unit last stride, cu_q and kv_lens must be contiguous")
-    return (*k_cache.shape, S)
+    return (*shape, S, (step, table[1]))
 
 
 def paged_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -559,45 +566,49 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
     replaces the cache positions in the rotation only.  With ``q`` [N, Hq, D], its norm and rotation run in the
     same launch into ``q_out`` (a new [N, Hq, D] tensor by default; q itself is allowed).
     """
-    _lib.require_cuda(k, v, k_cache, v_cache, block_table, cu_q, kv_lens)
-    pages, Hkv, page_size, D, S = _paged_shapes(k_cache, v_cache, block_table, cu_q, kv_lens, k.dtype)
-    if k.dim() != 3 or k.shape[1:] != (Hkv, D) or v.shape != k.shape or v.dtype != k.dtype:
+    device = _device_of(k, v, k_cache, v_cache, block_table, cu_q, kv_lens, q, rope, positions, q_weight, k_weight,
+                        q_out, status)
+    dtype = k.dtype
+    pages, Hkv, page_size, D, S, table = _paged_shapes(k_cache, v_cache, block_table, cu_q, kv_lens, dtype)
+    if k.dim() != 3 or k.shape[1] != Hkv or k.shape[2] != D or v.shape != k.shape or v.dtype != dtype:
         raise ValueError(f"k and v must be [N, {Hkv}, {D}] of one dtype, got {tuple(k.shape)} and {tuple(v.shape)}")
     N = k.shape[0]
-    k = k if k.stride(-1) == 1 else k.contiguous()
-    v = v if v.stride(-1) == 1 else v.contiguous()
+    k = k if k.stride(2) == 1 else k.contiguous()
+    v = v if v.stride(2) == 1 else v.contiguous()
     q_weight, k_weight = _head_weight(q_weight, D, "q_weight"), _head_weight(k_weight, D, "k_weight")
+    table_rows = rd = Hq = 0
     if rope is not None:
-        rope = _rope_table(rope, D)
+        _check_rope(rope, D)
+        table_rows, rd = rope.shape
     if positions is not None:
-        _lib.require_cuda(positions)
         if tuple(positions.shape) != (N,) or positions.is_floating_point():
             raise ValueError(f"positions must be integers [{N}]")
         positions = positions.to(torch.int64).contiguous()
-    Hq, qs, os = 0, None, None
+    qs = os = (0, 0)
     if q is not None:
-        _lib.require_cuda(q)
-        if q.dim() != 3 or q.shape[0] != N or q.shape[2] != D or q.dtype != k.dtype:
-            raise ValueError(f"q must be {k.dtype} [{N}, Hq, {D}], got {q.dtype} {tuple(q.shape)}")
-        q = q if q.stride(-1) == 1 else q.contiguous()
+        if q.dim() != 3 or q.shape[0] != N or q.shape[2] != D or q.dtype != dtype:
+            raise ValueError(f"q must be {dtype} [{N}, Hq, {D}], got {q.dtype} {tuple(q.shape)}")
+        q = q if q.stride(2) == 1 else q.contiguous()
         Hq = q.shape[1]
         if q_out is None:
-            q_out = torch.empty((N, Hq, D), device=q.device, dtype=q.dtype)
-        elif q_out.shape != q.shape or q_out.dtype != q.dtype or q_out.stride(-1) != 1:
-            raise ValueError(f"q_out must be {q.dtype} {tuple(q.shape)} with a unit last stride")
-        qs, os = _lib.strides(q, 2), _lib.strides(q_out, 2)
+            q_out = q.new_empty((N, Hq, D))
+        elif q_out.shape != q.shape or q_out.dtype != dtype or q_out.stride(2) != 1:
+            raise ValueError(f"q_out must be {dtype} {tuple(q.shape)} with a unit last stride")
+        qs, os = q.stride()[:2], q_out.stride()[:2]
     elif q_out is not None:
         raise ValueError("q_out without q")
-    _same_device(k, v, k_cache, v_cache, block_table, cu_q, kv_lens, q, rope, positions, q_weight, k_weight, q_out,
-                 status)
-    _lib.check(_lib.load().spruce_paged_append(
-        _ptr(q), qs, k.data_ptr(), _lib.strides(k, 2), v.data_ptr(), _lib.strides(v, 2), _dt(k), N, Hq, Hkv, D,
-        _ptr(rope), 0 if rope is None else rope.shape[0], 0 if rope is None else rope.shape[1], int(interleaved),
-        _ptr(positions), _ptr(q_weight), _ptr(k_weight), float(eps), _ptr(q_out), os, k_cache.data_ptr(),
-        _lib.strides(k_cache, 3), v_cache.data_ptr(), _lib.strides(v_cache, 3), pages, page_size,
-        block_table.data_ptr(), block_table.stride(0), block_table.shape[1], cu_q.data_ptr(), kv_lens.data_ptr(), S,
-        _ptr(status), _lib.stream_of(k)))
+    args = _lib.PAGED_APPEND_ARGS.pack(
+        _ptr(q), k.data_ptr(), v.data_ptr(), _ptr(q_out), k_cache.data_ptr(), v_cache.data_ptr(), _ptr(rope),
+        _ptr(positions), _ptr(q_weight), _ptr(k_weight), block_table.data_ptr(), cu_q.data_ptr(), kv_lens.data_ptr(),
+        _ptr(status), _lib.stream_on(device), *qs, *k.stride()[:2], *v.stride()[:2], *os, *k_cache.stride()[:3],
+        *v_cache.stride()[:3], _dt(k), N, S, Hq, Hkv, D, pages, page_size, *table, table_rows, rd, interleaved, eps)
+    _lib.check(_lib.load().spruce_paged_append(args))
     return q_out
+
+
+@functools.lru_cache(maxsize=256)
+def _paged_workspace_bytes(Hq: int, Hkv: int, D: int, max_q_len: int, dtype: int) -> int:
+    return int(_lib.load().spruce_paged_attention_workspace_bytes(Hq, Hkv, D, max_q_len, dtype))
 
 
 def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
@@ -610,28 +621,31 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     see none give zeros.  ``max_q_len`` and ``max_kv_len`` bound the sequences' new tokens and lengths (the lengths
     themselves stay on the device).  Returns [N, Hq, D]; rows past ``cu_q[-1]`` are not written.
     """
-    _lib.require_cuda(q, k_cache, v_cache, block_table, cu_q, kv_lens)
-    pages, Hkv, page_size, D, S = _paged_shapes(k_cache, v_cache, block_table, cu_q, kv_lens, q.dtype)
+    device = _device_of(q, k_cache, v_cache, block_table, cu_q, kv_lens, out, workspace, status)
+    dtype = q.dtype
+    pages, Hkv, page_size, D, S, table = _paged_shapes(k_cache, v_cache, block_table, cu_q, kv_lens, dtype)
     if q.dim() != 3 or q.shape[2] != D:
         raise ValueError(f"q must be [N, Hq, {D}], got {tuple(q.shape)}")
     N, Hq, _ = q.shape
-    q = _vec_ok(q)
+    qn, qh, qd = q.stride()
+    if qd != 1 or (qn | qh) % (16 // q.element_size()) or q.data_ptr() % 16:
+        q = q.contiguous()
+        qn, qh, _ = q.stride()
     if out is None:
-        out = torch.empty((N, Hq, D), device=q.device, dtype=q.dtype)
-    elif out.shape != q.shape or out.dtype != q.dtype or out.stride(-1) != 1:
-        raise ValueError(f"out must be {q.dtype} {tuple(q.shape)} with a unit last stride")
-    L = _lib.load()
-    need = L.spruce_paged_attention_workspace_bytes(Hq, Hkv, D, max_q_len, _dt(q))
-    if need < 0:
-        raise ValueError(f"bad paged attention shape: q {tuple(q.shape)}, cache {tuple(k_cache.shape)}, "
-                         f"max_q_len {max_q_len}")
+        out = q.new_empty((N, Hq, D))
+    elif out.shape != q.shape or out.dtype != dtype or out.stride(2) != 1:
+        raise ValueError(f"out must be {dtype} {tuple(q.shape)} with a unit last stride")
+    dt = _dt(q)
     if workspace is None:
-        workspace = torch.empty(need, device=q.device, dtype=torch.uint8)
-    _same_device(q, k_cache, v_cache, block_table, cu_q, kv_lens, out, workspace, status)
-    _lib.check(L.spruce_paged_attention(
-        q.data_ptr(), _lib.strides(q, 2), k_cache.data_ptr(), _lib.strides(k_cache, 3), v_cache.data_ptr(),
-        _lib.strides(v_cache, 3), _dt(q), N, Hq, Hkv, D, pages, page_size, block_table.data_ptr(),
-        block_table.stride(0), block_table.shape[1], cu_q.data_ptr(), kv_lens.data_ptr(), S, max_q_len, max_kv_len,
-        float(D ** -0.5 if scale is None else scale), out.data_ptr(), _lib.strides(out, 2), workspace.data_ptr(),
-        workspace.numel() * workspace.element_size(), _ptr(status), _lib.stream_of(q)))
+        need = _paged_workspace_bytes(Hq, Hkv, D, max_q_len, dt)
+        if need < 0:
+            raise ValueError(f"bad paged attention shape: q {tuple(q.shape)}, cache {tuple(k_cache.shape)}, "
+                             f"max_q_len {max_q_len}")
+        workspace = q.new_empty(need // q.element_size())
+    args = _lib.PAGED_ATTENTION_ARGS.pack(
+        q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), block_table.data_ptr(), cu_q.data_ptr(),
+        kv_lens.data_ptr(), workspace.data_ptr(), _ptr(status), _lib.stream_on(device), qn, qh, *k_cache.stride()[:3],
+        *v_cache.stride()[:3], *out.stride()[:2], dt, N, S, Hq, Hkv, D, pages, page_size, *table, max_q_len,
+        max_kv_len, workspace.nbytes, D ** -0.5 if scale is None else scale)
+    _lib.check(_lib.load().spruce_paged_attention(args))
     return out

@@ -79,29 +79,42 @@ def test_table_refusals():
 
 def test_entry_points_refuse_before_device_work():
     L = _lib.load()
-    s4, s3, s2 = _lib.int64s(64, 64, 64, 1), _lib.int64s(64, 64, 64), _lib.int64s(64, 64)
 
-    def rope(D=64, rd=64, rows=8, dtype=1, strides=s4, rope=1):
-        return L.spruce_qk_norm_rope(1, strides, 1, strides, dtype, 1, 2, 1, 4, D, rope, rows, rd, 0, None, None,
-                                     None, None, 1e-6, 1, strides, 1, strides, None, None)
+    def rope(D=64, rd=64, rows=8, dtype=1, last=1, rope=16, eps=1e-6):
+        strides = (64, 64, 64, last) * 4 + (0, 0)
+        return L.spruce_qk_norm_rope(_lib.QK_NORM_ROPE_ARGS.pack(16, 16, 16, 16, rope, 0, 0, 0, 0, 0, *strides, dtype,
+                                                                 1, 2, 1, 4, D, rows, rd, 0, eps))
 
     for kw, text in ((dict(D=258), "head_dim"), (dict(D=63), "head_dim"), (dict(rd=66), "rotary width"),
-                     (dict(rd=3), "rotary width"), (dict(rows=0), "empty"), (dict(rope=None), "empty"),
-                     (dict(dtype=3), "dtype"), (dict(strides=_lib.int64s(64, 64, 64, 2)), "unit last stride")):
+                     (dict(rd=3), "rotary width"), (dict(rows=0), "empty"), (dict(rope=0), "empty"),
+                     (dict(dtype=3), "dtype"), (dict(last=2), "unit last stride")):
         with pytest.raises(ValueError, match=text):
             _lib.check(rope(**kw))
 
-    def attend(D=64, Hq=4, Hkv=2, page=16, N=1, S=1, max_q=1, max_kv=16, cu=16, q=16, kc=s3, ws=256, ws_bytes=1 << 30,
-               scale=0.1, pages=4):
-        return L.spruce_paged_attention(q, s2, 16, kc, 16, s3, 1, N, Hq, Hkv, D, pages, page, 16, 2, 2, cu, 16, S, max_q,
-                                        max_kv, scale, 16, s2, ws, ws_bytes, None, None)
+    def append(N=1, page=16, D=64, k=16, rd=64, rows=8, S=1, table=16):
+        return L.spruce_paged_append(_lib.PAGED_APPEND_ARGS.pack(
+            0, k, 16, 0, 16, 16, 16, 0, 0, 0, table, 16, 16, 0, 0, *(64,) * 14, 1, N, S, 4, 2, D, 4, page, 2, 2, rows,
+            rd, 0, 1e-6))
+
+    for kw, text in ((dict(page=24), "page_size"), (dict(D=258), "head_dim"), (dict(rows=0), "empty"),
+                     (dict(k=0), "null"), (dict(table=0), "NULL"), (dict(N=-1), "bad shape"),
+                     (dict(N=1 << 31), "too large")):
+        with pytest.raises(ValueError, match=text):
+            _lib.check(append(**kw))
+    assert append(N=0) == _lib.OK and append(S=0) == _lib.OK
+
+    def attend(D=64, Hq=4, Hkv=2, page=16, N=1, S=1, max_q=1, max_kv=16, cu=16, q=16, head=64, ws=256,
+               ws_bytes=1 << 30, scale=0.1, pages=4):
+        return L.spruce_paged_attention(_lib.PAGED_ATTENTION_ARGS.pack(
+            q, 16, 16, 16, 16, cu, 16, ws, 0, 0, 64, 64, 64, head, 64, 64, 64, 64, 64, 64, 1, N, S, Hq, Hkv, D, pages,
+            page, 2, 2, max_q, max_kv, ws_bytes, scale))
 
     for kw, text in ((dict(D=96), "head_dim 64 or 128"), (dict(Hq=5), "divisible"), (dict(page=24), "page_size"),
                      (dict(page=8), "page_size"), (dict(N=-1), "bad shape"), (dict(max_q=-1), "negative"),
-                     (dict(max_q=1 << 30), "too long"), (dict(pages=0), "no pages"), (dict(scale=-1.0), "scale"), (dict(scale=float("nan")), "scale"),
-                     (dict(scale=float("inf")), "scale"), (dict(cu=None), "NULL"), (dict(q=None), "null"),
-                     (dict(q=8), "16-byte aligned"), (dict(kc=_lib.int64s(64, 60, 64)), "16-byte aligned"),
-                     (dict(ws=128), "256-byte")):
+                     (dict(max_q=1 << 30), "too long"), (dict(cu=0), "NULL"), (dict(q=0), "null"),
+                     (dict(pages=0), "no pages"), (dict(scale=-1.0), "scale"), (dict(scale=float("nan")), "scale"),
+                     (dict(scale=float("inf")), "scale"), (dict(q=8), "16-byte aligned"),
+                     (dict(head=60), "16-byte aligned"), (dict(ws=128), "256-byte")):
         with pytest.raises(ValueError, match=text):
             _lib.check(attend(**kw))
     with pytest.raises(RuntimeError, match="workspace"):
