@@ -28,36 +28,61 @@
 
 namespace spruce {
 
-constexpr int kChunkThreads = 320;
-constexpr int kChunkLoader = 8;
-constexpr int kChunkMma = 9;
+constexpr int kChunkThreads = 384;
+constexpr int kChunkMma = 8;
+constexpr int kChunkLoadK = 9;
+constexpr int kChunkLoadV = 10;
 constexpr int kChunkRows = kPagedChunkRows;
 constexpr int kChunkKeys = kPagedChunkKeys;
 
+constexpr int kChunkRoleBytes = 144;
+
 template <int D>
 struct ChunkLayout {
-  static constexpr int STAGES = D == 128 ? 2 : 4;
+  static constexpr int KST = D == 128 ? 3 : 5, VST = D == 128 ? 2 : 5;  // tiles of K and of V in flight
   static constexpr int NP = D / 64;           // 128-byte panels along the head dim
   static constexpr int PANEL = 128 * 128;     // 128 rows x 128 B
   static constexpr int TILE = NP * PANEL;
   static constexpr int OFF_Q = 0;
   static constexpr int OFF_K = 2 * TILE;
-  static constexpr int OFF_V = OFF_K + STAGES * TILE;
-  static constexpr int OFF_BAR = OFF_V + STAGES * TILE;
-  // q_full[2], k_full[S], v_full[S], kv_empty[S], v_tail, s_full[2], p_full[2][2], o_done[2], drain
-  static constexpr int NBAR = 2 + 3 * STAGES + 1 + 2 + 4 + 2 + 1;
+  static constexpr int OFF_V = OFF_K + KST * TILE;
+  static constexpr int OFF_BAR = OFF_V + VST * TILE;
+  // q_full[2], k_full[], k_empty[], v_full[], v_empty[], v_tail, s_full[2], p_full[2][2], o_done[2], drain
+  static constexpr int NBAR = 2 + 2 * (KST + VST) + 1 + 2 + 4 + 2 + 1;
   static constexpr int OFF_MISC = OFF_BAR + NBAR * 8;
   static constexpr int OFF_SCAN = (OFF_MISC + 16 + 15) / 16 * 16;
-  static constexpr int BYTES = 1024 + OFF_SCAN + 33 * 8;
+  static constexpr int OFF_ROLE = OFF_SCAN;   // a ChunkRole for each warp with a part, once the scan is done
+  static constexpr int BYTES = 1024 + OFF_ROLE + 11 * kChunkRoleBytes;
+  static_assert(BYTES + 16 <= 227 * 1024, "shared memory of a CTA");
   static constexpr int COL_S = 2 * D;         // S_t (and P_t) at COL_S + 128 t
 };
+
+// A warp's place in the CTA's run.  It lives in shared memory so that the softmax's inner loop, which wants every
+// register, does not carry it.
+struct ChunkRole {
+  PagedWalk<kChunkRows, kChunkKeys> walk;
+  PagedPiece x;
+};
+static_assert(sizeof(ChunkRole) <= kChunkRoleBytes, "fits its slot");
+__device__ __forceinline__ bool next_piece(const PagedParams& p, ChunkRole* r) {
+  PagedWalk<kChunkRows, kChunkKeys> w = r->walk;
+  PagedPiece x;
+  const bool more = w.next(p, x);
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) {
+    r->walk = w;
+    r->x = x;
+  }
+  __syncwarp();
+  return more;
+}
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kChunkThreads, 1)
     paged_chunk_sm100_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv,
-                             const PagedParams p, int box) {
+                             const __grid_constant__ PagedParams p, int box) {
   using L = ChunkLayout<D>;
-  constexpr int STAGES = L::STAGES;
+  constexpr int KST = L::KST, VST = L::VST;
   using Walk = PagedWalk<kChunkRows, kChunkKeys>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -69,9 +94,10 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::OFF_BAR);
   uint64_t* q_full = bars;                // [tile]: its Q rows are in shared memory (128 arrivals)
   uint64_t* k_full = q_full + 2;
-  uint64_t* v_full = k_full + STAGES;
-  uint64_t* kv_empty = v_full + STAGES;
-  uint64_t* v_tail = kv_empty + STAGES;   // the loader's own: a V tile whose tail it clears has landed
+  uint64_t* k_empty = k_full + KST;
+  uint64_t* v_full = k_empty + KST;
+  uint64_t* v_empty = v_full + VST;
+  uint64_t* v_tail = v_empty + VST;       // the loader's own: a V tile whose tail it clears has landed
   uint64_t* s_full = v_tail + 1;          // [tile]: S_t(j) written
   uint64_t* p_full = s_full + 2;          // [tile * 2 + half]: that half of P_t(j) written (128 arrivals)
   uint64_t* o_done = p_full + 4;          // [tile]: the piece's last PV_t complete
@@ -80,14 +106,11 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::OFF_MISC + 4);
   int64_t* scan = reinterpret_cast<int64_t*>(smem + L::OFF_SCAN);
 
-  if (warp == kChunkLoader) {
+  if (warp == kChunkLoadK) {
     if (lane == 0) {
       *abort_flag = 0;
-      for (int s = 0; s < STAGES; ++s) {
-        mbar_init(&k_full[s], 1);
-        mbar_init(&v_full[s], 1);
-        mbar_init(&kv_empty[s], 1);
-      }
+      for (int s = 0; s < 2 * KST; ++s) mbar_init(&k_full[s], 1);  // and k_empty
+      for (int s = 0; s < 2 * VST; ++s) mbar_init(&v_full[s], 1);  // and v_empty
       for (int t = 0; t < 2; ++t) {
         mbar_init(&q_full[t], 128);
         mbar_init(&s_full[t], 1);
@@ -114,49 +137,58 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   if (!any) walk.left = 0;
-  PagedPiece x;
+  ChunkRole* const role = reinterpret_cast<ChunkRole*>(smem + L::OFF_ROLE + min(warp, 10) * kChunkRoleBytes);
+  if (lane == 0 && warp < 11) role->walk = walk;
+  __syncwarp();
+  const PagedPiece& x = role->x;
 
-  if (warp == kChunkLoader) {
-    // ------------------------------------------------------------ K and V
-    const int boxes = kChunkKeys / box * L::NP;  // per tile and tensor; at most 16
-    const int pp = lane % L::NP, row0 = lane / L::NP * box;
-    const bool mine = lane < boxes;
-    int j = 0;         // tiles loaded by this CTA
-    uint32_t tails = 0;
+  if (warp == kChunkLoadK || warp == kChunkLoadV) {
+    // ------------------------------------------------------------ K or V
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    const bool v = warp == kChunkLoadV;
+    const CUtensorMap* const map = v ? &tmv : &tmk;
+    uint8_t* const base = smem + (v ? L::OFF_V : L::OFF_K);
+    uint64_t* const full = v ? v_full : k_full;
+    uint64_t* const empty = v ? v_empty : k_empty;
+    const int stages = v ? VST : KST;
+    const int boxes = kChunkKeys / box;  // of a tile's rows: at most 8
+    const bool leader = elect_one();
+    int st = 0, loaded = 0;              // the next tile's stage; tiles loaded
+    uint32_t turn = 1, tails = 0;        // parity of the stage's last release (none before the first round)
     bool ok = true;
-    while (ok && walk.next(p, x)) {
+    while (ok && next_piece(p, role)) {
       if (x.keys == 0) continue;
+      const int keys = x.keys, t1 = x.t1, g = x.g;
       const int32_t* table = p.a.block_table + x.s * p.a.table_stride;
-      auto page_of = [&](int t, int& row) {  // this lane's box of tile t
-        const int key = t * kChunkKeys + row0;
-        if (!mine || t >= x.t1 || key >= x.keys) return static_cast<int>(p.a.num_pages);
-        const int pi = key / p.a.page_size;
-        row = key - pi * p.a.page_size;
-        const int page = paged_page(p, table, pi);
+      // Lane b: page of box b of tile t; past the keys (or the table) a page index that reads zeros.
+      auto page_of = [&](int t) {
+        const int key = t * kChunkKeys + lane * box;
+        if (lane >= boxes || t >= t1 || key >= keys) return static_cast<int>(p.a.num_pages);
+        const int page = paged_page(p, table, key / p.a.page_size);
         return page < 0 ? static_cast<int>(p.a.num_pages) : page;
       };
-      int row = 0, page = page_of(x.t0, row);
-      for (int t = x.t0; t < x.t1; ++t, ++j) {
-        const int st = j % STAGES;
-        if (j >= STAGES && !__all_sync(0xffffffffu, mbar_wait(&kv_empty[st], ((j / STAGES) - 1) & 1, status, abort_flag))) {
-          ok = false;
-          break;
-        }
-        uint8_t* ks = smem + L::OFF_K + st * L::TILE;
-        uint8_t* vs = smem + L::OFF_V + st * L::TILE;
-        const int valid = x.keys - t * kChunkKeys;       // keys of this tile that exist
-        const bool tail = valid < kChunkKeys && valid % box != 0;
-        if (lane == 0) {
-          mbar_arrive_expect_tx(&k_full[st], L::TILE);
-          mbar_arrive_expect_tx(tail ? v_tail : &v_full[st], L::TILE);
-        }
+      int page = page_of(x.t0);
+      int row = (x.t0 * kChunkKeys) % p.a.page_size;       // of the next box in its page
+      for (int t = x.t0; t < t1; ++t) {
+        if (loaded >= stages && !(ok = __all_sync(0xffffffffu, mbar_wait(&empty[st], turn, status, abort_flag)))) break;
+        uint8_t* dst = base + st * L::TILE;
+        const int valid = keys - t * kChunkKeys;           // keys of this tile that exist
+        const bool tail = v && valid < kChunkKeys && valid % box != 0;
+        uint64_t* const bar = tail ? v_tail : &full[st];
+        if (leader) mbar_arrive_expect_tx(bar, L::TILE);
         __syncwarp();
-        if (mine) {
-          tma_load_4d(ks + pp * L::PANEL + row0 * 128, &tmk, &k_full[st], pp * 64, row, x.g, page);
-          tma_load_4d(vs + pp * L::PANEL + row0 * 128, &tmv, tail ? v_tail : &v_full[st], pp * 64, row, x.g, page);
+        for (int b = 0; b < boxes; ++b) {
+          const int pb = __shfl_sync(0xffffffffu, page, b);
+          if (leader) {
+#pragma unroll
+            for (int pp = 0; pp < L::NP; ++pp)
+              tma_load_4d(dst + pp * L::PANEL + b * box * 128, map, bar, pp * 64, row, g, pb);
+          }
+          __syncwarp();
+          row += box;
+          if (row == p.a.page_size) row = 0;
         }
-        row = 0;
-        page = page_of(t + 1, row);  // its latency passes behind the wait for the next stage
+        page = page_of(t + 1);  // its latency passes behind the wait for the next stage
         if (tail) {
           ok = __all_sync(0xffffffffu, mbar_wait(v_tail, tails & 1, status, abort_flag));
           ++tails;
@@ -164,23 +196,27 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
           const int end = min(kChunkKeys, (valid / box + 1) * box);
           for (int e = lane; e < (end - valid) * 8 * L::NP; e += 32) {
             const int panel = e / ((end - valid) * 8), c = e % ((end - valid) * 8);
-            *reinterpret_cast<uint4*>(vs + panel * L::PANEL + (valid + c / 8) * 128 + c % 8 * 16) = make_uint4(0, 0, 0, 0);
+            *reinterpret_cast<uint4*>(dst + panel * L::PANEL + (valid + c / 8) * 128 + c % 8 * 16) = make_uint4(0, 0, 0, 0);
           }
           fence_proxy_async_smem();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&v_full[st]);
-          if (!ok) break;
+          if (lane == 0) mbar_arrive(&full[st]);
         }
+        ++loaded;
+        if (++st == stages) {
+          st = 0;
+          turn ^= 1;
+        }
+        if (!ok) break;
       }
     }
     // No copy may be in flight when the CTA exits.
-    for (int i = max(0, j - STAGES); i < j; ++i) {
-      mbar_wait(&k_full[i % STAGES], (i / STAGES) & 1, status, nullptr);
-      mbar_wait(&v_full[i % STAGES], (i / STAGES) & 1, status, nullptr);
-    }
+    for (int k = max(0, loaded - stages); k < loaded; ++k)
+      mbar_wait(&full[k % stages], (k / stages) & 1, status, nullptr);
     __syncwarp();
   } else if (warp == kChunkMma) {
     // ------------------------------------------------------------ MMA issuer
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     const bool leader = elect_one();
     constexpr uint32_t fmt = UmmaFormat<T>::value;
     constexpr uint32_t idesc_qk = idesc_f16(fmt, 0, 0, 128, 128);
@@ -226,52 +262,61 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       ++np_[t];
       return true;
     };
-    int j = 0;
     uint32_t pieces[2] = {0, 0};
+    int kst = 0, vst = 0;            // stages of the next K and V tile, and the parities of their turns
+    uint32_t kturn = 0, vturn = 0;
     bool ok = true;
-    while (ok && walk.next(p, x)) {
-      const int rows = min(kChunkRows, x.q.qlen * p.rep - x.qt * kChunkRows);
-      const bool two = rows > 128;
+    while (ok && next_piece(p, role)) {
+      const bool two = x.q.qlen * p.rep - x.qt * kChunkRows > 128;
       if (x.keys == 0) continue;
-      ok = wait(&q_full[0], pieces[0]++ & 1) && (!two || wait(&q_full[1], pieces[1]++ & 1));
       const int n = x.t1 - x.t0;
+      ok = wait(&q_full[0], pieces[0]++ & 1) && (!two || wait(&q_full[1], pieces[1]++ & 1));
+      int vlast = 0;                 // V stage of tile i - 1
       for (int i = 0; ok && i <= n; ++i) {
-        const int st = (j + i) % STAGES;
-        const int sp = (j + i + STAGES - 1) % STAGES;  // stage of tile i - 1
-        const uint32_t ph = ((j + i) / STAGES) & 1;
         if (i < n) {
-          if (!(ok = wait(&k_full[st], ph))) break;
+          if (!(ok = wait(&k_full[kst], kturn))) break;
           tc_fence_after();
-          issue_qk(0, st);
+          issue_qk(0, kst);
         }
         if (i > 0 && two) {
-          if (!(ok = pv(1, sp, i == 1))) break;
+          if (!(ok = pv(1, vlast, i == 1))) break;
           if (i == n) commit(&o_done[1]);
         }
-        if (i > 0) commit(&kv_empty[sp]);  // every MMA reading that stage is issued before this
+        if (i > 0) commit(&v_empty[vlast]);  // every MMA reading that stage is issued before this
         if (i == n) break;
-        if (two) issue_qk(1, st);
-        if (!(ok = wait(&v_full[st], ph) && pv(0, st, i == 0))) break;
+        if (two) issue_qk(1, kst);
+        commit(&k_empty[kst]);
+        if (++kst == KST) {
+          kst = 0;
+          kturn ^= 1;
+        }
+        if (!(ok = wait(&v_full[vst], vturn) && pv(0, vst, i == 0))) break;
         if (i == n - 1) commit(&o_done[0]);
+        vlast = vst;
+        if (++vst == VST) {
+          vst = 0;
+          vturn ^= 1;
+        }
       }
-      j += n;
     }
     commit(drain);  // no MMA may be in flight when TMEM is released
     mbar_wait(drain, 0, status, nullptr);
     __syncwarp();
-  } else {
+  } else if (warp < kChunkMma) {
     // ------------------------------------------------------------ softmax + epilogue
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     const int t = warp >> 2;
     const int row = (warp & 3) * 32 + lane;  // TMEM lane == tile row
     const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t tO = tmem + lane_off + t * D;
     const uint32_t tS = tmem + lane_off + L::COL_S + 128 * t;
     const float sl2 = p.scale_log2;
-    int4 mine = make_int4(0, 0, 0, 0);
+    if (threadIdx.x == 0) p.desc[blockIdx.x] = make_int4(0, 0, 0, 0);
     uint32_t sj = 0, pieces = 0;  // tiles and pieces of this M-tile so far
     bool ok = true;
-    while (ok && walk.next(p, x)) {
-      if (x.parts > 0) mine = paged_desc(x, min(kChunkRows, x.q.qlen * p.rep - x.qt * kChunkRows));
+    while (ok && next_piece(p, role)) {
+      if (x.parts > 0 && threadIdx.x == 0)
+        p.desc[blockIdx.x] = paged_desc(x, min(kChunkRows, x.q.qlen * p.rep - x.qt * kChunkRows));
       const int rows = min(128, x.q.qlen * p.rep - x.qt * kChunkRows - t * 128);
       if (rows <= 0) continue;
       const int r0 = x.qt * kChunkRows + t * 128;  // the tile's first row in the sequence
@@ -295,10 +340,11 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         fence_proxy_async_smem();
         mbar_arrive(&q_full[t]);
       }
-      const int seen = min(x.q.first + (r0 + row) / p.rep + 1, x.keys);  // keys this row sees
+      // Columns of the piece's first key tile that this row sees; each tile further leaves 128 fewer.
+      int lim = min(x.q.first + (r0 + row) / p.rep + 1, x.keys) - x.t0 * kChunkKeys;
       float m_used = -INFINITY;  // reference max (log2 units) the exponentials use
       float l = 0.0f;
-      for (int j = 0; j < n; ++j, ++sj) {
+      for (int j = 0; j < n; ++j, ++sj, lim -= kChunkKeys) {
         ok = __all_sync(0xffffffffu, mbar_wait(&s_full[t], sj & 1, status, abort_flag));
         if (!ok) break;
         tc_fence_after();
@@ -306,7 +352,6 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
 #pragma unroll
         for (int q = 0; q < 4; ++q) tmem_ld32(tS + 32 * q, s[q]);
         tmem_wait_ld();
-        const int lim = seen - (x.t0 + j) * kChunkKeys;  // columns below it are seen
         const bool masked = __any_sync(0xffffffffu, lim < kChunkKeys);
         if (masked) {
 #pragma unroll
@@ -443,7 +488,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       }
       tc_fence_before();  // O and S are read before the next piece's MMAs, which wait for its Q
     }
-    if (threadIdx.x == 0) p.desc[blockIdx.x] = mine;
+  } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");  // the last warp only fills its warpgroup
   }
 
   tc_fence_before();
@@ -494,7 +540,7 @@ static cudaError_t launch_chunk(const PagedArgs& a, int dtype, int G, cudaStream
   static std::atomic<uint64_t> done{0};
   cudaError_t e = allow_smem(reinterpret_cast<const void*>(kern), L::BYTES, done);
   if (e != cudaSuccess) return e;
-  const PagedParams p = paged_params(a, kChunkRows, G, 1);
+  const PagedParams p = paged_params(a, kChunkRows, G, 8);
   kern<<<G, kChunkThreads, L::BYTES, stream>>>(mk, mv, p, box);
   e = cudaGetLastError();
   return e != cudaSuccess ? e : launch_paged_join<T>(p, kChunkRows, G, kChunkKeys, stream);

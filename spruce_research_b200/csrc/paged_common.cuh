@@ -23,7 +23,7 @@ struct PagedParams {
   PagedArgs a;
   int rep, row_tiles;     // Hq / Hkv; row tiles of the longest sequence allowed
   int kv_cap;             // keys a sequence may hold: min(max_kv, max_pages * page_size)
-  int min_tiles;          // shortest run
+  int unit_cost;          // of starting and ending a unit, in key tiles
   int4* desc;             // [G] split unit whose first part is the run's last: {first token, qt, g, parts | slot << 12 | rows << 16}
   float2* part_ml;        // [2 G][R] softmax maximum (log2 units) and sum
   float* part_o;          // [2 G][R][D]
@@ -46,7 +46,8 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedParams& p, int s) {
   return q;
 }
 
-// Keys that row tile qt sees (its last token's), and the tiles it counts as (an empty one still writes zeros).
+// Keys that row tile qt sees (its last token's), and the tiles it counts as (an empty one still writes zeros):
+// its key tiles and, after them, the fixed cost of a unit.
 template <int R>
 __device__ __forceinline__ int paged_keys(const PagedParams& p, const PagedSeq& q, int qt) {
   const int last_row = min((qt + 1) * R, q.qlen * p.rep) - 1;
@@ -54,7 +55,7 @@ __device__ __forceinline__ int paged_keys(const PagedParams& p, const PagedSeq& 
 }
 template <int R, int TK>
 __device__ __forceinline__ int paged_weight(const PagedParams& p, const PagedSeq& q, int qt) {
-  return max(1, (paged_keys<R>(p, q, qt) + TK - 1) / TK);
+  return max(1, (paged_keys<R>(p, q, qt) + TK - 1) / TK) + p.unit_cost;
 }
 
 // A piece of a unit that this CTA computes: key tiles [t0, t1) of n.
@@ -85,31 +86,34 @@ struct PagedWalk {
   bool head;        // the next piece begins the run
 
   __device__ __forceinline__ bool next(const PagedParams& p, PagedPiece& x) {
-    if (left <= 0) return false;
-    for (;;) {  // the next sequence with rows; one exists while tiles are left
-      if (s >= p.a.S) return false;
-      x.q = paged_seq(p, s);
-      if (qt * R < x.q.qlen * p.rep) break;
-      ++s;
-      qt = 0;
+    while (left > 0) {
+      for (;;) {  // the next sequence with rows; one exists while tiles are left
+        if (s >= p.a.S) return false;
+        x.q = paged_seq(p, s);
+        if (qt * R < x.q.qlen * p.rep) break;
+        ++s;
+        qt = 0;
+      }
+      x.s = s;
+      x.qt = qt;
+      x.g = g;
+      x.keys = paged_keys<R>(p, x.q, qt);
+      x.n = max(1, (x.keys + TK - 1) / TK);
+      const int take = static_cast<int>(min((int64_t)(x.n + p.unit_cost), t + left)) - t;
+      x.t0 = t;
+      x.t1 = min(x.n, t + take);
+      x.slot = x.t0 == 0 && x.t1 == x.n ? -1 : (head ? 0 : 1);
+      x.parts = x.t0 == 0 && x.t1 < x.n ? 1 + static_cast<int>((x.n - x.t1 + run - 1) / run) : 0;
+      left -= take;
+      head = false;
+      t = 0;
+      if (++g == p.a.Hkv) {
+        g = 0;
+        ++qt;
+      }
+      if (x.t0 < x.n) return true;  // else the run begins in the unit's fixed cost: nothing to do
     }
-    x.s = s;
-    x.qt = qt;
-    x.g = g;
-    x.keys = paged_keys<R>(p, x.q, qt);
-    x.n = max(1, (x.keys + TK - 1) / TK);
-    x.t0 = t;
-    x.t1 = static_cast<int>(min((int64_t)x.n, t + left));
-    left -= x.t1 - x.t0;
-    x.slot = x.t0 == 0 && x.t1 == x.n ? -1 : (head ? 0 : 1);
-    x.parts = x.t0 == 0 && x.t1 < x.n ? 1 + static_cast<int>((x.n - x.t1 + run - 1) / run) : 0;
-    head = false;
-    t = 0;
-    if (++g == p.a.Hkv) {
-      g = 0;
-      ++qt;
-    }
-    return true;
+    return false;
   }
 };
 
@@ -165,7 +169,7 @@ __device__ __forceinline__ bool paged_run(const PagedParams& p, PagedWalk<R, TK>
       b0 = before;
     }
   }
-  const int64_t run = max((int64_t)p.min_tiles, (total + G - 1) / G);
+  const int64_t run = max((int64_t)1, (total + G - 1) / G);
   const int64_t start = c * run;
   w.run = run;
   w.left = min(run, total - start);
@@ -249,7 +253,7 @@ template <typename T>
 cudaError_t launch_paged_join(const PagedParams& p, int R, int G, int TK, cudaStream_t stream);
 
 // Parameters of a launch with R-row tiles on at most G CTAs, its workspace carved up.
-inline PagedParams paged_params(const PagedArgs& a, int R, int G, int min_tiles) {
+inline PagedParams paged_params(const PagedArgs& a, int R, int G, int unit_cost) {
   PagedParams p;
   p.a = a;
   p.rep = a.Hq / a.Hkv;
@@ -257,7 +261,7 @@ inline PagedParams paged_params(const PagedArgs& a, int R, int G, int min_tiles)
   int64_t cap = (int64_t)a.max_pages * a.page_size;
   cap = cap < a.max_kv ? cap : a.max_kv;
   p.kv_cap = static_cast<int>(cap < (1 << 30) ? cap : 1 << 30);  // key indices stay ints with room for a tile more
-  p.min_tiles = min_tiles;
+  p.unit_cost = unit_cost;
   uint8_t* ws = static_cast<uint8_t*>(a.workspace);
   p.desc = reinterpret_cast<int4*>(ws);
   ws += ((int64_t)G * 16 + 255) / 256 * 256;
