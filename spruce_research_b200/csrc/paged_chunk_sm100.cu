@@ -8,7 +8,7 @@
 //
 // Warps: 0-3 softmax and epilogue of tile 0 (thread = row = TMEM lane), 4-7 of tile 1, 8 loads K and V, 9 issues the MMAs
 // and owns TMEM.  The softmax warps also bring in their own Q rows (once a unit).  O_0 O_1 S_0 S_1 fill TMEM's columns; P_t
-// is written over the first half of S_t.  One thread issues QK_0(j) PV_1(j-1) QK_1(j) PV_0(j) ..., in whose order they
+// is written over the first half of S_t.  One thread issues PV_0(j) QK_0(j+1) PV_1(j) QK_1(j+1) ..., in whose order they
 // execute, so QK_t(j+1) overwrites P_t(j) after PV_t(j) has read it, and while one tile's softmax runs the tensor core
 // works for the other.  P is announced in halves of 64 keys, so PV starts on the first while the second is
 // exponentiated.  O is rescaled only when the running maximum grew by more than 8 (log2 units): P stays below
@@ -243,59 +243,70 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       }
       commit(&s_full[t]);
     };
-    uint32_t np_[2] = {0, 0};  // PVs issued for each tile
-    auto pv = [&](int t, int st, bool first) {
-      for (int h = 0; h < 2; ++h) {
-        if (!wait(&p_full[2 * t + h], np_[t] & 1)) return false;
-        tc_fence_after();
-        const uint32_t a = tmem + L::COL_S + 128 * t;
-        const uint64_t vb = dv0 + (uint64_t)((st * L::TILE) >> 4);
+    uint32_t pvs[2] = {0, 0};  // PVs issued for each tile
+    auto pv_half = [&](int t, int st, int h, bool first) {
+      if (!wait(&p_full[2 * t + h], pvs[t] & 1)) return false;
+      tc_fence_after();
+      const uint32_t a = tmem + L::COL_S + 128 * t;
+      const uint64_t vb = dv0 + (uint64_t)((st * L::TILE) >> 4);
 #pragma unroll
-        for (int kk = 0; kk < 4; ++kk) {
-          const int ks = 4 * h + kk;
-          if (leader)
-            umma_f16_ts(tmem + t * D, a + ks * 8, vb + (uint64_t)((ks * 2048) >> 4), idesc_pv,
-                        (!first || ks > 0) ? 1u : 0u);
-          __syncwarp();
-        }
+      for (int kk = 0; kk < 4; ++kk) {
+        const int ks = 4 * h + kk;
+        if (leader)
+          umma_f16_ts(tmem + t * D, a + ks * 8, vb + (uint64_t)((ks * 2048) >> 4), idesc_pv,
+                      (!first || ks > 0) ? 1u : 0u);
+        __syncwarp();
       }
-      ++np_[t];
+      if (h == 1) ++pvs[t];
       return true;
     };
     uint32_t pieces[2] = {0, 0};
     int kst = 0, vst = 0;            // stages of the next K and V tile, and the parities of their turns
     uint32_t kturn = 0, vturn = 0;
     bool ok = true;
+    auto next_k = [&] {
+      if (++kst == KST) {
+        kst = 0;
+        kturn ^= 1;
+      }
+    };
     while (ok && next_piece(p, role)) {
       const bool two = x.q.qlen * p.rep - x.qt * kChunkRows > 128;
       if (x.keys == 0) continue;
       const int n = x.t1 - x.t0;
-      ok = wait(&q_full[0], pieces[0]++ & 1) && (!two || wait(&q_full[1], pieces[1]++ & 1));
-      int vlast = 0;                 // V stage of tile i - 1
-      for (int i = 0; ok && i <= n; ++i) {
-        if (i < n) {
-          if (!(ok = wait(&k_full[kst], kturn))) break;
-          tc_fence_after();
+      ok = wait(&q_full[0], pieces[0]++ & 1) && (!two || wait(&q_full[1], pieces[1]++ & 1)) &&
+           wait(&k_full[kst], kturn);
+      if (!ok) break;
+      tc_fence_after();
+      issue_qk(0, kst);
+      if (two) issue_qk(1, kst);
+      commit(&k_empty[kst]);
+      next_k();
+      for (int i = 0; i < n; ++i) {
+        // A check of a barrier waits behind this warp's queued MMAs, so what PV_t(i) and QK_t(i+1) need is checked
+        // before them and they are issued without a pause.
+        const bool more = i + 1 < n;
+        if (!(ok = wait(&v_full[vst], vturn) && (!more || wait(&k_full[kst], kturn)))) break;
+        if (!(ok = pv_half(0, vst, 0, i == 0) && pv_half(0, vst, 1, i == 0))) break;
+        if (more)
           issue_qk(0, kst);
+        else
+          commit(&o_done[0]);
+        if (two) {
+          if (!(ok = pv_half(1, vst, 0, i == 0) && pv_half(1, vst, 1, i == 0))) break;
+          if (more)
+            issue_qk(1, kst);
+          else
+            commit(&o_done[1]);
         }
-        if (i > 0 && two) {
-          if (!(ok = pv(1, vlast, i == 1))) break;
-          if (i == n) commit(&o_done[1]);
-        }
-        if (i > 0) commit(&v_empty[vlast]);  // every MMA reading that stage is issued before this
-        if (i == n) break;
-        if (two) issue_qk(1, kst);
-        commit(&k_empty[kst]);
-        if (++kst == KST) {
-          kst = 0;
-          kturn ^= 1;
-        }
-        if (!(ok = wait(&v_full[vst], vturn) && pv(0, vst, i == 0))) break;
-        if (i == n - 1) commit(&o_done[0]);
-        vlast = vst;
+        commit(&v_empty[vst]);  // every MMA reading these stages is issued before this
         if (++vst == VST) {
           vst = 0;
           vturn ^= 1;
+        }
+        if (more) {
+          commit(&k_empty[kst]);
+          next_k();
         }
       }
     }
