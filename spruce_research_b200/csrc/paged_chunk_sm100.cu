@@ -353,20 +353,29 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       const int r0 = x.qt * kChunkRows + t * 128;  // the tile's first row in the sequence
       const int n = x.keys == 0 ? 0 : x.t1 - x.t0;
       if (n > 0) {
-        // This warp's 32 rows of Q into the swizzled layout (rows past the end: zeros).
+        // This warp's 32 rows of Q into the swizzled layout (rows past the end: zeros), eight loads in flight a lane.
         constexpr int CH = D / 8;  // 16-byte chunks of a row
         uint8_t* qs = smem + L::OFF_Q + t * L::TILE;
-#pragma unroll 4
-        for (int e = lane; e < 32 * CH; e += 32) {
-          const int r = (warp & 3) * 32 + e / CH, c = e % CH;
-          uint4 v = make_uint4(0, 0, 0, 0);
-          if (r < rows) {
-            int64_t tok;
-            int head;
-            paged_row(p, x, r0 + r, tok, head);
-            v = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.a.q) + tok * p.a.qn + head * p.a.qh + c * 8);
+        const int c = lane % CH;
+#pragma unroll 1
+        for (int e0 = 0; e0 < CH; e0 += 8) {
+          uint4 v[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const int r = (warp & 3) * 32 + (e0 + e) * (32 / CH) + lane / CH;
+            v[e] = make_uint4(0, 0, 0, 0);
+            if (r < rows) {
+              int64_t tok;
+              int head;
+              paged_row(p, x, r0 + r, tok, head);
+              v[e] = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.a.q) + tok * p.a.qn + head * p.a.qh + c * 8);
+            }
           }
-          *reinterpret_cast<uint4*>(qs + (c >> 3) * L::PANEL + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const int r = (warp & 3) * 32 + (e0 + e) * (32 / CH) + lane / CH;
+            *reinterpret_cast<uint4*>(qs + (c >> 3) * L::PANEL + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v[e];
+          }
         }
         fence_proxy_async_smem();
         mbar_arrive(&q_full[t]);
@@ -469,48 +478,66 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         if (!ok) break;
         tc_fence_after();
       }
+      // The rows leave through this warp's rows of the Q tile, whose MMAs are complete: 128 bytes of each row a round,
+      // written row by thread and read back row by eight lanes, so that a store covers whole lines.
       const bool whole = x.slot < 0;
       const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-      T* dst = nullptr;
-      float* part_o = nullptr;
+      uint8_t* dst = nullptr;  // this row in the output, or among the parts
       if (row < rows) {
         if (whole) {
           int64_t tok;
           int head;
           paged_row(p, x, r0 + row, tok, head);
-          dst = static_cast<T*>(p.a.out) + tok * p.a.on + head * p.a.oh;
+          dst = reinterpret_cast<uint8_t*>(static_cast<T*>(p.a.out) + tok * p.a.on + head * p.a.oh);
         } else {
           const int64_t at = (int64_t)(2 * blockIdx.x + x.slot) * kChunkRows + t * 128 + row;
           p.part_ml[at] = make_float2(m_used, l);
-          part_o = p.part_o + at * D;
+          dst = reinterpret_cast<uint8_t*>(p.part_o + at * D);
         }
       }
+      uint8_t* const stage = smem + L::OFF_Q + t * L::TILE + (warp & 3) * 32 * 128;
+      const int rounds = whole ? D / 64 : D / 32;
 #pragma unroll 1
-      for (int cc = 0; cc < D / 32; ++cc) {
+      for (int c0 = 0; c0 < rounds; ++c0) {
+        uint4 v[8];
         float o[32];
-        if (n > 0) {
-          tmem_ld32(tO + cc * 32, o);
-          tmem_wait_ld();
-        } else {
+        if (whole) {
 #pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = 0.0f;
-        }
-        if (dst != nullptr) {
+          for (int half = 0; half < 2; ++half) {
+            if (n > 0) {
+              tmem_ld32(tO + c0 * 64 + half * 32, o);
+              tmem_wait_ld();
+            }
 #pragma unroll
-          for (int v4 = 0; v4 < 4; ++v4) {
-            uint4 v;
-            v.x = Pack2<T>::pack(o[v4 * 8 + 0] * inv, o[v4 * 8 + 1] * inv);
-            v.y = Pack2<T>::pack(o[v4 * 8 + 2] * inv, o[v4 * 8 + 3] * inv);
-            v.z = Pack2<T>::pack(o[v4 * 8 + 4] * inv, o[v4 * 8 + 5] * inv);
-            v.w = Pack2<T>::pack(o[v4 * 8 + 6] * inv, o[v4 * 8 + 7] * inv);
-            *reinterpret_cast<uint4*>(dst + cc * 32 + v4 * 8) = v;
+            for (int e = 0; e < 4; ++e) {
+              v[half * 4 + e].x = Pack2<T>::pack(o[e * 8 + 0] * inv, o[e * 8 + 1] * inv);
+              v[half * 4 + e].y = Pack2<T>::pack(o[e * 8 + 2] * inv, o[e * 8 + 3] * inv);
+              v[half * 4 + e].z = Pack2<T>::pack(o[e * 8 + 4] * inv, o[e * 8 + 5] * inv);
+              v[half * 4 + e].w = Pack2<T>::pack(o[e * 8 + 6] * inv, o[e * 8 + 7] * inv);
+              if (n == 0) v[half * 4 + e] = make_uint4(0, 0, 0, 0);  // no key seen: O was not written
+            }
           }
-        } else if (part_o != nullptr) {
+        } else {
+          tmem_ld32(tO + c0 * 32, o);
+          tmem_wait_ld();
 #pragma unroll
-          for (int v4 = 0; v4 < 8; ++v4)
-            *reinterpret_cast<float4*>(part_o + cc * 32 + v4 * 4) =
-                make_float4(o[v4 * 4], o[v4 * 4 + 1], o[v4 * 4 + 2], o[v4 * 4 + 3]);
+          for (int e = 0; e < 8; ++e)
+            v[e] = make_uint4(__float_as_uint(o[e * 4]), __float_as_uint(o[e * 4 + 1]), __float_as_uint(o[e * 4 + 2]),
+                              __float_as_uint(o[e * 4 + 3]));
         }
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          *reinterpret_cast<uint4*>(stage + lane * 128 + ((e ^ (lane & 7)) << 4)) = v[e];
+        __syncwarp();
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int r = e * 4 + (lane >> 3);
+          const uint4 y = *reinterpret_cast<const uint4*>(stage + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
+          uint8_t* const to = reinterpret_cast<uint8_t*>(
+              __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(dst), r));
+          if (to != nullptr) *reinterpret_cast<uint4*>(to + c0 * 128 + (lane & 7) * 16) = y;
+        }
+        __syncwarp();
       }
       tc_fence_before();  // O and S are read before the next piece's MMAs, which wait for its Q
     }
@@ -566,7 +593,7 @@ static cudaError_t launch_chunk(const PagedArgs& a, int dtype, int G, cudaStream
   static std::atomic<uint64_t> done{0};
   cudaError_t e = allow_smem(reinterpret_cast<const void*>(kern), L::BYTES, done);
   if (e != cudaSuccess) return e;
-  const PagedParams p = paged_params(a, kChunkRows, G, 8);
+  const PagedParams p = paged_params(a, kChunkRows, G, 5);
   kern<<<G, kChunkThreads, L::BYTES, stream>>>(mk, mv, p, box);
   e = cudaGetLastError();
   return e != cudaSuccess ? e : launch_paged_join<T>(p, kChunkRows, G, kChunkKeys, stream);

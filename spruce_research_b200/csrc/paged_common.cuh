@@ -196,12 +196,26 @@ __device__ __forceinline__ bool paged_run(const PagedParams& p, PagedWalk<R, TK>
   w.s = s_seq;
   int64_t rest = start - s_before;
   const PagedSeq q = paged_seq(p, w.s);
+  // The row tile that holds it: every warp looks at 32 of them at a time.
+  const int lane = threadIdx.x & 31;
+  const int tiles = (q.qlen * p.rep + R - 1) / R;
   w.qt = 0;
-  for (;;) {
-    const int64_t n = (int64_t)paged_weight<R, TK>(p, q, w.qt) * p.a.Hkv;
-    if (rest < n) break;
-    rest -= n;
-    ++w.qt;
+  for (int base = 0; base < tiles; base += 32) {
+    const int64_t v = base + lane < tiles ? (int64_t)paged_weight<R, TK>(p, q, base + lane) * p.a.Hkv : 0;
+    int64_t inc = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t y = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += y;
+    }
+    const unsigned past = __ballot_sync(0xffffffffu, rest < inc);
+    if (past != 0) {
+      const int at = __ffs(past) - 1;
+      w.qt = base + at;
+      rest -= __shfl_sync(0xffffffffu, inc - v, at);
+      break;
+    }
+    rest -= __shfl_sync(0xffffffffu, inc, 31);
   }
   const int n = paged_weight<R, TK>(p, q, w.qt);
   w.g = static_cast<int>(rest / n);
