@@ -29,6 +29,9 @@
 
 namespace spruce {
 
+// Starting and ending a unit takes about 16,000 cycles, five or six of the 3,200 a key tile takes (swept 2 - 8: a 16K
+// prompt, whose first units have one tile, 2.01 / 1.82 / 1.66 / 1.59 / 1.58 ms at 2 / 3 / 4 / 5 / 6; nothing else moves).
+constexpr int kChunkUnitCost = 6;
 constexpr int kChunkThreads = 384;
 constexpr int kChunkMma = 8;
 constexpr int kChunkLoadK = 9;
@@ -353,29 +356,26 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       const int r0 = x.qt * kChunkRows + t * 128;  // the tile's first row in the sequence
       const int n = x.keys == 0 ? 0 : x.t1 - x.t0;
       if (n > 0) {
-        // This warp's 32 rows of Q into the swizzled layout (rows past the end: zeros), eight loads in flight a lane.
+        // This warp's 32 rows of Q into the swizzled layout (rows past the end: zeros), all its loads in flight at once.
         constexpr int CH = D / 8;  // 16-byte chunks of a row
         uint8_t* qs = smem + L::OFF_Q + t * L::TILE;
         const int c = lane % CH;
-#pragma unroll 1
-        for (int e0 = 0; e0 < CH; e0 += 8) {
-          uint4 v[8];
+        uint4 v[CH];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const int r = (warp & 3) * 32 + (e0 + e) * (32 / CH) + lane / CH;
-            v[e] = make_uint4(0, 0, 0, 0);
-            if (r < rows) {
-              int64_t tok;
-              int head;
-              paged_row(p, x, r0 + r, tok, head);
-              v[e] = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.a.q) + tok * p.a.qn + head * p.a.qh + c * 8);
-            }
+        for (int e = 0; e < CH; ++e) {
+          const int r = (warp & 3) * 32 + e * (32 / CH) + lane / CH;
+          v[e] = make_uint4(0, 0, 0, 0);
+          if (r < rows) {
+            int64_t tok;
+            int head;
+            paged_row(p, x, r0 + r, tok, head);
+            v[e] = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.a.q) + tok * p.a.qn + head * p.a.qh + c * 8);
           }
+        }
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const int r = (warp & 3) * 32 + (e0 + e) * (32 / CH) + lane / CH;
-            *reinterpret_cast<uint4*>(qs + (c >> 3) * L::PANEL + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v[e];
-          }
+        for (int e = 0; e < CH; ++e) {
+          const int r = (warp & 3) * 32 + e * (32 / CH) + lane / CH;
+          *reinterpret_cast<uint4*>(qs + (c >> 3) * L::PANEL + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v[e];
         }
         fence_proxy_async_smem();
         mbar_arrive(&q_full[t]);
@@ -496,35 +496,16 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         }
       }
       uint8_t* const stage = smem + L::OFF_Q + t * L::TILE + (warp & 3) * 32 * 128;
-      const int rounds = whole ? D / 64 : D / 32;
-#pragma unroll 1
-      for (int c0 = 0; c0 < rounds; ++c0) {
-        uint4 v[8];
-        float o[32];
-        if (whole) {
+      float o[D];
+      if (n > 0) {
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            if (n > 0) {
-              tmem_ld32(tO + c0 * 64 + half * 32, o);
-              tmem_wait_ld();
-            }
+        for (int cc = 0; cc < D / 32; ++cc) tmem_ld32(tO + cc * 32, *reinterpret_cast<float(*)[32]>(o + cc * 32));
+        tmem_wait_ld();
+      } else {  // no key seen: O was not written
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              v[half * 4 + e].x = Pack2<T>::pack(o[e * 8 + 0] * inv, o[e * 8 + 1] * inv);
-              v[half * 4 + e].y = Pack2<T>::pack(o[e * 8 + 2] * inv, o[e * 8 + 3] * inv);
-              v[half * 4 + e].z = Pack2<T>::pack(o[e * 8 + 4] * inv, o[e * 8 + 5] * inv);
-              v[half * 4 + e].w = Pack2<T>::pack(o[e * 8 + 6] * inv, o[e * 8 + 7] * inv);
-              if (n == 0) v[half * 4 + e] = make_uint4(0, 0, 0, 0);  // no key seen: O was not written
-            }
-          }
-        } else {
-          tmem_ld32(tO + c0 * 32, o);
-          tmem_wait_ld();
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            v[e] = make_uint4(__float_as_uint(o[e * 4]), __float_as_uint(o[e * 4 + 1]), __float_as_uint(o[e * 4 + 2]),
-                              __float_as_uint(o[e * 4 + 3]));
-        }
+        for (int d = 0; d < D; ++d) o[d] = 0.0f;
+      }
+      auto send = [&](int round, const uint4 (&v)[8]) {
 #pragma unroll
         for (int e = 0; e < 8; ++e)
           *reinterpret_cast<uint4*>(stage + lane * 128 + ((e ^ (lane & 7)) << 4)) = v[e];
@@ -535,9 +516,32 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
           const uint4 y = *reinterpret_cast<const uint4*>(stage + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
           uint8_t* const to = reinterpret_cast<uint8_t*>(
               __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(dst), r));
-          if (to != nullptr) *reinterpret_cast<uint4*>(to + c0 * 128 + (lane & 7) * 16) = y;
+          if (to != nullptr) *reinterpret_cast<uint4*>(to + round * 128 + (lane & 7) * 16) = y;
         }
         __syncwarp();
+      };
+      uint4 v[8];
+      if (whole) {
+#pragma unroll
+        for (int round = 0; round < D / 64; ++round) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float* f = o + round * 64 + e * 8;
+            v[e] = make_uint4(Pack2<T>::pack(f[0] * inv, f[1] * inv), Pack2<T>::pack(f[2] * inv, f[3] * inv),
+                              Pack2<T>::pack(f[4] * inv, f[5] * inv), Pack2<T>::pack(f[6] * inv, f[7] * inv));
+          }
+          send(round, v);
+        }
+      } else {
+#pragma unroll
+        for (int round = 0; round < D / 32; ++round) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float* f = o + round * 32 + e * 4;
+            v[e] = make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+          }
+          send(round, v);
+        }
       }
       tc_fence_before();  // O and S are read before the next piece's MMAs, which wait for its Q
     }
@@ -593,7 +597,7 @@ static cudaError_t launch_chunk(const PagedArgs& a, int dtype, int G, cudaStream
   static std::atomic<uint64_t> done{0};
   cudaError_t e = allow_smem(reinterpret_cast<const void*>(kern), L::BYTES, done);
   if (e != cudaSuccess) return e;
-  const PagedParams p = paged_params(a, kChunkRows, G, 5);
+  const PagedParams p = paged_params(a, kChunkRows, G, kChunkUnitCost);
   kern<<<G, kChunkThreads, L::BYTES, stream>>>(mk, mv, p, box);
   e = cudaGetLastError();
   return e != cudaSuccess ? e : launch_paged_join<T>(p, kChunkRows, G, kChunkKeys, stream);
