@@ -4,11 +4,7 @@
 // For a query row q at position i: o = sum_j p_j v_j / sum_j p_j, p_j = 2^(q.k_j scale log2(e) - m), j <= i, over
 // key tiles in one pass with the running maximum m and sum.  Rows that see nothing are zero.  Cache rows at or past
 // the sequence's length are never loaded.
-//
-// A CTA of 256 threads holds R query rows and TK keys in shared memory as fp32; a thread forms TR x TC scores, then
-// TR rows x D / NC output dims.
 #include <algorithm>
-#include <climits>
 
 #include "attn_common.cuh"
 #include "paged_common.cuh"
@@ -26,31 +22,88 @@ static int sm_count() {
   return n > 0 ? n : 148;
 }
 
-template <int D, int R, int TK, int TR, int TC>
-__global__ void __launch_bounds__(256) paged_attn_f32_kernel(const PagedParams p) {
-  constexpr int NC = TK / TC;       // threads along the keys, and along D
-  constexpr int KP = D + 4;         // padded rows: float4 reads of adjacent keys hit distinct banks
-  constexpr int DV = D / NC;
-  constexpr int VN = 4;             // floats of a 16-byte load
-  static_assert((R / TR) * NC == 256 && NC <= 32, "256 threads");
+__device__ __forceinline__ void copy16_or_zero(float* dst, const float* src, bool in) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(in ? 16 : 0)
+               : "memory");
+}
+
+template <int D, int R, int TK, int STAGES>
+struct F32Layout {
+  static constexpr int TR = R == 64 ? 4 : 2, TC = R == 64 ? 4 : 2;  // rows and keys of a thread's scores
+  static constexpr int NC = TK / TC;                               // threads along the keys, and along D
+  static constexpr int THREADS = R / TR * NC;
+  static constexpr int KP = D + 4;    // padded rows: float4 reads of adjacent keys hit distinct banks
+  static constexpr int PP = TK + 4;
+  static constexpr int STAGE = TK * KP + TK * D;
+  // One stage: the probabilities take the place of the keys they were formed from.
+  static constexpr int FLOATS = R * D + STAGES * STAGE + (STAGES == 1 ? 0 : R * PP);
+  static_assert(STAGES > 1 || R * PP <= TK * KP, "probabilities fit over the keys");
+  static_assert(NC == 16, "half a warp a row group");
+};
+
+// A CTA holds R query rows and STAGES tiles of TK keys in shared memory; a thread forms TR x TC scores, then TR rows x
+// D / NC output dims.  Chunks are bound by the FMA pipe (4 x 4 scores a thread: 12 shared-memory wavefronts to 64
+// FMAs), with two CTAs an SM one of which loads while the other computes.  Few rows are bound by HBM on paper and in
+// practice by shared-memory reads (every key is read once a row group), so they take as few row groups as hold them,
+// eight or sixteen rows, and keep two tiles in flight.
+template <int D, int R, int TK, int STAGES>
+__global__ void __launch_bounds__(F32Layout<D, R, TK, STAGES>::THREADS) paged_attn_f32_kernel(const PagedParams p) {
+  using L = F32Layout<D, R, TK, STAGES>;
+  constexpr int TR = L::TR, TC = L::TC, NC = L::NC, KP = L::KP, PP = L::PP, THREADS = L::THREADS;
+  constexpr int DV = D / (4 * NC);  // float4s of an output row a thread holds, 4 NC dims apart
+  constexpr int CH = D / 4;
   extern __shared__ float fsm[];
-  float* Qs = fsm;                  // [R][D]
-  float* Ks = Qs + R * D;           // [TK][KP]
-  float* Vs = Ks + TK * KP;         // [TK][D]
-  float* Ps = Vs + TK * D;          // [R][TK + 1]
+  float* Qs = fsm;                   // [R][D]
+  float* KVs = Qs + R * D;           // [STAGES]: [TK][KP], [TK][D]
+  float* Ps = STAGES == 1 ? KVs : KVs + STAGES * L::STAGE;  // [R][PP]
   __shared__ int64_t scratch[33];
 
   const int tid = threadIdx.x;
   const int rg = tid / NC, cg = tid % NC;
   PagedWalk<R, TK> walk;
-  const bool any = paged_run<R, TK, 256>(p, walk, scratch);
+  const bool any = paged_run<R, TK, THREADS>(p, walk, scratch);
   int4 mine = make_int4(0, 0, 0, 0);
   PagedPiece x;
   while (any && walk.next(p, x)) {
     const int rows = min(R, x.q.qlen * p.rep - x.qt * R);
+    const int n = x.keys > 0 ? x.t1 - x.t0 : 0;
+    const int32_t* table = p.a.block_table + x.s * p.a.table_stride;
+    // Tile i of the piece into its stage: rows past the keys, or of no page, are zeros.
+    auto load = [&](int i) {
+      if (i < n) {
+        float* ks = KVs + i % STAGES * L::STAGE;
+        float* vs = ks + TK * KP;
+        const int key0 = (x.t0 + i) * TK, d = tid % CH * 4;
+#pragma unroll 1
+        for (int r0 = 0; r0 < TK; r0 += 16) {  // sixteen keys lie in one page
+          const int key = key0 + r0, pi = key / p.a.page_size;
+          const int64_t page = key < x.keys ? paged_page(p, table, pi) : -1;
+          const int64_t row = key - pi * p.a.page_size + tid / CH;
+          const float* k = static_cast<const float*>(p.a.kc);
+          const float* v = static_cast<const float*>(p.a.vc);
+          if (page >= 0) {
+            k += page * p.a.ks[0] + x.g * p.a.ks[1] + row * p.a.ks[2] + d;
+            v += page * p.a.vs[0] + x.g * p.a.vs[1] + row * p.a.vs[2] + d;
+          }
+#pragma unroll
+          for (int r = tid / CH; r < 16; r += THREADS / CH) {
+            const bool in = page >= 0 && key + r < x.keys;
+            copy16_or_zero(ks + (r0 + r) * KP + d, k, in);
+            copy16_or_zero(vs + (r0 + r) * D + d, v, in);
+            if (in) {
+              k += THREADS / CH * p.a.ks[2];
+              v += THREADS / CH * p.a.vs[2];
+            }
+          }
+        }
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
     __syncthreads();
-    for (int e = tid; e < R * (D / VN); e += 256) {
-      const int r = e / (D / VN), d = e % (D / VN) * VN;
+#pragma unroll
+    for (int i = 0; i + 1 < STAGES; ++i) load(i);
+    for (int e = tid; e < R * CH; e += THREADS) {
+      const int r = e / CH, d = e % CH * 4;
       float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
       if (r < rows) {
         int64_t tok;
@@ -60,7 +113,8 @@ __global__ void __launch_bounds__(256) paged_attn_f32_kernel(const PagedParams p
       }
       *reinterpret_cast<float4*>(Qs + r * D + d) = v;
     }
-    float o[TR][DV], m[TR], l[TR];
+    float4 o[TR][DV];
+    float m[TR], l[TR];
     int seen[TR];  // keys the row sees
 #pragma unroll
     for (int i = 0; i < TR; ++i) {
@@ -69,30 +123,15 @@ __global__ void __launch_bounds__(256) paged_attn_f32_kernel(const PagedParams p
       const int r = x.qt * R + rg * TR + i;
       seen[i] = min(x.q.first + r / p.rep + 1, x.keys);
 #pragma unroll
-      for (int d = 0; d < DV; ++d) o[i][d] = 0.0f;
+      for (int d = 0; d < DV; ++d) o[i][d] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     }
-    const int32_t* table = p.a.block_table + x.s * p.a.table_stride;
-    for (int t = x.t0; t < x.t1 && x.keys > 0; ++t) {
+    for (int t = 0; t < n; ++t) {
+      load(t + STAGES - 1);  // into the stage that the last tile's readers have left
+      if constexpr (STAGES == 1) asm volatile("cp.async.wait_group 0;" ::: "memory");
+      else asm volatile("cp.async.wait_group 1;" ::: "memory");
       __syncthreads();
-      for (int e = tid; e < TK * (D / VN); e += 256) {
-        const int r = e / (D / VN), d = e % (D / VN) * VN;
-        const int key = t * TK + r;
-        float4 kk = make_float4(0.0f, 0.0f, 0.0f, 0.0f), vv = kk;
-        if (key < x.keys) {
-          const int pi = key / p.a.page_size;
-          const int64_t page = paged_page(p, table, pi);
-          const int64_t row = key - pi * p.a.page_size;
-          if (page >= 0) {
-            kk = *reinterpret_cast<const float4*>(static_cast<const float*>(p.a.kc) + page * p.a.ks[0] +
-                                                  x.g * p.a.ks[1] + row * p.a.ks[2] + d);
-            vv = *reinterpret_cast<const float4*>(static_cast<const float*>(p.a.vc) + page * p.a.vs[0] +
-                                                  x.g * p.a.vs[1] + row * p.a.vs[2] + d);
-          }
-        }
-        *reinterpret_cast<float4*>(Ks + r * KP + d) = kk;
-        *reinterpret_cast<float4*>(Vs + r * D + d) = vv;
-      }
-      __syncthreads();
+      const float* Ks = KVs + t % STAGES * L::STAGE;
+      const float* Vs = Ks + TK * KP;
       float s[TR][TC];
 #pragma unroll
       for (int i = 0; i < TR; ++i)
@@ -112,12 +151,13 @@ __global__ void __launch_bounds__(256) paged_attn_f32_kernel(const PagedParams p
             s[i][j] = fmaf(qv[i].x, kv[j].x,
                            fmaf(qv[i].y, kv[j].y, fmaf(qv[i].z, kv[j].z, fmaf(qv[i].w, kv[j].w, s[i][j]))));
       }
+      if constexpr (STAGES == 1) __syncthreads();
 #pragma unroll
       for (int i = 0; i < TR; ++i) {
         float mx = -INFINITY;
 #pragma unroll
         for (int j = 0; j < TC; ++j) {
-          s[i][j] = t * TK + cg + j * NC < seen[i] ? s[i][j] * p.scale_log2 : -INFINITY;
+          s[i][j] = (x.t0 + t) * TK + cg + j * NC < seen[i] ? s[i][j] * p.scale_log2 : -INFINITY;
           mx = fmaxf(mx, s[i][j]);
         }
 #pragma unroll
@@ -129,7 +169,7 @@ __global__ void __launch_bounds__(256) paged_attn_f32_kernel(const PagedParams p
 #pragma unroll
         for (int j = 0; j < TC; ++j) {
           const float e = exp2f(s[i][j] - ref);
-          Ps[(rg * TR + i) * (TK + 1) + cg + j * NC] = e;
+          Ps[(rg * TR + i) * PP + cg + j * NC] = e;
           sum += e;
         }
 #pragma unroll
@@ -137,40 +177,58 @@ __global__ void __launch_bounds__(256) paged_attn_f32_kernel(const PagedParams p
         l[i] = l[i] * alpha + sum;
         m[i] = m_new;
 #pragma unroll
-        for (int d = 0; d < DV; ++d) o[i][d] *= alpha;
-      }
-      __syncwarp();  // a row's probabilities are written and read by the same NC lanes
-#pragma unroll 4
-      for (int j = 0; j < TK; ++j) {
-        float pr[TR];
-#pragma unroll
-        for (int i = 0; i < TR; ++i) pr[i] = Ps[(rg * TR + i) * (TK + 1) + j];
-#pragma unroll
         for (int d = 0; d < DV; ++d) {
-          const float v = Vs[j * D + cg * DV + d];
-#pragma unroll
-          for (int i = 0; i < TR; ++i) o[i][d] = fmaf(pr[i], v, o[i][d]);
+          o[i][d].x *= alpha;
+          o[i][d].y *= alpha;
+          o[i][d].z *= alpha;
+          o[i][d].w *= alpha;
         }
       }
+      __syncwarp();  // a row's probabilities are written and read by the same NC lanes
+#pragma unroll 2
+      for (int j = 0; j < TK; j += 4) {
+        float4 pr[TR];
+#pragma unroll
+        for (int i = 0; i < TR; ++i) pr[i] = *reinterpret_cast<const float4*>(Ps + (rg * TR + i) * PP + j);
+#pragma unroll
+        for (int jj = 0; jj < 4; ++jj)
+#pragma unroll
+          for (int d = 0; d < DV; ++d) {
+            const float4 v = *reinterpret_cast<const float4*>(Vs + (j + jj) * D + (d * NC + cg) * 4);
+#pragma unroll
+            for (int i = 0; i < TR; ++i) {
+              const float w = jj == 0 ? pr[i].x : (jj == 1 ? pr[i].y : (jj == 2 ? pr[i].z : pr[i].w));
+              o[i][d].x = fmaf(w, v.x, o[i][d].x);
+              o[i][d].y = fmaf(w, v.y, o[i][d].y);
+              o[i][d].z = fmaf(w, v.z, o[i][d].z);
+              o[i][d].w = fmaf(w, v.w, o[i][d].w);
+            }
+          }
+      }
+      __syncthreads();
     }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
 #pragma unroll
     for (int i = 0; i < TR; ++i) {
       const int r = rg * TR + i;
       if (r >= rows) continue;
+      float* dst;
+      float f = 1.0f;
       if (x.slot < 0) {
         int64_t tok;
         int head;
         paged_row(p, x, x.qt * R + r, tok, head);
-        float* dst = static_cast<float*>(p.a.out) + tok * p.a.on + head * p.a.oh + cg * DV;
-        const float inv = l[i] > 0.0f ? 1.0f / l[i] : 0.0f;
-#pragma unroll
-        for (int d = 0; d < DV; ++d) dst[d] = o[i][d] * inv;
+        dst = static_cast<float*>(p.a.out) + tok * p.a.on + head * p.a.oh;
+        f = l[i] > 0.0f ? 1.0f / l[i] : 0.0f;
       } else {
         const int64_t at = (int64_t)(2 * blockIdx.x + x.slot) * R + r;
         if (cg == 0) p.part_ml[at] = make_float2(m[i], l[i]);
-#pragma unroll
-        for (int d = 0; d < DV; ++d) p.part_o[at * D + cg * DV + d] = o[i][d];
+        dst = p.part_o + at * D;
       }
+#pragma unroll
+      for (int d = 0; d < DV; ++d)
+        *reinterpret_cast<float4*>(dst + (d * NC + cg) * 4) =
+            make_float4(o[i][d].x * f, o[i][d].y * f, o[i][d].z * f, o[i][d].w * f);
     }
     if (x.parts > 0) mine = paged_desc(x, rows);
   }
@@ -186,7 +244,7 @@ constexpr int kJoinThreads = 256, kJoinWarps = kJoinThreads / 32, kJoinPerSm = 4
 
 template <typename T>
 __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PagedParams p, int R, int G) {
-  static_assert(kPagedMaxRuns <= 2 * kJoinThreads, "two descriptions a thread");
+  constexpr int PER = (kPagedMaxRuns + kJoinThreads - 1) / kJoinThreads;  // descriptions a thread
   __shared__ int4 desc[kPagedMaxRuns];
   __shared__ int first[kPagedMaxRuns + 1];  // jobs before each unit
   __shared__ int sums[kJoinWarps], job_s;
@@ -196,31 +254,38 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PagedPar
   asm volatile("griddepcontrol.wait;" ::: "memory");
 
   // Jobs of each unit, summed.
-  int n[2] = {0, 0};
+  int n[PER], inc = 0;
 #pragma unroll
-  for (int u = 0; u < 2; ++u)
-    if (2 * tid + u < G) {
-      const int4 d = p.desc[2 * tid + u];
-      desc[2 * tid + u] = d;
+  for (int u = 0; u < PER; ++u) {
+    n[u] = 0;
+    if (PER * tid + u < G) {
+      const int4 d = p.desc[PER * tid + u];
+      desc[PER * tid + u] = d;
       const int parts = paged_desc_parts(d.w), rows = paged_desc_rows(d.w);
       n[u] = parts == 0 ? 0 : (parts <= kJoinWarps ? (rows + kJoinWarps - 1) / kJoinWarps : rows);
     }
-  int inc = n[0] + n[1];
+    inc += n[u];
+  }
+  int before = -inc;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int y = __shfl_up_sync(0xffffffffu, inc, o);
     if (lane >= o) inc += y;
   }
+  before += inc;
   if (lane == 31) sums[warp] = inc;
   __syncthreads();
-  int jobs = 0, before = inc - n[0] - n[1];
+  int jobs = 0;
 #pragma unroll
   for (int w = 0; w < kJoinWarps; ++w) {
     before += w < warp ? sums[w] : 0;
     jobs += sums[w];
   }
-  if (2 * tid < G) first[2 * tid] = before;
-  if (2 * tid + 1 < G) first[2 * tid + 1] = before + n[0];
+#pragma unroll
+  for (int u = 0; u < PER; ++u) {
+    if (PER * tid + u < G) first[PER * tid + u] = before;
+    before += n[u];
+  }
   if (tid == 0) first[G] = jobs;
   __syncthreads();
 
@@ -350,30 +415,38 @@ static int grid_for(const PagedArgs& a, int R, int TK, int resident) {
   return tiles < resident ? static_cast<int>(tiles) : resident;
 }
 
-constexpr int kF32Rows = 64, kF32PerSm = 2;
+constexpr int kF32Rows = 64, kF32PerSm = 2, kF32FewPerSm = 3;
 
-template <int D, int R, int TK, int TR, int TC>
-static cudaError_t launch_f32(const PagedArgs& a, cudaStream_t stream) {
-  const size_t smem = sizeof(float) * (R * D + TK * (D + 4) + TK * D + R * (TK + 1));
-  auto kern = paged_attn_f32_kernel<D, R, TK, TR, TC>;
+template <int D, int R, int TK, int STAGES>
+static cudaError_t launch_f32(const PagedArgs& a, int per_sm, cudaStream_t stream) {
+  using L = F32Layout<D, R, TK, STAGES>;
+  constexpr int smem = sizeof(float) * L::FLOATS;
+  auto kern = paged_attn_f32_kernel<D, R, TK, STAGES>;
   static std::atomic<uint64_t> done{0};
-  cudaError_t e = allow_smem(reinterpret_cast<const void*>(kern), (int)smem, done);
+  cudaError_t e = allow_smem(reinterpret_cast<const void*>(kern), smem, done);
   if (e != cudaSuccess) return e;
-  const int G = grid_for(a, R, TK, sm_count() * kF32PerSm);
+  const int G = grid_for(a, R, TK, sm_count() * per_sm);
   const PagedParams p = paged_params(a, R, G, 1);
-  kern<<<G, 256, smem, stream>>>(p);
+  kern<<<G, L::THREADS, smem, stream>>>(p);
   e = cudaGetLastError();
   return e != cudaSuccess ? e : launch_paged_join<float>(p, R, G, TK, stream);
 }
 
+template <int D>
+static cudaError_t launch_f32_rows(const PagedArgs& a, cudaStream_t stream) {
+  const int64_t rows = (int64_t)a.max_q * (a.Hq / a.Hkv);
+  if (rows <= 8) return launch_f32<D, 8, 32, 2>(a, kF32FewPerSm, stream);
+  if (rows <= 16) return launch_f32<D, 16, 32, 2>(a, kF32FewPerSm, stream);
+  return launch_f32<D, kF32Rows, 64, 1>(a, kF32PerSm, stream);
+}
+
 static cudaError_t launch_paged_f32(const PagedArgs& a, cudaStream_t stream) {
-  const bool few = (int64_t)a.max_q * (a.Hq / a.Hkv) <= 16;
-  if (a.D == 128) return few ? launch_f32<128, 16, 64, 2, 2>(a, stream) : launch_f32<128, kF32Rows, 32, 4, 2>(a, stream);
-  return few ? launch_f32<64, 16, 64, 2, 2>(a, stream) : launch_f32<64, kF32Rows, 32, 4, 2>(a, stream);
+  return a.D == 128 ? launch_f32_rows<128>(a, stream) : launch_f32_rows<64>(a, stream);
 }
 
 int64_t paged_workspace_bytes(int64_t Hq, int64_t Hkv, int64_t D, int64_t max_q, int dtype) {
-  if (dtype == SPRUCE_DTYPE_F32) return paged_params_bytes(kF32Rows, kMaxSms * kF32PerSm, D);
+  if (dtype == SPRUCE_DTYPE_F32)
+    return std::max(paged_params_bytes(kF32Rows, kMaxSms * kF32PerSm, D), paged_params_bytes(16, kMaxSms * kF32FewPerSm, D));
   if (max_q * (Hq / Hkv) <= kPagedRowsMax) return paged_params_bytes(kPagedRowsMax, kMaxSms * kPagedRowsPerSm, D);
   return paged_params_bytes(kPagedChunkRows, kMaxSms, D);
 }
@@ -382,7 +455,7 @@ cudaError_t launch_paged_attention(const PagedArgs& a, int dtype, cudaStream_t s
   if (dtype == SPRUCE_DTYPE_F32) return launch_paged_f32(a, stream);
   const int64_t rows = (int64_t)a.max_q * (a.Hq / a.Hkv);
   if (rows <= kPagedRowsMax) {
-    const int tiles = rows <= 16 ? 1 : (rows <= 32 ? 2 : 4);
+    const int tiles = rows <= 16 ? 1 : 2;
     return launch_paged_rows(a, dtype, tiles, grid_for(a, 16 * tiles, kPagedRowsKeys, sm_count() * kPagedRowsPerSm),
                              stream);
   }

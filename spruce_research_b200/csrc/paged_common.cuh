@@ -68,7 +68,7 @@ struct PagedPiece {
   int parts;        // > 0: the first part of a unit that this many runs share
 };
 
-constexpr int kMaxSms = 160, kPagedMaxRuns = 2 * kMaxSms;
+constexpr int kMaxSms = 160, kPagedMaxRuns = 3 * kMaxSms;
 static_assert(kPagedMaxRuns < 1 << 12, "parts of a unit fit their field");
 __device__ __forceinline__ int4 paged_desc(const PagedPiece& x, int rows) {
   return make_int4(x.q.q0, x.qt, x.g, x.parts | x.slot << 12 | rows << 16);
@@ -256,7 +256,7 @@ constexpr int kPagedChunkRows = 256, kPagedChunkKeys = 128;
 cudaError_t launch_paged_chunk(const PagedArgs& a, int dtype, int G, cudaStream_t stream);
 
 // Warp-MMA attention of at most 64 query rows a unit, in 1, 2 or 4 tiles of 16 (paged_rows_sm100.cu).
-constexpr int kPagedRowsMax = 64, kPagedRowsKeys = 64, kPagedRowsPerSm = 2;
+constexpr int kPagedRowsMax = 32, kPagedRowsKeys = 64, kPagedRowsPerSm = 2;
 cudaError_t launch_paged_rows(const PagedArgs& a, int dtype, int tiles, int G, cudaStream_t stream);
 // The cache's tensor maps, and the rows of a box of them, for key tiles of `tile` (paged_chunk_sm100.cu).
 bool paged_cache_maps(const PagedArgs& a, int dtype, int box, CUtensorMap* mk, CUtensorMap* mv);

@@ -1,4 +1,4 @@
-// Attention of single tokens and short drafts over a paged K/V cache (bf16 / fp16): up to 64 query rows a (sequence,
+// Attention of single tokens and short drafts over a paged K/V cache (bf16 / fp16): up to 32 query rows a (sequence,
 // KV head), bound by the HBM reads of K and V.
 //
 // The mathematics, the split of the work and its join are those of paged_common.cuh and paged_attn.cu.  Each byte of K
@@ -6,7 +6,7 @@
 // through TMEM would only add latency; warp-level MMAs (m16n8k16) on fragments from shared memory keep up with HBM.
 //
 // A CTA has one loader warp and four compute warps.  The loader keeps STAGES tiles of 64 keys (K and V) in flight by TMA,
-// page by page, across the borders of units; page ids come 32 boxes at a time, one batch ahead.  MT = 1, 2 or 4
+// page by page, across the borders of units; page ids come 32 boxes at a time, one batch ahead.  MT = 1 or 2
 // 16-row tiles (R = 16 MT) times 4 / MT slices of a tile's keys are dealt to the compute warps.  Each keeps its own
 // running maximum, sum and output, so the warps meet only at the end of a piece, where slices are joined through
 // shared memory.  Two CTAs an SM: one's joins and starts pass behind the other's loads.
@@ -348,8 +348,7 @@ static cudaError_t launch_rows(const PagedArgs& a, int dtype, int G, cudaStream_
 template <typename T, int D>
 static cudaError_t launch_rows_tiles(const PagedArgs& a, int dtype, int tiles, int G, cudaStream_t stream) {
   if (tiles == 1) return launch_rows<T, D, 1>(a, dtype, G, stream);
-  if (tiles == 2) return launch_rows<T, D, 2>(a, dtype, G, stream);
-  return launch_rows<T, D, 4>(a, dtype, G, stream);
+  return launch_rows<T, D, 2>(a, dtype, G, stream);
 }
 
 cudaError_t launch_paged_rows(const PagedArgs& a, int dtype, int tiles, int G, cudaStream_t stream) {
