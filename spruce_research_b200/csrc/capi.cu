@@ -858,9 +858,11 @@ int spruce_paged_append(const spruce_paged_append_args* args) {
   return cuda_status(spruce::launch_norm_rope(a, (int)x.dtype, as_stream(x.stream)), "paged append launch");
 }
 
+constexpr int64_t kMaxQueryRows = 1 << 30;  // of a sequence, over all heads: row numbers stay ints
+
 int64_t spruce_paged_attention_workspace_bytes(int64_t Hq, int64_t Hkv, int64_t D, int64_t max_q_len, int dtype) {
   if (!valid_dtype(dtype) || Hkv < 1 || Hq < 1 || Hq % Hkv || (D != 64 && D != 128) || max_q_len < 0 ||
-      max_q_len > INT32_MAX / Hq)
+      max_q_len > kMaxQueryRows / Hq)
     return -1;
   return spruce::paged_workspace_bytes(Hq, Hkv, D, max_q_len, dtype);
 }
@@ -875,7 +877,7 @@ int spruce_paged_attention(const spruce_paged_attention_args* args) {
     return fail(SPRUCE_ERR_UNSUPPORTED, "paged attention needs head_dim 64 or 128, got %lld", (long long)x.D);
   if (x.max_q_len < 0 || x.max_kv_len < 0)
     return fail(SPRUCE_ERR_INVALID, "max_q_len and max_kv_len must not be negative");
-  if (x.max_q_len > INT32_MAX / x.Hq || x.max_kv_len > INT32_MAX)
+  if (x.max_q_len > kMaxQueryRows / x.Hq || x.max_kv_len > INT32_MAX)
     return fail(SPRUCE_ERR_UNSUPPORTED, "sequence too long");
   const float scale = (float)x.scale;
   if (!(scale >= 0.0f && scale <= 3.0e38f))
@@ -889,6 +891,10 @@ int spruce_paged_attention(const spruce_paged_attention_args* args) {
   for (int i = 0; i < 2; ++i) ok = ok && x.q_strides[i] % vn == 0 && x.out_strides[i] % vn == 0;
   for (int i = 0; i < 3; ++i) ok = ok && x.kc_strides[i] % vn == 0 && x.vc_strides[i] % vn == 0;
   if (!ok) return fail(SPRUCE_ERR_UNSUPPORTED, "q, out and the cache need 16-byte aligned rows");
+  const int64_t sizes[3] = {x.num_pages, x.Hkv, x.page_size};
+  for (int i = 0; i < 3; ++i)  // what a tensor map can step by
+    if (sizes[i] > 1 && (x.kc_strides[i] < 1 || x.vc_strides[i] < 1))
+      return fail(SPRUCE_ERR_UNSUPPORTED, "the cache needs positive strides");
   const int64_t need = spruce::paged_workspace_bytes(x.Hq, x.Hkv, x.D, x.max_q_len, (int)x.dtype);
   if (x.workspace == nullptr || x.workspace_bytes < need)
     return fail(SPRUCE_ERR_WORKSPACE, "paged attention workspace needs %lld bytes, got %lld", (long long)need,

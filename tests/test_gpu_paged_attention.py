@@ -104,7 +104,12 @@ DTYPES = [torch.float32, torch.bfloat16, torch.float16]
     ([63, 0, 1, 130], [63, 40, 2, 257], 14, 2, 16),           # a chunk, an idle and a single-token sequence
     ([300], [1500], 28, 4, 64),
     ([256, 257], [256, 900], 4, 4, 256),
-    ([37], [37], 3, 1, 80)])                                  # a whole short prompt; rows of no power of two
+    ([37], [37], 3, 1, 80),                                   # a whole short prompt; rows of no power of two
+    ([1] * 400, [1 + (37 * i) % 300 for i in range(400)], 4, 2, 16),             # more sequences than threads scan at once
+    ([(11 * i) % 90 for i in range(41)], [(11 * i) % 90 + (53 * i) % 200 for i in range(41)], 4, 2, 16),
+    ([1900], [1900], 4, 4, 64),                               # a prompt in one chunk: units of every length
+    ([120, 120], [130, 1500], 8, 8, 64),                      # 65 to 128 rows: one tile of the pair
+    ([40, 3], [600, 4000], 1, 1, 32)])                        # 33 to 64 rows
 def test_matches_64_bits(dtype, D, qlens, kvs, Hq, Hkv, page):
     Batch(qlens, kvs, Hq, Hkv, D, page, dtype, seed=len(kvs) + page).check()
 
@@ -267,6 +272,9 @@ def test_refusals():
     with pytest.raises(ValueError, match="16-byte aligned"):
         odd = torch.zeros(b.kc.numel() + 8, device="cuda", dtype=torch.bfloat16)[1:1 + b.kc.numel()].view_as(b.kc)
         native.paged_attention(b.q, odd, b.vc, b.table, b.cu, b.kv, **call)
+    with pytest.raises(ValueError, match="positive"):
+        flat = b.kc[:, :1].expand(-1, 2, -1, -1)
+        native.paged_attention(b.q, flat, flat, b.table, b.cu, b.kv, **call)
     with pytest.raises(ValueError, match="new tokens' dtype"):
         native.paged_attention(b.q.half(), b.kc, b.vc, b.table, b.cu, b.kv, **call)
     with pytest.raises(ValueError, match="int32"):
