@@ -479,14 +479,14 @@ SPRUCE_API int spruce_paged_append(const spruce_paged_append_args *args);
  * q_len + i.  From single tokens to prefill chunks, of any mix of lengths; a
  * query that sees nothing (an empty sequence) yields zeros, rows past cu_q[S]
  * are not written.  Cache rows at or past kv_lens[s] never reach an output,
- * whatever they hold.  max_q_len and max_kv_len bound q_len and kv_lens (they
+ * whatever they hold; a value of the sequence itself that is not finite may
+ * reach every query whose key tile holds it.  max_q_len and max_kv_len bound q_len and kv_lens (they
  * size the launch); a longer sequence is cut to them and raises
  * SPRUCE_STATUS_BAD_LENGTH, a page id outside the cache reads zeros and raises
  * SPRUCE_STATUS_BAD_PAGE.  scale >= 0, D in {64, 128}, page_size a multiple of 16, every
  * row 16-byte aligned.  bf16 / fp16 run tensor-core kernels, fp32 a CUDA-core
  * kernel.  workspace (spruce_paged_attention_workspace_bytes, -1 for an invalid
- * shape; 256-byte aligned)
- * holds the parts of sequences that several CTAs share; a call uses it alone.
+ * shape; 256-byte aligned) holds the parts of sequences that several CTAs share; a call uses it alone.
  */
 SPRUCE_API int64_t spruce_paged_attention_workspace_bytes(int64_t Hq, int64_t Hkv, int64_t D, int64_t max_q_len,
                                                           int dtype);

@@ -10,5 +10,7 @@ Reference-named drop-ins:
   interfaces.validator     validate_selected_blocks
   route_overrides          charged_route_density
 Per-layer pipeline: pipeline.SparsePrefillLayer; multi-GPU split: sharding.
+Serving: rope.rope_table, paged.PagedKVCache, paged.PagedSparseLayer (over native.qk_norm_rope,
+native.paged_append and native.paged_attention).
 """
 __version__ = "0.1.0"

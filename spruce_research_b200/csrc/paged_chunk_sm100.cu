@@ -20,6 +20,11 @@
 // the last page past the end may hold anything, so the loader clears them in V (their scores are masked by selection)
 // before the MMA issuer may read the tile.
 //
+// Measured on a B200 (28 query / 4 KV heads, d = 128, bf16): 2048 tokens over 64K 1.60 ms (1190 TFLOP/s; 1.75 ms in a long run
+// under the power cap), a 16K prompt in one chunk 1.58 ms, 512 tokens over 32K 226 us.  A key tile of both M-tiles takes
+// 3,210 cycles, the MMAs alone 2,880 (90 each, not the 64 of their rate: Q and K are both read from shared memory), a
+// tile's softmax 1,900.  The registers go to the softmax (208 a thread by setmaxnreg: with 168 it ran a sixth slower).
+//
 // Every wait is bounded (common.cuh).
 #include <algorithm>
 #include <type_traits>
