@@ -61,6 +61,8 @@ __global__ void __launch_bounds__(F32Layout<D, R, TK, STAGES>::THREADS) paged_at
 
   const int tid = threadIdx.x;
   const int rg = tid / NC, cg = tid % NC;
+  let_next_kernel_start();
+  wait_for_earlier_kernels();
   PagedWalk<R, TK> walk;
   const bool any = paged_run<R, TK, THREADS>(p, walk, scratch);
   int4 mine = make_int4(0, 0, 0, 0);
@@ -68,6 +70,7 @@ __global__ void __launch_bounds__(F32Layout<D, R, TK, STAGES>::THREADS) paged_at
   while (any && walk.next(p, x)) {
     const int rows = min(R, x.q.qlen * p.rep - x.qt * R);
     const int n = x.keys > 0 ? x.t1 - x.t0 : 0;
+    const PagedRows row_at(p, x.q.q0, x.qt * R, x.g);
     const int32_t* table = p.a.block_table + x.s * p.a.table_stride;
     // Tile i of the piece into its stage: rows past the keys, or of no page, are zeros.
     auto load = [&](int i) {
@@ -107,10 +110,7 @@ __global__ void __launch_bounds__(F32Layout<D, R, TK, STAGES>::THREADS) paged_at
       const int r = e / CH, d = e % CH * 4;
       float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
       if (r < rows) {
-        int64_t tok;
-        int head;
-        paged_row(p, x, x.qt * R + r, tok, head);
-        v = *reinterpret_cast<const float4*>(static_cast<const float*>(p.a.q) + tok * p.a.qn + head * p.a.qh + d);
+        v = *reinterpret_cast<const float4*>(static_cast<const float*>(p.a.q) + row_at.offset(r, p.a.qn, p.a.qh) + d);
       }
       *reinterpret_cast<float4*>(Qs + r * D + d) = v;
     }
@@ -121,8 +121,7 @@ __global__ void __launch_bounds__(F32Layout<D, R, TK, STAGES>::THREADS) paged_at
     for (int i = 0; i < TR; ++i) {
       m[i] = -INFINITY;
       l[i] = 0.0f;
-      const int r = x.qt * R + rg * TR + i;
-      seen[i] = min(x.q.first + r / p.rep + 1, x.keys);
+      seen[i] = min(x.q.first + row_at.token(rg * TR + i) + 1, x.keys);
 #pragma unroll
       for (int d = 0; d < DV; ++d) o[i][d] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     }
@@ -216,10 +215,7 @@ __global__ void __launch_bounds__(F32Layout<D, R, TK, STAGES>::THREADS) paged_at
       float* dst;
       float f = 1.0f;
       if (x.slot < 0) {
-        int64_t tok;
-        int head;
-        paged_row(p, x, x.qt * R + r, tok, head);
-        dst = static_cast<float*>(p.a.out) + tok * p.a.on + head * p.a.oh;
+        dst = static_cast<float*>(p.a.out) + row_at.offset(r, p.a.on, p.a.oh);
         f = l[i] > 0.0f ? 1.0f / l[i] : 0.0f;
       } else {
         const int64_t at = (int64_t)(2 * blockIdx.x + x.slot) * R + r;
@@ -252,7 +248,8 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PagedPar
   __shared__ float l_s[kJoinWarps], o_s[kJoinWarps][128];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int D = p.a.D, dims = D / 32;  // 2 or 4 adjacent dims a lane
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  let_next_kernel_start();
+  wait_for_earlier_kernels();
 
   // Jobs of each unit, summed.
   int n[PER], inc = 0;
@@ -365,13 +362,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PagedPar
       }
     }
     if (r < rows && (few || warp == 0)) {
-      PagedPiece x;
-      x.q.q0 = d.x;
-      x.g = d.z;
-      int64_t tok;
-      int head;
-      paged_row(p, x, d.y * R + r, tok, head);
-      T* dst = static_cast<T*>(p.a.out) + tok * p.a.on + head * p.a.oh + lane * dims;
+      T* dst = static_cast<T*>(p.a.out) + PagedRows(p, d.x, d.y * R, d.z).offset(r, p.a.on, p.a.oh) + lane * dims;
       const float inv = l > 0.0f ? 1.0f / l : 0.0f;
       if constexpr (sizeof(T) == 4) {
         if (dims == 4)
@@ -393,16 +384,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PagedPar
 template <typename T>
 cudaError_t launch_paged_join(const PagedParams& p, int R, int G, int TK, cudaStream_t stream) {
   if (p.a.max_kv <= TK) return cudaSuccess;  // one key tile a unit: none is split
-  cudaLaunchConfig_t cfg{};
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.gridDim = dim3(kJoinPerSm * sm_count());
-  cfg.blockDim = dim3(kJoinThreads);
-  cfg.stream = stream;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, paged_join_kernel<T>, p, R, G);
+  return launch_early(paged_join_kernel<T>, kJoinPerSm * sm_count(), kJoinThreads, 0, stream, p, R, G);
 }
 template cudaError_t launch_paged_join<float>(const PagedParams&, int, int, int, cudaStream_t);
 template cudaError_t launch_paged_join<__nv_bfloat16>(const PagedParams&, int, int, int, cudaStream_t);
@@ -428,8 +410,7 @@ static cudaError_t launch_f32(const PagedArgs& a, int per_sm, cudaStream_t strea
   if (e != cudaSuccess) return e;
   const int G = grid_for(a, R, TK, sm_count() * per_sm);
   const PagedParams p = paged_params(a, R, G, 1);
-  kern<<<G, L::THREADS, smem, stream>>>(p);
-  e = cudaGetLastError();
+  e = launch_early(kern, G, L::THREADS, smem, stream, p);
   return e != cudaSuccess ? e : launch_paged_join<float>(p, R, G, TK, stream);
 }
 

@@ -13,6 +13,7 @@
 #pragma once
 
 #include <atomic>
+#include <utility>
 
 #include "common.cuh"
 #include "kernels.h"
@@ -28,6 +29,7 @@ struct PagedParams {
   float2* part_ml;        // [2 G][R] softmax maximum (log2 units) and sum
   float* part_o;          // [2 G][R][D]
   float scale_log2;
+  float inv_rep;
 };
 
 struct PagedSeq {
@@ -223,12 +225,25 @@ __device__ __forceinline__ bool paged_run(const PagedParams& p, PagedWalk<R, TK>
   return true;
 }
 
-// Start of row r of a piece in q / out; the caller keeps r below the tile's rows.
-__device__ __forceinline__ void paged_row(const PagedParams& p, const PagedPiece& x, int row, int64_t& tok, int& head) {
-  const int t = row / p.rep;
-  tok = x.q.q0 + t;
-  head = x.g * p.rep + row - t * p.rep;
-}
+// Tokens and heads of the rows of a tile: row r after row0 of sequence (q0 = its first token), KV head g.  One division a
+// tile; within it (row and remainder under 2^21) the quotient by a rounded reciprocal is exact.
+struct PagedRows {
+  int tok0, rem0, head0, rep;
+  int64_t q0;
+  float inv;
+  __device__ __forceinline__ PagedRows(const PagedParams& p, int first, int row0, int g)
+      : tok0(row0 / p.rep), rem0(row0 - row0 / p.rep * p.rep), head0(g * p.rep), rep(p.rep), q0(first), inv(p.inv_rep) {}
+  // Token of the sequence.
+  __device__ __forceinline__ int token(int r) const { return tok0 + in_tile(r); }
+  // Element offset in q or out.
+  __device__ __forceinline__ int64_t offset(int r, int64_t token_stride, int64_t head_stride) const {
+    const int t = in_tile(r);
+    return (q0 + tok0 + t) * token_stride + (head0 + rem0 + r - t * rep) * head_stride;
+  }
+
+ private:
+  __device__ __forceinline__ int in_tile(int r) const { return static_cast<int>((static_cast<float>(rem0 + r) + 0.5f) * inv); }
+};
 
 // Page of a key and the row in it; -1 (and a status) where the table names no page of the cache.
 __device__ __forceinline__ int paged_page(const PagedParams& p, const int32_t* table, int index) {
@@ -251,6 +266,26 @@ inline cudaError_t allow_smem(const void* kern, int bytes, std::atomic<uint64_t>
   return e;
 }
 
+// Launches a kernel that may start while the one before it in the stream ends; it waits (griddepcontrol) before it
+// touches memory.
+template <typename... Params, typename... Args>
+cudaError_t launch_early(void (*kern)(Params...), int grid, int threads, int smem, cudaStream_t stream, Args&&... args) {
+  cudaLaunchConfig_t cfg{};
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...);
+}
+// In a kernel: memory of the kernels before it is complete; the next kernel may start.
+__device__ __forceinline__ void wait_for_earlier_kernels() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void let_next_kernel_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 // Tensor-core attention of chunks (paged_chunk_sm100.cu), on G CTAs.
 constexpr int kPagedChunkRows = 256, kPagedChunkKeys = 128;
 cudaError_t launch_paged_chunk(const PagedArgs& a, int dtype, int G, cudaStream_t stream);
@@ -271,6 +306,7 @@ inline PagedParams paged_params(const PagedArgs& a, int R, int G, int unit_cost)
   PagedParams p;
   p.a = a;
   p.rep = a.Hq / a.Hkv;
+  p.inv_rep = 1.0f / static_cast<float>(p.rep);
   p.row_tiles = static_cast<int>(((int64_t)a.max_q * p.rep + R - 1) / R);
   int64_t cap = (int64_t)a.max_pages * a.page_size;
   cap = cap < a.max_kv ? cap : a.max_kv;

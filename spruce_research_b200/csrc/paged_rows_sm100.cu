@@ -92,7 +92,8 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
     prefetch_tmap(&tmk);
     prefetch_tmap(&tmv);
   }
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the join may take its place; it waits for our end
+  let_next_kernel_start();
+  wait_for_earlier_kernels();
   Walk walk;
   const bool any = paged_run<R, kRowsKeys, kRowsThreads>(p, walk, scan);
   __syncthreads();
@@ -156,6 +157,7 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
   while (walk.next(p, x)) {  // after a wait that ran out the warps still meet at the joins' barriers
     const int rows = min(R, x.q.qlen * p.rep - x.qt * R);
     if (x.parts > 0) mine = paged_desc(x, rows);
+    const PagedRows row_at(p, x.q.q0, x.qt * R, x.g);
     uint32_t q[D / 16][4];
     int seen[2];  // keys that this thread's two rows see
 #pragma unroll
@@ -163,12 +165,9 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
       const int r = mt * 16 + qr + 8 * i;
       const uint32_t* src = nullptr;
       if (r < rows) {
-        int64_t tok;
-        int head;
-        paged_row(p, x, x.qt * R + r, tok, head);
-        src = reinterpret_cast<const uint32_t*>(static_cast<const T*>(p.a.q) + tok * p.a.qn + head * p.a.qh);
+        src = reinterpret_cast<const uint32_t*>(static_cast<const T*>(p.a.q) + row_at.offset(r, p.a.qn, p.a.qh));
       }
-      seen[i] = min(x.q.first + (x.qt * R + r) / p.rep + 1, x.keys);
+      seen[i] = min(x.q.first + row_at.token(r) + 1, x.keys);
 #pragma unroll
       for (int k = 0; k < D / 16; ++k) {
         q[k][i] = src != nullptr ? src[k * 8 + qc] : 0u;
@@ -316,13 +315,10 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
           sum.w += v.w;
         }
         if (whole) {
-          int64_t tok;
-          int head;
-          paged_row(p, x, x.qt * R + r, tok, head);
           uint2 v;
           v.x = Pack2<T>::pack(sum.x, sum.y);
           v.y = Pack2<T>::pack(sum.z, sum.w);
-          *reinterpret_cast<uint2*>(static_cast<T*>(p.a.out) + tok * p.a.on + head * p.a.oh + c0 + wc) = v;
+          *reinterpret_cast<uint2*>(static_cast<T*>(p.a.out) + row_at.offset(r, p.a.on, p.a.oh) + c0 + wc) = v;
         } else {
           *reinterpret_cast<float4*>(p.part_o + (part + r) * D + c0 + wc) = sum;
         }
@@ -344,8 +340,7 @@ static cudaError_t launch_rows(const PagedArgs& a, int dtype, int G, cudaStream_
   cudaError_t e = allow_smem(reinterpret_cast<const void*>(kern), L::BYTES, done);
   if (e != cudaSuccess) return e;
   const PagedParams p = paged_params(a, 16 * MT, G, 1);
-  kern<<<G, kRowsThreads, L::BYTES, stream>>>(mk, mv, p, box);
-  e = cudaGetLastError();
+  e = launch_early(kern, G, kRowsThreads, L::BYTES, stream, mk, mv, p, box);
   return e != cudaSuccess ? e : launch_paged_join<T>(p, 16 * MT, G, kRowsKeys, stream);
 }
 

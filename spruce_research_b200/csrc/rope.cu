@@ -17,6 +17,7 @@
 // are brought in by cp.async, 16 KB a CTA and 128 KB an SM in flight, which registers could not hold (register loads: 436 us
 // at best for the layer; 256 threads or eight heads a group: 325-455 us, and slower at 4097 tokens).
 #include "attn_common.cuh"
+#include "paged_common.cuh"
 
 namespace spruce {
 
@@ -156,6 +157,7 @@ __device__ __forceinline__ const Rows& rows_of(const RowsArgs& a, int h, int& hh
 template <typename T, bool APPEND>
 __global__ void __launch_bounds__(kRowThreads, kRowCtasPerSm)
     norm_rope_kernel(const RowsArgs a, int lpr, int hc, int chunks) {
+  let_next_kernel_start();  // the attention over the cache sets up meanwhile, and waits for our end
   constexpr int HC = kHeadsPerGroup, VN = 16 / sizeof(T), NP = VN / 2;
   __shared__ uint4 stage[HC * 2][kRowThreads];  // a thread's own vectors: no barrier
   const int l = threadIdx.x & (lpr - 1);

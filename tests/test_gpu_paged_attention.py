@@ -250,6 +250,24 @@ def test_another_stream_and_a_graph():
     assert torch.equal(got, want)
     graph.replay()
     assert torch.equal(out, want)
+    # after a copy and after an append, eager and captured: an attention that starts early still waits for them
+    fresh = b.q.clone()
+    k, v = torch.zeros(2, 4, 128, device="cuda", dtype=torch.bfloat16), torch.zeros(2, 4, 128, device="cuda", dtype=torch.bfloat16)
+    last = [(b.kc[p, :, r].clone(), b.vc[p, :, r].clone()) for p, r in ((b.table[0, 1], 35), (b.table[1, 12], 31))]
+    k.copy_(torch.stack([x[0] for x in last]))
+    v.copy_(torch.stack([x[1] for x in last]))
+    torch.cuda.synchronize()
+    chain = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(chain):
+        b.q.copy_(fresh)
+        native.paged_append(k, v, b.kc, b.vc, b.table, b.cu, b.kv)
+        b.call(out=out)
+    for run in (chain.replay, lambda: (b.q.copy_(fresh), native.paged_append(k, v, b.kc, b.vc, b.table, b.cu, b.kv), b.call(out=out))):
+        for _ in range(20):
+            b.q.zero_()
+            b.kc[b.table[0, 1], :, 35] = 0
+            run()
+            assert torch.equal(out, want)
     b.kvs = [37, 700]
     b.kv.copy_(torch.tensor(b.kvs))
     graph.replay()
