@@ -451,14 +451,18 @@ def tree_topk(scores: torch.Tensor, valid: torch.Tensor, cand: torch.Tensor, k: 
     return out
 
 
-def _device_of(*tensors: torch.Tensor | None) -> int:
-    """The one CUDA device of these tensors (None: an argument that was left out)."""
-    device = tensors[0].get_device()
-    for t in tensors:
-        if t is not None and t.get_device() != device or device < 0:
-            _lib.require_cuda(*(t for t in tensors if t is not None))
-            raise ValueError(f"tensors on {tensors[0].device} and {t.device}")
-    return device
+def _on_one_device(device: int, *optional: torch.Tensor | None) -> bool:
+    for t in optional:
+        if t is not None and t.get_device() != device:
+            return False
+    return device >= 0
+
+
+def _refuse_devices(*tensors: torch.Tensor | None) -> None:
+    """The tensors are not on one CUDA device: say which."""
+    tensors = [t for t in tensors if t is not None]
+    _lib.require_cuda(*tensors)
+    raise ValueError(f"tensors on {', '.join(sorted({str(t.device) for t in tensors}))}")
 
 
 def _ptr(t: torch.Tensor | None) -> int:
@@ -493,14 +497,17 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, rope: torch.Tensor, positions
     token-major tensors viewed as [B, H, T, D] (the layout the selector and the attention take), or
     ``q_out`` / ``k_out``, which may be q and k themselves.
     """
-    device = _device_of(q, k, rope, positions, q_weight, k_weight, q_out, k_out, status)
+    device = q.get_device()
+    if not (device == k.get_device() == rope.get_device()
+            and _on_one_device(device, positions, q_weight, k_weight, q_out, k_out, status)):
+        _refuse_devices(q, k, rope, positions, q_weight, k_weight, q_out, k_out, status)
     B, Hq, T, D = q.shape
-    dtype = q.dtype
+    dtype, ks = q.dtype, k.shape
     if dtype != k.dtype:
         raise ValueError("q and k must share a dtype")
-    if k.dim() != 4 or k.shape[0] != B or k.shape[2:] != q.shape[2:]:
-        raise ValueError(f"k must be [{B}, Hkv, {T}, {D}], got {tuple(k.shape)}")
-    Hkv = k.shape[1]
+    if len(ks) != 4 or ks[0] != B or ks[2] != T or ks[3] != D:
+        raise ValueError(f"k must be [{B}, Hkv, {T}, {D}], got {tuple(ks)}")
+    Hkv = ks[1]
     _check_rope(rope, D)
     q_weight, k_weight = _head_weight(q_weight, D, "q_weight"), _head_weight(k_weight, D, "k_weight")
     pos_strides = (0, 0)
@@ -532,24 +539,24 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, rope: torch.Tensor, positions
 
 
 def _paged_shapes(k_cache, v_cache, block_table, cu_q, kv_lens, dtype):
-    """(num_pages, Hkv, page_size, D, S, (table stride, table width)) of a paged cache and its metadata, checked."""
-    shape = k_cache.shape
+    """A paged cache and its metadata, checked: its shape, both caches' strides, S and the table's (stride, width)."""
+    shape, ks, vs = k_cache.shape, k_cache.stride(), v_cache.stride()
     if len(shape) != 4 or v_cache.shape != shape:
         raise ValueError("the caches must be [pages, Hkv, page_size, D] of one shape")
     if k_cache.dtype != dtype or v_cache.dtype != dtype:
         raise ValueError("the caches must have the new tokens' dtype")
-    if k_cache.stride(3) != 1 or v_cache.stride(3) != 1:
+    if ks[3] != 1 or vs[3] != 1:
         raise ValueError("the caches need a unit last stride")
-    if not (block_table.dtype == cu_q.dtype == kv_lens.dtype == torch.int32):
+    if not (block_table.dtype is cu_q.dtype is kv_lens.dtype is torch.int32):
         raise ValueError("block_table, cu_q and kv_lens must be int32")
-    table, (S, *more) = block_table.shape, kv_lens.shape
-    if more or len(table) != 2 or table[0] != S or cu_q.shape != (S + 1,):
+    table, S = block_table.shape, kv_lens.numel()
+    if len(table) != 2 or table[0] != S or cu_q.shape != (S + 1,) or kv_lens.dim() != 1:
         raise ValueError(f"expected block_table [S, pages], cu_q [S + 1] and kv_lens [S], got "
                          f"{tuple(table)}, {tuple(cu_q.shape)}, {tuple(kv_lens.shape)}")
     step, unit = block_table.stride()
     if unit != 1 and table[1] > 1 or not (cu_q.is_contiguous() and kv_lens.is_contiguous()):
         raise ValueError("block_table needs a unit last stride, cu_q and kv_lens must be contiguous")
-    return (*shape, S, (step, table[1]))
+    return shape, ks, vs, S, step, table[1]
 
 
 def paged_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -566,15 +573,26 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
     replaces the cache positions in the rotation only.  With ``q`` [N, Hq, D], its norm and rotation run in the
     same launch into ``q_out`` (a new [N, Hq, D] tensor by default; q itself is allowed).
     """
-    device = _device_of(k, v, k_cache, v_cache, block_table, cu_q, kv_lens, q, rope, positions, q_weight, k_weight,
+    device = k.get_device()
+    if not (device == v.get_device() == k_cache.get_device() == v_cache.get_device() == block_table.get_device()
+            == cu_q.get_device() == kv_lens.get_device()
+            and _on_one_device(device, q, rope, positions, q_weight, k_weight, q_out, status)):
+        _refuse_devices(k, v, k_cache, v_cache, block_table, cu_q, kv_lens, q, rope, positions, q_weight, k_weight,
                         q_out, status)
-    dtype = k.dtype
-    pages, Hkv, page_size, D, S, table = _paged_shapes(k_cache, v_cache, block_table, cu_q, kv_lens, dtype)
-    if k.dim() != 3 or k.shape[1] != Hkv or k.shape[2] != D or v.shape != k.shape or v.dtype != dtype:
-        raise ValueError(f"k and v must be [N, {Hkv}, {D}] of one dtype, got {tuple(k.shape)} and {tuple(v.shape)}")
-    N = k.shape[0]
-    k = k if k.stride(2) == 1 else k.contiguous()
-    v = v if v.stride(2) == 1 else v.contiguous()
+    dtype, shape = k.dtype, k.shape
+    (pages, Hkv, page_size, D), kc_strides, vc_strides, S, step, width = _paged_shapes(k_cache, v_cache, block_table,
+                                                                                       cu_q, kv_lens, dtype)
+    if len(shape) != 3 or shape[1] != Hkv or shape[2] != D or v.shape != shape or v.dtype != dtype:
+        raise ValueError(f"k and v must be [N, {Hkv}, {D}] of one dtype, got {tuple(shape)} and {tuple(v.shape)}")
+    N = shape[0]
+    kn, kh, kd = k.stride()
+    if kd != 1:
+        k = k.contiguous()
+        kn, kh, _ = k.stride()
+    vn, vh, vd = v.stride()
+    if vd != 1:
+        v = v.contiguous()
+        vn, vh, _ = v.stride()
     q_weight, k_weight = _head_weight(q_weight, D, "q_weight"), _head_weight(k_weight, D, "k_weight")
     table_rows = rd = Hq = 0
     if rope is not None:
@@ -584,24 +602,30 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
         if tuple(positions.shape) != (N,) or positions.is_floating_point():
             raise ValueError(f"positions must be integers [{N}]")
         positions = positions.to(torch.int64).contiguous()
-    qs = os = (0, 0)
+    qn = qh = on = oh = 0
     if q is not None:
-        if q.dim() != 3 or q.shape[0] != N or q.shape[2] != D or q.dtype != dtype:
-            raise ValueError(f"q must be {dtype} [{N}, Hq, {D}], got {q.dtype} {tuple(q.shape)}")
-        q = q if q.stride(2) == 1 else q.contiguous()
-        Hq = q.shape[1]
+        shape = q.shape
+        if len(shape) != 3 or shape[0] != N or shape[2] != D or q.dtype != dtype:
+            raise ValueError(f"q must be {dtype} [{N}, Hq, {D}], got {q.dtype} {tuple(shape)}")
+        Hq = shape[1]
+        qn, qh, qd = q.stride()
+        if qd != 1:
+            q = q.contiguous()
+            qn, qh, _ = q.stride()
         if q_out is None:
             q_out = q.new_empty((N, Hq, D))
-        elif q_out.shape != q.shape or q_out.dtype != dtype or q_out.stride(2) != 1:
-            raise ValueError(f"q_out must be {dtype} {tuple(q.shape)} with a unit last stride")
-        qs, os = q.stride()[:2], q_out.stride()[:2]
+            on, oh = Hq * D, D
+        elif q_out.shape != shape or q_out.dtype != dtype or q_out.stride(2) != 1:
+            raise ValueError(f"q_out must be {dtype} {tuple(shape)} with a unit last stride")
+        else:
+            on, oh, _ = q_out.stride()
     elif q_out is not None:
         raise ValueError("q_out without q")
     args = _lib.PAGED_APPEND_ARGS.pack(
         _ptr(q), k.data_ptr(), v.data_ptr(), _ptr(q_out), k_cache.data_ptr(), v_cache.data_ptr(), _ptr(rope),
         _ptr(positions), _ptr(q_weight), _ptr(k_weight), block_table.data_ptr(), cu_q.data_ptr(), kv_lens.data_ptr(),
-        _ptr(status), _lib.stream_on(device), *qs, *k.stride()[:2], *v.stride()[:2], *os, *k_cache.stride()[:3],
-        *v_cache.stride()[:3], _dt(k), N, S, Hq, Hkv, D, pages, page_size, *table, table_rows, rd, interleaved, eps)
+        _ptr(status), _lib.stream_on(device), qn, qh, kn, kh, vn, vh, on, oh, *kc_strides[:3], *vc_strides[:3], _dt(k),
+        N, S, Hq, Hkv, D, pages, page_size, step, width, table_rows, rd, interleaved, eps)
     _lib.check(_lib.load().spruce_paged_append(args))
     return q_out
 
@@ -621,31 +645,40 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     see none give zeros.  ``max_q_len`` and ``max_kv_len`` bound the sequences' new tokens and lengths (the lengths
     themselves stay on the device).  Returns [N, Hq, D]; rows past ``cu_q[-1]`` are not written.
     """
-    device = _device_of(q, k_cache, v_cache, block_table, cu_q, kv_lens, out, workspace, status)
-    dtype = q.dtype
-    pages, Hkv, page_size, D, S, table = _paged_shapes(k_cache, v_cache, block_table, cu_q, kv_lens, dtype)
-    if q.dim() != 3 or q.shape[2] != D:
-        raise ValueError(f"q must be [N, Hq, {D}], got {tuple(q.shape)}")
-    N, Hq, _ = q.shape
+    device = q.get_device()
+    if not (device == k_cache.get_device() == v_cache.get_device() == block_table.get_device() == cu_q.get_device()
+            == kv_lens.get_device() and _on_one_device(device, out, workspace, status)):
+        _refuse_devices(q, k_cache, v_cache, block_table, cu_q, kv_lens, out, workspace, status)
+    dtype, shape = q.dtype, q.shape
+    (pages, Hkv, page_size, D), kc_strides, vc_strides, S, step, width = _paged_shapes(k_cache, v_cache, block_table,
+                                                                                       cu_q, kv_lens, dtype)
+    if len(shape) != 3 or shape[2] != D:
+        raise ValueError(f"q must be [N, Hq, {D}], got {tuple(shape)}")
+    N, Hq, _ = shape
+    dt, size = _dt(q), q.element_size()
     qn, qh, qd = q.stride()
-    if qd != 1 or (qn | qh) % (16 // q.element_size()) or q.data_ptr() % 16:
+    if qd != 1 or (qn | qh) % (16 // size) or q.data_ptr() % 16:
         q = q.contiguous()
         qn, qh, _ = q.stride()
     if out is None:
-        out = q.new_empty((N, Hq, D))
-    elif out.shape != q.shape or out.dtype != dtype or out.stride(2) != 1:
-        raise ValueError(f"out must be {dtype} {tuple(q.shape)} with a unit last stride")
-    dt = _dt(q)
+        out = torch.empty_like(q) if q.is_contiguous() else q.new_empty(shape)
+        on, oh = Hq * D, D
+    elif out.shape != shape or out.dtype != dtype or out.stride(2) != 1:
+        raise ValueError(f"out must be {dtype} {tuple(shape)} with a unit last stride")
+    else:
+        on, oh, _ = out.stride()
     if workspace is None:
-        need = _paged_workspace_bytes(Hq, Hkv, D, max_q_len, dt)
-        if need < 0:
-            raise ValueError(f"bad paged attention shape: q {tuple(q.shape)}, cache {tuple(k_cache.shape)}, "
+        nbytes = _paged_workspace_bytes(Hq, Hkv, D, max_q_len, dt)
+        if nbytes < 0:
+            raise ValueError(f"bad paged attention shape: q {tuple(shape)}, cache {tuple(k_cache.shape)}, "
                              f"max_q_len {max_q_len}")
-        workspace = q.new_empty(need // q.element_size())
+        workspace = q.new_empty(nbytes // size)
+    else:
+        nbytes = workspace.nbytes
     args = _lib.PAGED_ATTENTION_ARGS.pack(
         q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), block_table.data_ptr(), cu_q.data_ptr(),
-        kv_lens.data_ptr(), workspace.data_ptr(), _ptr(status), _lib.stream_on(device), qn, qh, *k_cache.stride()[:3],
-        *v_cache.stride()[:3], *out.stride()[:2], dt, N, S, Hq, Hkv, D, pages, page_size, *table, max_q_len,
-        max_kv_len, workspace.nbytes, D ** -0.5 if scale is None else scale)
+        kv_lens.data_ptr(), workspace.data_ptr(), _ptr(status), _lib.stream_on(device), qn, qh, *kc_strides[:3],
+        *vc_strides[:3], on, oh, dt, N, S, Hq, Hkv, D, pages, page_size, step, width, max_q_len, max_kv_len, nbytes,
+        D ** -0.5 if scale is None else scale)
     _lib.check(_lib.load().spruce_paged_attention(args))
     return out
