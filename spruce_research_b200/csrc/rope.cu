@@ -8,14 +8,18 @@
 // 131072, and any scaling of the frequencies costs the kernel nothing.
 //
 // Bound: HBM bandwidth (every row read once, written once; ~10 flops an element).  On a B200 Q and K of a 131072-token
-// layer (28 + 4 heads of 128, bf16, 2.2 GB) take 324 us, 6.8 TB/s; 4097 tokens with norms 18.5 us; the append of 8.2K tokens
-// 32.4 us, 5.0 TB/s.
+// layer (28 + 4 heads of 128, bf16, 2.2 GB) take 322 us, 6.9 TB/s; 16384 tokens with norms 45.3 us, 5.9 TB/s; 4097 tokens with
+// norms 14.4 us; the append of 8.2K tokens 30.8 us, 5.3 TB/s.
 //
-// Layout: a row is held by LPR lanes (8 at D = 128 in 16 bits), each with two 16-byte vectors that hold whole pairs
-// (half pairs: the same place in each half of the rotated dims; interleaved: any vector), so a rotation needs no exchange and the norm three
-// shuffles.  A lane group takes up to four heads of one token: the angles are loaded once for them, and their vectors
-// are brought in by cp.async, 16 KB a CTA and 128 KB an SM in flight, which registers could not hold (register loads: 436 us
-// at best for the layer; 256 threads or eight heads a group: 325-455 us, and slower at 4097 tokens).
+// Layout: a row is held by LPR lanes (8 at D = 128 in 16 bits), each with two 16-byte vectors that hold whole pairs (half
+// pairs: the same place in each half of the rotated dims; interleaved: any vector), so a rotation needs no exchange and the
+// norm three shuffles.  A lane group takes up to four heads of one token and one tensor: the angles and the norm's weights
+// are loaded once for them, addresses advance by a stride, and their vectors are brought in by cp.async, 16 KB a CTA and
+// 96 KB an SM in flight, which registers could not hold (register loads: 436 us at best for the layer; 256 threads or eight
+// heads a group: 325-455 us, and slower at 4097 tokens).  Issue slots are the second bound: groups that ran over tensors'
+// borders, with tensor, address and weights found anew for each head, took 285 instructions for a lane's 16 elements, and
+// 50.6 us for the 16384 tokens, 18.5 us for the 4097.  Weights in registers want 78 of them: six CTAs an SM (five: 49.6 us;
+// seven, with spills: 47.5 us).
 #include "attn_common.cuh"
 #include "paged_common.cuh"
 
@@ -23,7 +27,7 @@ namespace spruce {
 
 constexpr int kRowThreads = 128;
 constexpr int kHeadsPerGroup = 4;
-constexpr int kRowCtasPerSm = 8;
+constexpr int kRowCtasPerSm = 6;
 
 __device__ __forceinline__ uint64_t unpack2(uint32_t v, __nv_bfloat16) {
   return f2_pack(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
@@ -162,30 +166,33 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtasPerSm)
   __shared__ uint4 stage[HC * 2][kRowThreads];  // a thread's own vectors: no barrier
   const int l = threadIdx.x & (lpr - 1);
   const unsigned block = blockIdx.x / chunks;
-  const int h0 = static_cast<int>(blockIdx.x - block * chunks) * hc;
+  // The CTA's heads, of one tensor: its chunks are the queries', then the keys' (then the values').
+  int h0 = static_cast<int>(blockIdx.x - block * chunks) * hc;
+  const int hq = (a.Hq + hc - 1) / hc * hc, hk = (a.Hkv + hc - 1) / hc * hc;
+  const bool isq = h0 < hq, isv = h0 >= hq + hk;
+  const Rows& r = isq ? a.q : (isv ? a.v : a.k);
+  h0 -= isq ? 0 : (isv ? hq + hk : hq);
+  const int rows = min(hc, (isq ? a.Hq : a.Hkv) - h0);
   const int64_t n = (int64_t)block * (kRowThreads / lpr) + threadIdx.x / lpr;
-  const int heads = a.Hq + (APPEND ? 2 : 1) * a.Hkv;  // query rows, key rows, (value rows)
-  const int rows = min(hc, heads - h0);
   const bool live = n < (int64_t)a.B * a.T;
   const int b = a.B == 1 ? 0 : static_cast<int>(n / a.T), t = static_cast<int>(n - (int64_t)b * a.T);
-  const int items = a.D / (2 * VN), nrot = a.rd / (2 * VN);
+  const int rd = isv ? 0 : a.rd, items = a.D / (2 * VN), nrot = rd / (2 * VN);
   // This lane's two vectors.  Half pairs: the same place in each half of the rotated dims (or of the rest).  Interleaved:
   // of each half of the head, as a pair lies in one vector.  Adjacent lanes take adjacent vectors either way.
   const bool in = live && l < items;
-  const bool rot = a.interleaved ? l * VN < a.rd : l < nrot;
-  const int oa = a.interleaved || rot ? l * VN : a.rd + (l - nrot) * VN;
-  const int ob = a.interleaved ? a.D / 2 + oa : (rot ? a.rd / 2 : (a.D - a.rd) / 2) + oa;
-  const bool rot_b = a.interleaved ? ob < a.rd : rot;
+  const bool rot = a.interleaved ? l * VN < rd : l < nrot;
+  const int oa = a.interleaved || rot ? l * VN : rd + (l - nrot) * VN;
+  const int ob = a.interleaved ? a.D / 2 + oa : (rot ? rd / 2 : (a.D - rd) / 2) + oa;
+  const bool rot_b = a.interleaved ? ob < rd : rot;
 
   // The rows first: where they go and how they turn takes dependent loads of its own.
+  const T* src = static_cast<const T*>(r.x) + b * r.sb + h0 * r.sh + t * r.st;
 #pragma unroll
   for (int i = 0; i < HC; ++i) {
     if (in && i < rows) {
-      int hh;
-      const Rows& r = rows_of(a, h0 + i, hh);
-      const T* src = static_cast<const T*>(r.x) + b * r.sb + hh * r.sh + t * r.st;
       copy16(&stage[2 * i][threadIdx.x], src + oa);
       copy16(&stage[2 * i + 1][threadIdx.x], src + ob);
+      src += r.sh;
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   }
@@ -196,38 +203,45 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtasPerSm)
     if (rot && in) {
       const float* c = w.angles + (a.interleaved ? oa / 2 : oa);
       load_pairs(c, cs[0], cs[1]);
-      load_pairs(c + a.rd / 2, sn[0], sn[1]);
+      load_pairs(c + rd / 2, sn[0], sn[1]);
     }
     if (rot_b && in) {
       const float* c = w.angles + (a.interleaved ? ob / 2 : oa + 4);
       load_pairs(c, cs[2], cs[3]);
-      load_pairs(c + a.rd / 2, sn[2], sn[3]);
+      load_pairs(c + rd / 2, sn[2], sn[3]);
     }
   } else if (in) {
     if (a.interleaved) {
       if (rot) {
         cs[0] = load_pair(w.angles + oa / 2);
-        sn[0] = load_pair(w.angles + a.rd / 2 + oa / 2);
+        sn[0] = load_pair(w.angles + rd / 2 + oa / 2);
       }
       if (rot_b) {
         cs[1] = load_pair(w.angles + ob / 2);
-        sn[1] = load_pair(w.angles + a.rd / 2 + ob / 2);
+        sn[1] = load_pair(w.angles + rd / 2 + ob / 2);
       }
     } else if (rot) {
       load_pairs(w.angles + oa, cs[0], cs[1]);
-      load_pairs(w.angles + a.rd / 2 + oa, sn[0], sn[1]);
+      load_pairs(w.angles + rd / 2 + oa, sn[0], sn[1]);
     }
   }
-  const bool norm = a.q.weight != nullptr || a.k.weight != nullptr;
+  const bool norm = r.weight != nullptr, store = in && w.write && (!APPEND || isq || w.cached);
+  const float per_dim = 1.0f / static_cast<float>(a.D);
+  T* dst = static_cast<T*>(r.out) +
+           (APPEND && !isq ? w.page * r.ob + h0 * r.oh + w.slot * r.ot : b * r.ob + h0 * r.oh + t * r.ot);
+  uint64_t wa[NP], wb[NP];
+  if (norm && in) {
+#pragma unroll
+    for (int e = 0; e < NP; e += 2) {
+      load_pairs(r.weight + oa + 2 * e, wa[e], wa[e + 1]);
+      load_pairs(r.weight + ob + 2 * e, wb[e], wb[e + 1]);
+    }
+  }
 
 #pragma unroll
   for (int i = 0; i < HC; ++i) {
     wait_copies(HC - 1 - i);
     if (i >= rows) break;  // of the whole CTA
-    int hh;
-    const int h = h0 + i;
-    const Rows& r = rows_of(a, h, hh);
-    const bool isq = h < a.Hq, isv = h >= a.Hq + a.Hkv;
     uint4 ra = make_uint4(0, 0, 0, 0), rb = ra;
     if (in) {
       ra = stage[2 * i][threadIdx.x];
@@ -247,18 +261,13 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtasPerSm)
         f2_unpack(s2, s0, s1);
         float ss = s0 + s1;
         for (int o = lpr >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        const float inv = rsqrtf(ss / static_cast<float>(a.D) + a.eps);
-        if (r.weight != nullptr && in) {
-          const uint64_t inv2 = f2_pack(inv, inv);
+        const float inv = rsqrtf(fmaf(ss, per_dim, a.eps));
+        const uint64_t inv2 = f2_pack(inv, inv);
+        if (in) {
 #pragma unroll
-          for (int e = 0; e < NP; e += 2) {
-            uint64_t w0, w1;
-            load_pairs(r.weight + oa + 2 * e, w0, w1);
-            x[e] = f2_mul(x[e], f2_mul(w0, inv2));
-            x[e + 1] = f2_mul(x[e + 1], f2_mul(w1, inv2));
-            load_pairs(r.weight + ob + 2 * e, w0, w1);
-            y[e] = f2_mul(y[e], f2_mul(w0, inv2));
-            y[e + 1] = f2_mul(y[e + 1], f2_mul(w1, inv2));
+          for (int e = 0; e < NP; ++e) {
+            x[e] = f2_mul(x[e], f2_mul(wa[e], inv2));
+            y[e] = f2_mul(y[e], f2_mul(wb[e], inv2));
           }
         }
       }
@@ -279,11 +288,11 @@ __global__ void __launch_bounds__(kRowThreads, kRowCtasPerSm)
       ra = pack16<T>(x);
       rb = pack16<T>(y);
     }
-    if (!in || !w.write || (APPEND && !isq && !w.cached)) continue;
-    T* dst = static_cast<T*>(r.out) +
-             (APPEND && !isq ? w.page * r.ob + hh * r.oh + w.slot * r.ot : b * r.ob + hh * r.oh + t * r.ot);
-    *reinterpret_cast<uint4*>(dst + oa) = ra;
-    *reinterpret_cast<uint4*>(dst + ob) = rb;
+    if (store) {
+      *reinterpret_cast<uint4*>(dst + oa) = ra;
+      *reinterpret_cast<uint4*>(dst + ob) = rb;
+    }
+    dst += r.oh;
   }
 }
 
@@ -364,9 +373,10 @@ static cudaError_t launch_rows_typed(const RowsArgs& a, bool vec, cudaStream_t s
   const int64_t blocks = (tokens + per - 1) / per;
   // Four rows a group keep enough bytes in flight; where that leaves SMs without work, one: 64 single tokens of 36 rows take
   // 4.2 us so, 5.3 us with two.
+  auto chunks_of = [&](int hc) { return (a.Hq + hc - 1) / hc + (APPEND ? 2 : 1) * ((a.Hkv + hc - 1) / hc); };
   int hc = kHeadsPerGroup;
-  if (blocks * ((heads + hc - 1) / hc) < 2 * 148) hc = 1;
-  const int chunks = (heads + hc - 1) / hc;
+  if (blocks * chunks_of(hc) < 2 * 148) hc = 1;
+  const int chunks = chunks_of(hc);
   if (blocks * chunks > 0x7fffffff) return cudaErrorInvalidValue;
   norm_rope_kernel<T, APPEND><<<(unsigned)(blocks * chunks), kRowThreads, 0, stream>>>(a, lpr, hc, chunks);
   return cudaGetLastError();
