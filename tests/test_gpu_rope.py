@@ -176,6 +176,35 @@ def test_append_matches_64_bits_and_touches_nothing_else(dtype, qlens, clens, pa
     assert torch.equal(kc2, kc) and torch.equal(vc2, vc)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("D,rd,interleaved,sides", [
+    (128, 64, False, "qk"), (64, 64, True, "q"), (80, 48, True, "k"), (96, 64, False, "")])
+@pytest.mark.parametrize("Hq,Hkv", [(7, 3), (4, 5)])
+def test_many_tokens_whose_heads_leave_part_of_a_group(dtype, D, rd, interleaved, sides, Hq, Hkv):
+    """Enough tokens that a lane group takes four heads; the last group of each tensor is short; norms on either side."""
+    g = torch.Generator(device="cuda").manual_seed(11)
+    B, T = 2, 2003
+    qkv = torch.randn(B, T, Hq + 2 * Hkv, D, generator=g, device="cuda", dtype=dtype)
+    q, k, v = (x.transpose(1, 2) for x in qkv.split([Hq, Hkv, Hkv], 2))
+    table = torch.randn(B * T, rd, generator=g, device="cuda")
+    wq, wk = (torch.randn(D, generator=g, device="cuda") if side in sides else None for side in "qk")
+    qo, ko = native.qk_norm_rope(q, k, table, q_weight=wq, k_weight=wk, eps=1e-5, interleaved=interleaved)
+    check(qo, turned(q, wq, table[:T], rd, interleaved, 1e-5))
+    check(ko, turned(k, wk, table[:T], rd, interleaved, 1e-5))
+    # the same rows as one sequence of B * T tokens into pages
+    flat = qkv.flatten(0, 1)
+    q, k, v = flat.split([Hq, Hkv, Hkv], 1)
+    pages, cu, kv, count = _batch([B * T], [0], 32, 5)
+    kc, vc = (torch.zeros(count, Hkv, 32, D, device="cuda", dtype=dtype) for _ in range(2))
+    qo = native.paged_append(k, v, kc, vc, pages, cu, kv, q=q, rope=table, q_weight=wq, k_weight=wk, eps=1e-5,
+                             interleaved=interleaved)
+    at = torch.arange(B * T, device="cuda")
+    rows = pages[0, at // 32].long()
+    check(qo, turned(q, wq, table[:, None], rd, interleaved, 1e-5))
+    check(kc[rows, :, at % 32], turned(k, wk, table[:, None], rd, interleaved, 1e-5))
+    assert torch.equal(vc[rows, :, at % 32], v)
+
+
 def test_append_skips_bad_pages_and_lengths():
     D, page = 64, 16
     k = torch.randn(3, 1, D, device="cuda")
