@@ -469,6 +469,14 @@ def _ptr(t: torch.Tensor | None) -> int:
     return 0 if t is None else t.data_ptr()
 
 
+def _status_ptr(t: torch.Tensor | None) -> int:
+    if t is None:
+        return 0
+    if t.dtype is not torch.int32 or t.numel() < 1:
+        raise ValueError("status must be an int32 tensor of at least one element")
+    return t.data_ptr()
+
+
 def _head_weight(w: torch.Tensor | None, D: int, name: str) -> torch.Tensor | None:
     if w is None:
         return None
@@ -532,7 +540,7 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, rope: torch.Tensor, positions
         raise ValueError(f"an output must be {dtype} {tuple(k.shape)} with a unit last stride")
     args = _lib.QK_NORM_ROPE_ARGS.pack(
         q.data_ptr(), k.data_ptr(), q_out.data_ptr(), k_out.data_ptr(), rope.data_ptr(), _ptr(positions),
-        _ptr(q_weight), _ptr(k_weight), _ptr(status), _lib.stream_on(device), *q.stride(), *k.stride(),
+        _ptr(q_weight), _ptr(k_weight), _status_ptr(status), _lib.stream_on(device), *q.stride(), *k.stride(),
         *q_out.stride(), *k_out.stride(), *pos_strides, _dt(q), B, Hq, Hkv, T, D, *rope.shape, interleaved, eps)
     _lib.check(_lib.load().spruce_qk_norm_rope(args))
     return q_out, k_out
@@ -624,8 +632,8 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
     args = _lib.PAGED_APPEND_ARGS.pack(
         _ptr(q), k.data_ptr(), v.data_ptr(), _ptr(q_out), k_cache.data_ptr(), v_cache.data_ptr(), _ptr(rope),
         _ptr(positions), _ptr(q_weight), _ptr(k_weight), block_table.data_ptr(), cu_q.data_ptr(), kv_lens.data_ptr(),
-        _ptr(status), _lib.stream_on(device), qn, qh, kn, kh, vn, vh, on, oh, *kc_strides[:3], *vc_strides[:3], _dt(k),
-        N, S, Hq, Hkv, D, pages, page_size, step, width, table_rows, rd, interleaved, eps)
+        _status_ptr(status), _lib.stream_on(device), qn, qh, kn, kh, vn, vh, on, oh, *kc_strides[:3],
+        *vc_strides[:3], _dt(k), N, S, Hq, Hkv, D, pages, page_size, step, width, table_rows, rd, interleaved, eps)
     _lib.check(_lib.load().spruce_paged_append(args))
     return q_out
 
@@ -677,7 +685,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         nbytes = workspace.nbytes
     args = _lib.PAGED_ATTENTION_ARGS.pack(
         q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), block_table.data_ptr(), cu_q.data_ptr(),
-        kv_lens.data_ptr(), workspace.data_ptr(), _ptr(status), _lib.stream_on(device), qn, qh, *kc_strides[:3],
+        kv_lens.data_ptr(), workspace.data_ptr(), _status_ptr(status), _lib.stream_on(device), qn, qh, *kc_strides[:3],
         *vc_strides[:3], on, oh, dt, N, S, Hq, Hkv, D, pages, page_size, step, width, max_q_len, max_kv_len, nbytes,
         D ** -0.5 if scale is None else scale)
     _lib.check(_lib.load().spruce_paged_attention(args))

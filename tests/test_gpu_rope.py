@@ -269,3 +269,17 @@ def test_refusals():
         native.paged_append(x, x, cache, cache, bt, cu, kv, q=x[:2])
     with pytest.raises(ValueError, match="q_out without q"):
         native.paged_append(x, x, cache, cache, bt, cu, kv, q_out=x)
+
+
+@pytest.mark.parametrize("status", [torch.int64, torch.float32, None])
+def test_a_status_of_another_type_or_without_an_element_is_refused(status):
+    status = torch.zeros(int(status is not None), device="cuda", dtype=status or torch.int32)
+    x = torch.zeros(3, 2, 64, device="cuda", dtype=torch.bfloat16)
+    cache = torch.zeros(4, 2, 16, 64, device="cuda", dtype=torch.bfloat16)
+    bt, cu, kv = (torch.zeros(s, device="cuda", dtype=torch.int32) for s in ((1, 2), (2,), (1,)))
+    with pytest.raises(ValueError, match="status"):
+        native.qk_norm_rope(x[None], x[None], rope_table(64, 8), status=status)
+    with pytest.raises(ValueError, match="status"):
+        native.paged_append(x, x, cache, cache, bt, cu, kv, status=status)
+    with pytest.raises(ValueError, match="status"):
+        native.paged_attention(x, cache, cache, bt, cu, kv, max_q_len=3, max_kv_len=3, status=status)
