@@ -171,178 +171,182 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   __syncwarp();
   const PagedPiece& x = role->x;
 
-  if (warp == kChunkLoadK || warp == kChunkLoadV) {
-    // ------------------------------------------------------------ K or V
+  // All warps of a warpgroup execute the same setmaxnreg, the idle one included, before their roles part.
+  if (warp >= kChunkMma) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-    const bool v = warp == kChunkLoadV;
-    const CUtensorMap* const map = v ? &tmv : &tmk;
-    uint8_t* const base = smem + (v ? L::OFF_V : L::OFF_K);
-    uint64_t* const full = v ? v_full : k_full;
-    uint64_t* const empty = v ? v_empty : k_empty;
-    const int stages = v ? VST : KST;
-    const int boxes = kChunkKeys / box;  // of a tile's rows: at most 8
-    const bool leader = elect_one();
-    int st = 0, loaded = 0;              // the next tile's stage; tiles loaded
-    uint32_t turn = 1, tails = 0;        // parity of the stage's last release (none before the first round)
-    bool ok = true;
-    while (ok && next_piece(p, role)) {
-      if (x.keys == 0) continue;
-      const int keys = x.keys, t1 = x.t1, g = x.g;
-      const int32_t* table = p.a.block_table + x.s * p.a.table_stride;
-      // Lane b: page of box b of tile t; past the keys (or the table) a page index that reads zeros.
-      auto page_of = [&](int t) {
-        const int key = t * kChunkKeys + lane * box;
-        if (lane >= boxes || t >= t1 || key >= keys) return static_cast<int>(p.a.num_pages);
-        const int page = paged_page(p, table, key / p.a.page_size);
-        return page < 0 ? static_cast<int>(p.a.num_pages) : page;
-      };
-      int page = page_of(x.t0);
-      int row = (x.t0 * kChunkKeys) % p.a.page_size;       // of the next box in its page
-      for (int t = x.t0; t < t1; ++t) {
-        if (loaded >= stages && !(ok = __all_sync(0xffffffffu, mbar_wait(&empty[st], turn, status, abort_flag)))) break;
-        uint8_t* dst = base + st * L::TILE;
-        const int valid = keys - t * kChunkKeys;           // keys of this tile that exist
-        const bool tail = v && valid < kChunkKeys && valid % box != 0;
-        uint64_t* const bar = tail ? v_tail : &full[st];
-        if (leader) mbar_arrive_expect_tx(bar, L::TILE);
-        __syncwarp();
-        for (int b = 0; b < boxes; ++b) {
-          const int pb = __shfl_sync(0xffffffffu, page, b);
-          if (leader) {
+    if (warp == kChunkLoadK || warp == kChunkLoadV) {
+      // ------------------------------------------------------------ K or V
+      const bool v = warp == kChunkLoadV;
+      const CUtensorMap* const map = v ? &tmv : &tmk;
+      uint8_t* const base = smem + (v ? L::OFF_V : L::OFF_K);
+      uint64_t* const full = v ? v_full : k_full;
+      uint64_t* const empty = v ? v_empty : k_empty;
+      const int stages = v ? VST : KST;
+      const int boxes = kChunkKeys / box;  // of a tile's rows: at most 8
+      const bool leader = elect_one();
+      int st = 0, loaded = 0;              // the next tile's stage; tiles loaded
+      uint32_t turn = 1, tails = 0;        // parity of the stage's last release (none before the first round)
+      bool ok = true;
+      while (ok && next_piece(p, role)) {
+        if (x.keys == 0) continue;
+        const int keys = x.keys, t1 = x.t1, g = x.g;
+        const int32_t* table = p.a.block_table + x.s * p.a.table_stride;
+        // Lane b: page of box b of tile t; past the keys (or the table) a page index that reads zeros.
+        auto page_of = [&](int t) {
+          const int key = t * kChunkKeys + lane * box;
+          if (lane >= boxes || t >= t1 || key >= keys) return static_cast<int>(p.a.num_pages);
+          const int page = paged_page(p, table, key / p.a.page_size);
+          return page < 0 ? static_cast<int>(p.a.num_pages) : page;
+        };
+        int page = page_of(x.t0);
+        int row = (x.t0 * kChunkKeys) % p.a.page_size;       // of the next box in its page
+        for (int t = x.t0; t < t1; ++t) {
+          if (loaded >= stages && !(ok = __all_sync(0xffffffffu, mbar_wait(&empty[st], turn, status, abort_flag)))) break;
+          uint8_t* dst = base + st * L::TILE;
+          const int valid = keys - t * kChunkKeys;           // keys of this tile that exist
+          const bool tail = v && valid < kChunkKeys && valid % box != 0;
+          uint64_t* const bar = tail ? v_tail : &full[st];
+          if (leader) mbar_arrive_expect_tx(bar, L::TILE);
+          __syncwarp();
+          for (int b = 0; b < boxes; ++b) {
+            const int pb = __shfl_sync(0xffffffffu, page, b);
+            if (leader) {
 #pragma unroll
-            for (int pp = 0; pp < L::NP; ++pp)
-              tma_load_4d(dst + pp * L::PANEL + b * box * 128, map, bar, pp * 64, row, g, pb);
+              for (int pp = 0; pp < L::NP; ++pp)
+                tma_load_4d(dst + pp * L::PANEL + b * box * 128, map, bar, pp * 64, row, g, pb);
+            }
+            __syncwarp();
+            row += box;
+            if (row == p.a.page_size) row = 0;
           }
-          __syncwarp();
-          row += box;
-          if (row == p.a.page_size) row = 0;
-        }
-        page = page_of(t + 1);  // its latency passes behind the wait for the next stage
-        if (tail) {
-          ok = __all_sync(0xffffffffu, mbar_wait(v_tail, tails & 1, status, abort_flag));
-          ++tails;
-          // Rows past the end, to the end of their box (whole 16-byte chunks: any swizzle).
-          const int end = min(kChunkKeys, (valid / box + 1) * box);
-          for (int e = lane; e < (end - valid) * 8 * L::NP; e += 32) {
-            const int panel = e / ((end - valid) * 8), c = e % ((end - valid) * 8);
-            *reinterpret_cast<uint4*>(dst + panel * L::PANEL + (valid + c / 8) * 128 + c % 8 * 16) = make_uint4(0, 0, 0, 0);
+          page = page_of(t + 1);  // its latency passes behind the wait for the next stage
+          if (tail) {
+            ok = __all_sync(0xffffffffu, mbar_wait(v_tail, tails & 1, status, abort_flag));
+            ++tails;
+            // Rows past the end, to the end of their box (whole 16-byte chunks: any swizzle).
+            const int end = min(kChunkKeys, (valid / box + 1) * box);
+            for (int e = lane; e < (end - valid) * 8 * L::NP; e += 32) {
+              const int panel = e / ((end - valid) * 8), c = e % ((end - valid) * 8);
+              *reinterpret_cast<uint4*>(dst + panel * L::PANEL + (valid + c / 8) * 128 + c % 8 * 16) = make_uint4(0, 0, 0, 0);
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&full[st]);
           }
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&full[st]);
+          ++loaded;
+          if (++st == stages) {
+            st = 0;
+            turn ^= 1;
+          }
+          if (!ok) break;
         }
-        ++loaded;
-        if (++st == stages) {
-          st = 0;
-          turn ^= 1;
-        }
-        if (!ok) break;
       }
-    }
-    // No copy may be in flight when the CTA exits.
-    for (int k = max(0, loaded - stages); k < loaded; ++k)
-      mbar_wait(&full[k % stages], (k / stages) & 1, status, nullptr);
-    __syncwarp();
-  } else if (warp == kChunkMma) {
-    // ------------------------------------------------------------ MMA issuer
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-    const bool leader = elect_one();
-    constexpr uint32_t fmt = UmmaFormat<T>::value;
-    constexpr uint32_t idesc_qk = idesc_f16(fmt, 0, 0, 128, 128);
-    constexpr uint32_t idesc_pv = idesc_f16(fmt, 0, 1, D, 128);
-    const uint64_t dq0 = smem_desc(smem_u32(smem + L::OFF_Q), 16, 1024);
-    const uint64_t dk0 = smem_desc(smem_u32(smem + L::OFF_K), 16, 1024);
-    const uint64_t dv0 = smem_desc(smem_u32(smem + L::OFF_V), L::PANEL, 1024);
-    auto commit = [&](uint64_t* bar) {
-      if (leader) umma_commit(bar);
+      // No copy may be in flight when the CTA exits.
+      for (int k = max(0, loaded - stages); k < loaded; ++k)
+        mbar_wait(&full[k % stages], (k / stages) & 1, status, nullptr);
       __syncwarp();
-    };
-    auto wait = [&](uint64_t* bar, uint32_t parity) {
-      return __all_sync(0xffffffffu, mbar_wait(bar, parity, status, abort_flag));
-    };
-    auto issue_qk = [&](int t, int st) {
-      const uint32_t d = tmem + L::COL_S + 128 * t;
-      const uint64_t qa = dq0 + (uint64_t)((t * L::TILE) >> 4);
-      const uint64_t kb = dk0 + (uint64_t)((st * L::TILE) >> 4);
-#pragma unroll
-      for (int ks = 0; ks < D / 16; ++ks) {
-        const uint32_t off = ((ks >> 2) * L::PANEL + (ks & 3) * 32) >> 4;
-        if (leader) umma_f16_ss(d, qa + off, kb + off, idesc_qk, ks > 0 ? 1u : 0u);
+    } else if (warp == kChunkMma) {
+      // ------------------------------------------------------------ MMA issuer
+      const bool leader = elect_one();
+      constexpr uint32_t fmt = UmmaFormat<T>::value;
+      constexpr uint32_t idesc_qk = idesc_f16(fmt, 0, 0, 128, 128);
+      constexpr uint32_t idesc_pv = idesc_f16(fmt, 0, 1, D, 128);
+      const uint64_t dq0 = smem_desc(smem_u32(smem + L::OFF_Q), 16, 1024);
+      const uint64_t dk0 = smem_desc(smem_u32(smem + L::OFF_K), 16, 1024);
+      const uint64_t dv0 = smem_desc(smem_u32(smem + L::OFF_V), L::PANEL, 1024);
+      auto commit = [&](uint64_t* bar) {
+        if (leader) umma_commit(bar);
         __syncwarp();
-      }
-      commit(&s_full[t]);
-    };
-    uint32_t pvs[2] = {0, 0};  // PVs issued for each tile
-    auto pv_half = [&](int t, int st, int h, bool first) {
-      if (!wait(&p_full[2 * t + h], pvs[t] & 1)) return false;
-      tc_fence_after();
-      const uint32_t a = tmem + L::COL_S + 128 * t;
-      const uint64_t vb = dv0 + (uint64_t)((st * L::TILE) >> 4);
+      };
+      auto wait = [&](uint64_t* bar, uint32_t parity) {
+        return __all_sync(0xffffffffu, mbar_wait(bar, parity, status, abort_flag));
+      };
+      auto issue_qk = [&](int t, int st) {
+        const uint32_t d = tmem + L::COL_S + 128 * t;
+        uint64_t qa = dq0 + (uint64_t)((t * L::TILE) >> 4);
+        uint64_t kb = dk0 + (uint64_t)((st * L::TILE) >> 4);
+        asm volatile("" : "+l"(qa), "+l"(kb));  // steps added here: kept ahead of the loop they spill at 88 registers
 #pragma unroll
-      for (int kk = 0; kk < 4; ++kk) {
-        const int ks = 4 * h + kk;
-        if (leader)
-          umma_f16_ts(tmem + t * D, a + ks * 8, vb + (uint64_t)((ks * 2048) >> 4), idesc_pv,
-                      (!first || ks > 0) ? 1u : 0u);
-        __syncwarp();
-      }
-      if (h == 1) ++pvs[t];
-      return true;
-    };
-    uint32_t pieces[2] = {0, 0};
-    int kst = 0, vst = 0;            // stages of the next K and V tile, and the parities of their turns
-    uint32_t kturn = 0, vturn = 0;
-    bool ok = true;
-    auto next_k = [&] {
-      if (++kst == KST) {
-        kst = 0;
-        kturn ^= 1;
-      }
-    };
-    while (ok && next_piece(p, role)) {
-      const bool two = x.q.qlen * p.rep - x.qt * kChunkRows > 128;
-      if (x.keys == 0) continue;
-      const int n = x.t1 - x.t0;
-      ok = wait(&q_full[0], pieces[0]++ & 1) && (!two || wait(&q_full[1], pieces[1]++ & 1)) &&
-           wait(&k_full[kst], kturn);
-      if (!ok) break;
-      tc_fence_after();
-      issue_qk(0, kst);
-      if (two) issue_qk(1, kst);
-      commit(&k_empty[kst]);
-      next_k();
-      for (int i = 0; i < n; ++i) {
-        // A check of a barrier waits behind this warp's queued MMAs, so what PV_t(i) and QK_t(i+1) need is checked
-        // before them and they are issued without a pause.
-        const bool more = i + 1 < n;
-        if (!(ok = wait(&v_full[vst], vturn) && (!more || wait(&k_full[kst], kturn)))) break;
-        if (!(ok = pv_half(0, vst, 0, i == 0) && pv_half(0, vst, 1, i == 0))) break;
-        if (more)
-          issue_qk(0, kst);
-        else
-          commit(&o_done[0]);
-        if (two) {
-          if (!(ok = pv_half(1, vst, 0, i == 0) && pv_half(1, vst, 1, i == 0))) break;
+        for (int ks = 0; ks < D / 16; ++ks) {
+          const uint32_t off = ((ks >> 2) * L::PANEL + (ks & 3) * 32) >> 4;
+          if (leader) umma_f16_ss(d, qa + off, kb + off, idesc_qk, ks > 0 ? 1u : 0u);
+          __syncwarp();
+        }
+        commit(&s_full[t]);
+      };
+      uint32_t pvs[2] = {0, 0};  // PVs issued for each tile
+      auto pv_half = [&](int t, int st, int h, bool first) {
+        if (!wait(&p_full[2 * t + h], pvs[t] & 1)) return false;
+        tc_fence_after();
+        const uint32_t a = tmem + L::COL_S + 128 * t;
+        uint64_t vb = dv0 + (uint64_t)((st * L::TILE) >> 4);
+        asm volatile("" : "+l"(vb));
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) {
+          const int ks = 4 * h + kk;
+          if (leader)
+            umma_f16_ts(tmem + t * D, a + ks * 8, vb + (uint64_t)((ks * 2048) >> 4), idesc_pv,
+                        (!first || ks > 0) ? 1u : 0u);
+          __syncwarp();
+        }
+        if (h == 1) ++pvs[t];
+        return true;
+      };
+      uint32_t pieces[2] = {0, 0};
+      int kst = 0, vst = 0;            // stages of the next K and V tile, and the parities of their turns
+      uint32_t kturn = 0, vturn = 0;
+      bool ok = true;
+      auto next_k = [&] {
+        if (++kst == KST) {
+          kst = 0;
+          kturn ^= 1;
+        }
+      };
+      while (ok && next_piece(p, role)) {
+        const bool two = x.q.qlen * p.rep - x.qt * kChunkRows > 128;
+        if (x.keys == 0) continue;
+        const int n = x.t1 - x.t0;
+        ok = wait(&q_full[0], pieces[0]++ & 1) && (!two || wait(&q_full[1], pieces[1]++ & 1)) &&
+             wait(&k_full[kst], kturn);
+        if (!ok) break;
+        tc_fence_after();
+        issue_qk(0, kst);
+        if (two) issue_qk(1, kst);
+        commit(&k_empty[kst]);
+        next_k();
+        for (int i = 0; i < n; ++i) {
+          // A check of a barrier waits behind this warp's queued MMAs, so what PV_t(i) and QK_t(i+1) need is checked
+          // before them and they are issued without a pause.
+          const bool more = i + 1 < n;
+          if (!(ok = wait(&v_full[vst], vturn) && (!more || wait(&k_full[kst], kturn)))) break;
+          if (!(ok = pv_half(0, vst, 0, i == 0) && pv_half(0, vst, 1, i == 0))) break;
           if (more)
-            issue_qk(1, kst);
+            issue_qk(0, kst);
           else
-            commit(&o_done[1]);
-        }
-        commit(&v_empty[vst]);  // every MMA reading these stages is issued before this
-        if (++vst == VST) {
-          vst = 0;
-          vturn ^= 1;
-        }
-        if (more) {
-          commit(&k_empty[kst]);
-          next_k();
+            commit(&o_done[0]);
+          if (two) {
+            if (!(ok = pv_half(1, vst, 0, i == 0) && pv_half(1, vst, 1, i == 0))) break;
+            if (more)
+              issue_qk(1, kst);
+            else
+              commit(&o_done[1]);
+          }
+          commit(&v_empty[vst]);  // every MMA reading these stages is issued before this
+          if (++vst == VST) {
+            vst = 0;
+            vturn ^= 1;
+          }
+          if (more) {
+            commit(&k_empty[kst]);
+            next_k();
+          }
         }
       }
+      commit(drain);  // no MMA may be in flight when TMEM is released
+      mbar_wait(drain, 0, status, nullptr);
+      __syncwarp();
     }
-    commit(drain);  // no MMA may be in flight when TMEM is released
-    mbar_wait(drain, 0, status, nullptr);
-    __syncwarp();
-  } else if (warp < kChunkMma) {
+  } else {
     // ------------------------------------------------------------ softmax + epilogue
     asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     const int t = warp >> 2;
@@ -547,8 +551,6 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       }
       tc_fence_before();  // O and S are read before the next piece's MMAs, which wait for its Q
     }
-  } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");  // the last warp only fills its warpgroup
   }
 
   tc_fence_before();
