@@ -455,8 +455,8 @@ SPRUCE_API int spruce_qk_norm_rope(const spruce_qk_norm_rope_args *args);
  * `positions` [N] gives them.  rd = 0: no rotation.  q_out [N, Hq, D] (NULL with
  * q) may be q.  Strides of packed tensors are (token, head).  A token whose
  * position lies outside its table row, or whose page id lies outside the cache,
- * is not written and raises SPRUCE_STATUS_BAD_LENGTH / _BAD_PAGE; tokens past
- * cu_q[S] are left out.
+ * is not written and raises SPRUCE_STATUS_BAD_LENGTH / _BAD_PAGE; tokens before
+ * cu_q[0] and past cu_q[S] are of no sequence and left out, their rows of q_out too.
  */
 typedef struct {
   const void *q, *k, *v;
@@ -477,8 +477,8 @@ SPRUCE_API int spruce_paged_append(const spruce_paged_append_args *args);
  * Causal GQA attention of new tokens over a paged cache: sequence s's query i
  * (packed as above, already in the cache) sees positions 0 .. kv_lens[s] -
  * q_len + i.  From single tokens to prefill chunks, of any mix of lengths; a
- * query that sees nothing (an empty sequence) yields zeros, rows past cu_q[S]
- * are not written.  Cache rows at or past kv_lens[s] never reach an output,
+ * query that sees nothing (an empty sequence) yields zeros, rows before cu_q[0]
+ * and past cu_q[S] are not written.  Cache rows at or past kv_lens[s] never reach an output,
  * whatever they hold; a value of the sequence itself that is not finite may
  * reach every query whose key tile holds it.  max_q_len and max_kv_len bound q_len and kv_lens (they
  * size the launch); a longer sequence is cut to them and raises

@@ -126,8 +126,10 @@ __device__ __forceinline__ TokenPlace place_token(const RowsArgs& a, bool live, 
           else hi = mid;
         }
         s = lo;
+        first = a.cu_q[s];
         next = a.cu_q[s + 1];
         kv = a.kv_lens[s];
+        w.write = first <= n && n < next;  // else the token is before the first sequence
       }
       pos = (int64_t)kv - next + n;
       const int p = pos >= 0 && pos < 0x7fffffff ? static_cast<int>(pos) : -1;

@@ -575,8 +575,8 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
                  q_out: torch.Tensor | None = None, status: torch.Tensor | None = None) -> torch.Tensor | None:
     """Write new keys and values [N, Hkv, D] into a paged cache, normed and rotated on the way; returns q likewise.
 
-    The packed tokens of sequence s are ``cu_q[s] .. cu_q[s+1]``; ``kv_lens[s]`` is its length after the call, so its
-    token i lands at position ``kv_lens[s] - q_len + i`` (page ``block_table[s, position // page_size]`` of
+    The packed tokens of sequence s are ``cu_q[s] .. cu_q[s+1]`` (those before ``cu_q[0]`` or past ``cu_q[-1]`` are left
+    out, in the result too); ``kv_lens[s]`` is its length after the call, so its token i lands at position ``kv_lens[s] - q_len + i`` (page ``block_table[s, position // page_size]`` of
     ``k_cache`` / ``v_cache`` [pages, Hkv, page_size, D]).  ``rope`` None: no rotation.  ``positions`` int [N]
     replaces the cache positions in the rotation only.  With ``q`` [N, Hq, D], its norm and rotation run in the
     same launch into ``q_out`` (a new [N, Hq, D] tensor by default; q itself is allowed).
@@ -651,7 +651,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
 
     The last new token of sequence s sees ``kv_lens[s]`` keys, the one before it one fewer, and so on; queries that
     see none give zeros.  ``max_q_len`` and ``max_kv_len`` bound the sequences' new tokens and lengths (the lengths
-    themselves stay on the device).  Returns [N, Hq, D]; rows past ``cu_q[-1]`` are not written.
+    themselves stay on the device).  Returns [N, Hq, D]; rows before ``cu_q[0]`` and past ``cu_q[-1]`` are not written.
     """
     device = q.get_device()
     if not (device == k_cache.get_device() == v_cache.get_device() == block_table.get_device() == cu_q.get_device()
