@@ -2,7 +2,11 @@
 import os
 import re
 
-from spruce_research_b200 import build
+import pytest
+import torch
+
+from spruce_research_b200 import build, native
+from spruce_research_b200.paged import PagedKVCache, PagedSparseLayer
 
 CSRC = build.CSRC
 
@@ -17,3 +21,34 @@ def test_a_warpgroup_gives_up_registers_by_one_instruction():
     assert re.search(r"\} else \{\s*asm volatile\(\"setmaxnreg\.inc", code)
     roles = {k: int(v) for k, v in re.findall(r"constexpr int kChunk(Mma|Threads) = (\d+);", code)}
     assert roles["Mma"] % 4 == 0 and roles["Threads"] == 32 * (roles["Mma"] + 4)   # whole warpgroups either side
+
+
+def _cache(pages=6, page=16):
+    return PagedKVCache(1, pages, page, 2, 64, torch.float32, "cpu")
+
+
+def _no_kernels(monkeypatch):
+    """Entry points that only note that they were called."""
+    calls = []
+    for name in ("paged_append", "paged_attention", "qk_norm_rope"):
+        def call(*args, called=name, **kw):
+            calls.append(called)
+            return args[:2] if called == "qk_norm_rope" else args[0]
+        monkeypatch.setattr(native, name, call)
+    return calls
+
+
+def test_a_layer_refuses_a_step_past_its_rotation_table(monkeypatch):
+    calls = _no_kernels(monkeypatch)
+    c = _cache()
+    layer = PagedSparseLayer(c, 0, torch.zeros(20, 64), prefill=lambda q, k, v: (q, None))
+    x = torch.zeros(21, 2, 64)
+    layer.extend(x[:20], x[:20], x[:20], c.step([("a", 20)]))
+    assert calls == ["paged_append", "paged_attention"]
+    step = c.step([("a", 1), ("b", 3)])
+    with pytest.raises(ValueError, match="21 tokens need a rotation table"):
+        layer.extend(x[:4], x[:4], x[:4], step)
+    step = c.step([("c", 21)])
+    with pytest.raises(ValueError, match="21 tokens need a rotation table"):
+        layer.prefill(x, x, x, step)
+    assert calls == ["paged_append", "paged_attention"]
