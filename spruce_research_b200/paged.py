@@ -116,16 +116,22 @@ class PagedSparseLayer:
         self.rope, self.sparse = rope, prefill
         self.rotation = dict(q_weight=q_weight, k_weight=k_weight, eps=eps, interleaved=interleaved)
 
-    def _check(self, step: PagedStep) -> None:
-        """What the host knows: the kernels would only report it in a status word and take the nearest angles."""
+    def _check(self, tensors, step: PagedStep, spare: bool) -> None:
+        """What the host knows: the kernels would leave rows out, take the nearest angles and only report it in a status."""
+        rows = [x.shape[0] for x in tensors]
+        if min(rows) < step.tokens or not spare and max(rows) > step.tokens:
+            raise ValueError(f"the step has {step.tokens} tokens, q, k and v have {rows}")
         if self.rope is not None and step.max_kv_len > self.rope.shape[0]:
             raise ValueError(f"sequences of {step.max_kv_len} tokens need a rotation table of as many positions, got "
                              f"{self.rope.shape[0]}")
 
     def extend(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, step: PagedStep,
                out: torch.Tensor | None = None) -> torch.Tensor:
-        """Append the step's tokens and attend over all each sequence holds: [N, Hq, D]."""
-        self._check(step)
+        """Append the step's tokens and attend over all each sequence holds: [N, Hq, D].
+
+        N may exceed the step's tokens; the rows past them are not written.
+        """
+        self._check((q, k, v), step, spare=True)
         q = native.paged_append(k, v, self.k_cache, self.v_cache, step.block_table, step.cu_q, step.kv_lens, q=q,
                                 rope=self.rope, **self.rotation)
         return native.paged_attention(q, self.k_cache, self.v_cache, step.block_table, step.cu_q, step.kv_lens,
@@ -140,7 +146,7 @@ class PagedSparseLayer:
             raise ValueError("this layer was made without a SparsePrefillLayer")
         if len(step.seq_ids) != 1 or step.max_q_len != step.max_kv_len:
             raise ValueError("the sparse prefill takes one whole prompt: one sequence that held nothing before")
-        self._check(step)
+        self._check((q, k, v), step, spare=False)
         qs, ks, vs = (x.transpose(0, 1).unsqueeze(0) for x in (q, k, v))       # [1, H, T, D] views
         qr, kr = native.qk_norm_rope(qs, ks, self.rope, **self.rotation)
         native.paged_append(kr[0].transpose(0, 1), v, self.k_cache, self.v_cache, step.block_table, step.cu_q,

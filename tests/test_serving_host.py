@@ -52,3 +52,23 @@ def test_a_layer_refuses_a_step_past_its_rotation_table(monkeypatch):
     with pytest.raises(ValueError, match="21 tokens need a rotation table"):
         layer.prefill(x, x, x, step)
     assert calls == ["paged_append", "paged_attention"]
+
+
+def test_a_layer_refuses_tensors_of_another_number_of_tokens(monkeypatch):
+    """Fewer rows than the step has tokens would leave cache rows unwritten that its lengths count."""
+    calls = _no_kernels(monkeypatch)
+    c = _cache()
+    layer = PagedSparseLayer(c, 0, torch.zeros(64, 64), prefill=lambda q, k, v: (q, None))
+    x = torch.zeros(5, 2, 64)
+    step = c.step([("a", 4)])
+    for bad in ((x[:3], x[:4], x[:4]), (x[:4], x[:3], x[:4]), (x[:4], x[:4], x[:3])):
+        with pytest.raises(ValueError, match="the step has 4 tokens"):
+            layer.extend(*bad, step)
+        with pytest.raises(ValueError, match="the step has 4 tokens"):
+            layer.prefill(*bad, step)
+    with pytest.raises(ValueError, match="the step has 4 tokens"):      # the selector would pool the rows past the prompt
+        layer.prefill(x, x, x, step)
+    assert not calls
+    layer.prefill(x[:4], x[:4], x[:4], step)
+    layer.extend(x, x, x, step)                                         # a buffer of a fixed size
+    assert calls == ["qk_norm_rope", "paged_append", "paged_append", "paged_attention"]
