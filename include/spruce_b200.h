@@ -3,7 +3,8 @@
  *
  * Plain pointers, element strides and sizes; no torch or CUDA types.  All
  * pointers are device pointers unless noted, `stream` is a cudaStream_t (NULL
- * = legacy default stream).  No entry point allocates device memory or
+ * = legacy default stream) of the current device, which has to be the tensors'.
+ * No entry point allocates device memory or
  * synchronises the stream: work is enqueued and the call returns.  Inputs are
  * borrowed; outputs are written in place.
  *

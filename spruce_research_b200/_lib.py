@@ -147,6 +147,19 @@ def stream_on(device: int) -> int:
     return torch._C._cuda_getCurrentRawStream(device)
 
 
+def current_device() -> int:
+    return torch._C._cuda_getDevice()
+
+
+def launch(entry, args: bytes, device: int) -> None:
+    """Call an entry point with the tensors' GPU current: its launches go to a stream of that GPU."""
+    if current_device() == device:
+        check(entry(args))
+    else:
+        with torch.cuda.device(device):
+            check(entry(args))
+
+
 def require_cuda(*tensors: torch.Tensor, what: str = "the SPRUCE B200 kernels") -> None:
     for t in tensors:
         if not t.is_cuda:

@@ -11,15 +11,16 @@
 
 namespace spruce {
 
+// SMs of the current GPU, asked for once.
 static int sm_count() {
-  static int n = 0;
-  if (n == 0) {
-    int dev = 0, v = 0;
-    if (cudaGetDevice(&dev) == cudaSuccess &&
-        cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess && v > 0)
-      n = std::min(v, kMaxSms);
-  }
-  return n > 0 ? n : 148;
+  static std::atomic<int> known[64];
+  int dev = 0, v = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 148;
+  if (dev < 64 && (v = known[dev].load()) > 0) return v;
+  if (cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || v < 1) return 148;
+  v = std::min(v, kMaxSms);
+  if (dev < 64) known[dev].store(v);
+  return v;
 }
 
 __device__ __forceinline__ void copy16_or_zero(float* dst, const float* src, bool in) {

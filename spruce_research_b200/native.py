@@ -542,7 +542,7 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, rope: torch.Tensor, positions
         q.data_ptr(), k.data_ptr(), q_out.data_ptr(), k_out.data_ptr(), rope.data_ptr(), _ptr(positions),
         _ptr(q_weight), _ptr(k_weight), _status_ptr(status), _lib.stream_on(device), *q.stride(), *k.stride(),
         *q_out.stride(), *k_out.stride(), *pos_strides, _dt(q), B, Hq, Hkv, T, D, *rope.shape, interleaved, eps)
-    _lib.check(_lib.load().spruce_qk_norm_rope(args))
+    _lib.launch(_lib.load().spruce_qk_norm_rope, args, device)
     return q_out, k_out
 
 
@@ -634,7 +634,7 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cach
         _ptr(positions), _ptr(q_weight), _ptr(k_weight), block_table.data_ptr(), cu_q.data_ptr(), kv_lens.data_ptr(),
         _status_ptr(status), _lib.stream_on(device), qn, qh, kn, kh, vn, vh, on, oh, *kc_strides[:3],
         *vc_strides[:3], _dt(k), N, S, Hq, Hkv, D, pages, page_size, step, width, table_rows, rd, interleaved, eps)
-    _lib.check(_lib.load().spruce_paged_append(args))
+    _lib.launch(_lib.load().spruce_paged_append, args, device)
     return q_out
 
 
@@ -688,5 +688,5 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         kv_lens.data_ptr(), workspace.data_ptr(), _status_ptr(status), _lib.stream_on(device), qn, qh, *kc_strides[:3],
         *vc_strides[:3], on, oh, dt, N, S, Hq, Hkv, D, pages, page_size, step, width, max_q_len, max_kv_len, nbytes,
         D ** -0.5 if scale is None else scale)
-    _lib.check(_lib.load().spruce_paged_attention(args))
+    _lib.launch(_lib.load().spruce_paged_attention, args, device)
     return out

@@ -72,3 +72,49 @@ def test_a_layer_refuses_tensors_of_another_number_of_tokens(monkeypatch):
     layer.prefill(x[:4], x[:4], x[:4], step)
     layer.extend(x, x, x, step)                                         # a buffer of a fixed size
     assert calls == ["qk_norm_rope", "paged_append", "paged_append", "paged_attention"]
+
+
+class _Elsewhere(torch.Tensor):
+    """A host tensor that says it is on GPU 1."""
+
+    def get_device(self):
+        return 1
+
+
+def _elsewhere(*shape, dtype=torch.float32):
+    return torch.zeros(*shape, dtype=dtype).as_subclass(_Elsewhere)
+
+
+def test_calls_run_on_the_gpu_of_their_tensors(monkeypatch):
+    """Tensors of GPU 1 while GPU 0 is current: the stream is GPU 1's, so the launch has to be made with GPU 1 current."""
+    current, made = [0], []
+
+    class Device:
+        def __init__(self, index):
+            self.index = index
+
+        def __enter__(self):
+            self.before, current[0] = current[0], self.index
+
+        def __exit__(self, *exc):
+            current[0] = self.before
+
+    class Library:
+        def __getattr__(self, entry):
+            return lambda args: made.append((entry, current[0])) or 0
+
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setattr(native._lib, "current_device", lambda: current[0], raising=False)
+    monkeypatch.setattr(native._lib, "stream_on", lambda device: 0)
+    monkeypatch.setattr(native._lib, "load", Library)
+    monkeypatch.setattr(native, "_paged_workspace_bytes", lambda *a: 256)
+    x, cache = _elsewhere(3, 2, 64), _elsewhere(4, 2, 16, 64)
+    table, cu, kv = (_elsewhere(*s, dtype=torch.int32) for s in ((1, 2), (2,), (1,)))
+    names = ["spruce_qk_norm_rope", "spruce_paged_append", "spruce_paged_attention"]
+    for device in (0, 1):
+        current[0] = device
+        native.qk_norm_rope(x[None], x[None], _elsewhere(8, 64))
+        native.paged_append(x, x, cache, cache, table, cu, kv)
+        native.paged_attention(x, cache, cache, table, cu, kv, max_q_len=3, max_kv_len=3)
+        assert made == [(name, 1) for name in names] and current[0] == device
+        made.clear()
