@@ -480,8 +480,9 @@ SPRUCE_API int spruce_paged_append(const spruce_paged_append_args *args);
  * q_len + i.  From single tokens to prefill chunks, of any mix of lengths; a
  * query that sees nothing (an empty sequence) yields zeros, rows before cu_q[0]
  * and past cu_q[S] are not written.  Cache rows at or past kv_lens[s] never reach an output,
- * whatever they hold; a value of the sequence itself that is not finite may
- * reach every query whose key tile holds it.  max_q_len and max_kv_len bound q_len and kv_lens (they
+ * whatever they hold.  A score that is NaN or +inf makes the outputs of the
+ * queries that see it NaN; a V element of the sequence itself that is not finite
+ * may reach every query whose key tile holds it, as 0 times it is NaN.  max_q_len and max_kv_len bound q_len and kv_lens (they
  * size the launch); a longer sequence is cut to them and raises
  * SPRUCE_STATUS_BAD_LENGTH, a page id outside the cache reads zeros and raises
  * SPRUCE_STATUS_BAD_PAGE.  scale >= 0, D in {64, 128}, page_size a multiple of 16, every

@@ -85,6 +85,13 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const float (&v)[16]) 
   tmem_st16u(taddr, r);
 }
 
+// max(a, b, c), NaN where one of them is.
+__device__ __forceinline__ float fmax3_nan(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
 // A warp's place in the CTA's run.  It lives in shared memory so that the softmax's inner loop, which wants every
 // register, does not carry it.
 struct ChunkRole {
@@ -410,17 +417,18 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         float mx8[8];
 #pragma unroll
         for (int u = 0; u < 8; ++u) {
-          float a = fmax3(s[0][u], s[0][u + 8], s[0][u + 16]);
-          a = fmax3(a, s[0][u + 24], s[1][u]);
-          a = fmax3(a, s[1][u + 8], s[1][u + 16]);
-          a = fmax3(a, s[1][u + 24], s[2][u]);
-          a = fmax3(a, s[2][u + 8], s[2][u + 16]);
-          a = fmax3(a, s[2][u + 24], s[3][u]);
-          a = fmax3(a, s[3][u + 8], s[3][u + 16]);
-          mx8[u] = fmaxf(a, s[3][u + 24]);
+          float a = fmax3_nan(s[0][u], s[0][u + 8], s[0][u + 16]);
+          a = fmax3_nan(a, s[0][u + 24], s[1][u]);
+          a = fmax3_nan(a, s[1][u + 8], s[1][u + 16]);
+          a = fmax3_nan(a, s[1][u + 24], s[2][u]);
+          a = fmax3_nan(a, s[2][u + 8], s[2][u + 16]);
+          a = fmax3_nan(a, s[2][u + 24], s[3][u]);
+          a = fmax3_nan(a, s[3][u + 8], s[3][u + 16]);
+          mx8[u] = fmax3_nan(a, s[3][u + 24], a);
         }
-        const float mx = fmaxf(fmax3(mx8[0], mx8[1], mx8[2]), fmax3(mx8[3], mx8[4], fmax3(mx8[5], mx8[6], mx8[7])));
-        const float m_new = fmaxf(m_used, mx * sl2);
+        const float mx = fmax3_nan(fmax3_nan(mx8[0], mx8[1], mx8[2]), fmax3_nan(mx8[3], mx8[4], mx8[5]), fmax3_nan(mx8[6], mx8[7], mx8[7]));
+        const float top = mx * sl2;
+        const float m_new = fmaxf(m_used, top);  // a NaN is not taken over
         const bool rescale = m_new > m_used + 8.0f;  // the first tile's too
         if (__any_sync(0xffffffffu, rescale)) {
           // PV_t(j-1) is complete and PV_t(j) waits for this tile's P.
@@ -439,7 +447,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
             }
           }
         }
-        const float neg_ref = (m_used == -INFINITY) ? 0.0f : -m_used;
+        // A tile with a score of NaN or +inf makes the row NaN whichever column holds it: the polynomial, whose clamp takes NaN
+        // for a number, would lose it in the columns that it serves.
+        const float neg_ref = top < INFINITY ? (m_used == -INFINITY ? 0.0f : -m_used) : __int_as_float(0x7fffffff);
         uint64_t sum2[2] = {f2_pack(0.0f, 0.0f), f2_pack(0.0f, 0.0f)};
         const uint64_t sl2x2 = f2_pack(sl2, sl2), nref2 = f2_pack(neg_ref, neg_ref);
 #pragma unroll

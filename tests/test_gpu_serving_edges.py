@@ -31,3 +31,38 @@ def test_append_leaves_out_tokens_before_the_first_sequence(shift, with_q):
     assert torch.equal(kc, want_k) and torch.equal(vc, want_v)
     if with_q:
         assert torch.equal(out[3:7], q[3:7]) and (out[:3] == 7).all() and (out[7:] == 7).all()
+
+
+def _attend(q, k, v, page=16, **kw):
+    """One sequence: q [Nq, Hq, D] are the last tokens of k, v [N, Hkv, D]."""
+    N, Hkv, D = k.shape
+    pages = -(-N // page)
+    kc, vc = (torch.zeros(pages * page, Hkv, D, device="cuda", dtype=q.dtype) for _ in range(2))
+    kc[:N], vc[:N] = k, v
+    kc, vc = (x.view(pages, page, Hkv, D).transpose(1, 2).contiguous() for x in (kc, vc))
+    table = torch.arange(pages, device="cuda", dtype=torch.int32)[None]
+    cu, kv = (torch.tensor(x, device="cuda", dtype=torch.int32) for x in ([0, q.shape[0]], [N]))
+    return native.paged_attention(q, kc, vc, table, cu, kv, **dict(max_q_len=q.shape[0], max_kv_len=N) | kw)
+
+
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("q", [1, 300])                    # single tokens and chunks are two kernels
+@pytest.mark.parametrize("key", [28, 29, 30, 31, 190, 351, 383, 639])
+@pytest.mark.parametrize("bad", ["nan", "inf"])
+@pytest.mark.parametrize("heads", [2, 300])                # units split over CTAs and joined, or whole
+def test_a_score_that_is_not_a_number_reaches_every_query_that_sees_it(dtype, q, key, bad, heads):
+    """A NaN in a key, or a key that is so large that its scores are +inf, makes the rows that see it NaN, wherever in a
+    tile it stands; rows before it are as they are without it."""
+    g = torch.Generator(device="cuda").manual_seed(2)
+    n = 700
+    x, k, v = (torch.randn(m, heads, 128, generator=g, device="cuda").to(dtype) for m in (q, n, n))
+    x[:, :, 3] = 1.0
+    clean = _attend(x, k, v)
+    k[key, :, 3] = float(bad)
+    got = _attend(x, k, v)
+    sees = torch.arange(n - q, n, device="cuda") >= key
+    assert got[sees].isnan().all()
+    assert torch.equal(got[~sees], clean[~sees]) and clean.isfinite().all()
