@@ -52,8 +52,9 @@ template <> struct Pack2<__half> {
 // evaluation, against 3.9e-3 = the bf16 precision P is rounded to), and
 // 2^n applied as 2^(n+1) in the exponent field times 0.5 (the product rounds correctly
 // where the result is subnormal, e.g. x = -126, where p(0) < 1 would otherwise land in
-// the subnormal encoding).  x is clamped at -126; callers only pass x <= 8 (lazy
-// rescale) and never -inf.
+// the subnormal encoding).  x is clamped at -126: -inf and NaN give 2^-126.  The prefill
+// kernels only pass x <= 8 (lazy rescale) and never -inf; the paged one sees to rows with
+// scores that are not finite itself.
 __device__ __forceinline__ float poly_exp2(float x) {
   x = fmaxf(x, -126.0f);
   const float kRound = 12582912.0f;  // 1.5 * 2^23

@@ -499,7 +499,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       // The rows leave through this warp's rows of the Q tile, whose MMAs are complete: 128 bytes of each row a round,
       // written row by thread and read back row by eight lanes, so that a store covers whole lines.
       const bool whole = x.slot < 0;
-      const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+      // No maximum: no key, or scores of -inf alone, of which the polynomial's columns made 2^-126.
+      const float inv = l > 0.0f && m_used > -INFINITY ? 1.0f / l : 0.0f;
       uint8_t* dst = nullptr;  // this row in the output, or among the parts
       if (row < rows) {
         if (whole) {

@@ -66,3 +66,31 @@ def test_a_score_that_is_not_a_number_reaches_every_query_that_sees_it(dtype, q,
     sees = torch.arange(n - q, n, device="cuda") >= key
     assert got[sees].isnan().all()
     assert torch.equal(got[~sees], clean[~sees]) and clean.isfinite().all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])     # fp16's largest products do not overflow fp32
+@pytest.mark.parametrize("q", [1, 300])
+@pytest.mark.parametrize("heads", [2, 300])
+def test_rows_whose_scores_are_all_minus_infinity_are_zero(dtype, q, heads):
+    """Scores that overflow to -inf weigh nothing, as masked ones: a row of nothing else is zero, and the rows of head 1,
+    whose scores are ordinary, are as they are beside ordinary ones."""
+    g = torch.Generator(device="cuda").manual_seed(3)
+    n = 700
+    x, k, v = (torch.randn(m, heads, 128, generator=g, device="cuda").to(dtype) for m in (q, n, n))
+    low = torch.arange(heads, device="cuda") != 1
+    ordinary = k[:, 1].clone(), x[:, 1].clone()
+    k = k.abs() * 1e20 + 1e20
+    x[:] = -1e20
+    k[:, 1], x[:, 1] = ordinary
+    got = _attend(x, k, v)
+    assert (got[:, low] == 0).all()
+    k[:, low] = 0
+    assert torch.equal(got[:, 1], _attend(x, k, v)[:, 1]) and (got[:, 1] != 0).any()
+    # -inf for the first half of the keys only: the second half decides
+    k[:n // 2, low] = 1e20
+    half = _attend(x, k, v)[:, low].double()
+    total = v.double().cumsum(0)[:, low]
+    mean = (total[n - q:] - total[n // 2 - 1]) / torch.arange(n - q - n // 2 + 1, n - n // 2 + 1, device="cuda")[:, None, None]
+    # flat weights: the probabilities are 1 exactly, so the store rounds by u |o| and the sums by n 2^-24 of max |v|
+    u = 2.0 ** -24 if dtype == torch.float32 else 2.0 ** -8
+    assert ((half - mean).abs() <= u * mean.abs() + 2 * n * 2.0 ** -24 * v.abs().max()).all()
