@@ -482,9 +482,11 @@ SPRUCE_API int spruce_paged_append(const spruce_paged_append_args *args);
  * and past cu_q[S] are not written.  Cache rows at or past kv_lens[s] never reach an output,
  * whatever they hold.  A score that is NaN or +inf makes the outputs of the
  * queries that see it NaN; a V element of the sequence itself that is not finite
- * may reach every query whose key tile holds it, as 0 times it is NaN.  max_q_len and max_kv_len bound q_len and kv_lens (they
- * size the launch); a longer sequence is cut to them and raises
- * SPRUCE_STATUS_BAD_LENGTH, a page id outside the cache reads zeros and raises
+ * may reach every query whose key tile holds it, as 0 times it is NaN.
+ * max_q_len and max_kv_len bound q_len and kv_lens (they size the launch); a
+ * longer sequence is cut to them and raises SPRUCE_STATUS_BAD_LENGTH: its
+ * queries past max_q_len are not written (none are where that is 0), its keys
+ * past max_kv_len not seen.  A page id outside the cache reads zeros and raises
  * SPRUCE_STATUS_BAD_PAGE.  scale >= 0, D in {64, 128}, page_size a multiple of 16, every
  * row 16-byte aligned.  bf16 / fp16 run tensor-core kernels, fp32 a CUDA-core
  * kernel.  workspace (spruce_paged_attention_workspace_bytes, -1 for an invalid

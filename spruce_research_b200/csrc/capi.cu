@@ -882,7 +882,8 @@ int spruce_paged_attention(const spruce_paged_attention_args* args) {
   const float scale = (float)x.scale;
   if (!(scale >= 0.0f && scale <= 3.0e38f))
     return fail(SPRUCE_ERR_INVALID, "scale must be finite and not negative, got %g", x.scale);
-  if (x.N == 0 || x.S == 0 || x.max_q_len == 0) return SPRUCE_OK;
+  if (x.N == 0 || x.S == 0) return SPRUCE_OK;
+  if (x.max_q_len == 0 && x.status == nullptr) return SPRUCE_OK;  // with a status, sequences that have tokens are reported
   if (x.num_pages < 1) return fail(SPRUCE_ERR_INVALID, "the cache has no pages");
   if (x.q == nullptr || x.out == nullptr || x.k_cache == nullptr || x.v_cache == nullptr)
     return fail(SPRUCE_ERR_INVALID, "null pointer");

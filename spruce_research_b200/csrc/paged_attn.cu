@@ -391,12 +391,13 @@ template cudaError_t launch_paged_join<float>(const PagedParams&, int, int, int,
 template cudaError_t launch_paged_join<__nv_bfloat16>(const PagedParams&, int, int, int, cudaStream_t);
 template cudaError_t launch_paged_join<__half>(const PagedParams&, int, int, int, cudaStream_t);
 
-// CTAs worth launching: all resident ones, or fewer where the tiles cannot be more.
+// CTAs worth launching: all resident ones, or fewer where the tiles cannot be more.  One where there are none (no room for
+// new tokens): it reports the sequences that have some.
 static int grid_for(const PagedArgs& a, int R, int TK, int resident) {
   const int64_t rt = ((int64_t)a.max_q * (a.Hq / a.Hkv) + R - 1) / R;
   const int64_t kt = std::max<int64_t>(1, ((int64_t)a.max_kv + TK - 1) / TK);
   const __int128 tiles = (__int128)a.S * rt * kt * a.Hkv;
-  return tiles < resident ? static_cast<int>(tiles) : resident;
+  return tiles < 1 ? 1 : (tiles < resident ? static_cast<int>(tiles) : resident);
 }
 
 constexpr int kF32Rows = 64, kF32PerSm = 2, kF32FewPerSm = 3;

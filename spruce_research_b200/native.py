@@ -651,7 +651,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
 
     The last new token of sequence s sees ``kv_lens[s]`` keys, the one before it one fewer, and so on; queries that
     see none give zeros.  ``max_q_len`` and ``max_kv_len`` bound the sequences' new tokens and lengths (the lengths
-    themselves stay on the device).  Returns [N, Hq, D]; rows before ``cu_q[0]`` and past ``cu_q[-1]`` are not written.
+    themselves stay on the device); longer ones are cut to them, their queries past ``max_q_len`` are not written, and only
+    ``status`` says so.  Returns [N, Hq, D]; rows before ``cu_q[0]`` and past ``cu_q[-1]`` are not written.
     """
     device = q.get_device()
     if not (device == k_cache.get_device() == v_cache.get_device() == block_table.get_device() == cu_q.get_device()

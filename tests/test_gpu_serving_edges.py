@@ -3,7 +3,7 @@ not finite, weights near the end of fp16's range, tensors at odd addresses."""
 import pytest
 import torch
 
-from spruce_research_b200 import native
+from spruce_research_b200 import _lib, native
 
 pytestmark = pytest.mark.gpu
 
@@ -94,3 +94,17 @@ def test_rows_whose_scores_are_all_minus_infinity_are_zero(dtype, q, heads):
     # flat weights: the probabilities are 1 exactly, so the store rounds by u |o| and the sums by n 2^-24 of max |v|
     u = 2.0 ** -24 if dtype == torch.float32 else 2.0 ** -8
     assert ((half - mean).abs() <= u * mean.abs() + 2 * n * 2.0 ** -24 * v.abs().max()).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("heads", [4, 28])
+def test_no_room_for_new_tokens_sets_the_status(dtype, heads):
+    """max_q_len 0 while a sequence has new tokens: every one is cut off, which the status reports."""
+    x = torch.randn(3, heads, 64, device="cuda").to(dtype)
+    k = torch.randn(90, 4, 64, device="cuda").to(dtype)
+    status = torch.zeros(1, device="cuda", dtype=torch.int32)
+    out = torch.full_like(x, 5.0)
+    _attend(x, k, k, max_q_len=0, out=out, status=status)
+    assert status.item() == _lib.STATUS_BAD_LENGTH and (out == 5).all()
+    _attend(x, k, k, max_q_len=0, out=out)
+    assert (out == 5).all()
