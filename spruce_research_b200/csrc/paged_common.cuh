@@ -40,11 +40,11 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedParams& p, int s) {
   const int c0 = p.a.cu_q[s], c1 = p.a.cu_q[s + 1], k = p.a.kv_lens[s];
   PagedSeq q;
   q.q0 = min(max(c0, 0), p.a.N);
-  q.qlen = min(max(c1, q.q0), p.a.N) - q.q0;
-  q.qlen = min(q.qlen, p.a.max_q);
-  q.kv = min(max(k, 0), p.kv_cap);
+  const int held = max(k, 0), added = min(max(c1, q.q0), p.a.N) - q.q0;
+  q.qlen = min(added, p.a.max_q);
+  q.kv = min(held, p.kv_cap);
   if (q.qlen != c1 - c0 || q.kv != k) raise_status(p.a.status, SPRUCE_STATUS_BAD_LENGTH);
-  q.first = q.kv - q.qlen;
+  q.first = min(held, 1 << 30) - added;  // of the uncut lengths; positions stay ints
   return q;
 }
 

@@ -108,3 +108,27 @@ def test_no_room_for_new_tokens_sets_the_status(dtype, heads):
     assert status.item() == _lib.STATUS_BAD_LENGTH and (out == 5).all()
     _attend(x, k, k, max_q_len=0, out=out)
     assert (out == 5).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("q,cut", [(3, 1), (200, 1), (200, 100)])
+def test_a_sequence_cut_to_the_bounds_keeps_its_positions(dtype, q, cut):
+    """With max_q_len below its new tokens the first ones are computed and see what they saw; with max_kv_len below its
+    length the keys past it are left out."""
+    g = torch.Generator(device="cuda").manual_seed(4)
+    n = 500
+    x, k, v = (torch.randn(m, 4, 64, generator=g, device="cuda").to(dtype) for m in (q, n, n))
+    want = _attend(x[:cut], k[:n - q + cut], v[:n - q + cut])
+    status = torch.zeros(1, device="cuda", dtype=torch.int32)
+    out = torch.full_like(x, 5.0)
+    _attend(x, k, v, max_q_len=cut, out=out, status=status)
+    assert status.item() == _lib.STATUS_BAD_LENGTH and (out[cut:] == 5).all()
+    # the same sums in another split: see the bounds of the attention's tests, here at scores of order 1
+    u = {torch.float32: 2.0 ** -18, torch.bfloat16: 2.0 ** -6, torch.float16: 2.0 ** -9}[dtype]
+    assert (out[:cut].double() - want.double()).abs().max().item() <= u * v.abs().max().item()
+    status.zero_()
+    got = _attend(x, k, v, max_kv_len=n - q // 2, status=status)
+    assert status.item() == _lib.STATUS_BAD_LENGTH
+    seen = q - q // 2                                        # tokens whose keys all lie within the bound
+    want = _attend(x[:seen], k[:n - q // 2], v[:n - q // 2])
+    assert (got[:seen].double() - want.double()).abs().max().item() <= u * v.abs().max().item()
