@@ -11,9 +11,9 @@
 // is written over the first half of S_t.  One thread issues PV_0(j) QK_0(j+1) PV_1(j) QK_1(j+1) ..., in whose order they
 // execute, so QK_t(j+1) overwrites P_t(j) after PV_t(j) has read it, and while one tile's softmax runs the tensor core
 // works for the other.  P is announced in halves of 64 keys, so PV starts on the first while the second is
-// exponentiated.  O is rescaled only when the running maximum grew by more than 8 (log2 units): P stays below
-// 2^8, which both 16-bit types hold, and O / l is exact for any reference.  P is rounded to the input type (the MMA's
-// operand); the sum l is of the unrounded fp32 values.
+// exponentiated.  O is rescaled only when the running maximum grew by more than 8 (log2 units; fp16: 2), which
+// O / l cancels.  P is rounded to the input type (the MMA's operand) and stays below 2^8 in bf16; in fp16 it carries 2^13 and
+// stays below 2^15, so weights keep all their bits down to 2^-27 of the row's largest.  The sum l is of the unrounded fp32 values.
 //
 // Pages: one TMA box of a page's rows (or of 128 of them, or of its largest power-of-two divisor) lands as rows of the
 // 128-byte-swizzled tile.  Boxes past the sequence's end take a page index past the cache, which reads zeros; the rows of
@@ -397,6 +397,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       }
       // Columns of the piece's first key tile that this row sees; each tile further leaves 128 fewer.
       int lim = min(x.q.first + row_at.token(row) + 1, x.keys) - x.t0 * kChunkKeys;
+      // Growth of the maximum that O is not rescaled for, and the factor of P: together P's range.
+      constexpr float kLag = std::is_same<T, __half>::value ? 2.0f : 8.0f;
+      constexpr float kScale = PScale<T>::log2 > 0.0f ? PScale<T>::log2 - kLag : 0.0f;
       float m_used = -INFINITY;  // reference max (log2 units) the exponentials use
       float l = 0.0f;
       // One key tile.  Masked tiles are a unit's last ones; they have a body of their own because a branch within the
@@ -429,7 +432,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         const float mx = fmax3_nan(fmax3_nan(mx8[0], mx8[1], mx8[2]), fmax3_nan(mx8[3], mx8[4], mx8[5]), fmax3_nan(mx8[6], mx8[7], mx8[7]));
         const float top = mx * sl2;
         const float m_new = fmaxf(m_used, top);  // a NaN is not taken over
-        const bool rescale = m_new > m_used + 8.0f;  // the first tile's too
+        const bool rescale = m_new > m_used + kLag;  // the first tile's too
         if (__any_sync(0xffffffffu, rescale)) {
           // PV_t(j-1) is complete and PV_t(j) waits for this tile's P.
           const float alpha = rescale ? fast_exp2(m_used - m_new) : 1.0f;
@@ -449,7 +452,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         }
         // A tile with a score of NaN or +inf makes the row NaN whichever column holds it: the polynomial, whose clamp takes NaN
         // for a number, would lose it in the columns that it serves.
-        const float neg_ref = top < INFINITY ? (m_used == -INFINITY ? 0.0f : -m_used) : __int_as_float(0x7fffffff);
+        const float neg_ref = top < INFINITY ? (m_used == -INFINITY ? 0.0f : kScale - m_used) : __int_as_float(0x7fffffff);
         uint64_t sum2[2] = {f2_pack(0.0f, 0.0f), f2_pack(0.0f, 0.0f)};
         const uint64_t sl2x2 = f2_pack(sl2, sl2), nref2 = f2_pack(neg_ref, neg_ref);
 #pragma unroll

@@ -253,6 +253,13 @@ __device__ __forceinline__ int paged_page(const PagedParams& p, const int32_t* t
   return -1;
 }
 
+// log2 of the factor that all probabilities of a kernel carry until O / l cancels it.  P is rounded to the inputs' type for
+// its product with V (the operand of the MMA), the sum l is of the fp32 values.  bf16 has fp32's range.  fp16 ends at 2^-24
+// and loses bits below 2^-14: with the largest P at 1, weights under 2^-25 of it would be in l and not in O, and a long
+// context has many of those.  With P up to 2^15 (fp16 holds 65504) a weight keeps all its bits down to 2^-29 of the largest.
+template <typename T> struct PScale { static constexpr float log2 = 0.0f; };
+template <> struct PScale<__half> { static constexpr float log2 = 15.0f; };
+
 // Opts a kernel into `bytes` of dynamic shared memory, once a device (`done` is the kernel's own mask of devices).
 inline cudaError_t allow_smem(const void* kern, int bytes, std::atomic<uint64_t>& done) {
   int dev = 0;

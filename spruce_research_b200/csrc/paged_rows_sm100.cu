@@ -11,6 +11,8 @@
 // running maximum, sum and output, so the warps meet only at the end of a piece, where slices are joined through
 // shared memory.  Two CTAs an SM: one's joins and starts pass behind the other's loads.
 //
+// P is rounded to the inputs' type for its product with V, scaled as PScale says; sums, maxima and O are fp32.
+//
 // Cache rows past the sequence's end may hold anything: their scores are masked by selection and their V
 // fragments cleared.
 //
@@ -225,8 +227,9 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
           const float ref = m_new == -INFINITY ? 0.0f : m_new;
           alpha[i2] = fast_exp2(m[i2] - ref);
           m[i2] = m_new;
-          const float e0 = fast_exp2(e[0][2 * i2] - ref), e1 = fast_exp2(e[0][2 * i2 + 1] - ref);
-          const float e2 = fast_exp2(e[1][2 * i2] - ref), e3 = fast_exp2(e[1][2 * i2 + 1] - ref);
+          const float low = ref - PScale<T>::log2;
+          const float e0 = fast_exp2(e[0][2 * i2] - low), e1 = fast_exp2(e[0][2 * i2 + 1] - low);
+          const float e2 = fast_exp2(e[1][2 * i2] - low), e3 = fast_exp2(e[1][2 * i2 + 1] - low);
           l[i2] = l[i2] * alpha[i2] + ((e0 + e1) + (e2 + e3));
           pa[i2] = Pack2<T>::pack(e0, e1);
           pa[2 + i2] = Pack2<T>::pack(e2, e3);

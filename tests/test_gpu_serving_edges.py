@@ -132,3 +132,25 @@ def test_a_sequence_cut_to_the_bounds_keeps_its_positions(dtype, q, cut):
     seen = q - q // 2                                        # tokens whose keys all lie within the bound
     want = _attend(x[:seen], k[:n - q // 2], v[:n - q // 2])
     assert (got[:seen].double() - want.double()).abs().max().item() <= u * v.abs().max().item()
+
+
+@pytest.mark.parametrize("q,n", [(1, 2000), (300, 20000)])
+@pytest.mark.parametrize("gap", [17.0, 24.0, 25.5])
+def test_fp16_keeps_many_small_weights(q, n, gap):
+    """One key outweighs each other by 2^gap but holds zeros: what is left is the sum of the small weights, which has to
+    be right relative to itself as long as each is above 2^-26 of the largest."""
+    D = 128
+    x = torch.zeros(q, 1, D, device="cuda", dtype=torch.float16)
+    x[:, :, 0] = 1.0
+    k = torch.zeros(n, 1, D, device="cuda", dtype=torch.float16)
+    k[0] = gap * 0.6931471805599453 / D ** -0.5              # score gap ln 2
+    v = torch.ones(n, 1, D, device="cuda", dtype=torch.float16)
+    v[0] = 0
+    score = k[0, 0, 0].double() * D ** -0.5
+    got = _attend(x, k, v)[:, 0].double()
+    small = torch.arange(n - q, n, device="cuda").double()[:, None]      # keys besides the first that the row sees
+    want = small * torch.exp(-score) / (1 + small * torch.exp(-score))
+    # each weight: rounded to fp16 (2^-11) and its exponential (1e-4 and the exponent's 2^-24 |x|); the store 2^-11, or
+    # half of fp16's smallest step; sums n 2^-24
+    rel = 2 * 2.0 ** -11 + 1e-4 + n * 2.0 ** -24 + 40 * 2.0 ** -23
+    assert ((got - want).abs() <= rel * want + 2.0 ** -25).all()
