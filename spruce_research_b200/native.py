@@ -667,7 +667,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     dt, size = _dt(q), q.element_size()
     qn, qh, qd = q.stride()
     if qd != 1 or (qn | qh) % (16 // size) or q.data_ptr() % 16:
-        q = q.contiguous()
+        q = q.clone(memory_format=torch.contiguous_format)  # contiguous() returns a q at an odd address as it is
         qn, qh, _ = q.stride()
     if out is None:
         out = torch.empty_like(q) if q.is_contiguous() else q.new_empty(shape)

@@ -154,3 +154,16 @@ def test_fp16_keeps_many_small_weights(q, n, gap):
     # half of fp16's smallest step; sums n 2^-24
     rel = 2 * 2.0 ** -11 + 1e-4 + n * 2.0 ** -24 + 40 * 2.0 ** -23
     assert ((got - want).abs() <= rel * want + 2.0 ** -25).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_queries_at_an_odd_address_are_copied(dtype):
+    """A contiguous q that does not begin on 16 bytes, or whose only token has any stride."""
+    g = torch.Generator(device="cuda").manual_seed(5)
+    flat = torch.randn(3 * 4 * 64 + 1, generator=g, device="cuda").to(dtype)
+    k, v = (torch.randn(70, 2, 64, generator=g, device="cuda").to(dtype) for _ in range(2))
+    q = flat[1:].view(3, 4, 64)
+    assert q.is_contiguous()
+    assert torch.equal(_attend(q, k, v), _attend(q.clone(), k, v))
+    one = flat[:256].as_strided((1, 4, 64), (257, 64, 1))
+    assert torch.equal(_attend(one, k, v), _attend(one.clone(memory_format=torch.contiguous_format), k, v))
