@@ -682,6 +682,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
             raise ValueError(f"bad paged attention shape: q {tuple(shape)}, cache {tuple(k_cache.shape)}, "
                              f"max_q_len {max_q_len}")
         workspace = q.new_empty(nbytes // size)
+    elif not workspace.is_contiguous():
+        raise ValueError("workspace must be contiguous")
     else:
         nbytes = workspace.nbytes
     args = _lib.PAGED_ATTENTION_ARGS.pack(

@@ -85,8 +85,9 @@ def _elsewhere(*shape, dtype=torch.float32):
     return torch.zeros(*shape, dtype=dtype).as_subclass(_Elsewhere)
 
 
-def test_calls_run_on_the_gpu_of_their_tensors(monkeypatch):
-    """Tensors of GPU 1 while GPU 0 is current: the stream is GPU 1's, so the launch has to be made with GPU 1 current."""
+@pytest.fixture
+def fake_gpus(monkeypatch):
+    """Entry points that note their name and the current GPU; returns (the current GPU, the calls)."""
     current, made = [0], []
 
     class Device:
@@ -108,8 +109,18 @@ def test_calls_run_on_the_gpu_of_their_tensors(monkeypatch):
     monkeypatch.setattr(native._lib, "stream_on", lambda device: 0)
     monkeypatch.setattr(native._lib, "load", Library)
     monkeypatch.setattr(native, "_paged_workspace_bytes", lambda *a: 256)
-    x, cache = _elsewhere(3, 2, 64), _elsewhere(4, 2, 16, 64)
-    table, cu, kv = (_elsewhere(*s, dtype=torch.int32) for s in ((1, 2), (2,), (1,)))
+    return current, made
+
+
+def _paged():
+    return (_elsewhere(3, 2, 64), _elsewhere(4, 2, 16, 64), _elsewhere(1, 2, dtype=torch.int32),
+            _elsewhere(2, dtype=torch.int32), _elsewhere(1, dtype=torch.int32))
+
+
+def test_calls_run_on_the_gpu_of_their_tensors(fake_gpus):
+    """Tensors of GPU 1 while GPU 0 is current: the stream is GPU 1's, so the launch has to be made with GPU 1 current."""
+    current, made = fake_gpus
+    x, cache, table, cu, kv = _paged()
     names = ["spruce_qk_norm_rope", "spruce_paged_append", "spruce_paged_attention"]
     for device in (0, 1):
         current[0] = device
@@ -118,3 +129,12 @@ def test_calls_run_on_the_gpu_of_their_tensors(monkeypatch):
         native.paged_attention(x, cache, cache, table, cu, kv, max_q_len=3, max_kv_len=3)
         assert made == [(name, 1) for name in names] and current[0] == device
         made.clear()
+
+
+def test_a_workspace_with_gaps_or_repeats_is_refused(fake_gpus):
+    """The kernels take its bytes as one block: an expanded element has the size of a workspace and not its memory."""
+    x, cache, table, cu, kv = _paged()
+    for bad in (_elsewhere(1).expand(1 << 20), _elsewhere(1 << 10, 2)[:, 0]):
+        with pytest.raises(ValueError, match="workspace must be contiguous"):
+            native.paged_attention(x, cache, cache, table, cu, kv, max_q_len=3, max_kv_len=3, workspace=bad)
+    assert not fake_gpus[1]
