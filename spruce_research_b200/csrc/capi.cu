@@ -764,6 +764,7 @@ static int check_rope(int64_t D, const float* rope, int64_t table_rows, int64_t 
 }
 
 int spruce_qk_norm_rope(const spruce_qk_norm_rope_args* args) {
+  if (args == nullptr) return fail(SPRUCE_ERR_INVALID, "null arguments");
   const spruce_qk_norm_rope_args& x = *args;
   if (x.dtype != (int)x.dtype || !valid_dtype((int)x.dtype))
     return fail(SPRUCE_ERR_INVALID, "unsupported dtype code %lld", (long long)x.dtype);
@@ -820,6 +821,7 @@ static int check_paged(const Args& x) {
 }
 
 int spruce_paged_append(const spruce_paged_append_args* args) {
+  if (args == nullptr) return fail(SPRUCE_ERR_INVALID, "null arguments");
   const spruce_paged_append_args& x = *args;
   if (int rc = check_paged(x)) return rc;
   if (int rc = check_rope(x.D, x.rope, x.table_rows, x.rd)) return rc;
@@ -868,6 +870,7 @@ int64_t spruce_paged_attention_workspace_bytes(int64_t Hq, int64_t Hkv, int64_t 
 }
 
 int spruce_paged_attention(const spruce_paged_attention_args* args) {
+  if (args == nullptr) return fail(SPRUCE_ERR_INVALID, "null arguments");
   const spruce_paged_attention_args& x = *args;
   if (int rc = check_paged(x)) return rc;
   if (x.Hq < 1 || x.Hq % x.Hkv)

@@ -1,6 +1,8 @@
 """What the serving operators do on the host, and rules of their kernels that only the source shows (CPU)."""
 import os
 import re
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -138,3 +140,14 @@ def test_a_workspace_with_gaps_or_repeats_is_refused(fake_gpus):
         with pytest.raises(ValueError, match="workspace must be contiguous"):
             native.paged_attention(x, cache, cache, table, cu, kv, max_q_len=3, max_kv_len=3, workspace=bad)
     assert not fake_gpus[1]
+
+
+def test_no_arguments_are_an_error_and_not_a_crash():
+    """A null argument struct at the C entries; in a process of its own, as it could end it."""
+    code = ("from spruce_research_b200 import _lib\n"
+            "L = _lib.load()\n"
+            "for f in (L.spruce_qk_norm_rope, L.spruce_paged_append, L.spruce_paged_attention):\n"
+            "    assert f(None) == _lib.ERR_INVALID and b'null' in L.spruce_last_error()\n")
+    done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300,
+                          cwd=build.REPO)
+    assert done.returncode == 0, (done.returncode, done.stderr[-500:])
