@@ -104,10 +104,10 @@ class PagedSparseLayer:
     """One attention layer over a :class:`PagedKVCache`: sparse prefill of prompts, then chunks and single tokens.
 
     Takes the projections before norms and rotation, packed ``q [N, Hq, D]``, ``k`` / ``v`` [N, Hkv, D].  ``rope`` is a
-    :func:`rope.rope_table` of the longest sequence; ``q_weight`` / ``k_weight`` are head norms (None: no norm).
+    :func:`rope.rope_table` of the longest sequence (None: no rotation); ``q_weight`` / ``k_weight`` are head norms (None: no norm).
     """
 
-    def __init__(self, cache: PagedKVCache, layer_idx: int, rope: torch.Tensor, *,
+    def __init__(self, cache: PagedKVCache, layer_idx: int, rope: torch.Tensor | None, *,
                  prefill: SparsePrefillLayer | None = None, q_weight: torch.Tensor | None = None,
                  k_weight: torch.Tensor | None = None, eps: float = 1e-6, interleaved: bool = False):
         if not 0 <= layer_idx < cache.k.shape[0]:
@@ -148,7 +148,8 @@ class PagedSparseLayer:
             raise ValueError("the sparse prefill takes one whole prompt: one sequence that held nothing before")
         self._check((q, k, v), step, spare=False)
         qs, ks, vs = (x.transpose(0, 1).unsqueeze(0) for x in (q, k, v))       # [1, H, T, D] views
-        qr, kr = native.qk_norm_rope(qs, ks, self.rope, **self.rotation)
+        rope = self.rope if self.rope is not None else q.new_empty((step.tokens, 0), dtype=torch.float32)  # norms alone
+        qr, kr = native.qk_norm_rope(qs, ks, rope, **self.rotation)
         native.paged_append(kr[0].transpose(0, 1), v, self.k_cache, self.v_cache, step.block_table, step.cu_q,
                             step.kv_lens)
         out, selected = self.sparse(qr, kr, vs)

@@ -4,6 +4,9 @@ import pytest
 import torch
 
 from spruce_research_b200 import _lib, native
+from spruce_research_b200.paged import PagedKVCache, PagedSparseLayer
+from spruce_research_b200.pipeline import SparsePrefillLayer
+from spruce_research_b200.synthetic import make_gate_weights
 
 pytestmark = pytest.mark.gpu
 
@@ -167,3 +170,20 @@ def test_queries_at_an_odd_address_are_copied(dtype):
     assert torch.equal(_attend(q, k, v), _attend(q.clone(), k, v))
     one = flat[:256].as_strided((1, 4, 64), (257, 64, 1))
     assert torch.equal(_attend(one, k, v), _attend(one.clone(memory_format=torch.contiguous_format), k, v))
+
+
+@pytest.mark.parametrize("norm", [True, False])
+def test_a_layer_without_a_rotation_table_prefills_as_with_angles_of_zero(norm):
+    g = torch.Generator(device="cuda").manual_seed(6)
+    n, Hq, Hkv, D = 200, 4, 2, 64
+    q, k, v = torch.randn(n + 1, Hq + 2 * Hkv, D, generator=g, device="cuda", dtype=torch.bfloat16).split([Hq, Hkv, Hkv], 1)
+    w = (1 + 0.1 * torch.randn(D, generator=g, device="cuda")) if norm else None
+    gq, gk = make_gate_weights(1, D, D, seed=3, device="cuda")
+    still = torch.cat([torch.ones(n + 1, D // 2), torch.zeros(n + 1, D // 2)], 1).cuda()      # cos 1, sin 0
+    results = []
+    for table in (None, still):
+        cache = PagedKVCache(1, 20, 16, Hkv, D)
+        layer = PagedSparseLayer(cache, 0, table, prefill=SparsePrefillLayer(gq[0], gk[0], 3), q_weight=w, k_weight=w)
+        out, _ = layer.prefill(q[:n], k[:n], v[:n], cache.step([("a", n)]))
+        results.append((out, layer.extend(q[n:], k[n:], v[n:], cache.step([("a", 1)]))))
+    assert torch.equal(results[0][0], results[1][0]) and torch.equal(results[0][1], results[1][1])

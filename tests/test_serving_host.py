@@ -151,3 +151,18 @@ def test_no_arguments_are_an_error_and_not_a_crash():
     done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300,
                           cwd=build.REPO)
     assert done.returncode == 0, (done.returncode, done.stderr[-500:])
+
+
+def test_a_layer_without_a_rotation_table_prefills(monkeypatch):
+    """paged_append takes no table for projections that need no rotation; so does the layer, in prefill as in extend."""
+    seen = []
+    monkeypatch.setattr(native, "qk_norm_rope", lambda q, k, rope, **kw: seen.append((rope, kw)) or (q, k))
+    monkeypatch.setattr(native, "paged_append", lambda k, v, *a, **kw: seen.append(kw.get("rope")))
+    c = _cache()
+    w = torch.ones(64)
+    layer = PagedSparseLayer(c, 0, None, prefill=lambda q, k, v: (q, None), q_weight=w)
+    x = torch.zeros(20, 2, 64)
+    out, _ = layer.prefill(x, x, x, c.step([("a", 20)]))
+    (rope, kw), appended = seen
+    assert rope.shape == (20, 0) and rope.dtype == torch.float32 and kw["q_weight"] is w     # norms, and no angle
+    assert appended is None and out.shape == (2, 20, 64)
