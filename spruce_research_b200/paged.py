@@ -67,10 +67,22 @@ class PagedKVCache:
         self._free.extend(reversed(self._pages.pop(seq_id, [])))
         self._length.pop(seq_id, None)
 
+    def truncate(self, seq_id, length: int) -> None:
+        """Keep a sequence's first ``length`` tokens: drafts that were rejected, or a step whose forward did not run."""
+        held = self.length(seq_id)
+        if not 0 <= length <= held:
+            raise ValueError(f"a sequence of {held} tokens cannot be cut to {length}")
+        if seq_id in self._pages:
+            pages, keep = self._pages[seq_id], -(-length // self.page_size)
+            self._free.extend(reversed(pages[keep:]))
+            del pages[keep:]
+            self._length[seq_id] = length
+
     def step(self, new_tokens) -> PagedStep:
         """Make room for ``new_tokens``, pairs (seq_id, count), and describe the batch on the device.
 
         Unknown sequences start empty.  Nothing changes when the pages do not suffice (RuntimeError).
+        The lengths count the new tokens from here on: :meth:`truncate` takes them back if they are not written.
         """
         new_tokens = [(s, int(n)) for s, n in new_tokens]
         if len({s for s, _ in new_tokens}) < len(new_tokens):

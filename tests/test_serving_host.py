@@ -166,3 +166,29 @@ def test_a_layer_without_a_rotation_table_prefills(monkeypatch):
     (rope, kw), appended = seen
     assert rope.shape == (20, 0) and rope.dtype == torch.float32 and kw["q_weight"] is w     # norms, and no angle
     assert appended is None and out.shape == (2, 20, 64)
+
+
+def test_a_step_that_was_not_run_can_be_taken_back(monkeypatch):
+    """A refused forward leaves the cache counting tokens that were never written, until they are truncated."""
+    _no_kernels(monkeypatch)
+    c = _cache(pages=6)
+    layer = PagedSparseLayer(c, 0, torch.zeros(40, 64))
+    x = torch.zeros(41, 2, 64)
+    layer.extend(x[:20], x[:20], x[:20], c.step([("a", 20)]))
+    pages = c.step([("a", 0)]).block_table[0].tolist()
+    step = c.step([("a", 21), ("b", 16)])
+    with pytest.raises(ValueError, match="rotation table"):
+        layer.extend(x, x, x, step)
+    assert c.length("a") == 41 and c.free_pages == 2
+    c.truncate("a", 20)
+    c.truncate("b", 0)
+    c.truncate("nobody", 0)
+    assert c.length("a") == 20 and c.length("b") == 0 and c.free_pages == 4
+    s = c.step([("a", 12)])                     # the rest of its second page
+    assert s.block_table[0].tolist() == pages and s.kv_lens.tolist() == [32] and c.free_pages == 4
+    s = c.step([("c", 64)])                     # the returned pages, none of them still a's
+    assert len({*pages, *s.block_table[0].tolist()}) == 6
+    for seq, bad in (("a", 33), ("a", -1), ("nobody", 1)):
+        with pytest.raises(ValueError, match="cannot be cut"):
+            c.truncate(seq, bad)
+    assert c.length("a") == 32
