@@ -114,10 +114,11 @@ __device__ __forceinline__ TokenPlace place_token(const RowsArgs& a, bool live, 
   if constexpr (APPEND) {
     if (live) {
       // A sequence of one token most often: s == n.  These loads do not wait for one another.
-      const int end = a.cu_q[a.S];
+      const int begin = a.cu_q[0], end = a.cu_q[a.S];
       int s = min(n, a.S - 1);
-      int first = a.cu_q[s], next = a.cu_q[s + 1], kv = a.kv_lens[s];
-      w.write = n < end;
+      const int first = a.cu_q[s];
+      int next = a.cu_q[s + 1], kv = a.kv_lens[s];
+      w.write = begin <= n && n < end;  // the search then ends at a sequence that holds n
       if (w.write && (first > n || next <= n)) {
         int lo = 0, hi = a.S;  // the largest s with cu_q[s] <= n
         while (hi - lo > 1) {
@@ -126,10 +127,8 @@ __device__ __forceinline__ TokenPlace place_token(const RowsArgs& a, bool live, 
           else hi = mid;
         }
         s = lo;
-        first = a.cu_q[s];
         next = a.cu_q[s + 1];
         kv = a.kv_lens[s];
-        w.write = first <= n && n < next;  // else the token is before the first sequence
       }
       pos = (int64_t)kv - next + n;
       const int p = pos >= 0 && pos < 0x7fffffff ? static_cast<int>(pos) : -1;
