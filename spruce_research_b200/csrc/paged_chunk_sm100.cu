@@ -268,15 +268,18 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       auto wait = [&](uint64_t* bar, uint32_t parity) {
         return __all_sync(0xffffffffu, mbar_wait(bar, parity, status, abort_flag));
       };
+      // A descriptor's address is in its low word, which alone is stepped, where an MMA is issued (the asm statements below
+      // see to that): all steps kept ahead of the loop spill at 88 registers, and 64-bit additions cost 2.8% of a long chunk.
+      auto at_address = [](uint64_t d, uint32_t low) { return (d & 0xffffffff00000000ull) | low; };
       auto issue_qk = [&](int t, int st) {
         const uint32_t d = tmem + L::COL_S + 128 * t;
-        uint64_t qa = dq0 + (uint64_t)((t * L::TILE) >> 4);
-        uint64_t kb = dk0 + (uint64_t)((st * L::TILE) >> 4);
-        asm volatile("" : "+l"(qa), "+l"(kb));  // steps added here: kept ahead of the loop they spill at 88 registers
+        uint32_t qa = static_cast<uint32_t>(dq0) + ((t * L::TILE) >> 4);
+        uint32_t kb = static_cast<uint32_t>(dk0) + ((st * L::TILE) >> 4);
+        asm volatile("" : "+r"(qa), "+r"(kb));
 #pragma unroll
         for (int ks = 0; ks < D / 16; ++ks) {
           const uint32_t off = ((ks >> 2) * L::PANEL + (ks & 3) * 32) >> 4;
-          if (leader) umma_f16_ss(d, qa + off, kb + off, idesc_qk, ks > 0 ? 1u : 0u);
+          if (leader) umma_f16_ss(d, at_address(dq0, qa + off), at_address(dk0, kb + off), idesc_qk, ks > 0 ? 1u : 0u);
           __syncwarp();
         }
         commit(&s_full[t]);
@@ -286,13 +289,13 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         if (!wait(&p_full[2 * t + h], pvs[t] & 1)) return false;
         tc_fence_after();
         const uint32_t a = tmem + L::COL_S + 128 * t;
-        uint64_t vb = dv0 + (uint64_t)((st * L::TILE) >> 4);
-        asm volatile("" : "+l"(vb));
+        uint32_t vb = static_cast<uint32_t>(dv0) + ((st * L::TILE) >> 4);
+        asm volatile("" : "+r"(vb));
 #pragma unroll
         for (int kk = 0; kk < 4; ++kk) {
           const int ks = 4 * h + kk;
           if (leader)
-            umma_f16_ts(tmem + t * D, a + ks * 8, vb + (uint64_t)((ks * 2048) >> 4), idesc_pv,
+            umma_f16_ts(tmem + t * D, a + ks * 8, at_address(dv0, vb + ((ks * 2048) >> 4)), idesc_pv,
                         (!first || ks > 0) ? 1u : 0u);
           __syncwarp();
         }
