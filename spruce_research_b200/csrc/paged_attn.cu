@@ -47,7 +47,7 @@ struct F32Layout {
 // FMAs), with two CTAs an SM one of which loads while the other computes.  Few rows are bound by HBM on paper and in
 // practice by shared-memory reads (every key is read once a row group), so they take as few row groups as hold them,
 // eight or sixteen rows, and keep two tiles in flight.  On a B200: 512 tokens over 8K (28 heads of 128) 1.66 ms, 37 TFLOP/s;
-// one token over 32K 58 us, 2.3 TB/s.
+// one token over 32K 58 us, 2.3 TB/s.  At D = 128 the 64-row form spills 96 bytes of a thread's 128 registers.
 template <int D, int R, int TK, int STAGES>
 __global__ void __launch_bounds__(F32Layout<D, R, TK, STAGES>::THREADS) paged_attn_f32_kernel(const PagedParams p) {
   using L = F32Layout<D, R, TK, STAGES>;

@@ -6,24 +6,27 @@
 //   S_t = Q_t K^T   M128 N128 K16, D / 16 MMAs      O_t += P_t V   M128 N = D K16, 8 MMAs.
 // A CTA per SM walks its run of key tiles, from unit to unit, with the loads running ahead across the units' border.
 //
-// Warps: 0-3 softmax and epilogue of tile 0 (thread = row = TMEM lane), 4-7 of tile 1, 8 loads K and V, 9 issues the MMAs
-// and owns TMEM.  The softmax warps also bring in their own Q rows (once a unit).  O_0 O_1 S_0 S_1 fill TMEM's columns; P_t
-// is written over the first half of S_t.  One thread issues PV_0(j) QK_0(j+1) PV_1(j) QK_1(j+1) ..., in whose order they
-// execute, so QK_t(j+1) overwrites P_t(j) after PV_t(j) has read it, and while one tile's softmax runs the tensor core
-// works for the other.  P is announced in halves of 64 keys, so PV starts on the first while the second is
-// exponentiated.  O is rescaled only when the running maximum grew by more than 8 (log2 units; fp16: 2), which
-// O / l cancels.  P is rounded to the input type (the MMA's operand) and stays below 2^8 in bf16; in fp16 it carries 2^13 and
-// stays below 2^15, so weights keep all their bits down to 2^-27 of the row's largest.  The sum l is of the unrounded fp32 values.
+// Warps: 0-3 softmax and epilogue of tile 0 (thread = row = TMEM lane), 4-7 of tile 1, 8 issues the MMAs and owns TMEM,
+// 9 loads K, 10 loads V, 11 only fills its warpgroup.  The softmax warps also bring in their own Q rows (once a unit).
+// O_0 O_1 S_0 S_1 fill TMEM's columns; P_t is written over the first half of S_t.  One thread issues PV_0(j) QK_0(j+1)
+// PV_1(j) QK_1(j+1) ..., in whose order they execute, so QK_t(j+1) overwrites P_t(j) after PV_t(j) has read it, and while
+// one tile's softmax runs the tensor core works for the other.  P is announced in halves of 64 keys, so PV starts on the
+// first while the second is exponentiated.  O is rescaled only when the running maximum grew by more than 8 (log2 units;
+// fp16: 2), which O / l cancels.  P is rounded to the input type (the MMA's operand) and stays below 2^8 in bf16; in fp16 it
+// carries 2^13 and stays below 2^15, so weights keep all their bits down to 2^-27 of the row's largest.  The sum l is of the
+// unrounded fp32 values.
 //
 // Pages: one TMA box of a page's rows (or of 128 of them, or of its largest power-of-two divisor) lands as rows of the
 // 128-byte-swizzled tile.  Boxes past the sequence's end take a page index past the cache, which reads zeros; the rows of
 // the last page past the end may hold anything, so the loader clears them in V (their scores are masked by selection)
 // before the MMA issuer may read the tile.
 //
-// Measured on a B200 (28 query / 4 KV heads, d = 128, bf16): 2048 tokens over 64K 1.60 ms (1190 TFLOP/s; 1.75 ms in a long run
-// under the power cap), a 16K prompt in one chunk 1.58 ms, 512 tokens over 32K 226 us.  A key tile of both M-tiles takes
-// 3,210 cycles, the MMAs alone 2,880 (90 each, not the 64 of their rate: Q and K are both read from shared memory), a
-// tile's softmax 1,900.  The registers go to the softmax (208 a thread by setmaxnreg: with 168 it ran a sixth slower).
+// Measured on a B200 (28 query / 4 KV heads, d = 128, bf16): 2048 tokens over 64K 1.62-1.65 ms in short runs from idle (1,150
+// TFLOP/s), 1.80 ms in runs of a hundred under the power cap, 1.90 ms in longer ones (995 TFLOP/s); fp16 1.76 and 1.92 ms in the
+// first two.  A 16K prompt in one chunk 1.65 ms, 512 tokens over 32K 224 us, 247 us in long runs.  A key tile of both M-tiles was
+// traced at 3,210 cycles, the MMAs alone 2,880 (90 each, not the 64 of their rate: Q and K are both read from shared
+// memory), a tile's softmax 1,900.  The registers go to the softmax (208 a thread by setmaxnreg: with 168 it ran a sixth
+// slower; 200, 192 and 216 with what is left for the other warps 1-5% slower).
 //
 // Every wait is bounded (common.cuh).
 #include <algorithm>
@@ -455,7 +458,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         }
         // A tile with a score of NaN or +inf makes the row NaN whichever column holds it: the polynomial, whose clamp takes NaN
         // for a number, would lose it in the columns that it serves.
-        const float neg_ref = top < INFINITY ? (m_used == -INFINITY ? 0.0f : kScale - m_used) : __int_as_float(0x7fffffff);
+        const float lost = __int_as_float(0x7fffffff);
+        const float neg_ref = top < INFINITY ? (m_used == -INFINITY ? 0.0f : kScale - m_used) : lost;
         uint64_t sum2[2] = {f2_pack(0.0f, 0.0f), f2_pack(0.0f, 0.0f)};
         const uint64_t sl2x2 = f2_pack(sl2, sl2), nref2 = f2_pack(neg_ref, neg_ref);
 #pragma unroll

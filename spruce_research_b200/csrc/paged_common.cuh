@@ -297,7 +297,7 @@ __device__ __forceinline__ void let_next_kernel_start() { asm volatile("griddepc
 constexpr int kPagedChunkRows = 256, kPagedChunkKeys = 128;
 cudaError_t launch_paged_chunk(const PagedArgs& a, int dtype, int G, cudaStream_t stream);
 
-// Warp-MMA attention of at most 64 query rows a unit, in 1, 2 or 4 tiles of 16 (paged_rows_sm100.cu).
+// Warp-MMA attention of at most 32 query rows a unit, in 1 or 2 tiles of 16 (paged_rows_sm100.cu).
 constexpr int kPagedRowsMax = 32, kPagedRowsKeys = 64, kPagedRowsPerSm = 2;
 cudaError_t launch_paged_rows(const PagedArgs& a, int dtype, int tiles, int G, cudaStream_t stream);
 // The cache's tensor maps, and the rows of a box of them, for key tiles of `tile` (paged_chunk_sm100.cu).

@@ -9,7 +9,8 @@
 //
 // Bound: HBM bandwidth (every row read once, written once; ~10 flops an element).  On a B200 Q and K of a 131072-token
 // layer (28 + 4 heads of 128, bf16, 2.2 GB) take 322 us, 6.9 TB/s; 16384 tokens with norms 45.3 us, 5.9 TB/s; 4097 tokens with
-// norms 14.4 us; the append of 8.2K tokens 30.8 us, 5.3 TB/s.
+// norms 14.4 us; the append of 8.2K tokens 30.6 us, 5.3 TB/s.  fp32, 16384 tokens with norms: 84.2 us, 6.5 TB/s.  Rows that 16-byte
+// vectors do not fit, a warp a row: 16384 tokens 202 us in bf16 (1.4 TB/s), 199 us in fp32 (2.7 TB/s), bound by element loads.
 //
 // Layout: a row is held by LPR lanes (8 at D = 128 in 16 bits), each with two 16-byte vectors that hold whole pairs (half
 // pairs: the same place in each half of the rotated dims; interleaved: any vector), so a rotation needs no exchange and the
