@@ -40,6 +40,7 @@ extern "C" {
 #define SPRUCE_STATUS_BAD_PAGE 4u  /* a page id outside the cache was needed */
 #define SPRUCE_STATUS_BAD_LENGTH 8u    /* a sequence length or offset outside its bounds */
 #define SPRUCE_STATUS_BAD_POSITION 16u /* a position outside the rotation table */
+#define SPRUCE_STATUS_BAD_INDEX 32u    /* a teacher's column past the visible ones */
 
 #define SPRUCE_DTYPE_F32 0
 #define SPRUCE_DTYPE_BF16 1
@@ -507,6 +508,113 @@ typedef struct {
   double scale;
 } spruce_paged_attention_args;
 SPRUCE_API int spruce_paged_attention(const spruce_paged_attention_args *args);
+
+/* The same, and the natural log of each query row's softmax sum (of exp(score * scale)) to lse, fp32 [N, Hq] by
+ * strides (token, head); -inf for a query that sees nothing.  Rows that out does not get are not written here either. */
+typedef struct {
+  spruce_paged_attention_args attention;
+  float *lse;
+  int64_t lse_strides[2];
+} spruce_paged_attention_lse_args;
+SPRUCE_API int spruce_paged_attention_lse(const spruce_paged_attention_lse_args *args);
+
+/*
+ * Softmax weight that each cached key receives from new tokens (packed as above, already in the cache), summed over the
+ * queries that see it and the query heads of its group:
+ *   mass_out[j] = decay * mass[j] + sum_i sum_h exp(scale * q_ih . k_j - lse_ih)
+ * for every slot j of a sequence that has new tokens; slots of the new tokens themselves start from 0, whatever mass
+ * holds there, and with decay = 0 no old value is read.  Sequences without new tokens, and all other slots, are left as they are.
+ * lse is spruce_paged_attention_lse's; a row whose lse is -inf gives nothing.  mass and mass_out are fp32 [num_pages,
+ * Hkv, page_size] by strides (page, head, row) and may be one.  Bounds, pages and alignment are spruce_paged_attention's: keys
+ * of a bad page get no weight written, queries past max_q_len give none.  Each sum is formed in a fixed order.
+ */
+typedef struct {
+  const void *q, *k_cache;
+  const float *lse, *mass;
+  float *mass_out;
+  const int32_t *block_table, *cu_q, *kv_lens;
+  uint32_t *status;
+  void *stream;
+  int64_t q_strides[2], kc_strides[3], lse_strides[2], mass_strides[3], mass_out_strides[3];
+  int64_t dtype, N, S, Hq, Hkv, D, num_pages, page_size, table_stride, max_pages, max_q_len, max_kv_len;
+  double scale, decay;
+} spruce_paged_key_mass_args;
+SPRUCE_API int spruce_paged_key_mass(const spruce_paged_key_mass_args *args);
+
+/*
+ * Eviction from a paged cache by weight.  A sequence that holds more than `keep` tokens keeps, in each KV head, its first
+ * `sinks` slots, its last `recent` ones and of those between the ones of the largest mass, `keep` in all (equal masses:
+ * the lowest slot; NaN counts as the largest); where keep < sinks + recent, sinks go first.  The kept rows of K, V and mass move, in
+ * their order, to slots 0 .. keep - 1 of the pages that out_table names, in the caches *_out.  Shorter sequences keep all.
+ * In place (the outputs are the inputs, out_table is block_table), or into pages that no sequence of the call reads.  In
+ * place, no page may belong to two sequences of the call.  Slots past the kept ones are left as they are.
+ * kept int32 [S, Hkv, width] receives the old slots, -1 past the kept ones; width >= min(keep, max_kv_len).  new_lens int32
+ * [S] receives the new lengths and may not be kv_lens.  A sequence longer than max_kv_len or its table is left as it is (kept
+ * -1, its length unchanged) and raises SPRUCE_STATUS_BAD_LENGTH; masses and rows of a bad page count as 0 and
+ * are not moved, and raise SPRUCE_STATUS_BAD_PAGE.  K and V rows are 16-byte aligned.
+ */
+typedef struct {
+  const void *k_cache, *v_cache;
+  const float *mass;
+  void *k_out, *v_out;
+  float *mass_out;
+  const int32_t *block_table, *out_table, *kv_lens;
+  int32_t *kept, *new_lens;
+  uint32_t *status;
+  void *stream;
+  int64_t kc_strides[3], vc_strides[3], mass_strides[3], k_out_strides[3], v_out_strides[3], mass_out_strides[3];
+  int64_t dtype, S, Hkv, D, num_pages, page_size, table_stride, max_pages, out_pages, out_table_stride, out_max_pages,
+      max_kv_len, width, keep, sinks, recent;
+} spruce_paged_evict_args;
+SPRUCE_API int spruce_paged_evict(const spruce_paged_evict_args *args);
+
+/*
+ * Softmax weight of whole key blocks, a gate's teacher: of causal attention of q [B, Hq, T, D] over k [B, Hkv, T, D]
+ * (element strides, unit last),
+ *   out[b, g, i, j] = mean over heads h of group g and tokens t of query block i of sum_{u in block j, u <= t} p_tu,
+ * fp32 [B, Hkv, qb, qb] contiguous, qb = ceil(T / 64); rows sum to 1 and are 0 past the diagonal.  A token whose scores
+ * are all -inf gives nothing; one with a score of NaN or +inf makes its block's row NaN.  D in {64, 128}, rows 16-byte aligned,
+ * scale >= 0.  workspace: spruce_block_mass_workspace_bytes (-1 for an invalid shape), 256-byte aligned; a call uses it alone.
+ */
+SPRUCE_API int64_t spruce_block_mass_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t T, int64_t D, int dtype);
+typedef struct {
+  const void *q, *k;
+  float *out;
+  void *workspace;
+  uint32_t *status;
+  void *stream;
+  int64_t q_strides[4], k_strides[4];
+  int64_t dtype, B, Hq, Hkv, T, D, workspace_bytes;
+  double scale;
+} spruce_block_mass_args;
+SPRUCE_API int spruce_block_mass(const spruce_block_mass_args *args);
+
+/*
+ * Distillation of a teacher's top entries into rows of scores [R, n] (row stride, unit last): with
+ *   p = softmax over the row's entries k of teacher[r, k] / tau,   q = softmax over its visible columns of scores[r, j] / tau,
+ *   loss[r] = sum_k p_k (ln p_k - ln q_ids[r,k]),
+ *   grad[r, j] = weight[r] / tau * (q_j - sum_{k: ids[r,k] = j} p_k),  0 past the visible columns.
+ * ids [R, K] are int32, or int64 (ids64 != 0); negative ones are padding; one past the visible columns counts as padding
+ * and raises SPRUCE_STATUS_BAD_INDEX.  A column named twice counts twice.  visible int32 [R] (NULL: all n columns); one outside
+ * [0, n] is cut to it and raises SPRUCE_STATUS_BAD_LENGTH.  A row without a column above -inf, or without a teacher entry above it,
+ * has loss and gradient 0.  teacher has a dtype of its own.  Outputs: loss fp32 [R] and stats fp32 [R, 2] (what the
+ * gradient needs of the scores' softmax; NULL: not wanted), grad in the scores' dtype [R, n] by row stride (NULL: not wanted; needs
+ * weight fp32 [R] by stride).  With stats_in, of a call on the same scores, visible and tau, only grad is formed.
+ * tau > 0, K <= 2048.  Outputs may not overlap the scores.
+ */
+typedef struct {
+  const void *scores, *ids, *teacher;
+  const int32_t *visible;
+  float *loss, *stats;
+  const float *stats_in, *weight;
+  void *grad;
+  uint32_t *status;
+  void *stream;
+  int64_t score_stride, id_stride, teacher_stride, weight_stride, grad_stride;
+  int64_t dtype, teacher_dtype, ids64, R, n, K;
+  double tau;
+} spruce_topk_distill_args;
+SPRUCE_API int spruce_topk_distill(const spruce_topk_distill_args *args);
 
 #ifdef __cplusplus
 }

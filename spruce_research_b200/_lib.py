@@ -26,6 +26,7 @@ STATUS_EMPTY_ROW = 2
 STATUS_BAD_PAGE = 4
 STATUS_BAD_LENGTH = 8
 STATUS_BAD_POSITION = 16
+STATUS_BAD_INDEX = 32
 
 DTYPE_CODE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
@@ -81,12 +82,23 @@ SIGNATURES = {
     "spruce_paged_append": ([_P], _INT),
     "spruce_paged_attention_workspace_bytes": ([_I64, _I64, _I64, _I64, _INT], _I64),
     "spruce_paged_attention": ([_P], _INT),
+    "spruce_paged_attention_lse": ([_P], _INT),
+    "spruce_paged_key_mass": ([_P], _INT),
+    "spruce_paged_evict": ([_P], _INT),
+    "spruce_block_mass_workspace_bytes": ([_I64, _I64, _I64, _I64, _I64, _INT], _I64),
+    "spruce_block_mass": ([_P], _INT),
+    "spruce_topk_distill": ([_P], _INT),
 }
 
-# The argument structs of the serving operators: 8-byte pointers and integers, a double at the end.
+# The argument structs of the serving and weight operators: 8-byte pointers and integers, doubles after them.
 QK_NORM_ROPE_ARGS = struct.Struct("=37qd")
 PAGED_APPEND_ARGS = struct.Struct("=42qd")
 PAGED_ATTENTION_ARGS = struct.Struct("=33qd")
+PAGED_ATTENTION_LSE_ARGS = struct.Struct("=33qd3q")
+PAGED_KEY_MASS_ARGS = struct.Struct("=35q2d")
+PAGED_EVICT_ARGS = struct.Struct("=47q")
+BLOCK_MASS_ARGS = struct.Struct("=21qd")
+TOPK_DISTILL_ARGS = struct.Struct("=22qd")
 
 _lib = None
 

@@ -869,9 +869,7 @@ int64_t spruce_paged_attention_workspace_bytes(int64_t Hq, int64_t Hkv, int64_t 
   return spruce::paged_workspace_bytes(Hq, Hkv, D, max_q_len, dtype);
 }
 
-int spruce_paged_attention(const spruce_paged_attention_args* args) {
-  if (args == nullptr) return fail(SPRUCE_ERR_INVALID, "null arguments");
-  const spruce_paged_attention_args& x = *args;
+static int paged_attention_impl(const spruce_paged_attention_args& x, float* lse, int64_t ln, int64_t lh) {
   if (int rc = check_paged(x)) return rc;
   if (x.Hq < 1 || x.Hq % x.Hkv)
     return fail(SPRUCE_ERR_INVALID, "query heads (%lld) must be divisible by KV heads (%lld)", (long long)x.Hq,
@@ -935,7 +933,279 @@ int spruce_paged_attention(const spruce_paged_attention_args* args) {
   a.scale = scale;
   a.workspace = x.workspace;
   a.status = x.status;
+  a.lse = lse;
+  a.ln = ln;
+  a.lh = lh;
   return cuda_status(spruce::launch_paged_attention(a, (int)x.dtype, as_stream(x.stream)), "paged attention launch");
+}
+
+int spruce_paged_attention(const spruce_paged_attention_args* args) {
+  if (args == nullptr) return fail(SPRUCE_ERR_INVALID, "null arguments");
+  return paged_attention_impl(*args, nullptr, 0, 0);
+}
+
+int spruce_paged_attention_lse(const spruce_paged_attention_lse_args* args) {
+  if (args == nullptr) return fail(SPRUCE_ERR_INVALID, "null arguments");
+  if (args->lse == nullptr && args->attention.N > 0 && args->attention.S > 0) return fail(SPRUCE_ERR_INVALID, "lse is NULL");
+  return paged_attention_impl(args->attention, args->lse, args->lse_strides[0], args->lse_strides[1]);
+}
+
+int spruce_paged_key_mass(const spruce_paged_key_mass_args* args) {
+  if (args == nullptr) return fail(SPRUCE_ERR_INVALID, "null arguments");
+  const spruce_paged_key_mass_args& x = *args;
+  if (int rc = check_paged(x)) return rc;
+  if (x.Hq < 1 || x.Hq % x.Hkv)
+    return fail(SPRUCE_ERR_INVALID, "query heads (%lld) must be divisible by KV heads (%lld)", (long long)x.Hq,
+                (long long)x.Hkv);
+  if (x.D != 64 && x.D != 128)
+    return fail(SPRUCE_ERR_UNSUPPORTED, "key mass needs head_dim 64 or 128, got %lld", (long long)x.D);
+  if (x.max_q_len < 0 || x.max_kv_len < 0)
+    return fail(SPRUCE_ERR_INVALID, "max_q_len and max_kv_len must not be negative");
+  if (x.max_q_len > kMaxQueryRows / x.Hq || x.max_kv_len > INT32_MAX)
+    return fail(SPRUCE_ERR_UNSUPPORTED, "sequence too long");
+  const float scale = (float)x.scale, decay = (float)x.decay;
+  if (!(scale >= 0.0f && scale <= 3.0e38f))
+    return fail(SPRUCE_ERR_INVALID, "scale must be finite and not negative, got %g", x.scale);
+  if (!(decay >= 0.0f && decay <= 1.0f)) return fail(SPRUCE_ERR_INVALID, "decay must be in [0, 1], got %g", x.decay);
+  if (x.N == 0 || x.S == 0) return SPRUCE_OK;
+  if (x.num_pages < 1) return fail(SPRUCE_ERR_INVALID, "the cache has no pages");
+  if (x.q == nullptr || x.k_cache == nullptr || x.lse == nullptr || x.mass == nullptr || x.mass_out == nullptr)
+    return fail(SPRUCE_ERR_INVALID, "null pointer");
+  const int64_t vn = 16 / elem_size((int)x.dtype);
+  bool ok = aligned16(x.q) && aligned16(x.k_cache);
+  for (int i = 0; i < 2; ++i) ok = ok && x.q_strides[i] % vn == 0;
+  for (int i = 0; i < 3; ++i) ok = ok && x.kc_strides[i] % vn == 0;
+  if (!ok) return fail(SPRUCE_ERR_UNSUPPORTED, "q and the cache need 16-byte aligned rows");
+  const int64_t sizes[3] = {x.num_pages, x.Hkv, x.page_size};
+  for (int i = 0; i < 3; ++i)  // what a tensor map can step by
+    if (sizes[i] > 1 && x.kc_strides[i] < 1) return fail(SPRUCE_ERR_UNSUPPORTED, "the cache needs positive strides");
+  spruce::KeyMassArgs m{};
+  spruce::PagedArgs& a = m.a;
+  a.q = x.q;
+  a.qn = x.q_strides[0];
+  a.qh = x.q_strides[1];
+  a.kc = a.vc = x.k_cache;
+  for (int i = 0; i < 3; ++i) {
+    a.ks[i] = a.vs[i] = x.kc_strides[i];
+    m.ms[i] = x.mass_strides[i];
+    m.os[i] = x.mass_out_strides[i];
+  }
+  a.block_table = x.block_table;
+  a.table_stride = x.table_stride;
+  a.cu_q = x.cu_q;
+  a.kv_lens = x.kv_lens;
+  a.S = (int)x.S;
+  a.N = (int)x.N;
+  a.Hq = (int)x.Hq;
+  a.Hkv = (int)x.Hkv;
+  a.D = (int)x.D;
+  a.page_size = (int)x.page_size;
+  a.max_pages = (int)x.max_pages;
+  a.max_q = (int)x.max_q_len;
+  a.max_kv = (int)x.max_kv_len;
+  a.num_pages = x.num_pages;
+  a.scale = scale;
+  a.status = x.status;
+  m.lse = x.lse;
+  m.ln = x.lse_strides[0];
+  m.lh = x.lse_strides[1];
+  m.mass = x.mass;
+  m.out = x.mass_out;
+  m.decay = decay;
+  return cuda_status(spruce::launch_key_mass(m, (int)x.dtype, as_stream(x.stream)), "key mass launch");
+}
+
+int spruce_paged_evict(const spruce_paged_evict_args* args) {
+  if (args == nullptr) return fail(SPRUCE_ERR_INVALID, "null arguments");
+  const spruce_paged_evict_args& x = *args;
+  if (x.dtype != (int)x.dtype || !valid_dtype((int)x.dtype))
+    return fail(SPRUCE_ERR_INVALID, "unsupported dtype code %lld", (long long)x.dtype);
+  if (x.S < 0 || x.Hkv < 1 || x.Hkv > 65535 || x.D < 1 || x.num_pages < 0 || x.max_pages < 0 || x.out_pages < 0 ||
+      x.out_max_pages < 0 || x.max_kv_len < 0 || x.width < 0)
+    return fail(SPRUCE_ERR_INVALID, "bad shape");
+  if (x.page_size < 16 || x.page_size % 16)
+    return fail(SPRUCE_ERR_UNSUPPORTED, "page_size must be a multiple of 16, got %lld", (long long)x.page_size);
+  if (x.keep < 0 || x.sinks < 0 || x.recent < 0)
+    return fail(SPRUCE_ERR_INVALID, "keep, sinks and recent must not be negative");
+  const int64_t row = x.D * elem_size((int)x.dtype);
+  if (x.D > 512 || row % 16)
+    return fail(SPRUCE_ERR_UNSUPPORTED, "rows of %lld elements: at most 512, a multiple of 16 bytes", (long long)x.D);
+  // Blocks of the moves: two slices of 16 bytes at least and one of weights a (sequence, head).
+  if (x.max_pages > INT32_MAX || x.page_size > INT32_MAX || x.num_pages > INT32_MAX || x.out_pages > INT32_MAX ||
+      x.max_kv_len > (1 << 30) || x.width > (1 << 30) || x.S > INT32_MAX / (2 * (row / 16) + 1) / x.Hkv)
+    return fail(SPRUCE_ERR_UNSUPPORTED, "shape too large");
+  if (x.width < (x.keep < x.max_kv_len ? x.keep : x.max_kv_len))
+    return fail(SPRUCE_ERR_INVALID, "kept is %lld wide, sequences keep up to %lld", (long long)x.width,
+                (long long)(x.keep < x.max_kv_len ? x.keep : x.max_kv_len));
+  if (x.S == 0) return SPRUCE_OK;
+  if (x.kv_lens == nullptr || x.new_lens == nullptr || (x.kept == nullptr && x.width > 0))
+    return fail(SPRUCE_ERR_INVALID, "null pointer");
+  if (x.kv_lens == x.new_lens) return fail(SPRUCE_ERR_INVALID, "new_lens may not be kv_lens");
+  int64_t cap = x.max_pages > x.max_kv_len / x.page_size ? x.max_kv_len : x.max_pages * x.page_size;
+  if (cap > 0 && (x.num_pages < 1 || x.k_cache == nullptr || x.v_cache == nullptr || x.mass == nullptr ||
+                  x.block_table == nullptr))
+    return fail(SPRUCE_ERR_INVALID, "null pointer");
+  const int64_t most = x.keep < cap ? x.keep : cap;
+  if (most > 0 && (x.k_out == nullptr || x.v_out == nullptr || x.mass_out == nullptr || x.out_table == nullptr))
+    return fail(SPRUCE_ERR_INVALID, "null pointer");
+  if (most > 0 && (x.out_max_pages < (most + x.page_size - 1) / x.page_size || x.out_pages < 1))
+    return fail(SPRUCE_ERR_INVALID, "the output's table has %lld pages a sequence, %lld tokens stay",
+                (long long)x.out_max_pages, (long long)most);
+  const int64_t vn = 16 / elem_size((int)x.dtype);
+  bool ok = aligned16(x.k_cache) && aligned16(x.v_cache) && aligned16(x.k_out) && aligned16(x.v_out);
+  for (int i = 0; i < 3; ++i)
+    ok = ok && x.kc_strides[i] % vn == 0 && x.vc_strides[i] % vn == 0 && x.k_out_strides[i] % vn == 0 &&
+         x.v_out_strides[i] % vn == 0;
+  if (!ok) return fail(SPRUCE_ERR_UNSUPPORTED, "the caches need 16-byte aligned rows");
+  const bool in_place = x.k_out == x.k_cache;
+  if (in_place) {
+    bool same = x.v_out == x.v_cache && x.mass_out == x.mass && x.out_table == x.block_table &&
+                x.out_table_stride == x.table_stride && x.out_pages == x.num_pages;
+    for (int i = 0; i < 3; ++i)
+      same = same && x.kc_strides[i] == x.k_out_strides[i] && x.vc_strides[i] == x.v_out_strides[i] &&
+             x.mass_strides[i] == x.mass_out_strides[i];
+    // The keys alone may lie in the same cache: then the other pages are the caller's promise.
+    if (!same && x.out_table == x.block_table)
+      return fail(SPRUCE_ERR_INVALID, "in place, every output has to be its input");
+  }
+  spruce::EvictArgs a{};
+  a.k = x.k_cache;
+  a.v = x.v_cache;
+  a.mass = x.mass;
+  a.k_out = x.k_out;
+  a.v_out = x.v_out;
+  a.mass_out = x.mass_out;
+  for (int i = 0; i < 3; ++i) {
+    a.ks[i] = x.kc_strides[i];
+    a.vs[i] = x.vc_strides[i];
+    a.ms[i] = x.mass_strides[i];
+    a.kos[i] = x.k_out_strides[i];
+    a.vos[i] = x.v_out_strides[i];
+    a.mos[i] = x.mass_out_strides[i];
+  }
+  a.table = x.block_table;
+  a.to_table = x.out_table;
+  a.table_stride = x.table_stride;
+  a.to_table_stride = x.out_table_stride;
+  a.kv_lens = x.kv_lens;
+  a.kept = x.kept;
+  a.new_lens = x.new_lens;
+  a.S = (int)x.S;
+  a.Hkv = (int)x.Hkv;
+  a.D = (int)x.D;
+  a.es = elem_size((int)x.dtype);
+  a.page_size = (int)x.page_size;
+  a.cap = (int)cap;
+  a.width = (int)x.width;
+  a.keep = (int)(x.keep < cap ? x.keep : cap);
+  a.sinks = (int)(x.sinks < cap ? x.sinks : cap);
+  a.recent = (int)(x.recent < cap ? x.recent : cap);
+  a.num_pages = x.num_pages;
+  a.to_pages = x.out_pages;
+  a.in_place = in_place && x.out_table == x.block_table;
+  a.status = x.status;
+  return cuda_status(spruce::launch_evict(a, as_stream(x.stream)), "eviction launch");
+}
+
+int64_t spruce_block_mass_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t T, int64_t D, int dtype) {
+  if (!valid_dtype(dtype) || B < 0 || Hkv < 1 || Hq < 1 || Hq % Hkv || Hq > 65535 || (D != 64 && D != 128) || T < 0 ||
+      T > (1 << 24) || B > INT32_MAX / Hq / ((T + 63) / 64 + 1))
+    return -1;
+  return spruce::block_mass_workspace_bytes(B, Hq, Hkv, T, D, dtype);
+}
+
+int spruce_block_mass(const spruce_block_mass_args* args) {
+  if (args == nullptr) return fail(SPRUCE_ERR_INVALID, "null arguments");
+  const spruce_block_mass_args& x = *args;
+  if (x.dtype != (int)x.dtype || !valid_dtype((int)x.dtype))
+    return fail(SPRUCE_ERR_INVALID, "unsupported dtype code %lld", (long long)x.dtype);
+  if (x.B < 0 || x.T < 0 || x.Hkv < 1 || x.Hq < 1) return fail(SPRUCE_ERR_INVALID, "bad shape");
+  if (x.Hq % x.Hkv)
+    return fail(SPRUCE_ERR_INVALID, "query heads (%lld) must be divisible by KV heads (%lld)", (long long)x.Hq,
+                (long long)x.Hkv);
+  if (x.D != 64 && x.D != 128)
+    return fail(SPRUCE_ERR_UNSUPPORTED, "block mass needs head_dim 64 or 128, got %lld", (long long)x.D);
+  const float scale = (float)x.scale;
+  if (!(scale >= 0.0f && scale <= 3.0e38f / 1.5f))
+    return fail(SPRUCE_ERR_INVALID, "scale must be finite and not negative, got %g", x.scale);
+  const int64_t need = spruce_block_mass_workspace_bytes(x.B, x.Hq, x.Hkv, x.T, x.D, (int)x.dtype);
+  if (need < 0) return fail(SPRUCE_ERR_UNSUPPORTED, "shape too large");
+  if (x.B == 0 || x.T == 0) return SPRUCE_OK;
+  if (x.q == nullptr || x.k == nullptr || x.out == nullptr) return fail(SPRUCE_ERR_INVALID, "null pointer");
+  if (!aligned16(x.q) || !aligned16(x.k) || !vec_strides_ok(x.q_strides, (int)x.dtype, x.D) ||
+      !vec_strides_ok(x.k_strides, (int)x.dtype, x.D))
+    return fail(SPRUCE_ERR_UNSUPPORTED, "q and k need 16-byte aligned rows with a unit last stride");
+  const int64_t sizes[3] = {x.B, x.Hq, x.T};
+  for (int i = 0; i < 3; ++i)  // what a tensor map can step by
+    if (sizes[i] > 1 && (x.q_strides[i] < 1 || (x.k_strides[i] < 1 && !(i == 1 && x.Hkv == 1))))
+      return fail(SPRUCE_ERR_UNSUPPORTED, "q and k need positive strides");
+  if (x.workspace == nullptr || x.workspace_bytes < need)
+    return fail(SPRUCE_ERR_WORKSPACE, "block mass workspace needs %lld bytes, got %lld", (long long)need,
+                (long long)x.workspace_bytes);
+  if (reinterpret_cast<uintptr_t>(x.workspace) & 255u)
+    return fail(SPRUCE_ERR_UNSUPPORTED, "workspace must be 256-byte aligned");
+  spruce::BlockMassArgs a{};
+  a.q = x.q;
+  a.k = x.k;
+  for (int i = 0; i < 3; ++i) {
+    a.qs[i] = x.q_strides[i];
+    a.ks[i] = x.k_strides[i];
+  }
+  a.B = (int)x.B;
+  a.Hq = (int)x.Hq;
+  a.Hkv = (int)x.Hkv;
+  a.T = (int)x.T;
+  a.D = (int)x.D;
+  // Not 0: a masked score (-inf) times 0 is not a number.  1e-30 makes every finite score 0 as well.
+  a.scale_log2 = scale > 0.0f ? scale * 1.4426950408889634f : 1e-30f;
+  a.out = x.out;
+  a.workspace = static_cast<float*>(x.workspace);
+  a.status = x.status;
+  return cuda_status(spruce::launch_block_mass(a, (int)x.dtype, as_stream(x.stream)), "block mass launch");
+}
+
+int spruce_topk_distill(const spruce_topk_distill_args* args) {
+  if (args == nullptr) return fail(SPRUCE_ERR_INVALID, "null arguments");
+  const spruce_topk_distill_args& x = *args;
+  if (x.dtype != (int)x.dtype || !valid_dtype((int)x.dtype) || x.teacher_dtype != (int)x.teacher_dtype ||
+      !valid_dtype((int)x.teacher_dtype))
+    return fail(SPRUCE_ERR_INVALID, "unsupported dtype code");
+  if (x.R < 0 || x.n < 0 || x.K < 0) return fail(SPRUCE_ERR_INVALID, "bad shape");
+  if (x.n > (1 << 30) || x.R > (int64_t(1) << 40)) return fail(SPRUCE_ERR_UNSUPPORTED, "shape too large");
+  if (x.K > 2048) return fail(SPRUCE_ERR_UNSUPPORTED, "at most 2048 teacher entries a row, got %lld", (long long)x.K);
+  const float inv_tau = (float)(1.0 / x.tau);
+  if (!(x.tau > 0.0 && inv_tau > 1e-30f && inv_tau < 1e30f))
+    return fail(SPRUCE_ERR_INVALID, "temperature must be positive and finite, got %g", x.tau);
+  if (x.R == 0) return SPRUCE_OK;
+  if ((x.scores == nullptr && x.n > 0) || ((x.ids == nullptr || x.teacher == nullptr) && x.K > 0) ||
+      (x.loss == nullptr && x.grad == nullptr) || (x.grad != nullptr && x.weight == nullptr) ||
+      (x.stats_in != nullptr && x.grad == nullptr))
+    return fail(SPRUCE_ERR_INVALID, "null pointer");
+  if (x.stats_in != nullptr && (x.loss != nullptr || x.stats != nullptr))
+    return fail(SPRUCE_ERR_INVALID, "stats_in is for the gradient alone");
+  spruce::DistillArgs a{};
+  a.scores = x.scores;
+  a.score_stride = x.score_stride;
+  a.ids = x.ids;
+  a.id_stride = x.id_stride;
+  a.ids64 = x.ids64 != 0;
+  a.teacher = x.teacher;
+  a.teacher_stride = x.teacher_stride;
+  a.teacher_dtype = (int)x.teacher_dtype;
+  a.visible = x.visible;
+  a.loss = x.loss;
+  a.stats = x.stats;
+  a.stats_in = x.stats_in;
+  a.weight = x.weight;
+  a.weight_stride = x.weight_stride;
+  a.grad = x.grad;
+  a.grad_stride = x.grad_stride;
+  a.R = x.R;
+  a.n = (int)x.n;
+  a.K = (int)x.K;
+  a.inv_tau = inv_tau;
+  a.status = x.status;
+  return cuda_status(spruce::launch_distill(a, (int)x.dtype, as_stream(x.stream)), "distillation launch");
 }
 
 }  // extern "C"

@@ -186,9 +186,82 @@ struct PagedArgs {
   float scale;
   void* workspace;
   uint32_t* status;
+  float* lse;                 // [N, Hq], or nullptr
+  int64_t ln, lh;
 };
 int64_t paged_workspace_bytes(int64_t Hq, int64_t Hkv, int64_t D, int64_t max_q, int dtype);
 cudaError_t launch_paged_attention(const PagedArgs& a, int dtype, cudaStream_t stream);
+
+// Softmax weight that each cached key receives from the new tokens (mass*.cu).
+struct KeyMassArgs {
+  PagedArgs a;                // vc, out, workspace unused
+  const float* lse;           // [N, Hq], natural log
+  int64_t ln, lh;
+  const float* mass;          // [num_pages, Hkv, page_size]
+  float* out;
+  int64_t ms[3], os[3];       // element strides: page, head, row
+  float decay;
+};
+cudaError_t launch_key_mass(const KeyMassArgs& a, int dtype, cudaStream_t stream);
+
+// Mean softmax weight of whole key blocks (mass*.cu).
+struct BlockMassArgs {
+  const void* q;              // [B, Hq, T, D], element strides b, h, t
+  const void* k;              // [B, Hkv, T, D]
+  int64_t qs[3], ks[3];
+  int B, Hq, Hkv, T, D;
+  float scale_log2;
+  float* out;                 // [B, Hkv, qb, qb]
+  float* workspace;
+  uint32_t* status;
+};
+int64_t block_mass_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t T, int64_t D, int dtype);
+cudaError_t launch_block_mass(const BlockMassArgs& a, int dtype, cudaStream_t stream);
+
+// Eviction from a paged cache by weight (evict.cu).
+struct EvictArgs {
+  const void *k, *v;          // [num_pages, Hkv, page_size, D]
+  const float* mass;          // [num_pages, Hkv, page_size]
+  void *k_out, *v_out;        // [to_pages, Hkv, page_size, D]
+  float* mass_out;
+  int64_t ks[3], vs[3], ms[3], kos[3], vos[3], mos[3];  // element strides: page, head, row
+  const int32_t* table;       // [S, max_pages]
+  const int32_t* to_table;
+  int64_t table_stride, to_table_stride;
+  const int32_t* kv_lens;     // [S]
+  int32_t* kept;              // [S, Hkv, width]
+  int32_t* new_lens;          // [S]
+  int S, Hkv, D, es, page_size, cap, width, keep, sinks, recent;
+  int64_t num_pages, to_pages;
+  bool in_place;
+  uint32_t* status;
+};
+cudaError_t launch_evict(const EvictArgs& a, cudaStream_t stream);
+
+// Distillation of a teacher's top entries (distill.cu).
+struct DistillArgs {
+  const void* scores;         // [R, n]
+  int64_t score_stride;
+  const void* ids;            // [R, K] int32 or int64
+  int64_t id_stride;
+  bool ids64;
+  const void* teacher;        // [R, K]
+  int64_t teacher_stride;
+  int teacher_dtype;
+  const int32_t* visible;     // [R] or nullptr
+  float* loss;                // [R] or nullptr
+  float* stats;               // [R, 2] or nullptr: the student's maximum and log2 of its sum
+  const float* stats_in;      // those of an earlier call, or nullptr
+  const float* weight;        // [R] (by stride) of the gradient
+  int64_t weight_stride;
+  void* grad;                 // [R, n] or nullptr
+  int64_t grad_stride;
+  int64_t R;
+  int n, K;
+  float inv_tau;
+  uint32_t* status;
+};
+cudaError_t launch_distill(const DistillArgs& a, int dtype, cudaStream_t stream);
 
 // K/V summary table of the residual tree (summaries.cu).
 struct KvSummaryArgs {

@@ -11,8 +11,7 @@
 
 namespace spruce {
 
-// SMs of the current GPU, asked for once.
-static int sm_count() {
+int sm_count() {
   static std::atomic<int> known[64];
   int dev = 0, v = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return 148;
@@ -218,6 +217,7 @@ __global__ void __launch_bounds__(F32Layout<D, R, TK, STAGES>::THREADS) paged_at
       if (x.slot < 0) {
         dst = static_cast<float*>(p.a.out) + row_at.offset(r, p.a.on, p.a.oh);
         f = l[i] > 0.0f ? 1.0f / l[i] : 0.0f;
+        if (p.a.lse != nullptr && cg == 0) p.a.lse[row_at.offset(r, p.a.ln, p.a.lh)] = paged_lse(p, m[i], l[i]);
       } else {
         const int64_t at = (int64_t)(2 * blockIdx.x + x.slot) * R + r;
         if (cg == 0) p.part_ml[at] = make_float2(m[i], l[i]);
@@ -298,7 +298,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PagedPar
     const bool few = parts <= kJoinWarps;
     const int r = few ? (job - first[c]) * kJoinWarps + warp : job - first[c];
     const int step = few ? 1 : kJoinWarps, start = few ? 0 : warp;
-    float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f}, l = 0.0f;
+    float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f}, l = 0.0f, top = -INFINITY;
     if (r < rows) {
       // Part i > 0 begins its run (slot 0); part 0 has the described slot.
       auto at = [&](int i) { return (int64_t)(2 * (c + i) + (i == 0 ? paged_desc_slot(d.w) : 0)) * R + r; };
@@ -328,7 +328,6 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PagedPar
         }
       };
       load(start);
-      float top = -INFINITY;
       for (int i = lane; i < parts; i += 32) top = fmaxf(top, p.part_ml[at(i)].x);
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
@@ -363,7 +362,9 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PagedPar
       }
     }
     if (r < rows && (few || warp == 0)) {
-      T* dst = static_cast<T*>(p.a.out) + PagedRows(p, d.x, d.y * R, d.z).offset(r, p.a.on, p.a.oh) + lane * dims;
+      const PagedRows row_at(p, d.x, d.y * R, d.z);
+      if (p.a.lse != nullptr && lane == 0) p.a.lse[row_at.offset(r, p.a.ln, p.a.lh)] = paged_lse(p, top, l);
+      T* dst = static_cast<T*>(p.a.out) + row_at.offset(r, p.a.on, p.a.oh) + lane * dims;
       const float inv = l > 0.0f ? 1.0f / l : 0.0f;
       if constexpr (sizeof(T) == 4) {
         if (dims == 4)

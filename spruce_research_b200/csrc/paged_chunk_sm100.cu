@@ -115,6 +115,11 @@ __device__ __forceinline__ bool next_piece(const PagedParams& p, ChunkRole* r) {
   return more;
 }
 
+template <typename T> struct ChunkScale {
+  static constexpr float lag = std::is_same<T, __half>::value ? 2.0f : 8.0f;
+  static constexpr float log2 = PScale<T>::log2 > 0.0f ? PScale<T>::log2 - lag : 0.0f;
+};
+
 template <typename T, int D>
 __global__ void __launch_bounds__(kChunkThreads, 1)
     paged_chunk_sm100_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv,
@@ -404,8 +409,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       // Columns of the piece's first key tile that this row sees; each tile further leaves 128 fewer.
       int lim = min(x.q.first + row_at.token(row) + 1, x.keys) - x.t0 * kChunkKeys;
       // Growth of the maximum that O is not rescaled for, and the factor of P: together P's range.
-      constexpr float kLag = std::is_same<T, __half>::value ? 2.0f : 8.0f;
-      constexpr float kScale = PScale<T>::log2 > 0.0f ? PScale<T>::log2 - kLag : 0.0f;
+      constexpr float kLag = ChunkScale<T>::lag, kScale = ChunkScale<T>::log2;
       float m_used = -INFINITY;  // reference max (log2 units) the exponentials use
       float l = 0.0f;
       // One key tile.  Masked tiles are a unit's last ones; they have a body of their own because a branch within the
@@ -516,6 +520,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         if (whole) {
           dst = reinterpret_cast<uint8_t*>(static_cast<T*>(p.a.out) +
                                            PagedRows(p, x.q.q0, r0, x.g).offset(row, p.a.on, p.a.oh));
+          if (p.a.lse != nullptr)
+            p.a.lse[PagedRows(p, x.q.q0, r0, x.g).offset(row, p.a.ln, p.a.lh)] = paged_lse(p, m_used, l);
         } else {
           const int64_t at = (int64_t)(2 * blockIdx.x + x.slot) * kChunkRows + t * 128 + row;
           p.part_ml[at] = make_float2(m_used, l);
@@ -622,7 +628,7 @@ static cudaError_t launch_chunk(const PagedArgs& a, int dtype, int G, cudaStream
   static std::atomic<uint64_t> done{0};
   cudaError_t e = allow_smem(reinterpret_cast<const void*>(kern), L::BYTES, done);
   if (e != cudaSuccess) return e;
-  const PagedParams p = paged_params(a, kChunkRows, G, kChunkUnitCost);
+  const PagedParams p = paged_params(a, kChunkRows, G, kChunkUnitCost, ChunkScale<T>::log2);
   // An early start saves short calls two microseconds (512-token prompt 26.7 -> 23.8 us, 8 x 64 tokens over 1000 41.2 -> 38.3)
   // and costs calls whose CTAs take several units some (4K prompt 168 -> 180 us, 16K prompt 1.62 -> 1.65 ms).
   if ((int64_t)a.S * p.row_tiles * a.Hkv <= G) {

@@ -30,6 +30,7 @@ struct PagedParams {
   float* part_o;          // [2 G][R][D]
   float scale_log2;
   float inv_rep;
+  float sum_log2;         // log2 of the factor that the kernel's sums carry
 };
 
 struct PagedSeq {
@@ -260,6 +261,11 @@ __device__ __forceinline__ int paged_page(const PagedParams& p, const int32_t* t
 template <typename T> struct PScale { static constexpr float log2 = 0.0f; };
 template <> struct PScale<__half> { static constexpr float log2 = 15.0f; };
 
+// Natural log of a row's softmax sum from its maximum (log2 units) and sum; -inf where nothing is above -inf.
+__device__ __forceinline__ float paged_lse(const PagedParams& p, float m, float l) {
+  return m == -INFINITY && !(l != l) ? -INFINITY : (m + (log2f(l) - p.sum_log2)) * 0.6931471805599453f;
+}
+
 // Opts a kernel into `bytes` of dynamic shared memory, once a device (`done` is the kernel's own mask of devices).
 inline cudaError_t allow_smem(const void* kern, int bytes, std::atomic<uint64_t>& done) {
   int dev = 0;
@@ -272,6 +278,9 @@ inline cudaError_t allow_smem(const void* kern, int bytes, std::atomic<uint64_t>
   if (e == cudaSuccess) done.fetch_or(uint64_t(1) << dev);
   return e;
 }
+
+// SMs of the current GPU (at most kMaxSms), asked for once (paged_attn.cu).
+int sm_count();
 
 // Launches a kernel that may start while the one before it in the stream ends; it waits (griddepcontrol) before it
 // touches memory.
@@ -309,8 +318,9 @@ template <typename T>
 cudaError_t launch_paged_join(const PagedParams& p, int R, int G, int TK, cudaStream_t stream);
 
 // Parameters of a launch with R-row tiles on at most G CTAs, its workspace carved up.
-inline PagedParams paged_params(const PagedArgs& a, int R, int G, int unit_cost) {
+inline PagedParams paged_params(const PagedArgs& a, int R, int G, int unit_cost, float sum_log2 = 0.0f) {
   PagedParams p;
+  p.sum_log2 = sum_log2;
   p.a = a;
   p.rep = a.Hq / a.Hkv;
   p.inv_rep = 1.0f / static_cast<float>(p.rep);

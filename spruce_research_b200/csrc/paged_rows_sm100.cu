@@ -291,9 +291,11 @@ __global__ void __launch_bounds__(kRowsThreads, 2)
 #pragma unroll
       for (int w = 0; w < KS; ++w) sum += ml[w * R + r].y * fast_exp2(ml[w * R + r].x - ref);
       f[i] = fast_exp2(m[i] - ref);
-      if (whole)
+      if (whole) {
         f[i] *= sum > 0.0f ? 1.0f / sum : 0.0f;
-      else if (ks == 0 && qc == 0 && r < rows)
+        if (p.a.lse != nullptr && ks == 0 && qc == 0 && r < rows)
+          p.a.lse[row_at.offset(r, p.a.ln, p.a.lh)] = paged_lse(p, top, sum);
+      } else if (ks == 0 && qc == 0 && r < rows)
         p.part_ml[part + r] = make_float2(top, sum);
     }
     const int wr = threadIdx.x >> 3, wc = (threadIdx.x & 7) * 4;  // written by this thread: row of each 16, 4 columns
@@ -343,7 +345,7 @@ static cudaError_t launch_rows(const PagedArgs& a, int dtype, int G, cudaStream_
   static std::atomic<uint64_t> done{0};
   cudaError_t e = allow_smem(reinterpret_cast<const void*>(kern), L::BYTES, done);
   if (e != cudaSuccess) return e;
-  const PagedParams p = paged_params(a, 16 * MT, G, 1);
+  const PagedParams p = paged_params(a, 16 * MT, G, 1, PScale<T>::log2);
   e = launch_early(kern, G, kRowsThreads, L::BYTES, stream, mk, mv, p, box);
   return e != cudaSuccess ? e : launch_paged_join<T>(p, 16 * MT, G, kRowsKeys, stream);
 }

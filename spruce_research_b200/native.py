@@ -646,18 +646,21 @@ def _paged_workspace_bytes(Hq: int, Hkv: int, D: int, max_q_len: int, dtype: int
 def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
                     cu_q: torch.Tensor, kv_lens: torch.Tensor, *, max_q_len: int, max_kv_len: int,
                     scale: float | None = None, out: torch.Tensor | None = None,
-                    workspace: torch.Tensor | None = None, status: torch.Tensor | None = None) -> torch.Tensor:
+                    workspace: torch.Tensor | None = None, status: torch.Tensor | None = None,
+                    lse: torch.Tensor | None = None) -> torch.Tensor:
     """Causal GQA attention of packed new tokens q [N, Hq, D] over a paged cache (see :func:`paged_append`).
 
     The last new token of sequence s sees ``kv_lens[s]`` keys, the one before it one fewer, and so on; queries that
     see none give zeros.  ``max_q_len`` and ``max_kv_len`` bound the sequences' new tokens and lengths (the lengths
     themselves stay on the device); longer ones are cut to them, their queries past ``max_q_len`` are not written, and only
     ``status`` says so.  Returns [N, Hq, D]; rows before ``cu_q[0]`` and past ``cu_q[-1]`` are not written.
+    ``lse`` float32 [N, Hq] receives each row's log of the softmax sum (natural; -inf where it sees nothing), which
+    :func:`paged_key_mass` takes.
     """
     device = q.get_device()
     if not (device == k_cache.get_device() == v_cache.get_device() == block_table.get_device() == cu_q.get_device()
-            == kv_lens.get_device() and _on_one_device(device, out, workspace, status)):
-        _refuse_devices(q, k_cache, v_cache, block_table, cu_q, kv_lens, out, workspace, status)
+            == kv_lens.get_device() and _on_one_device(device, out, workspace, status, lse)):
+        _refuse_devices(q, k_cache, v_cache, block_table, cu_q, kv_lens, out, workspace, status, lse)
     dtype, shape = q.dtype, q.shape
     (pages, Hkv, page_size, D), kc_strides, vc_strides, S, step, width = _paged_shapes(k_cache, v_cache, block_table,
                                                                                        cu_q, kv_lens, dtype)
@@ -686,10 +689,243 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         raise ValueError("workspace must be contiguous")
     else:
         nbytes = workspace.nbytes
-    args = _lib.PAGED_ATTENTION_ARGS.pack(
+    fields = (
         q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), block_table.data_ptr(), cu_q.data_ptr(),
         kv_lens.data_ptr(), workspace.data_ptr(), _status_ptr(status), _lib.stream_on(device), qn, qh, *kc_strides[:3],
         *vc_strides[:3], on, oh, dt, N, S, Hq, Hkv, D, pages, page_size, step, width, max_q_len, max_kv_len, nbytes,
         D ** -0.5 if scale is None else scale)
-    _lib.launch(_lib.load().spruce_paged_attention, args, device)
+    if lse is None:
+        _lib.launch(_lib.load().spruce_paged_attention, _lib.PAGED_ATTENTION_ARGS.pack(*fields), device)
+    else:
+        _check_lse(lse, N, Hq)
+        _lib.launch(_lib.load().spruce_paged_attention_lse,
+                    _lib.PAGED_ATTENTION_LSE_ARGS.pack(*fields, lse.data_ptr(), *lse.stride()), device)
     return out
+
+
+def _check_lse(lse: torch.Tensor, N: int, Hq: int) -> None:
+    if tuple(lse.shape) != (N, Hq) or lse.dtype != torch.float32:
+        raise ValueError(f"lse must be float32 [{N}, {Hq}], got {lse.dtype} {tuple(lse.shape)}")
+
+
+def _check_mass(mass: torch.Tensor, shape, name: str) -> None:
+    if tuple(mass.shape) != tuple(shape[:3]) or mass.dtype != torch.float32:
+        raise ValueError(f"{name} must be float32 {tuple(shape[:3])}, got {mass.dtype} {tuple(mass.shape)}")
+
+
+def paged_key_mass(q: torch.Tensor, k_cache: torch.Tensor, mass: torch.Tensor, block_table: torch.Tensor,
+                   cu_q: torch.Tensor, kv_lens: torch.Tensor, lse: torch.Tensor, *, max_q_len: int, max_kv_len: int,
+                   decay: float = 1.0, scale: float | None = None, out: torch.Tensor | None = None,
+                   status: torch.Tensor | None = None) -> torch.Tensor:
+    """Add the softmax weight that cached keys receive from the new tokens q [N, Hq, D] to ``mass`` [pages, Hkv, page_size].
+
+    ``mass'[j] = decay * mass[j] + sum over queries i that see j and heads h of j's group of exp(scale q_ih.k_j - lse_ih)``
+    for each slot of a sequence with new tokens; the new tokens' own slots start from 0.  With ``decay`` 0 nothing old
+    is read.  The batch is described as for :func:`paged_attention`, whose ``lse`` [N, Hq] this takes.  ``out`` (``mass`` itself
+    by default) receives the sums; slots of no such sequence are left as they are.
+    """
+    out = mass if out is None else out
+    device = q.get_device()
+    if not (device == k_cache.get_device() == mass.get_device() == block_table.get_device() == cu_q.get_device()
+            == kv_lens.get_device() == lse.get_device() == out.get_device() and _on_one_device(device, status)):
+        _refuse_devices(q, k_cache, mass, block_table, cu_q, kv_lens, lse, out, status)
+    dtype, shape = q.dtype, q.shape
+    (pages, Hkv, page_size, D), kc_strides, _, S, step, width = _paged_shapes(k_cache, k_cache, block_table, cu_q,
+                                                                              kv_lens, dtype)
+    if len(shape) != 3 or shape[2] != D:
+        raise ValueError(f"q must be [N, Hq, {D}], got {tuple(shape)}")
+    N, Hq, _ = shape
+    _check_lse(lse, N, Hq)
+    _check_mass(mass, k_cache.shape, "mass")
+    _check_mass(out, k_cache.shape, "out")
+    dt, size = _dt(q), q.element_size()
+    qn, qh, qd = q.stride()
+    if qd != 1 or (qn | qh) % (16 // size) or q.data_ptr() % 16:
+        q = q.clone(memory_format=torch.contiguous_format)
+        qn, qh, _ = q.stride()
+    args = _lib.PAGED_KEY_MASS_ARGS.pack(
+        q.data_ptr(), k_cache.data_ptr(), lse.data_ptr(), mass.data_ptr(), out.data_ptr(), block_table.data_ptr(),
+        cu_q.data_ptr(), kv_lens.data_ptr(), _status_ptr(status), _lib.stream_on(device), qn, qh, *kc_strides[:3],
+        *lse.stride(), *mass.stride(), *out.stride(), dt, N, S, Hq, Hkv, D, pages, page_size, step, width, max_q_len,
+        max_kv_len, D ** -0.5 if scale is None else scale, decay)
+    _lib.launch(_lib.load().spruce_paged_key_mass, args, device)
+    return out
+
+
+def paged_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, mass: torch.Tensor, block_table: torch.Tensor,
+                kv_lens: torch.Tensor, keep: int, *, max_kv_len: int, sinks: int = 0, recent: int = 0,
+                into: tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor] | None = None,
+                status: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Cut sequences of a paged cache to ``keep`` tokens, each KV head to the ones of the largest ``mass``.
+
+    A sequence longer than ``keep`` keeps its first ``sinks`` slots, its last ``recent`` ones and the heaviest of those
+    between (ties: the lowest slot).  K, V and mass rows that stay move, in their order, to the first slots: in place, or
+    of the pages of ``into = (k, v, mass, block_table)``, which no sequence of the call reads.  In place, no
+    page may belong to two sequences.  ``kv_lens`` int32 [S] are the lengths, at most ``max_kv_len`` (a longer one is left as
+    it is, and only ``status`` says so).  Returns ``kept`` int32 [S, Hkv, min(keep, max_kv_len)], the old slots (-1 past
+    them), and the new lengths int32 [S].
+    """
+    k_out, v_out, mass_out, out_table = (k_cache, v_cache, mass, block_table) if into is None else into
+    device = k_cache.get_device()
+    if not (device == v_cache.get_device() == mass.get_device() == block_table.get_device() == kv_lens.get_device()
+            == k_out.get_device() == v_out.get_device() == mass_out.get_device() == out_table.get_device()
+            and _on_one_device(device, status)):
+        _refuse_devices(k_cache, v_cache, mass, block_table, kv_lens, k_out, v_out, mass_out, out_table, status)
+    shape, to_shape = k_cache.shape, k_out.shape
+    if len(shape) != 4 or v_cache.shape != shape or len(to_shape) != 4 or v_out.shape != to_shape:
+        raise ValueError("the caches must be [pages, Hkv, page_size, D] of one shape")
+    pages, Hkv, page_size, D = shape
+    if to_shape[1:] != shape[1:]:
+        raise ValueError(f"the caches of `into` must be [pages, {Hkv}, {page_size}, {D}], got {tuple(to_shape)}")
+    if not k_cache.dtype == v_cache.dtype == k_out.dtype == v_out.dtype:
+        raise ValueError("the caches must share a dtype")
+    if any(x.stride(3) != 1 for x in (k_cache, v_cache, k_out, v_out)):
+        raise ValueError("the caches need a unit last stride")
+    _check_mass(mass, shape, "mass")
+    _check_mass(mass_out, to_shape, "the mass of `into`")
+    S = kv_lens.numel()
+    for table in (block_table, out_table):
+        if table.dtype != torch.int32 or table.dim() != 2 or table.shape[0] != S:
+            raise ValueError(f"a block table must be int32 [{S}, pages], got {table.dtype} {tuple(table.shape)}")
+        if table.shape[1] > 1 and table.stride(1) != 1:
+            raise ValueError("a block table needs a unit last stride")
+    if kv_lens.dtype != torch.int32 or kv_lens.dim() != 1 or not kv_lens.is_contiguous():
+        raise ValueError("kv_lens must be contiguous int32 [S]")
+    keep, max_kv_len = int(keep), int(max_kv_len)
+    if keep < 0 or max_kv_len < 0:
+        raise ValueError("keep and max_kv_len must not be negative")
+    kept = kv_lens.new_empty((S, Hkv, min(keep, max_kv_len)))
+    lens = torch.empty_like(kv_lens)
+    args = _lib.PAGED_EVICT_ARGS.pack(
+        k_cache.data_ptr(), v_cache.data_ptr(), mass.data_ptr(), k_out.data_ptr(), v_out.data_ptr(),
+        mass_out.data_ptr(), block_table.data_ptr(), out_table.data_ptr(), kv_lens.data_ptr(), kept.data_ptr(),
+        lens.data_ptr(), _status_ptr(status), _lib.stream_on(device), *k_cache.stride()[:3], *v_cache.stride()[:3],
+        *mass.stride(), *k_out.stride()[:3], *v_out.stride()[:3], *mass_out.stride(), _dt(k_cache), S, Hkv, D, pages,
+        page_size, block_table.stride(0), block_table.shape[1], to_shape[0], out_table.stride(0), out_table.shape[1],
+        max_kv_len, kept.shape[2], keep, sinks, recent)
+    _lib.launch(_lib.load().spruce_paged_evict, args, device)
+    return kept, lens
+
+
+def block_mass(q: torch.Tensor, k: torch.Tensor, *, scale: float | None = None, out: torch.Tensor | None = None,
+               workspace: torch.Tensor | None = None, status: torch.Tensor | None = None) -> torch.Tensor:
+    """Softmax weight of whole key blocks of 64 tokens, the teacher of a gate: float32 [B, Hkv, qb, qb].
+
+    ``out[b, g, i, j]`` is the mean over the heads of group g and the tokens of query block i of the weight that causal
+    attention of q [B, Hq, T, D] over k [B, Hkv, T, D] gives to key block j; rows sum to 1.
+    """
+    device = q.get_device()
+    if not (device == k.get_device() and _on_one_device(device, out, workspace, status)):
+        _refuse_devices(q, k, out, workspace, status)
+    if q.dim() != 4 or k.dim() != 4:
+        raise ValueError("q and k must be [B, H, T, D]")
+    B, Hq, T, D = q.shape
+    Hkv = k.shape[1]
+    if q.dtype != k.dtype:
+        raise ValueError("q and k must share a dtype")
+    if k.shape[0] != B or k.shape[2] != T or k.shape[3] != D:
+        raise ValueError(f"k must be [{B}, Hkv, {T}, {D}], got {tuple(k.shape)}")
+    dt, qb = _dt(q), (T + BLOCK - 1) // BLOCK
+    q, k = _tma_ok(q), _tma_ok(k)
+    if out is None:
+        out = torch.empty((B, Hkv, qb, qb), device=q.device, dtype=torch.float32)
+    elif tuple(out.shape) != (B, Hkv, qb, qb) or out.dtype != torch.float32 or not out.is_contiguous():
+        raise ValueError(f"out must be contiguous float32 {(B, Hkv, qb, qb)}")
+    if workspace is None:
+        nbytes = _lib.load().spruce_block_mass_workspace_bytes(B, Hq, Hkv, T, D, dt)
+        if nbytes < 0:
+            raise ValueError(f"bad block mass shape: q {tuple(q.shape)}, k {tuple(k.shape)}")
+        workspace = torch.empty(nbytes // 4, device=q.device, dtype=torch.float32)
+    elif not workspace.is_contiguous():
+        raise ValueError("workspace must be contiguous")
+    else:
+        nbytes = workspace.nbytes
+    args = _lib.BLOCK_MASS_ARGS.pack(
+        q.data_ptr(), k.data_ptr(), out.data_ptr(), workspace.data_ptr(), _status_ptr(status), _lib.stream_on(device),
+        *q.stride(), *k.stride(), dt, B, Hq, Hkv, T, D, nbytes, D ** -0.5 if scale is None else scale)
+    _lib.launch(_lib.load().spruce_block_mass, args, device)
+    return out
+
+
+def _tma_ok(t: torch.Tensor) -> torch.Tensor:
+    """A view whose rows are 16-byte aligned and that steps forwards (a copy only if it is not)."""
+    vn = 16 // t.element_size()
+    if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(
+            n == 1 or (s > 0 and s % vn == 0) for n, s in zip(t.shape[:-1], t.stride()[:-1])):
+        if all(s % vn == 0 and s > 0 for s in t.stride()[:-1]):
+            return t
+        # A dimension of one element never steps: any stride will do.
+        return t.as_strided(t.shape, [s if n > 1 else t.shape[-1] for n, s in zip(t.shape[:-1], t.stride()[:-1])] + [1])
+    return t.clone(memory_format=torch.contiguous_format)
+
+
+def _row_major(t: torch.Tensor, rows: int) -> torch.Tensor:
+    """[..., n] as [rows, n] with a unit last stride."""
+    t = t.reshape(rows, t.shape[-1])
+    return t if t.stride(1) == 1 or t.shape[1] <= 1 else t.contiguous()
+
+
+def _distill(scores, ids, teacher, visible, temperature, status, *, loss=False, stats=None, want_stats=False,
+             weight=None):
+    """One call of spruce_topk_distill on checked arguments: (loss, stats, grad), None where not asked for."""
+    device = scores.get_device()
+    if not (device == ids.get_device() == teacher.get_device()
+            and _on_one_device(device, visible, stats, weight, status)):
+        _refuse_devices(scores, ids, teacher, visible, stats, weight, status)
+    if scores.dim() < 1 or ids.dim() != scores.dim() or ids.shape[:-1] != scores.shape[:-1] or teacher.shape != ids.shape:
+        raise ValueError(f"expected scores [..., n], ids [..., K] and teacher [..., K], got {tuple(scores.shape)}, "
+                         f"{tuple(ids.shape)}, {tuple(teacher.shape)}")
+    if ids.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"ids must be int32 or int64, got {ids.dtype}")
+    lead, n, K = scores.shape[:-1], scores.shape[-1], ids.shape[-1]
+    R = math.prod(lead)
+    if visible is not None:
+        if visible.dtype != torch.int32 or visible.shape != lead:
+            raise ValueError(f"visible must be int32 {tuple(lead)}, got {visible.dtype} {tuple(visible.shape)}")
+        visible = visible.reshape(R).contiguous()
+    if weight is not None:
+        if weight.dtype != torch.float32 or weight.shape != lead:
+            raise ValueError(f"the rows' weights must be float32 {tuple(lead)}, got {weight.dtype} {tuple(weight.shape)}")
+        weight = weight.reshape(R)
+    x, i, t = _row_major(scores, R), _row_major(ids, R), _row_major(teacher, R)
+    out = torch.empty(lead, device=x.device, dtype=torch.float32) if loss else None
+    made = torch.empty((R, 2), device=x.device, dtype=torch.float32) if want_stats else None
+    grad = torch.empty(scores.shape, device=x.device, dtype=x.dtype) if weight is not None else None
+    args = _lib.TOPK_DISTILL_ARGS.pack(
+        x.data_ptr(), i.data_ptr(), t.data_ptr(), _ptr(visible), _ptr(out), _ptr(made), _ptr(stats), _ptr(weight),
+        _ptr(grad), _status_ptr(status), _lib.stream_on(device), x.stride(0), i.stride(0), t.stride(0),
+        weight.stride(0) if weight is not None else 0, n, _dt(x), _dt(t), i.dtype == torch.int64, R, n, K, temperature)
+    _lib.launch(_lib.load().spruce_topk_distill, args, device)
+    return out, made, grad
+
+
+def topk_distill(scores: torch.Tensor, ids: torch.Tensor, teacher: torch.Tensor, *, visible: torch.Tensor | None = None,
+                 temperature: float = 1.0, grad_weight: torch.Tensor | None = None,
+                 status: torch.Tensor | None = None):
+    """Distillation of a teacher's top entries into rows of scores [..., n]: the rows' losses float32 [...].
+
+    With p the softmax of ``teacher`` [..., K] / temperature over the entries whose ``ids`` [..., K] are not negative, and q
+    the softmax of scores / temperature over the first ``visible`` [...] columns (all by default), a row's loss is
+    ``sum_k p_k (ln p_k - ln q[ids_k])``.  A column named twice counts twice; one past the visible ones counts as padding, and
+    only ``status`` says so.  Rows without a visible score or a teacher entry above -inf have loss and gradient 0.
+
+    With ``grad_weight`` float32 [...], returns ``(loss, grad)``, grad [..., n] being the gradient of the sum of
+    ``grad_weight * loss`` by the scores, in the scores' dtype: both in one pass over the scores.  Not recorded by autograd;
+    :func:`spruce_research_b200.selector.loss.topk_distill_loss` is.
+    """
+    loss, _, grad = _distill(scores, ids, teacher, visible, temperature, status, loss=True, weight=grad_weight)
+    return loss if grad_weight is None else (loss, grad)
+
+
+def topk_distill_forward(scores, ids, teacher, *, visible=None, temperature=1.0, status=None):
+    """``(loss, stats)``: as :func:`topk_distill`, with what :func:`topk_distill_backward` needs of the scores' softmax."""
+    loss, stats, _ = _distill(scores, ids, teacher, visible, temperature, status, loss=True, want_stats=True)
+    return loss, stats
+
+
+def topk_distill_backward(scores, ids, teacher, stats, weight, *, visible=None, temperature=1.0, status=None):
+    """Gradient [..., n] of the sum of ``weight * loss`` by the scores; ``stats`` are of the forward call on them."""
+    R = math.prod(scores.shape[:-1])
+    if tuple(stats.shape) != (R, 2) or stats.dtype != torch.float32 or not stats.is_contiguous():
+        raise ValueError(f"stats must be contiguous float32 [{R}, 2]")
+    return _distill(scores, ids, teacher, visible, temperature, status, stats=stats, weight=weight)[2]
