@@ -152,7 +152,7 @@ cudaError_t launch_key_mass(const KeyMassArgs& a, int dtype, cudaStream_t stream
 
 // ------------------------------------------------------------------ block mass
 // One (batch, KV head, query block) at a time: its heads one after another, 64 x 64 scores a step.
-template <typename T, int D>
+template <int D>
 __global__ void __launch_bounds__(kTileThreads) block_mass_tile_kernel(const BlockMassArgs a, int qb) {
   constexpr int P = D + 4;
   extern __shared__ float sm[];
@@ -170,7 +170,7 @@ __global__ void __launch_bounds__(kTileThreads) block_mass_tile_kernel(const Blo
     float* out = a.out + ((int64_t)bg * qb + i) * qb;
     for (int h = 0; h < rep; ++h) {
       __syncthreads();
-      const T* q = static_cast<const T*>(a.q) + b * a.qs[0] + (g * rep + h) * a.qs[1];
+      const float* q = static_cast<const float*>(a.q) + b * a.qs[0] + (g * rep + h) * a.qs[1];
       for (int e = tid; e < 64 * (D / 4); e += kTileThreads) {
         const int r = e / (D / 4), d = e % (D / 4) * 4;
         float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -183,7 +183,7 @@ __global__ void __launch_bounds__(kTileThreads) block_mass_tile_kernel(const Blo
         m[x] = -INFINITY;
         l[x] = 0.0f;
       }
-      const T* k = static_cast<const T*>(a.k) + b * a.ks[0] + g * a.ks[1];
+      const float* k = static_cast<const float*>(a.k) + b * a.ks[0] + g * a.ks[1];
       for (int j = 0; j <= i; ++j) {
         __syncthreads();
         for (int e = tid; e < 64 * (D / 4); e += kTileThreads) {
@@ -243,15 +243,16 @@ __global__ void __launch_bounds__(kTileThreads) block_mass_tile_kernel(const Blo
 constexpr int kBlockTilePerSm = 2;
 
 int64_t block_mass_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t T, int64_t D, int dtype) {
-  (void)Hq, (void)D, (void)dtype;
+  (void)D;
+  if (dtype != SPRUCE_DTYPE_F32) return block_mass_sm100_workspace_bytes(B, Hq, Hkv, T);
   const int64_t qb = (T + 63) / 64;
   return std::min<int64_t>(B * Hkv * qb, kMaxSms * kBlockTilePerSm) * qb * 64 * 4;
 }
 
-template <typename T, int D>
+template <int D>
 static cudaError_t launch_block_tile(const BlockMassArgs& a, cudaStream_t stream) {
   constexpr int smem = sizeof(float) * (128 * (D + 4) + 64);
-  auto kern = block_mass_tile_kernel<T, D>;
+  auto kern = block_mass_tile_kernel<D>;
   static std::atomic<uint64_t> done{0};
   cudaError_t e = allow_smem(reinterpret_cast<const void*>(kern), smem, done);
   if (e != cudaSuccess) return e;
@@ -261,17 +262,9 @@ static cudaError_t launch_block_tile(const BlockMassArgs& a, cudaStream_t stream
   return cudaGetLastError();
 }
 
-template <typename T>
-static cudaError_t launch_block_t(const BlockMassArgs& a, cudaStream_t stream) {
-  return a.D == 128 ? launch_block_tile<T, 128>(a, stream) : launch_block_tile<T, 64>(a, stream);
-}
-
 cudaError_t launch_block_mass(const BlockMassArgs& a, int dtype, cudaStream_t stream) {
-  switch (dtype) {
-    case SPRUCE_DTYPE_F32: return launch_block_t<float>(a, stream);
-    case SPRUCE_DTYPE_BF16: return launch_block_t<__nv_bfloat16>(a, stream);
-    default: return launch_block_t<__half>(a, stream);
-  }
+  if (dtype != SPRUCE_DTYPE_F32) return launch_block_mass_sm100(a, dtype, stream);
+  return a.D == 128 ? launch_block_tile<128>(a, stream) : launch_block_tile<64>(a, stream);
 }
 
 }  // namespace spruce

@@ -33,6 +33,10 @@ inline KeyMassParams key_mass_params(const KeyMassArgs& a, int tile) {
   return p;
 }
 
+// Block mass in 16 bits (block_mass_sm100.cu).
+int64_t block_mass_sm100_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t T);
+cudaError_t launch_block_mass_sm100(const BlockMassArgs& a, int dtype, cudaStream_t stream);
+
 // Page of the 16 keys from `key` on; -1 past the sequence's keys, or where the table names no page of the cache.
 __device__ __forceinline__ int mass_page(const KeyMassParams& p, int s, int key, int kv) {
   if (key >= kv) return -1;
