@@ -5,13 +5,18 @@
 //   S_t = Q_t K^T   M128 N128 K16, D / 16 MMAs.
 // Nothing follows S: for each row and block of 64 keys the softmax warps form b = log2(sum 2^(s - m)) + m over the running
 // maximum m, keep it in the workspace (written and read by the same thread) and add it to the row's total.  When a unit's
-// keys are through, 2^(b - total) is summed over the 64 rows of a query block: 32 blocks a round by a transposing butterfly, 31
+// keys are through, 2^(b - total) is summed over the 64 rows of a query block: 32 a round by a transposing butterfly, 31
 // shuffles for 32 sums of a warp.  Heads are added by a second kernel in their order, so nothing depends on timing.
 //
-// Warps: 0-3 softmax of tile 0 (thread = row = TMEM lane), 4-7 of tile 1, 8 issues the MMAs and owns TMEM, 9 loads Q and
-// K.  Each S_t has two buffers, which fill TMEM: the tensor core runs a tile ahead of the exponentials, which bound the kernel
+// Warps: 0-3 the first 64 keys of tile 0 (thread = row = TMEM lane), 4-7 the others, 8-15 likewise of tile 1, 16 issues the
+// MMAs and owns TMEM, 17 loads Q and K.  Four warps a scheduler hide each other's latencies (two of 128 keys a row: 4.72 ms
+// where these take 4.58).  Each S_t has two buffers, which fill TMEM: the tensor core runs a tile ahead of the exponentials, which bound the kernel
 // (16 a clock and SM, against 32 scores a clock of the MMAs at d = 128).  Part of them runs on the FMA pipe instead, as a
-// polynomial of degree 4 with a relative error of 2.7e-6.
+// polynomial of degree 4 with a relative error of 2.7e-6: an eighth (none, 1/8, 1/4, 3/8: 4.65, 4.58, 4.58, 4.78 ms; the
+// issue slots bound what the exponentials leave).  Exponentials over an old maximum, without a pass for the block's own,
+// measured 1.5% slower: the branch for a row that outgrows it keeps blocks from overlapping.
+//
+// On a B200, 28 query / 4 KV heads of 128 in bf16: 32768 tokens 4.58 ms, 840 TFLOP/s; the exponentials' pipe 78% busy.
 //
 // Units go to the CTAs longest first, back and forth over them.
 //
@@ -24,9 +29,9 @@
 
 namespace spruce {
 
-constexpr int kBmThreads = 320, kBmMma = 8, kBmLoad = 9;
+constexpr int kBmThreads = 576, kBmMma = 16, kBmLoad = 17;
 constexpr int kBmKeys = 128;
-constexpr int kBmMufu = 5;  // of 8 pairs of exponentials; the others by polynomial
+constexpr int kBmMufu = 7;  // of 8 pairs of exponentials; the others by polynomial
 
 template <int D>
 struct BlockLayout {
@@ -36,8 +41,9 @@ struct BlockLayout {
   static constexpr int TILE = NP * PANEL;
   static constexpr int OFF_Q = 0;
   static constexpr int OFF_K = 2 * TILE;
-  static constexpr int OFF_SUM = OFF_K + KST * TILE;     // [8 warps][2][32] floats: sums handed to the other warp of a block
-  static constexpr int OFF_BAR = OFF_SUM + 8 * 2 * 32 * 4;
+  static constexpr int OFF_SUM = OFF_K + KST * TILE;     // [8 pairs of warps][2][32] floats: sums handed to the other warp of a block
+  static constexpr int OFF_ML = OFF_SUM + 8 * 2 * 32 * 4;  // [2][2 tiles][2 halves][128] maxima and sums
+  static constexpr int OFF_BAR = OFF_ML + 2 * 512 * 8;
   // k_full[], k_empty[], q_full, q_empty, s_full[2][2], s_empty[2][2], drain
   static constexpr int NBAR = 2 * KST + 2 + 4 + 4 + 1;
   static constexpr int OFF_MISC = OFF_BAR + NBAR * 8;
@@ -47,11 +53,11 @@ struct BlockLayout {
 
 struct BlockParams {
   BlockMassArgs a;
-  int rep, tiles, qb, kbp;   // token tiles of 128; query blocks; key blocks rounded up to 32
+  int rep, tiles, qb, kbp;   // token tiles of 128; query blocks; key blocks rounded up to 64
   int pairs;                 // pairs of row tiles of a (batch, KV head)
   int units;
   float* blocks;             // [CTA][kbp][256]
-  float* part;               // [B Hkv][tiles * rep][2][kbp]
+  float* part;               // [B Hkv][tiles * rep][2 query blocks][2 halves][kbp / 2]
 };
 
 // 2^x of two values on the FMA pipe: n = round(x) by the 1.5 * 2^23 trick, 2^(x - n) by a polynomial fitted for minimal relative
@@ -116,7 +122,7 @@ __global__ void __launch_bounds__(kBmThreads, 1)
   uint64_t* q_full = k_empty + KST;
   uint64_t* q_empty = q_full + 1;
   uint64_t* s_full = q_empty + 1;      // [tile * 2 + buffer]
-  uint64_t* s_empty = s_full + 4;      // 128 arrivals
+  uint64_t* s_empty = s_full + 4;      // 256 arrivals
   uint64_t* drain = s_empty + 4;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::OFF_MISC);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::OFF_MISC + 4);
@@ -127,7 +133,7 @@ __global__ void __launch_bounds__(kBmThreads, 1)
       for (int s = 0; s < 2 * KST + 2; ++s) mbar_init(&k_full[s], 1);  // and k_empty, q_full, q_empty
       for (int s = 0; s < 4; ++s) {
         mbar_init(&s_full[s], 1);
-        mbar_init(&s_empty[s], 128);
+        mbar_init(&s_empty[s], 256);
       }
       mbar_init(drain, 1);
       fence_barrier_init();
@@ -204,14 +210,18 @@ __global__ void __launch_bounds__(kBmThreads, 1)
       if (!(ok = wait(q_full, r & 1))) break;
       const int n = max(u.keys[0], u.keys[1]);
       for (int j = 0; ok && j < n; ++j) {
-        if (!(ok = wait(&k_full[st], turn))) break;
+        // A check of a barrier waits behind this warp's queued MMAs: all that a step needs is checked before its MMAs.
+        ok = wait(&k_full[st], turn);
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+          if (ok && j < u.keys[t] && issued[t] >= 2)
+            ok = wait(&s_empty[2 * t + (issued[t] & 1)], ((issued[t] >> 1) - 1) & 1);
+        if (!ok) break;
         tc_fence_after();
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
           if (j >= u.keys[t]) continue;
-          const uint32_t buf = issued[t] & 1;
-          if (issued[t] >= 2 && !(ok = wait(&s_empty[2 * t + buf], ((issued[t] >> 1) - 1) & 1))) break;
-          tc_fence_after();
+          const uint32_t buf = issued[t]++ & 1;
 #pragma unroll
           for (int ks = 0; ks < D / 16; ++ks) {
             const uint32_t off = ((ks >> 2) * L::PANEL + (ks & 3) * 32) >> 4;
@@ -221,9 +231,7 @@ __global__ void __launch_bounds__(kBmThreads, 1)
             __syncwarp();
           }
           commit(&s_full[2 * t + buf]);
-          ++issued[t];
         }
-        if (!ok) break;
         commit(&k_empty[st]);
         if (++st == KST) {
           st = 0;
@@ -237,22 +245,23 @@ __global__ void __launch_bounds__(kBmThreads, 1)
     __syncwarp();
   } else {
     // ------------------------------------------------------------ softmax and sums
-    const int t = warp >> 2;
-    const uint32_t tS = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + t * 256;
+    const int t = warp >> 3, half = (warp >> 2) & 1;  // tile, and which 64 of its keys
+    const uint32_t tS = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + t * 256 + half * 64;
     const int row = (warp & 3) * 32 + lane;
-    float* const mine = p.blocks + (int64_t)blockIdx.x * p.kbp * 256 + t * 128 + row;  // [block] at stride 256
-    float* const given = reinterpret_cast<float*>(smem + L::OFF_SUM) + (warp & ~1) * 64;  // [2][32] of this pair of warps
+    float* const mine = p.blocks + ((int64_t)blockIdx.x * p.kbp + half) * 256 + t * 128 + row;  // [key tile] at stride 512
+    float* const given = reinterpret_cast<float*>(smem + L::OFF_SUM) + (warp >> 1) * 64;        // [2][32] of this pair of warps
+    float2* const ml = reinterpret_cast<float2*>(smem + L::OFF_ML) + t * 256 + row;             // [half] at stride 128
     const float sl2 = p.a.scale_log2;
     const uint64_t sl2x2 = f2_pack(sl2, sl2);
     uint32_t sj = 0, rounds = 0;
     bool ok = true;
-    // After a wait that ran out the warps still meet at the rounds' barriers.
+    // After a wait that ran out the warps still meet at the barriers.
     for (int r = 0; block_unit(p, r, u); ++r) {
       const int n = u.keys[t];
       if (n == 0) continue;
       float m = -INFINITY, l = 0.0f;
       // 64 keys: b of the block, the total moved on.  lim: columns that the row sees.
-      auto block = [&](const float (&s)[64], auto masked_c, int lim, int at) {
+      auto block = [&](const float (&s)[64], auto masked_c, int lim, int j) {
         constexpr bool masked = decltype(masked_c)::value;
         float z[64];
 #pragma unroll
@@ -290,40 +299,40 @@ __global__ void __launch_bounds__(kBmThreads, 1)
         const float sum = (a0 + a1) + (a2 + a3);
         l = fmaf(l, fast_exp2(m - ref), sum);
         m = up;
-        mine[(int64_t)at * 256] = ref + __log2f(sum);
+        mine[(int64_t)j * 512] = ref + __log2f(sum);
       };
       for (int j = 0; ok && j < n; ++j, ++sj) {
         const uint32_t buf = sj & 1;
         ok = __all_sync(0xffffffffu, mbar_wait(&s_full[2 * t + buf], (sj >> 1) & 1, status, abort_flag));
         if (!ok) break;
         tc_fence_after();
-        float s0[64], s1[64];
-        auto load = [&](float (&s)[64], int col) {
-          tmem_ld32(tS + buf * 128 + col, *reinterpret_cast<float(*)[32]>(s));
-          tmem_ld32(tS + buf * 128 + col + 32, *reinterpret_cast<float(*)[32]>(s + 32));
-        };
-        load(s0, 0);
-        load(s1, 64);
+        float s[64];
+        tmem_ld32(tS + buf * 128, *reinterpret_cast<float(*)[32]>(s));
+        tmem_ld32(tS + buf * 128 + 32, *reinterpret_cast<float(*)[32]>(s + 32));
         tmem_wait_ld();
         tc_fence_before();
         mbar_arrive(&s_empty[2 * t + buf]);
-        if (j + 1 < n) {
-          block(s0, std::false_type{}, 0, 2 * j);
-          block(s1, std::false_type{}, 0, 2 * j + 1);
-        } else {  // the diagonal
-          block(s0, std::true_type{}, row + 1, 2 * j);
-          block(s1, std::true_type{}, row - 63, 2 * j + 1);
-        }
+        if (j + 1 < n)
+          block(s, std::false_type{}, 0, j);
+        else  // the diagonal
+          block(s, std::true_type{}, row + 1 - half * 64, j);
       }
+      // The row's total over both halves.
+      float2* const x = ml + (r & 1) * 512;
+      x[half * 128] = make_float2(m, l);
+      named_barrier_sync(9 + t, 256);
+      const float2 other = x[128 - half * 128];
+      const bool in = u.tile[t] / p.rep * 128 + row < p.a.T;
+      const float top = fmaxf(m, other.x), ref = top == -INFINITY ? 0.0f : top;
+      const float all = l * fast_exp2(m - ref) + other.y * fast_exp2(other.x - ref);
+      const float total = top == -INFINITY && all == all ? INFINITY : ref + __log2f(all);
       // Weights of this warp's 32 rows, summed, and those of the other warp of the query block.
-      const int tt = u.tile[t] / p.rep;
-      const bool in = tt * 128 + row < p.a.T;
-      const float total = in ? (m == -INFINITY && l == l ? INFINITY : m + __log2f(l)) : INFINITY;
-      float* const out = p.part + (((int64_t)u.bg * p.tiles * p.rep + u.tile[t]) * 2 + ((warp >> 1) & 1)) * p.kbp;
-      for (int j0 = 0; j0 < 2 * n; j0 += 32, ++rounds) {
+      float* const out = p.part + (((int64_t)u.bg * p.tiles * p.rep + u.tile[t]) * 2 + ((warp >> 1) & 1)) * p.kbp +
+                         half * (p.kbp / 2);
+      for (int j0 = 0; j0 < n; j0 += 32, ++rounds) {
         float v[32];
 #pragma unroll
-        for (int k = 0; k < 32; ++k) v[k] = in && j0 + k < 2 * n ? mine[(int64_t)(j0 + k) * 256] : -INFINITY;
+        for (int k = 0; k < 32; ++k) v[k] = in && j0 + k < n ? mine[(int64_t)(j0 + k) * 512] : -INFINITY;
 #pragma unroll
         for (int k = 0; k < 32; ++k) v[k] = fast_exp2(v[k] - total);
         // Halves of the values change sides with a lane half away, until lane k holds the sum of value k.
@@ -360,7 +369,7 @@ __global__ void __launch_bounds__(256) block_mass_join_kernel(const BlockParams 
   for (int j = threadIdx.x; j < p.qb; j += 256) {
     float sum = 0.0f;
     if (j <= i)
-      for (int h = 0; h < p.rep; ++h) sum += part[(int64_t)h * 2 * p.kbp + j];
+      for (int h = 0; h < p.rep; ++h) sum += part[(int64_t)h * 2 * p.kbp + (j & 1) * (p.kbp / 2) + j / 2];
     out[j] = sum * share;
   }
 }
@@ -370,7 +379,7 @@ static BlockParams block_params(int64_t B, int64_t Hq, int64_t Hkv, int64_t T) {
   p.rep = static_cast<int>(Hq / Hkv);
   p.tiles = static_cast<int>((T + 127) / 128);
   p.qb = static_cast<int>((T + 63) / 64);
-  p.kbp = (p.qb + 31) / 32 * 32;
+  p.kbp = (p.qb + 63) / 64 * 64;
   p.pairs = (p.tiles * p.rep + 1) / 2;
   p.units = static_cast<int>(B * Hkv * p.pairs);
   return p;
