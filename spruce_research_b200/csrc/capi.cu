@@ -979,6 +979,8 @@ int spruce_paged_key_mass(const spruce_paged_key_mass_args* args) {
   const int64_t sizes[3] = {x.num_pages, x.Hkv, x.page_size};
   for (int i = 0; i < 3; ++i)  // what a tensor map can step by
     if (sizes[i] > 1 && x.kc_strides[i] < 1) return fail(SPRUCE_ERR_UNSUPPORTED, "the cache needs positive strides");
+  if ((x.N > 1 && x.q_strides[0] < 1) || (x.Hq > 1 && x.q_strides[1] < 1))
+    return fail(SPRUCE_ERR_UNSUPPORTED, "q needs positive strides");
   spruce::KeyMassArgs m{};
   spruce::PagedArgs& a = m.a;
   a.q = x.q;

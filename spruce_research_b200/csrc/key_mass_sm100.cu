@@ -1,0 +1,422 @@
+// Softmax weight of cached keys under many query rows, on the tcgen05 tensor cores (bf16 / fp16).
+//
+// The formula is mass.cu's.  Scores are formed as S^T, keys by rows: M = 128 keys are the lanes of TMEM, so the sum over
+// the rows runs along a thread's own columns and nothing crosses lanes:
+//   S^T_t = K_t Q^T   M128 N128 K16, D / 16 MMAs     sum_j += sum_r 2^(S^T_jr c - lse_r).
+// An item is 256 keys (two tiles) of a (sequence, KV head); the query rows that see them stream by in tiles of as many whole
+// tokens as fit 128 rows, each a TMA box of (token, head of the group) rows.  Items go to the CTAs round robin; where a
+// cluster of CTAs can be had for each, it shares the item's rows and its first CTA adds the sums up in their order.
+//
+// Warps: 0-3 the first 64 rows of tile 0 (thread = key = TMEM lane), 4-7 the others, 8-15 likewise of tile 1, 16 issues the
+// MMAs and owns TMEM, 17 loads K (an item ahead) and Q, 18 brings the rows' lse and limits.  Each S^T_t has two buffers.
+//
+// Every wait is bounded (common.cuh).
+#include <algorithm>
+#include <type_traits>
+
+#include "attn_common.cuh"
+#include "mass_common.cuh"
+
+namespace spruce {
+
+constexpr int kKmThreads = 608, kKmMma = 16, kKmLoad = 17, kKmLse = 18;
+constexpr int kKmKeys = 256;
+
+template <int D>
+struct KeyMassLayout {
+  static constexpr int QST = D == 128 ? 2 : 4, LST = 4;
+  static constexpr int NP = D / 64;
+  static constexpr int PANEL = 128 * 128;
+  static constexpr int TILE = NP * PANEL;
+  static constexpr int OFF_K = 0;                       // [2 items][2 tiles]
+  static constexpr int OFF_Q = OFF_K + 4 * TILE;
+  static constexpr int OFF_ROW = OFF_Q + QST * TILE;    // [LST]: 128 lse, 128 limits
+  static constexpr int OFF_SUM = OFF_ROW + LST * 1024;  // [2][256] sums handed over
+  static constexpr int OFF_PART = OFF_SUM + 2 * 1024;   // [8 CTAs][256] sums of a cluster
+  static constexpr int OFF_BAR = OFF_PART + 8 * 1024;
+  // k_full[2], k_empty[2], q_full[], q_empty[], l_full[], l_empty[], s_full[4], s_empty[4], drain
+  static constexpr int NBAR = 4 + 2 * QST + 2 * LST + 8 + 1;
+  static constexpr int OFF_MISC = OFF_BAR + NBAR * 8;
+  static constexpr int BYTES = 1024 + OFF_MISC + 16;
+  static_assert(BYTES <= 227 * 1024, "shared memory of a CTA");
+};
+
+// An item of a CTA: its keys, and its share of the rows that see them.
+struct KeyMassItem {
+  PagedSeq q;
+  int s, g, key0;
+  int tok0, steps;  // first token of this CTA's rows, and its row tiles
+};
+
+// The item at `at` of all; false where there is nothing to write.
+__device__ __forceinline__ bool key_mass_item(const KeyMassParams& p, int64_t at, int ntok, int rank, int parts, KeyMassItem& x) {
+  const int per = p.key_tiles * p.v.a.Hkv;
+  x.s = static_cast<int>(at / per);
+  const int rest = static_cast<int>(at % per);
+  x.g = rest % p.v.a.Hkv;
+  x.key0 = rest / p.v.a.Hkv * kKmKeys;
+  x.q = paged_seq(p.v, x.s);
+  if (x.q.qlen == 0 || x.key0 >= x.q.kv) return false;
+  // Tokens before the item's first key do not see it.
+  const int lo = min(max(x.key0 - x.q.first, 0), x.q.qlen);
+  const int tiles = (x.q.qlen - lo + ntok - 1) / ntok, each = (tiles + parts - 1) / parts;
+  x.tok0 = lo + rank * each * ntok;
+  x.steps = max(0, min(each, tiles - rank * each));
+  return true;
+}
+
+// All threads of the cluster's CTAs.
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kKmThreads, 1)
+    key_mass_sm100_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ CUtensorMap tmk,
+                          const __grid_constant__ KeyMassParams p, int box, int ntok, int parts, int64_t items) {
+  using L = KeyMassLayout<D>;
+  constexpr int QST = L::QST, LST = L::LST;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  uint32_t* const status = p.v.a.status;
+  uint64_t* k_full = reinterpret_cast<uint64_t*>(smem + L::OFF_BAR);
+  uint64_t* k_empty = k_full + 2;
+  uint64_t* q_full = k_empty + 2;
+  uint64_t* q_empty = q_full + QST;
+  uint64_t* l_full = q_empty + QST;    // 32 arrivals
+  uint64_t* l_empty = l_full + LST;    // 16: a lane of each softmax warp
+  uint64_t* s_full = l_empty + LST;    // [tile * 2 + buffer]
+  uint64_t* s_empty = s_full + 4;      // 256 arrivals
+  uint64_t* drain = s_empty + 4;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::OFF_MISC);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::OFF_MISC + 4);
+  const int rank = blockIdx.x % parts;
+  const int64_t first = blockIdx.x / parts, stride = gridDim.x / parts;
+  const int rows = ntok * p.v.rep;     // of a row tile that a box fills
+
+  if (warp == kKmLoad) {
+    if (lane == 0) {
+      *abort_flag = 0;
+      for (int i = 0; i < 4 + 2 * QST; ++i) mbar_init(&k_full[i], 1);  // and k_empty, q_full, q_empty
+      for (int i = 0; i < LST; ++i) {
+        mbar_init(&l_full[i], 32);
+        mbar_init(&l_empty[i], 16);
+      }
+      for (int i = 0; i < 4; ++i) {
+        mbar_init(&s_full[i], 1);
+        mbar_init(&s_empty[i], 256);
+      }
+      mbar_init(drain, 1);
+      fence_barrier_init();
+      prefetch_tmap(&tmq);
+      prefetch_tmap(&tmk);
+    }
+    __syncwarp();
+  } else if (warp == kKmMma) {
+    tmem_alloc(tmem_slot, 512u);
+    tmem_relinquish();
+  }
+  // Rows of a stage that no box fills stay zero: what they multiply into is not summed, but must be a number.
+  for (int e = threadIdx.x; e < QST * L::NP * (128 - rows) * 8; e += kKmThreads) {
+    const int c = e % 8, r = rows + e / 8 % (128 - rows), panel = e / 8 / (128 - rows);
+    *reinterpret_cast<uint4*>(smem + L::OFF_Q + panel * L::PANEL + r * 128 + c * 16) = make_uint4(0, 0, 0, 0);
+  }
+  fence_proxy_async_smem();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  if (parts > 1) cluster_sync();       // the others' shared memory is there
+  KeyMassItem x;
+  float* to = nullptr;                 // where a sum that the cluster shares goes
+  float old_part = 0.0f;
+
+  if (warp == kKmLoad) {
+    // ------------------------------------------------------------ K and Q
+    const bool leader = elect_one();
+    const int boxes = kKmKeys / box;  // at most 16
+    int kb = 0, kn = 0, st = 0, qn = 0;
+    bool ok = true;
+    for (int64_t at = first; ok && at < items; at += stride) {
+      if (!key_mass_item(p, at, ntok, rank, parts, x) || x.steps == 0) continue;
+      const int32_t* table = p.v.a.block_table + x.s * p.v.a.table_stride;
+      const int key = x.key0 + lane * box;
+      int page = static_cast<int>(p.v.a.num_pages);  // reads zeros
+      if (lane < boxes && key < x.q.kv) {
+        page = paged_page(p.v, table, key / p.v.a.page_size);
+        if (page < 0) page = static_cast<int>(p.v.a.num_pages);
+      }
+      if (kn >= 2 && !(ok = __all_sync(0xffffffffu, mbar_wait(&k_empty[kb], ((kn >> 1) - 1) & 1, status, abort_flag)))) break;
+      if (leader) mbar_arrive_expect_tx(&k_full[kb], 2 * L::TILE);
+      __syncwarp();
+      for (int b = 0; b < boxes; ++b) {
+        const int pb = __shfl_sync(0xffffffffu, page, b);
+        const int r = b * box;  // of the item's keys
+        if (leader)
+#pragma unroll
+          for (int pp = 0; pp < L::NP; ++pp)
+            tma_load_4d(smem + L::OFF_K + (2 * kb + (r >> 7)) * L::TILE + pp * L::PANEL + (r & 127) * 128, &tmk, &k_full[kb],
+                        pp * 64, (x.key0 + r) % p.v.a.page_size, x.g, pb);
+        __syncwarp();
+      }
+      kb ^= 1;
+      ++kn;
+      for (int i = 0; i < x.steps; ++i) {
+        if (qn >= QST && !(ok = __all_sync(0xffffffffu, mbar_wait(&q_empty[st], ((qn / QST) - 1) & 1, status, abort_flag)))) break;
+        if (leader) {
+          mbar_arrive_expect_tx(&q_full[st], L::NP * rows * 128);
+#pragma unroll
+          for (int pp = 0; pp < L::NP; ++pp)
+            tma_load_4d(smem + L::OFF_Q + st * L::TILE + pp * L::PANEL, &tmq, &q_full[st], pp * 64, x.g * p.v.rep,
+                        x.q.q0 + x.tok0 + i * ntok, 0);
+        }
+        __syncwarp();
+        ++qn;
+        if (++st == QST) st = 0;
+      }
+    }
+    // No copy may be in flight when the CTA exits.
+    for (int i = max(0, kn - 2); i < kn; ++i) mbar_wait(&k_full[i & 1], (i >> 1) & 1, status, nullptr);
+    for (int i = max(0, qn - QST); i < qn; ++i) mbar_wait(&q_full[i % QST], (i / QST) & 1, status, nullptr);
+    __syncwarp();
+  } else if (warp == kKmLse) {
+    // ------------------------------------------------------------ lse and limits of the rows
+    int ln = 0;
+    bool ok = true;
+    for (int64_t at = first; ok && at < items; at += stride) {
+      if (!key_mass_item(p, at, ntok, rank, parts, x)) continue;
+      for (int i = 0; i < x.steps; ++i, ++ln) {
+        const int st = ln % LST, tok = x.tok0 + i * ntok;
+        float v[4];
+        int lim[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int r = lane + 32 * k;
+          const int t = static_cast<int>((static_cast<float>(r) + 0.5f) * p.v.inv_rep), h = r - t * p.v.rep;
+          v[k] = INFINITY;
+          lim[k] = -1;
+          if (r < rows && tok + t < x.q.qlen) {
+            v[k] = mass_row_lse(p.lse[(int64_t)(x.q.q0 + tok + t) * p.ln + (int64_t)(x.g * p.v.rep + h) * p.lh]);
+            lim[k] = x.q.first + tok + t - x.key0;
+          }
+        }
+        if (ln >= LST && !(ok = __all_sync(0xffffffffu, mbar_wait(&l_empty[st], ((ln / LST) - 1) & 1, status, abort_flag)))) break;
+        float* dst = reinterpret_cast<float*>(smem + L::OFF_ROW + st * 1024);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          dst[lane + 32 * k] = v[k];
+          reinterpret_cast<int*>(dst)[128 + lane + 32 * k] = lim[k];
+        }
+        mbar_arrive(&l_full[st]);
+      }
+    }
+  } else if (warp == kKmMma) {
+    // ------------------------------------------------------------ MMA issuer
+    const bool leader = elect_one();
+    constexpr uint32_t idesc = idesc_f16(UmmaFormat<T>::value, 0, 0, 128, 128);
+    const uint64_t dq0 = smem_desc(smem_u32(smem + L::OFF_Q), 16, 1024);
+    const uint64_t dk0 = smem_desc(smem_u32(smem + L::OFF_K), 16, 1024);
+    auto commit = [&](uint64_t* bar) {
+      if (leader) umma_commit(bar);
+      __syncwarp();
+    };
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+      return __all_sync(0xffffffffu, mbar_wait(bar, parity, status, abort_flag));
+    };
+    int kn = 0, qn = 0;
+    bool ok = true;
+    for (int64_t at = first; ok && at < items; at += stride) {
+      if (!key_mass_item(p, at, ntok, rank, parts, x) || x.steps == 0) continue;
+      if (!(ok = wait(&k_full[kn & 1], (kn >> 1) & 1))) break;
+      for (int i = 0; i < x.steps; ++i, ++qn) {
+        const int st = qn % QST;
+        const uint32_t buf = qn & 1;
+        // A check of a barrier waits behind this warp's queued MMAs: all that a step needs is checked before its MMAs.
+        ok = wait(&q_full[st], (qn / QST) & 1);
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+          if (ok && qn >= 2) ok = wait(&s_empty[2 * t + buf], ((qn >> 1) - 1) & 1);
+        if (!ok) break;
+        tc_fence_after();
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+#pragma unroll
+          for (int ks = 0; ks < D / 16; ++ks) {
+            const uint32_t off = ((ks >> 2) * L::PANEL + (ks & 3) * 32) >> 4;
+            if (leader)
+              umma_f16_ss(tmem + (2 * t + buf) * 128, dk0 + (((2 * (kn & 1) + t) * L::TILE) >> 4) + off,
+                          dq0 + ((st * L::TILE) >> 4) + off, idesc, ks > 0 ? 1u : 0u);
+            __syncwarp();
+          }
+          commit(&s_full[2 * t + buf]);
+        }
+        commit(&q_empty[st]);
+      }
+      if (ok) commit(&k_empty[kn & 1]);
+      ++kn;
+    }
+    commit(drain);  // no MMA may be in flight when TMEM is released
+    mbar_wait(drain, 0, status, nullptr);
+    __syncwarp();
+  } else {
+    // ------------------------------------------------------------ weights and sums
+    const int t = warp >> 3, half = (warp >> 2) & 1;  // tile, and which 64 of the rows
+    const uint32_t tS = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + t * 256 + half * 64;
+    const int key = t * 128 + (warp & 3) * 32 + lane;  // of the item
+    float* const given = reinterpret_cast<float*>(smem + L::OFF_SUM);
+    const float sl2 = p.v.scale_log2;
+    const uint64_t sl2x2 = f2_pack(sl2, sl2);
+    int qn = 0, done = 0;
+    bool ok = true;
+    // After a wait that ran out the warps still meet at the barriers.
+    for (int64_t at = first; at < items; at += stride) {
+      if (!key_mass_item(p, at, ntok, rank, parts, x)) continue;
+      // Where the sum goes, and the old weight, fetched while the rows stream by.
+      int page = -1;
+      float old = 0.0f;
+      const int pos = x.key0 + key, slot = pos % p.v.a.page_size;
+      if (half == 0 && rank == 0 && pos < x.q.kv) {
+        page = paged_page(p.v, p.v.a.block_table + x.s * p.v.a.table_stride, pos / p.v.a.page_size);
+        if (page >= 0 && pos < x.q.first && p.decay != 0.0f)
+          old = p.decay * p.mass[page * p.ms[0] + x.g * p.ms[1] + slot * p.ms[2]];
+      }
+      uint64_t sum2[2] = {f2_pack(0.0f, 0.0f), f2_pack(0.0f, 0.0f)};
+      auto rows_of = [&](const float (&s)[64], const float* lse, auto masked_c) {
+        constexpr bool masked = decltype(masked_c)::value;
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+          const float4 v = *reinterpret_cast<const float4*>(lse + 4 * k);
+          float x0, x1, x2, x3;
+          f2_unpack(f2_fma(f2_pack(s[4 * k], s[4 * k + 1]), sl2x2, f2_pack(-v.x, -v.y)), x0, x1);
+          f2_unpack(f2_fma(f2_pack(s[4 * k + 2], s[4 * k + 3]), sl2x2, f2_pack(-v.z, -v.w)), x2, x3);
+          float e0 = fast_exp2(x0), e1 = fast_exp2(x1), e2 = fast_exp2(x2), e3 = fast_exp2(x3);
+          if constexpr (masked) {
+            const int4 lim = *reinterpret_cast<const int4*>(lse + 128 + 4 * k);
+            e0 = key <= lim.x ? e0 : 0.0f;
+            e1 = key <= lim.y ? e1 : 0.0f;
+            e2 = key <= lim.z ? e2 : 0.0f;
+            e3 = key <= lim.w ? e3 : 0.0f;
+          }
+          sum2[0] = f2_add(sum2[0], f2_pack(e0, e1));
+          sum2[1] = f2_add(sum2[1], f2_pack(e2, e3));
+        }
+      };
+      for (int i = 0; ok && i < x.steps; ++i, ++qn) {
+        const uint32_t buf = qn & 1;
+        ok = __all_sync(0xffffffffu, mbar_wait(&l_full[qn % LST], (qn / LST) & 1, status, abort_flag) &&
+                                         mbar_wait(&s_full[2 * t + buf], (qn >> 1) & 1, status, abort_flag));
+        if (!ok) break;
+        tc_fence_after();
+        float s[64];
+        tmem_ld32(tS + buf * 128, *reinterpret_cast<float(*)[32]>(s));
+        tmem_ld32(tS + buf * 128 + 32, *reinterpret_cast<float(*)[32]>(s + 32));
+        tmem_wait_ld();
+        tc_fence_before();
+        mbar_arrive(&s_empty[2 * t + buf]);
+        const float* lse = reinterpret_cast<const float*>(smem + L::OFF_ROW + (qn % LST) * 1024) + half * 64;
+        // All tokens of the tile are the sequence's and see all the item's keys, or its rows have limits.
+        if (x.q.first + x.tok0 + i * ntok >= x.key0 + kKmKeys - 1 && x.tok0 + (i + 1) * ntok <= x.q.qlen)
+          rows_of(s, lse, std::false_type{});
+        else
+          rows_of(s, lse, std::true_type{});
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&l_empty[qn % LST]);
+      }
+      float a0, a1, a2, a3;
+      f2_unpack(sum2[0], a0, a1);
+      f2_unpack(sum2[1], a2, a3);
+      float sum = (a0 + a1) + (a2 + a3);
+      // Two buffers: what is handed over now is read before the barrier of the item after the next.
+      float* const mine = given + (done & 1) * 256;
+      if (half == 1) mine[key] = sum;
+      named_barrier_sync(1 + t, 256);
+      if (half == 0) sum += mine[key];
+      float* const dst = page >= 0 ? p.out + page * p.os[0] + x.g * p.os[1] + slot * p.os[2] : nullptr;
+      if (parts == 1) {
+        if (dst != nullptr) *dst = sum + old;
+      } else if (half == 0) {  // the only item: to the cluster's first CTA
+        uint32_t there;
+        asm("mapa.shared::cluster.u32 %0, %1, %2;"
+            : "=r"(there)
+            : "r"(smem_u32(smem + L::OFF_PART) + static_cast<uint32_t>(rank * 256 + key) * 4), "r"(0));
+        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(there), "f"(sum) : "memory");
+        to = dst;
+        old_part = old;
+      }
+      ++done;
+    }
+  }
+
+  if (parts > 1) {
+    cluster_sync();
+    if (to != nullptr) {  // half 0 of the first CTA
+      const float* const part = reinterpret_cast<const float*>(smem + L::OFF_PART) + (warp >> 3) * 128 + (warp & 3) * 32 + lane;
+      float sum = 0.0f;
+      for (int c = 0; c < parts; ++c) sum += part[c * 256];
+      *to = sum + old_part;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kKmMma) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512u);
+  }
+}
+
+// q as [N][Hq][D]: boxes of 64 dims x the heads of a group x `ntok` tokens, whose rows are those of a row tile in order.
+static bool rows_map(CUtensorMap* m, const KeyMassArgs& x, CUtensorMapDataType dt, int ntok) {
+  EncodeTiledFn fn = encode_fn();
+  if (fn == nullptr) return false;
+  const PagedArgs& a = x.a;
+  const cuuint64_t dims[4] = {(cuuint64_t)a.D, (cuuint64_t)a.Hq, (cuuint64_t)a.N, 1};
+  // A dimension of one element never steps: any valid stride will do.
+  const cuuint64_t row = (cuuint64_t)a.D * 2;
+  const cuuint64_t strides[3] = {a.Hq > 1 ? (cuuint64_t)a.qh * 2 : row, a.N > 1 ? (cuuint64_t)a.qn * 2 : row, row};
+  const cuuint32_t b[4] = {64, (cuuint32_t)(a.Hq / a.Hkv), (cuuint32_t)ntok, 1};
+  const cuuint32_t estr[4] = {1, 1, 1, 1};
+  return fn(m, dt, 4, const_cast<void*>(a.q), dims, strides, b, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename T, int D>
+static cudaError_t launch_rows(const KeyMassArgs& a, int dtype, cudaStream_t stream) {
+  using L = KeyMassLayout<D>;
+  const int ntok = 128 / (a.a.Hq / a.a.Hkv), box = paged_box(a.a.page_size, 128);
+  CUtensorMap mq, mk, mv;
+  if (!rows_map(&mq, a, dtype == SPRUCE_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, ntok) ||
+      !paged_cache_maps(a.a, dtype, box, &mk, &mv))
+    return cudaErrorInvalidValue;
+  auto kern = key_mass_sm100_kernel<T, D>;
+  static std::atomic<uint64_t> done{0};
+  cudaError_t e = allow_smem(reinterpret_cast<const void*>(kern), L::BYTES, done);
+  if (e != cudaSuccess) return e;
+  const KeyMassParams p = key_mass_params(a, kKmKeys);
+  const int64_t items = (int64_t)a.a.S * p.key_tiles * a.a.Hkv;
+  const int sms = sm_count();
+  // CTAs of an item: as many as leave one item each, and a row tile each of the longest sequence allowed.
+  int parts = 1;
+  while (parts < 8 && items * parts * 2 <= sms && 2 * parts * ntok <= a.a.max_q) parts *= 2;
+  cudaLaunchConfig_t cfg{};
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = parts;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.gridDim = dim3(static_cast<unsigned>(parts * std::min<int64_t>(items, sms / parts)));
+  cfg.blockDim = dim3(kKmThreads);
+  cfg.dynamicSmemBytes = L::BYTES;
+  cfg.stream = stream;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kern, mq, mk, p, box, ntok, parts, items);
+}
+
+cudaError_t launch_key_mass_sm100(const KeyMassArgs& a, int dtype, cudaStream_t stream) {
+  if (dtype == SPRUCE_DTYPE_BF16)
+    return a.a.D == 128 ? launch_rows<__nv_bfloat16, 128>(a, dtype, stream) : launch_rows<__nv_bfloat16, 64>(a, dtype, stream);
+  return a.a.D == 128 ? launch_rows<__half, 128>(a, dtype, stream) : launch_rows<__half, 64>(a, dtype, stream);
+}
+
+}  // namespace spruce

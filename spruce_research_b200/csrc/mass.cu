@@ -143,6 +143,9 @@ static cudaError_t launch_key_mass_t(const KeyMassArgs& a, int sms, cudaStream_t
 cudaError_t launch_key_mass(const KeyMassArgs& a, int dtype, cudaStream_t stream) {
   const int sms = sm_count();
   if (key_mass_params(a, kTileKeys).key_tiles == 0) return cudaSuccess;
+  const int rep = a.a.Hq / a.a.Hkv;
+  if (dtype != SPRUCE_DTYPE_F32 && (int64_t)a.a.max_q * rep > kKmFewRows && rep <= 128)
+    return launch_key_mass_sm100(a, dtype, stream);
   switch (dtype) {
     case SPRUCE_DTYPE_F32: return launch_key_mass_t<float>(a, sms, stream);
     case SPRUCE_DTYPE_BF16: return launch_key_mass_t<__nv_bfloat16>(a, sms, stream);

@@ -33,6 +33,10 @@ inline KeyMassParams key_mass_params(const KeyMassArgs& a, int tile) {
   return p;
 }
 
+// Key mass of more than kKmFewRows query rows a sequence and KV head, in 16 bits (key_mass_sm100.cu).
+constexpr int kKmFewRows = 32;
+cudaError_t launch_key_mass_sm100(const KeyMassArgs& a, int dtype, cudaStream_t stream);
+
 // Block mass in 16 bits (block_mass_sm100.cu).
 int64_t block_mass_sm100_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t T);
 cudaError_t launch_block_mass_sm100(const BlockMassArgs& a, int dtype, cudaStream_t stream);

@@ -740,7 +740,7 @@ def paged_key_mass(q: torch.Tensor, k_cache: torch.Tensor, mass: torch.Tensor, b
     _check_mass(out, k_cache.shape, "out")
     dt, size = _dt(q), q.element_size()
     qn, qh, qd = q.stride()
-    if qd != 1 or (qn | qh) % (16 // size) or q.data_ptr() % 16:
+    if qd != 1 or (qn | qh) % (16 // size) or q.data_ptr() % 16 or min(qn, qh) < 1:
         q = q.clone(memory_format=torch.contiguous_format)
         qn, qh, _ = q.stride()
     args = _lib.PAGED_KEY_MASS_ARGS.pack(
