@@ -44,7 +44,7 @@ struct KeyMassLayout {
 // An item of a CTA: its keys, and its share of the rows that see them.
 struct KeyMassItem {
   PagedSeq q;
-  int s, g, key0;
+  int s, g, key0, keys;  // keys: of the sequence, that its new tokens see
   int tok0, steps;  // first token of this CTA's rows, and its row tiles
 };
 
@@ -56,7 +56,8 @@ __device__ __forceinline__ bool key_mass_item(const KeyMassParams& p, int64_t at
   x.g = rest % p.v.a.Hkv;
   x.key0 = rest / p.v.a.Hkv * kKmKeys;
   x.q = paged_seq(p.v, x.s);
-  if (x.q.qlen == 0 || x.key0 >= x.q.kv) return false;
+  x.keys = mass_keys(x.q);
+  if (x.q.qlen == 0 || x.key0 >= x.keys) return false;
   // Tokens before the item's first key do not see it.
   const int lo = min(max(x.key0 - x.q.first, 0), x.q.qlen);
   const int tiles = (x.q.qlen - lo + ntok - 1) / ntok, each = (tiles + parts - 1) / parts;
@@ -143,7 +144,7 @@ __global__ void __launch_bounds__(kKmThreads, 1)
       const int32_t* table = p.v.a.block_table + x.s * p.v.a.table_stride;
       const int key = x.key0 + lane * box;
       int page = static_cast<int>(p.v.a.num_pages);  // reads zeros
-      if (lane < boxes && key < x.q.kv) {
+      if (lane < boxes && key < x.keys) {
         page = paged_page(p.v, table, key / p.v.a.page_size);
         if (page < 0) page = static_cast<int>(p.v.a.num_pages);
       }
@@ -276,7 +277,7 @@ __global__ void __launch_bounds__(kKmThreads, 1)
       int page = -1;
       float old = 0.0f;
       const int pos = x.key0 + key, slot = pos % p.v.a.page_size;
-      if (half == 0 && rank == 0 && pos < x.q.kv) {
+      if (half == 0 && rank == 0 && pos < x.keys) {
         page = paged_page(p.v, p.v.a.block_table + x.s * p.v.a.table_stride, pos / p.v.a.page_size);
         if (page >= 0 && pos < x.q.first && p.decay != 0.0f)
           old = p.decay * p.mass[page * p.ms[0] + x.g * p.ms[1] + slot * p.ms[2]];

@@ -68,14 +68,15 @@ __global__ void __launch_bounds__(kTileThreads) key_mass_tile_kernel(const KeyMa
     const int s = static_cast<int>(item / per_seq), rest = static_cast<int>(item % per_seq);
     const int g = rest / p.key_tiles, key0 = rest % p.key_tiles * kTileKeys;
     const PagedSeq q = paged_seq(p.v, s);
-    if (q.qlen == 0 || key0 >= q.kv) continue;
+    const int keys = mass_keys(q);
+    if (q.qlen == 0 || key0 >= keys) continue;
     __syncthreads();
-    if (tid < kTileKeys / 16) pages[tid] = mass_page(p, s, key0 + 16 * tid, q.kv);
+    if (tid < kTileKeys / 16) pages[tid] = mass_page(p, s, key0 + 16 * tid, keys);
     __syncthreads();
     for (int e = tid; e < kTileKeys * (D / 4); e += kTileThreads) {
       const int r = e / (D / 4), d = e % (D / 4) * 4, key = key0 + r, page = pages[r / 16];
       float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      if (page >= 0 && key < q.kv)
+      if (page >= 0 && key < keys)
         v = load4(static_cast<const T*>(p.v.a.kc) + page * p.v.a.ks[0] + g * p.v.a.ks[1] + key % p.v.a.page_size * p.v.a.ks[2] + d);
       *reinterpret_cast<float4*>(Ks + r * P + d) = v;
     }
@@ -96,7 +97,7 @@ __global__ void __launch_bounds__(kTileThreads) key_mass_tile_kernel(const KeyMa
         Ts[tid] = -1;
         if (r0 + tid < rows) {
           Ls[tid] = mass_row_lse(p.lse[row_at.offset(tid, p.ln, p.lh)]);
-          Ts[tid] = min(q.first + row_at.token(tid), q.kv - 1);
+          Ts[tid] = q.first + row_at.token(tid);
         }
       }
       __syncthreads();
@@ -115,7 +116,7 @@ __global__ void __launch_bounds__(kTileThreads) key_mass_tile_kernel(const KeyMa
     if (rr < 4) {
       const int key = key0 + kk * 4 + rr, page = pages[kk / 4];
       const float sum = rr == 0 ? acc[0] : (rr == 1 ? acc[1] : (rr == 2 ? acc[2] : acc[3]));
-      if (page >= 0 && key < q.kv) mass_store(p, page, g, key % p.v.a.page_size, key < q.first, sum);
+      if (page >= 0 && key < keys) mass_store(p, page, g, key % p.v.a.page_size, key < q.first, sum);
     }
   }
 }
@@ -144,8 +145,10 @@ cudaError_t launch_key_mass(const KeyMassArgs& a, int dtype, cudaStream_t stream
   const int sms = sm_count();
   if (key_mass_params(a, kTileKeys).key_tiles == 0) return cudaSuccess;
   const int rep = a.a.Hq / a.a.Hkv;
-  if (dtype != SPRUCE_DTYPE_F32 && (int64_t)a.a.max_q * rep > kKmFewRows && rep <= 128)
-    return launch_key_mass_sm100(a, dtype, stream);
+  if (dtype != SPRUCE_DTYPE_F32) {
+    if ((int64_t)a.a.max_q * rep <= kKmFewRows) return launch_key_mass_rows(a, dtype, stream);
+    if (rep <= 128) return launch_key_mass_sm100(a, dtype, stream);
+  }
   switch (dtype) {
     case SPRUCE_DTYPE_F32: return launch_key_mass_t<float>(a, sms, stream);
     case SPRUCE_DTYPE_BF16: return launch_key_mass_t<__nv_bfloat16>(a, sms, stream);

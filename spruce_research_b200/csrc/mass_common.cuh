@@ -36,6 +36,8 @@ inline KeyMassParams key_mass_params(const KeyMassArgs& a, int tile) {
 // Key mass of more than kKmFewRows query rows a sequence and KV head, in 16 bits (key_mass_sm100.cu).
 constexpr int kKmFewRows = 32;
 cudaError_t launch_key_mass_sm100(const KeyMassArgs& a, int dtype, cudaStream_t stream);
+// At most that many, in 16 bits (key_mass_rows.cu).
+cudaError_t launch_key_mass_rows(const KeyMassArgs& a, int dtype, cudaStream_t stream);
 
 // Block mass in 16 bits (block_mass_sm100.cu).
 int64_t block_mass_sm100_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t T);
@@ -46,6 +48,9 @@ __device__ __forceinline__ int mass_page(const KeyMassParams& p, int s, int key,
   if (key >= kv) return -1;
   return paged_page(p.v, p.v.a.block_table + s * p.v.a.table_stride, key / p.v.a.page_size);
 }
+
+// Keys that the new tokens see.  All the sequence holds, but where its tokens are cut to max_q.
+__device__ __forceinline__ int mass_keys(const PagedSeq& q) { return min(max(q.first + q.qlen, 0), q.kv); }
 
 // A row's lse in log2 units.  A row that saw nothing (-inf) counts for nothing.
 __device__ __forceinline__ float mass_row_lse(float lse) {
