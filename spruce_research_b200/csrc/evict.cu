@@ -9,7 +9,7 @@
 // Moving in place: slot j takes row kept[j] >= j, so going up in j a row is read before it is written over, if
 // all rows of a round are read before any is written: one barrier a round.  Rows are cut into slices of columns, which
 // never touch each other, so a (sequence, head) is spread over many CTAs that need not wait for one another.  Into other
-// pages there is nothing to wait for: a CTA takes 128 whole rows.
+// pages there is nothing to wait for: a warp takes 32 whole rows.
 #include <algorithm>
 
 #include "mass_common.cuh"
@@ -21,6 +21,24 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
   if (w != w) return 0xffffffffu;
   const uint32_t b = __float_as_uint(w + 0.0f);
   return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+
+// n / page_size for 0 <= n < 2^31 by a product: exact, as d - 1 <= 2^l - 1 bounds the rounding of 2^(31 + l) / d.
+struct PageDiv {
+  uint32_t mul;
+  int shift, size;
+  __device__ __forceinline__ int page(int n) const {
+    return static_cast<int>((static_cast<uint64_t>(static_cast<uint32_t>(n)) * mul) >> shift);
+  }
+};
+static PageDiv page_div(int size) {
+  PageDiv d;
+  int l = 0;
+  while ((int64_t(1) << l) < size) ++l;
+  d.shift = 31 + l;
+  d.mul = static_cast<uint32_t>(((uint64_t(1) << d.shift) + size - 1) / size);
+  d.size = size;
+  return d;
 }
 
 struct EvictSeq {
@@ -66,7 +84,7 @@ __device__ __forceinline__ void together(int ctas) {
     __syncthreads();
 }
 
-__global__ void __launch_bounds__(kSelectThreads, 1) evict_select_kernel(const EvictArgs a, int ctas, int cached) {
+__global__ void __launch_bounds__(kSelectThreads, 1) evict_select_kernel(const EvictArgs a, const PageDiv pd, int ctas, int cached, bool vec) {
   extern __shared__ uint32_t keys[];  // [cached]
   __shared__ int hist[2][kSelectBins];
   __shared__ int sums[2][kSelectWarps];
@@ -90,8 +108,8 @@ __global__ void __launch_bounds__(kSelectThreads, 1) evict_select_kernel(const E
   const int begin = min(rank * each, q.kv), n = min(each, q.kv - begin);
   const int32_t* table = a.table + s * a.table_stride;
   auto read = [&](int j) {
-    const int page = evict_page(table, j / a.page_size, a.num_pages, a.status);
-    return weight_key(page < 0 ? 0.0f : a.mass[page * a.ms[0] + g * a.ms[1] + j % a.page_size * a.ms[2]]);
+    const int pi = pd.page(j), page = evict_page(table, pi, a.num_pages, a.status);
+    return weight_key(page < 0 ? 0.0f : a.mass[page * a.ms[0] + g * a.ms[1] + (j - pi * pd.size) * a.ms[2]]);
   };
   auto key_of = [&](int i) { return i < cached ? keys[i] : read(begin + i); };
   auto always = [&](int j) { return j < q.sinks || j >= q.tail; };
@@ -103,7 +121,20 @@ __global__ void __launch_bounds__(kSelectThreads, 1) evict_select_kernel(const E
   for (int pass = 0; pass < 3; ++pass) {
     const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0), bins = pass == 2 ? 1024 : 2048;
     int* const h = hist[pass & 1];
-    if (pass == 0) {
+    if (pass == 0 && vec && n <= cached) {  // four slots a load; they lie in one page, and `begin` is a multiple of 32
+#pragma unroll 4
+      for (int i = 4 * tid; i < n; i += 4 * kSelectThreads) {
+        const int j = begin + i, pi = pd.page(j), page = evict_page(table, pi, a.num_pages, a.status);
+        float4 w = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (page >= 0) w = *reinterpret_cast<const float4*>(a.mass + page * a.ms[0] + g * a.ms[1] + (j - pi * pd.size));
+        const uint4 k = make_uint4(weight_key(w.x), weight_key(w.y), weight_key(w.z), weight_key(w.w));
+        *reinterpret_cast<uint4*>(keys + i) = k;
+        if (i < n && !always(j)) atomicAdd(&h[k.x >> 21], 1);
+        if (i + 1 < n && !always(j + 1)) atomicAdd(&h[k.y >> 21], 1);
+        if (i + 2 < n && !always(j + 2)) atomicAdd(&h[k.z >> 21], 1);
+        if (i + 3 < n && !always(j + 3)) atomicAdd(&h[k.w >> 21], 1);
+      }
+    } else if (pass == 0) {
 #pragma unroll 4
       for (int i = tid; i < n; i += kSelectThreads) {
         const uint32_t k = read(begin + i);
@@ -221,76 +252,128 @@ __global__ void __launch_bounds__(kSelectThreads, 1) evict_select_kernel(const E
   if (ctas > 1) together(ctas);  // the others read this CTA's counts
 }
 
-// Bytes a thread moves of a row at a time, and rows that it holds.
+// In place: a CTA takes a slice of the columns of all rows, so that the rows' order is its own affair.  A round is kMoveRows rows a
+// thread; the places of the next are looked up while this one's rows are on their way.
 constexpr int kMoveThreads = 256, kMoveRows = 8;
-constexpr int kMoveSlice = 32;  // bytes of a row that a CTA of a move in place takes
+constexpr int kMoveSlice = 32;  // bytes of a row that a CTA takes
 
-// Rows [j0, j1) from their old slots: bytes [at, at + lanes * sizeof(V)) of each.
 template <typename V>
-__device__ __forceinline__ void move_rows(const EvictArgs& a, const EvictSeq& q, int s, int g, const void* from, const int64_t* fs,
-                                          void* to, const int64_t* ts, int es, int lanes, int at, int j0, int j1) {
+__device__ __forceinline__ void move_rows(const EvictArgs& a, const PageDiv& pd, const EvictSeq& q, int s, int g, char* data,
+                                          const int64_t* st, int es, int lanes, int at) {
   const int32_t* kept = a.kept + ((int64_t)s * a.Hkv + g) * a.width;
   const int32_t* table = a.table + s * a.table_stride;
-  const int32_t* to_table = a.to_table + s * a.to_table_stride;
   const int r = threadIdx.x / lanes, c = threadIdx.x % lanes, per = kMoveThreads / lanes;
-  int src[kMoveRows];
-  auto slots = [&](int base) {
+  data += g * st[1] * es + at + c * sizeof(V);
+  int64_t from[kMoveRows], to[kMoveRows];  // -1: nothing to move
+  auto look = [&](int base) {
+    int src[kMoveRows];
 #pragma unroll
     for (int u = 0; u < kMoveRows; ++u) {
       const int j = base + u * per + r;
-      src[u] = r < per && j < j1 ? kept[j] : -1;
+      src[u] = j < q.keep ? kept[j] : -1;
+    }
+#pragma unroll
+    for (int u = 0; u < kMoveRows; ++u) {
+      const int j = base + u * per + r;
+      from[u] = -1;
+      if (src[u] < 0 || src[u] >= q.kv || src[u] == j) continue;
+      const int i0 = pd.page(src[u]), i1 = pd.page(j);
+      const int p0 = evict_page(table, i0, a.num_pages, a.status), p1 = evict_page(table, i1, a.num_pages, a.status);
+      if (p0 < 0 || p1 < 0) continue;
+      from[u] = (p0 * st[0] + (src[u] - i0 * pd.size) * st[2]) * es;
+      to[u] = (p1 * st[0] + (j - i1 * pd.size) * st[2]) * es;
     }
   };
-  slots(j0);
-  for (int base = j0; base < j1; base += per * kMoveRows) {
+  look(0);
+  for (int base = 0; base < q.keep; base += per * kMoveRows) {
     V v[kMoveRows];
     V* dst[kMoveRows];
 #pragma unroll
     for (int u = 0; u < kMoveRows; ++u) {
       dst[u] = nullptr;
-      const int j = base + u * per + r;
-      if (src[u] < 0 || src[u] >= q.kv || (a.in_place && src[u] == j)) continue;
-      const int p0 = evict_page(table, src[u] / a.page_size, a.num_pages, a.status);
-      const int p1 = evict_page(to_table, j / a.page_size, a.to_pages, a.status);
-      if (p0 < 0 || p1 < 0) continue;
-      v[u] = *reinterpret_cast<const V*>(static_cast<const char*>(from) +
-                                         (p0 * fs[0] + g * fs[1] + src[u] % a.page_size * fs[2]) * es + at + c * sizeof(V));
-      dst[u] = reinterpret_cast<V*>(static_cast<char*>(to) + (p1 * ts[0] + g * ts[1] + j % a.page_size * ts[2]) * es + at +
-                                    c * sizeof(V));
+      if (from[u] < 0) continue;
+      v[u] = *reinterpret_cast<const V*>(data + from[u]);
+      dst[u] = reinterpret_cast<V*>(data + to[u]);
     }
-    slots(base + per * kMoveRows);
-    if (a.in_place) __syncthreads();
+    look(base + per * kMoveRows);
+    __syncthreads();
 #pragma unroll
     for (int u = 0; u < kMoveRows; ++u)
       if (dst[u] != nullptr) *dst[u] = v[u];
   }
 }
 
-// In place: blocks of a (sequence, head) are `parts` slices of K, as many of V, and one of the weights.  Into other pages: `parts`
-// pieces of `rows` rows of K with the weights, and as many of V.
-__global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const EvictArgs a, int parts, int lanes, int rows) {
-  const int blocks = a.in_place ? 2 * parts + 1 : 2 * parts, x = blockIdx.x % blocks;
+// Blocks of a (sequence, head): `slices` of K, as many of V, and one of the weights.
+__global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(const EvictArgs a, const PageDiv pd, int slices, int lanes) {
+  const int blocks = 2 * slices + 1, x = blockIdx.x % blocks;
   const int sg = blockIdx.x / blocks, s = sg / a.Hkv, g = sg % a.Hkv;
   let_next_kernel_start();
   wait_for_earlier_kernels();
   const EvictSeq q = evict_seq(a, s, false);
-  if (a.in_place) {
-    if (q.keep == q.kv) return;
-    const int at = x % parts * lanes * 16;
-    if (x == 2 * parts)
-      move_rows<float>(a, q, s, g, a.mass, a.ms, a.mass_out, a.mos, 4, 1, 0, 0, q.keep);
-    else if (x < parts)
-      move_rows<uint4>(a, q, s, g, a.k, a.ks, a.k_out, a.kos, a.es, lanes, at, 0, q.keep);
-    else
-      move_rows<uint4>(a, q, s, g, a.v, a.vs, a.v_out, a.vos, a.es, lanes, at, 0, q.keep);
-  } else {
-    const int j0 = x % parts * rows, j1 = min(q.keep, j0 + rows);
-    if (j0 >= j1) return;
-    if (x < parts) {
-      move_rows<float>(a, q, s, g, a.mass, a.ms, a.mass_out, a.mos, 4, 1, 0, j0, j1);
-      move_rows<uint4>(a, q, s, g, a.k, a.ks, a.k_out, a.kos, a.es, lanes, 0, j0, j1);
-    } else {
-      move_rows<uint4>(a, q, s, g, a.v, a.vs, a.v_out, a.vos, a.es, lanes, 0, j0, j1);
+  if (q.keep == q.kv) return;
+  const int at = x % slices * lanes * 16;
+  if (x == 2 * slices)
+    move_rows<float>(a, pd, q, s, g, reinterpret_cast<char*>(a.mass_out), a.ms, 4, 1, 0);
+  else if (x < slices)
+    move_rows<uint4>(a, pd, q, s, g, static_cast<char*>(a.k_out), a.ks, a.es, lanes, at);
+  else
+    move_rows<uint4>(a, pd, q, s, g, static_cast<char*>(a.v_out), a.vs, a.es, lanes, at);
+}
+
+// Into other pages: a warp takes 32 rows of a (sequence, head).  Each lane looks up the places of one, then all copy K and V
+// rows 16 bytes a lane, eight loads in flight.
+constexpr int kCopyThreads = 256, kCopyRows = 32, kCopyFlight = 8;
+
+__global__ void __launch_bounds__(kCopyThreads) evict_copy_kernel(const EvictArgs a, const PageDiv pd, const PageDiv vecs, int chunks) {
+  const int lane = threadIdx.x & 31;
+  const int64_t at = (int64_t)blockIdx.x * (kCopyThreads / 32) + threadIdx.x / 32;
+  let_next_kernel_start();
+  wait_for_earlier_kernels();
+  const int64_t sg = at / chunks;
+  if (sg >= (int64_t)a.S * a.Hkv) return;
+  const int s = static_cast<int>(sg / a.Hkv), g = static_cast<int>(sg % a.Hkv), j0 = static_cast<int>(at % chunks) * kCopyRows;
+  const EvictSeq q = evict_seq(a, s, false);
+  const int n = min(kCopyRows, q.keep - j0);
+  if (n <= 0) return;
+  // Places of this lane's row: pages and rows of them; -1: no such page.
+  int p0 = -1, p1 = -1, r0 = 0, r1 = 0;
+  if (lane < n) {
+    const int src = a.kept[sg * a.width + j0 + lane];
+    if (src >= 0 && src < q.kv) {
+      const int i0 = pd.page(src), i1 = pd.page(j0 + lane);
+      r0 = src - i0 * pd.size;
+      r1 = j0 + lane - i1 * pd.size;
+      p0 = evict_page(a.table + s * a.table_stride, i0, a.num_pages, a.status);
+      p1 = evict_page(a.to_table + s * a.to_table_stride, i1, a.to_pages, a.status);
+    }
+  }
+  const bool ok = p0 >= 0 && p1 >= 0;
+  if (ok) a.mass_out[p1 * a.mos[0] + g * a.mos[1] + r1 * a.mos[2]] = a.mass[p0 * a.ms[0] + g * a.ms[1] + r0 * a.ms[2]];
+  const unsigned rows_ok = __ballot_sync(0xffffffffu, ok);
+#pragma unroll
+  for (int kv = 0; kv < 2; ++kv) {
+    const int64_t* fs = kv == 0 ? a.ks : a.vs;
+    const int64_t* ts = kv == 0 ? a.kos : a.vos;
+    const char* from = static_cast<const char*>(kv == 0 ? a.k : a.v) + g * fs[1] * a.es;
+    char* to = static_cast<char*>(kv == 0 ? a.k_out : a.v_out) + g * ts[1] * a.es;
+    const int64_t f = (p0 * fs[0] + r0 * fs[2]) * a.es, t = (p1 * ts[0] + r1 * ts[2]) * a.es;
+    const int total = n * vecs.size;  // 16-byte pieces
+    for (int i0 = 0; i0 < total; i0 += 32 * kCopyFlight) {
+      uint4 v[kCopyFlight];
+      char* dst[kCopyFlight];
+#pragma unroll
+      for (int u = 0; u < kCopyFlight; ++u) {
+        const int i = i0 + 32 * u + lane, row = vecs.page(min(i, total - 1));
+        const int64_t fr = __shfl_sync(0xffffffffu, f, row), tr = __shfl_sync(0xffffffffu, t, row);
+        dst[u] = nullptr;
+        if (i >= total || !(rows_ok >> row & 1)) continue;
+        const int c = (i - row * vecs.size) * 16;
+        v[u] = __ldcs(reinterpret_cast<const uint4*>(from + fr + c));
+        dst[u] = to + tr + c;
+      }
+#pragma unroll
+      for (int u = 0; u < kCopyFlight; ++u)
+        if (dst[u] != nullptr) *reinterpret_cast<uint4*>(dst[u]) = v[u];
     }
   }
 }
@@ -317,23 +400,21 @@ cudaError_t launch_evict(const EvictArgs& a, cudaStream_t stream) {
   cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  e = cudaLaunchKernelEx(&cfg, evict_select_kernel, a, ctas, cached);
+  const bool vec = a.ms[2] == 1 && a.ms[0] % 4 == 0 && a.ms[1] % 4 == 0 && (reinterpret_cast<uintptr_t>(a.mass) & 15u) == 0;
+  const PageDiv pd = page_div(a.page_size);
+  e = cudaLaunchKernelEx(&cfg, evict_select_kernel, a, pd, ctas, cached, vec);
   const int most = std::min(a.keep, a.cap);  // rows that a head keeps
   if (e != cudaSuccess || most == 0) return e;
   const int row = a.D * a.es;
-  int parts, lanes, rows = 0;
   if (a.in_place) {
     const int slice = row % kMoveSlice == 0 ? kMoveSlice : 16;
-    parts = row / slice;
-    lanes = slice / 16;
-  } else {
-    lanes = row / 16;
-    rows = std::max(1, kMoveThreads / lanes) * kMoveRows;
-    parts = (most + rows - 1) / rows;
+    return launch_early(evict_move_kernel, static_cast<int>(heads * (2 * (row / slice) + 1)), kMoveThreads, 0, stream, a, pd,
+                        row / slice, slice / 16);
   }
-  const int64_t blocks = heads * (a.in_place ? 2 * parts + 1 : 2 * (int64_t)parts);
+  const int chunks = (most + kCopyRows - 1) / kCopyRows;
+  const int64_t blocks = (heads * chunks + kCopyThreads / 32 - 1) / (kCopyThreads / 32);
   if (blocks > INT32_MAX) return cudaErrorInvalidConfiguration;
-  return launch_early(evict_move_kernel, static_cast<int>(blocks), kMoveThreads, 0, stream, a, parts, lanes, rows);
+  return launch_early(evict_copy_kernel, static_cast<int>(blocks), kCopyThreads, 0, stream, a, pd, page_div(row / 16), chunks);
 }
 
 }  // namespace spruce
