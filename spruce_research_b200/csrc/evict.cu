@@ -16,9 +16,10 @@
 
 namespace spruce {
 
-// Order of the weights as unsigned integers; NaN above all, -0 as +0.
+// Order of the weights as unsigned integers; NaN above all, -0 as +0.  kAlways, above that, is a slot that stays anyway.
+constexpr uint32_t kAlways = 0xffffffffu, kNan = 0xfffffffeu;
 __device__ __forceinline__ uint32_t weight_key(float w) {
-  if (w != w) return 0xffffffffu;
+  if (w != w) return kNan;
   const uint32_t b = __float_as_uint(w + 0.0f);
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
@@ -65,16 +66,22 @@ __device__ __forceinline__ int evict_page(const int32_t* table, int index, int64
   return -1;
 }
 
-constexpr int kSelectThreads = 1024, kSelectWarps = kSelectThreads / 32;
-constexpr int kSelectBins = 2048, kSelectMostCtas = 8;
+constexpr int kSelectThreads = 512, kSelectWarps = kSelectThreads / 32;
+constexpr int kSelectBins = 2048, kSelectMostCtas = 16;
 constexpr int kSelectCached = 48 * 1024;  // slots of a CTA whose weights fit in shared memory; longer pieces are read again
 
-__device__ __forceinline__ int remote_int(const int* p, int cta) {
+__device__ __forceinline__ uint32_t at_cta(const int* p, int cta) {
   uint32_t at;
-  int v;
   asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(p)), "r"(cta));
-  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+  return at;
+}
+__device__ __forceinline__ int remote_int(const int* p, int cta) {
+  int v;
+  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(at_cta(p, cta)) : "memory");
   return v;
+}
+__device__ __forceinline__ void remote_store(int* p, int cta, int v) {
+  asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(at_cta(p, cta)), "r"(v) : "memory");
 }
 // All threads of the CTAs that share a head.
 __device__ __forceinline__ void together(int ctas) {
@@ -84,15 +91,18 @@ __device__ __forceinline__ void together(int ctas) {
     __syncthreads();
 }
 
-__global__ void __launch_bounds__(kSelectThreads, 1) evict_select_kernel(const EvictArgs a, const PageDiv pd, int ctas, int cached, bool vec) {
-  extern __shared__ uint32_t keys[];  // [cached]
-  __shared__ int hist[2][kSelectBins];
+__global__ void __launch_bounds__(kSelectThreads, 2)
+    evict_select_kernel(const EvictArgs a, const PageDiv pd, int ctas, int cached, bool vec) {
+  extern __shared__ __align__(16) uint32_t keys[];  // [cached, to a multiple of 4]
+  __shared__ int hist[kSelectBins];
+  __shared__ int shares[kSelectMostCtas];
   __shared__ int sums[2][kSelectWarps];
-  __shared__ int found[2];            // digit of the last one kept, and how many are left to take within it
-  __shared__ int counts[2];           // of this CTA: above the last weight (or always kept), and equal to it
+  __shared__ int found[2];               // digit of the last one kept, and how many are left to take within it
+  __shared__ int counts[2];              // of this CTA: above the last weight (or always kept), and equal to it
   const int sg = blockIdx.x / ctas, rank = blockIdx.x % ctas;
   const int s = sg / a.Hkv, g = sg % a.Hkv;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  for (int b = tid; b < kSelectBins; b += kSelectThreads) hist[b] = 0;
   let_next_kernel_start();
   wait_for_earlier_kernels();
   const EvictSeq q = evict_seq(a, s, g == 0 && rank == 0 && tid == 0);
@@ -103,68 +113,81 @@ __global__ void __launch_bounds__(kSelectThreads, 1) evict_select_kernel(const E
     for (int j = rank * kSelectThreads + tid; j < q.keep; j += ctas * kSelectThreads) kept[j] = j;
     return;
   }
-  // This CTA's slots, a whole number of warps' steps.
+  // This CTA's slots.
   const int each = ((q.kv + ctas - 1) / ctas + 31) / 32 * 32;
   const int begin = min(rank * each, q.kv), n = min(each, q.kv - begin);
   const int32_t* table = a.table + s * a.table_stride;
+  auto key = [&](int j, float w) { return j < q.sinks || j >= q.tail ? kAlways : weight_key(w); };
   auto read = [&](int j) {
     const int pi = pd.page(j), page = evict_page(table, pi, a.num_pages, a.status);
-    return weight_key(page < 0 ? 0.0f : a.mass[page * a.ms[0] + g * a.ms[1] + (j - pi * pd.size) * a.ms[2]]);
+    return key(j, page < 0 ? 0.0f : a.mass[page * a.ms[0] + g * a.ms[1] + (j - pi * pd.size) * a.ms[2]]);
   };
-  auto key_of = [&](int i) { return i < cached ? keys[i] : read(begin + i); };
-  auto always = [&](int j) { return j < q.sinks || j >= q.tail; };
-  for (int b = tid; b < kSelectBins; b += kSelectThreads) hist[0][b] = 0;
-  __syncthreads();
+  auto count = [&](int* h, uint32_t k, int digit) {
+    if (k != kAlways) atomicAdd(&h[digit], 1);
+  };
+  together(ctas);  // the histograms are empty
+  if (vec && n <= cached) {  // four slots a load; they lie in one page, and `begin` is a multiple of 32
+#pragma unroll 4
+    for (int i = 4 * tid; i < n; i += 4 * kSelectThreads) {
+      const int j = begin + i, pi = pd.page(j), page = evict_page(table, pi, a.num_pages, a.status);
+      float4 w = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if (page >= 0) w = *reinterpret_cast<const float4*>(a.mass + page * a.ms[0] + g * a.ms[1] + (j - pi * pd.size));
+      const uint4 k = make_uint4(key(j, w.x), key(j + 1, w.y), key(j + 2, w.z), key(j + 3, w.w));
+      *reinterpret_cast<uint4*>(keys + i) = k;  // past the sequence's slots: those of the tail, kAlways
+      count(hist, k.x, k.x >> 21);
+      count(hist, k.y, k.y >> 21);
+      count(hist, k.z, k.z >> 21);
+      count(hist, k.w, k.w >> 21);
+    }
+  } else {
+#pragma unroll 4
+    for (int i = tid; i < n; i += kSelectThreads) {
+      const uint32_t k = read(begin + i);
+      if (i < cached) keys[i] = k;
+      count(hist, k, k >> 21);
+    }
+    if (tid < 4 && n + tid < cached) keys[n + tid] = kAlways;
+  }
   int left = q.keep - q.sinks - (q.kv - q.tail);  // to be taken between sinks and tail
-  uint32_t prefix = 0, mask = 0;
+  uint32_t prefix = left > 0 ? 0u : kNan, mask = 0;
 #pragma unroll
   for (int pass = 0; pass < 3; ++pass) {
     const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0), bins = pass == 2 ? 1024 : 2048;
-    int* const h = hist[pass & 1];
-    if (pass == 0 && vec && n <= cached) {  // four slots a load; they lie in one page, and `begin` is a multiple of 32
-#pragma unroll 4
-      for (int i = 4 * tid; i < n; i += 4 * kSelectThreads) {
-        const int j = begin + i, pi = pd.page(j), page = evict_page(table, pi, a.num_pages, a.status);
-        float4 w = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (page >= 0) w = *reinterpret_cast<const float4*>(a.mass + page * a.ms[0] + g * a.ms[1] + (j - pi * pd.size));
-        const uint4 k = make_uint4(weight_key(w.x), weight_key(w.y), weight_key(w.z), weight_key(w.w));
-        *reinterpret_cast<uint4*>(keys + i) = k;
-        if (i < n && !always(j)) atomicAdd(&h[k.x >> 21], 1);
-        if (i + 1 < n && !always(j + 1)) atomicAdd(&h[k.y >> 21], 1);
-        if (i + 2 < n && !always(j + 2)) atomicAdd(&h[k.z >> 21], 1);
-        if (i + 3 < n && !always(j + 3)) atomicAdd(&h[k.w >> 21], 1);
+    if (pass > 0 && left > 0) {
+      auto look = [&](uint32_t k) {
+        if ((k & mask) == prefix) count(hist, k, (k >> shift) & (bins - 1));
+      };
+      const int there = min(n, cached);
+      for (int i = 4 * tid; i < there; i += 4 * kSelectThreads) {
+        const uint4 k = *reinterpret_cast<const uint4*>(keys + i);
+        look(k.x);
+        if (i + 1 < there) look(k.y);
+        if (i + 2 < there) look(k.z);
+        if (i + 3 < there) look(k.w);
       }
-    } else if (pass == 0) {
-#pragma unroll 4
-      for (int i = tid; i < n; i += kSelectThreads) {
-        const uint32_t k = read(begin + i);
-        if (i < cached) keys[i] = k;
-        if (!always(begin + i)) atomicAdd(&h[k >> 21], 1);
-      }
-    } else {
-      for (int i = tid; i < n; i += kSelectThreads) {
-        const uint32_t k = key_of(i);
-        if ((k & mask) == prefix && !always(begin + i)) atomicAdd(&h[(k >> shift) & (bins - 1)], 1);
-      }
+      for (int i = cached + tid; i < n; i += kSelectThreads) look(read(begin + i));
     }
     together(ctas);
-    // The other buffer was read by all before they came here.
-    for (int b = tid; b < kSelectBins; b += kSelectThreads) hist[(pass + 1) & 1][b] = 0;
-    // Bins from the highest down, two a thread.
-    const int hi = bins - 1 - 2 * tid;
-    int c0 = 0, c1 = 0;
-    if (hi > 0) {
-      if (ctas == 1) {
-        c0 = h[hi];
-        c1 = h[hi - 1];
-      } else {
-        for (int c = 0; c < ctas; ++c) {
-          c0 += remote_int(&h[hi], c);
-          c1 += remote_int(&h[hi - 1], c);
+    // Bins from the highest down.  A CTA adds up an equal share of them over all CTAs; the shares' sums tell every CTA whose share
+    // holds the last one kept, and that one finds it.  (All CTAs reading one CTA's totals took four times as long.)
+    const int share = bins / ctas, top = bins - 1 - rank * share;
+    const int bins_of = max(1, share / kSelectThreads);  // bins of a thread: 1, 2 or 4
+    int c[4] = {0, 0, 0, 0}, inc = 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int b = bins_of * tid + k;
+      if (k < bins_of && b < share) {
+        if (ctas == 1) {
+          c[k] = hist[top - b];
+        } else {
+#pragma unroll 16
+          for (int x = 0; x < kSelectMostCtas; ++x)
+            if (x < ctas) c[k] += remote_int(&hist[top - b], x);
         }
       }
+      inc += c[k];
     }
-    int inc = c0 + c1;
+    int before = -inc;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int y = __shfl_up_sync(0xffffffffu, inc, o);
@@ -172,84 +195,110 @@ __global__ void __launch_bounds__(kSelectThreads, 1) evict_select_kernel(const E
     }
     if (lane == 31) sums[0][warp] = inc;
     __syncthreads();
-    int before = inc - c0 - c1;
-    for (int w = 0; w < warp; ++w) before += sums[0][w];
-    if (left > 0 && hi > 0) {  // one thread of the block finds it
-      if (before < left && left <= before + c0) {
-        found[0] = hi;
-        found[1] = left - before;
-      } else if (before + c0 < left && left <= before + c0 + c1) {
-        found[0] = hi - 1;
-        found[1] = left - before - c0;
+    before += inc + __reduce_add_sync(0xffffffffu, lane < warp ? sums[0][lane] : 0);
+    bool here = true;
+    if (ctas > 1) {
+      const int all = __reduce_add_sync(0xffffffffu, lane < kSelectWarps ? sums[0][lane] : 0);
+      if (warp == 0 && lane < ctas) remote_store(&shares[rank], lane, all);
+      together(ctas);
+      const int higher = __reduce_add_sync(0xffffffffu, lane < rank ? shares[lane] : 0);
+      before += higher;
+      here = higher < left && left <= higher + all;
+    }
+    if (left > 0 && here) {  // one thread of the head finds it
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if (before < left && left <= before + c[k])
+          for (int x = 0; x < ctas; ++x) {
+            remote_store(&found[0], x, top - bins_of * tid - k);
+            remote_store(&found[1], x, left - before);
+          }
+        before += c[k];
       }
     }
-    __syncthreads();
+    for (int b = tid; b < kSelectBins; b += kSelectThreads) hist[b] = 0;
+    together(ctas);
     if (left > 0) {
       prefix |= static_cast<uint32_t>(found[0]) << shift;
       left = found[1];
       mask |= static_cast<uint32_t>(bins - 1) << shift;
     }
   }
-  // `left` slots of exactly the weight `prefix` stay, and all above it; none between sinks and tail where none is to be taken.
-  const bool any = mask != 0;
-  const int per = (n + kSelectWarps * 32 - 1) / (kSelectWarps * 32) * 32, w0 = min(warp * per, n), w1 = min(w0 + per, n);
-  auto look = [&](int i, unsigned& above, unsigned& equal) {  // of 32 slots
-    bool up = false, eq = false;
-    if (i < w1) {
-      const int j = begin + i;
-      up = always(j);
-      if (!up && any) {
-        const uint32_t k = key_of(i);
-        up = k > prefix;
-        eq = k == prefix;
-      }
+  // All above `prefix` stay and, of its equals, the first `left`.  128 slots a warp and step, four a lane.
+  const int per = (n + kSelectWarps * 128 - 1) / (kSelectWarps * 128) * 128, w0 = min(warp * per, n), w1 = min(w0 + per, n);
+  auto four = [&](int i) {
+    uint4 k = make_uint4(0, 0, 0, 0);  // below all: neither above nor, as `prefix` is at least that of -inf, equal
+    if (i + 3 < min(w1, cached)) {
+      k = *reinterpret_cast<const uint4*>(keys + i);
+    } else {
+      if (i < w1) k.x = i < cached ? keys[i] : read(begin + i);
+      if (i + 1 < w1) k.y = i + 1 < cached ? keys[i + 1] : read(begin + i + 1);
+      if (i + 2 < w1) k.z = i + 2 < cached ? keys[i + 2] : read(begin + i + 2);
+      if (i + 3 < w1) k.w = i + 3 < cached ? keys[i + 3] : read(begin + i + 3);
     }
-    above = __ballot_sync(0xffffffffu, up);
-    equal = __ballot_sync(0xffffffffu, eq);
+    return k;
   };
+  auto above = [&](const uint4& k) { return (k.x > prefix) + (k.y > prefix) + (k.z > prefix) + (k.w > prefix); };
+  auto equal = [&](const uint4& k) { return (k.x == prefix) + (k.y == prefix) + (k.z == prefix) + (k.w == prefix); };
   int ups = 0, eqs = 0;
-  for (int i = w0; i < w1; i += 32) {
-    unsigned above, equal;
-    look(i + lane, above, equal);
-    ups += __popc(above);
-    eqs += __popc(equal);
+  for (int i = w0; i < w1; i += 128) {
+    const uint4 k = four(i + 4 * lane);
+    ups += above(k);
+    eqs += equal(k);
   }
+  ups = __reduce_add_sync(0xffffffffu, ups);
+  eqs = __reduce_add_sync(0xffffffffu, eqs);
   if (lane == 0) {
     sums[0][warp] = ups;
     sums[1][warp] = eqs;
   }
   __syncthreads();
-  int up0 = 0, eq0 = 0;
-  for (int w = 0; w < kSelectWarps; ++w) {
-    if (w == warp) {
-      ups = up0;
-      eqs = eq0;
-    }
-    up0 += sums[0][w];
-    eq0 += sums[1][w];
-  }
-  if (ctas > 1) {
-    if (tid == 0) {
-      counts[0] = up0;
-      counts[1] = eq0;
-    }
-    together(ctas);
-    for (int c = 0; c < rank; ++c) {
-      ups += remote_int(&counts[0], c);
-      eqs += remote_int(&counts[1], c);
+  {
+    const int u = lane < kSelectWarps ? sums[0][lane] : 0, e = lane < kSelectWarps ? sums[1][lane] : 0;
+    ups = __reduce_add_sync(0xffffffffu, lane < warp ? u : 0);
+    eqs = __reduce_add_sync(0xffffffffu, lane < warp ? e : 0);
+    if (ctas > 1) {
+      const int all_u = __reduce_add_sync(0xffffffffu, u), all_e = __reduce_add_sync(0xffffffffu, e);
+      if (tid == 0) {
+        counts[0] = all_u;
+        counts[1] = all_e;
+      }
+      together(ctas);
+      const bool before = lane < rank;
+      ups += __reduce_add_sync(0xffffffffu, before ? remote_int(&counts[0], lane) : 0);
+      eqs += __reduce_add_sync(0xffffffffu, before ? remote_int(&counts[1], lane) : 0);
     }
   }
-  for (int i = w0; i < w1; i += 32) {
-    unsigned above, equal;
-    look(i + lane, above, equal);
-    const unsigned lower = (1u << lane) - 1;
-    const int rank_eq = eqs + __popc(equal & lower);
-    const int at = ups + __popc(above & lower) + min(rank_eq, left);
-    if (((above >> lane & 1) || ((equal >> lane & 1) && rank_eq < left)) && at < q.keep) kept[at] = begin + i + lane;
-    ups += __popc(above);
-    eqs += __popc(equal);
+  for (int i = w0; i < w1; i += 128) {
+    const uint4 k = four(i + 4 * lane);
+    // Both counts in one scan: a step has at most 128 of each.
+    const int mine = above(k) | equal(k) << 16;
+    int inc = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += y;
+    }
+    const int all = __shfl_sync(0xffffffffu, inc, 31);
+    int up = ups + ((inc - mine) & 0xffff), eq = eqs + ((inc - mine) >> 16);
+    auto put = [&](uint32_t x, int j) {
+      if (x > prefix) {
+        kept[up + min(eq, left)] = j;
+        ++up;
+      } else if (x == prefix) {
+        if (eq < left) kept[up + eq] = j;
+        ++eq;
+      }
+    };
+    const int j = begin + i + 4 * lane;
+    put(k.x, j);
+    put(k.y, j + 1);
+    put(k.z, j + 2);
+    put(k.w, j + 3);
+    ups += all & 0xffff;
+    eqs += all >> 16;
   }
-  if (ctas > 1) together(ctas);  // the others read this CTA's counts
+  if (ctas > 1) together(ctas);  // the others read this CTA's shared memory
 }
 
 // In place: a CTA takes a slice of the columns of all rows, so that the rows' order is its own affair.  A round is kMoveRows rows a
@@ -383,9 +432,11 @@ cudaError_t launch_evict(const EvictArgs& a, cudaStream_t stream) {
   // CTAs of a head: as many as the GPU has room for, while each gets 2048 slots of the longest sequence allowed.
   int ctas = 1;
   while (ctas < kSelectMostCtas && heads * ctas * 2 <= sm_count() && a.cap / (ctas * 2) >= 2048) ctas *= 2;
-  const int each = ((a.cap + ctas - 1) / ctas + 31) / 32 * 32, cached = std::min(each, kSelectCached);
+  const int each = ((a.cap + ctas - 1) / ctas + 31) / 32 * 32, cached = std::min(each, kSelectCached);  // a multiple of 4
   static std::atomic<uint64_t> done{0};
   cudaError_t e = allow_smem(reinterpret_cast<const void*>(evict_select_kernel), kSelectCached * 4, done);
+  if (e == cudaSuccess && ctas > 8)
+    e = cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg{};
   cudaLaunchAttribute attr[2]{};
