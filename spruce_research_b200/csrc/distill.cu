@@ -3,15 +3,21 @@
 //   p = softmax_k(t_k / tau) over the row's teacher entries, q = softmax_j(s_j / tau) over its visible columns
 //   loss = sum_k p_k (ln p_k - ln q_id(k))         d loss / d s_j = (q_j - sum_{k: id(k) = j} p_k) / tau
 //
-// One CTA a row.  The first pass keeps a running maximum and sum; the gradient's pass reads the row again (it is in L2 when
-// both run in one call) and the columns of the teacher are written again after it, so that each element is rounded once.
+// Bound by HBM: the scores are read once (twice by a separate backward pass) and the gradient written once.  Rows of up to 2048
+// columns (a gate's) take a warp each, which holds the row in registers between the sums and the gradient.  Longer ones (a
+// vocabulary's) take a CTA each, which keeps a running maximum and sum; its gradient pass reads the row again, from L2 when both
+// run in one call: two CTAs an SM, so that their rows stay there.  The teacher's columns are written again after the others,
+// so that each element is rounded once.  A column named twice is found by a bitmap; only rows that have one search for it.
 #include <algorithm>
 
 #include "mass_common.cuh"
 
 namespace spruce {
 
-constexpr int kDistillThreads = 256;
+constexpr int kDistillThreads = 512, kDistillWarps = kDistillThreads / 32;
+constexpr int kRowWarps = 8;            // rows of a CTA of the warp kernel
+constexpr int kRowMost = 2048, kRowEntries = 512;  // columns and teacher entries that it takes
+constexpr int kRowBits = 64, kDistillBits = 1024;  // words of the bitmaps; columns share bits modulo their size
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 __device__ __forceinline__ float load_as_float(const void* p, int dtype, int64_t i) {
@@ -20,78 +26,276 @@ __device__ __forceinline__ float load_as_float(const void* p, int dtype, int64_t
   return __half2float(static_cast<const __half*>(p)[i]);
 }
 
-__device__ __forceinline__ float2 block_join(float m, float l, float2* red) {
-  auto join = [](float2 a, float2 b) {
-    const float m = fmaxf(a.x, b.x), ref = m == -INFINITY ? 0.0f : m;
-    return make_float2(m, a.y * exp2f(a.x - ref) + b.y * exp2f(b.x - ref));
-  };
-  float2 v = make_float2(m, l);
+// A maximum and the sum of 2^((x - maximum) c) over it.  Differences are formed before they are scaled: the types' lowest
+// values, as masks, stay finite.
+__device__ __forceinline__ float2 join(float2 a, float2 b, float c) {
+  const float m = fmaxf(a.x, b.x), ref = m == -INFINITY ? 0.0f : m;
+  return make_float2(m, a.y * fast_exp2((a.x - ref) * c) + b.y * fast_exp2((b.x - ref) * c));
+}
+__device__ __forceinline__ float2 warp_join(float2 v, float c) {
+#pragma unroll
   for (int o = 16; o > 0; o >>= 1)
-    v = join(v, make_float2(__shfl_xor_sync(0xffffffffu, v.x, o), __shfl_xor_sync(0xffffffffu, v.y, o)));
+    v = join(v, make_float2(__shfl_xor_sync(0xffffffffu, v.x, o), __shfl_xor_sync(0xffffffffu, v.y, o)), c);
+  return v;
+}
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// Columns of the row that count.
+__device__ __forceinline__ int row_seen(const DistillArgs& a, int64_t row, bool report) {
+  if (a.visible == nullptr) return a.n;
+  const int seen = a.visible[row];
+  if (report && (seen < 0 || seen > a.n)) raise_status(a.status, SPRUCE_STATUS_BAD_LENGTH);
+  return min(max(seen, 0), a.n);
+}
+// A teacher entry: its column (-1: padding) and logit (-inf).
+__device__ __forceinline__ void row_entry(const DistillArgs& a, int64_t row, int k, int seen, int& column, float& logit) {
+  const int64_t id = a.ids64 ? static_cast<const int64_t*>(a.ids)[row * a.id_stride + k]
+                             : static_cast<const int32_t*>(a.ids)[row * a.id_stride + k];
+  if (id >= seen) raise_status(a.status, SPRUCE_STATUS_BAD_INDEX);
+  const bool use = id >= 0 && id < seen;
+  column = use ? static_cast<int>(id) : -1;
+  logit = use ? load_as_float(a.teacher, a.teacher_dtype, row * a.teacher_stride + k) : -INFINITY;
+}
+template <typename T>
+__device__ __forceinline__ void unpack16(const uint4& v, float (&x)[16 / sizeof(T)]) {
+  const T* e = reinterpret_cast<const T*>(&v);
+#pragma unroll
+  for (int i = 0; i < static_cast<int>(16 / sizeof(T)); ++i) x[i] = Elem<T>::to_f(e[i]);
+}
+template <typename T>
+__device__ __forceinline__ uint4 pack16(const float (&x)[16 / sizeof(T)]) {
+  uint4 v;
+  T* e = reinterpret_cast<T*>(&v);
+#pragma unroll
+  for (int i = 0; i < static_cast<int>(16 / sizeof(T)); ++i) e[i] = Elem<T>::from_f(x[i]);
+  return v;
+}
+
+// ------------------------------------------------------------------ a warp a row
+// NV: 16-byte vectors of a lane.  Lane l holds columns V (32 i + l) ..; the order of the sums does not depend on alignment.
+template <typename T, int NV>
+__global__ void __launch_bounds__(32 * kRowWarps) distill_rows_kernel(const DistillArgs a, bool vec_in, bool vec_out) {
+  constexpr int V = 16 / sizeof(T);
+  extern __shared__ float sm[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  float* P = sm + warp * (2 * a.K + kRowBits);     // [K] teacher weights
+  int* I = reinterpret_cast<int*>(P + a.K);        // [K] columns
+  uint32_t* bits = reinterpret_cast<uint32_t*>(I + a.K);
+  const int64_t row = (int64_t)blockIdx.x * kRowWarps + warp;
+  if (row >= a.R) return;
+  const float c = a.inv_tau * kLog2e;
+  const T* s = static_cast<const T*>(a.scores) + row * a.score_stride;
+  const int seen = row_seen(a, row, lane == 0);
+  float v[NV][V];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int col = (32 * i + lane) * V;
+    if (vec_in && col + V <= seen) {
+      unpack16<T>(__ldcs(reinterpret_cast<const uint4*>(s + col)), v[i]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < V; ++e) v[i][e] = col + e < seen ? Elem<T>::to_f(s[col + e]) : -INFINITY;
+    }
+  }
+  // Teacher.
+  for (int b = lane; b < kRowBits; b += 32) bits[b] = 0;
+  float tm = -INFINITY;
+  __syncwarp();
+  bool twice = false;
+  for (int k = lane; k < a.K; k += 32) {
+    int column;
+    float logit;
+    row_entry(a, row, k, seen, column, logit);
+    I[k] = column;
+    P[k] = logit;
+    tm = fmaxf(tm, logit);
+    if (a.grad != nullptr && column >= 0)
+      twice = twice || (atomicOr(&bits[(column >> 5) % kRowBits], 1u << (column & 31)) >> (column & 31) & 1);
+  }
+  twice = __any_sync(0xffffffffu, twice);
+  tm = warp_max(tm);
+  const float tref = tm == -INFINITY ? 0.0f : tm;
+  float tsum = 0.0f;
+  for (int k = lane; k < a.K; k += 32) tsum += I[k] < 0 ? 0.0f : fast_exp2((P[k] - tref) * c);
+  tsum = warp_sum(tsum);
+  // Student.
+  float2 st;
+  if (a.stats_in != nullptr) {
+    st = make_float2(a.stats_in[2 * row], a.stats_in[2 * row + 1]);
+  } else {
+    float m = -INFINITY, l = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int e = 0; e < V; ++e) m = fmaxf(m, v[i][e]);
+    m = warp_max(m);
+    const float ref = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int e = 0; e < V; ++e) l += fast_exp2((v[i][e] - ref) * c);
+    st = make_float2(ref, log2f(warp_sum(l)));  // -inf: nothing to see
+  }
+  const bool empty = st.y == -INFINITY || tsum == 0.0f;
+  const float tlog = log2f(tsum), inv = 1.0f / tsum;
+  float loss = 0.0f;
+  for (int k = lane; k < a.K; k += 32) {
+    if (I[k] < 0 || empty) continue;
+    const float e = (P[k] - tref) * c, p = fast_exp2(e) * inv;
+    if (a.loss != nullptr && p != 0.0f) loss += p * ((e - tlog) - ((Elem<T>::to_f(s[I[k]]) - st.x) * c - st.y));
+    P[k] = p;
+  }
+  if (a.loss != nullptr) {
+    loss = warp_sum(loss) * kLn2;
+    if (lane == 0) {
+      a.loss[row] = empty ? 0.0f : loss;
+      if (a.stats != nullptr) {
+        a.stats[2 * row] = st.x;
+        a.stats[2 * row + 1] = st.y;
+      }
+    }
+  }
+  if (a.grad == nullptr) return;
+  T* grad = static_cast<T*>(a.grad) + row * a.grad_stride;
+  const float w = a.weight[row * a.weight_stride] * a.inv_tau;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int col = (32 * i + lane) * V;
+    float g[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) g[e] = col + e < seen && !empty ? w * fast_exp2((v[i][e] - st.x) * c - st.y) : 0.0f;
+    if (vec_out && col + V <= a.n) {
+      __stcs(reinterpret_cast<uint4*>(grad + col), pack16<T>(g));
+    } else {
+#pragma unroll
+      for (int e = 0; e < V; ++e)
+        if (col + e < a.n) grad[col + e] = Elem<T>::from_f(g[e]);
+    }
+  }
+  __syncwarp();
+  for (int k = lane; k < a.K; k += 32) {
+    const int j = I[k];
+    if (j < 0 || empty) continue;
+    float p = P[k];
+    if (twice) {
+      p = 0.0f;
+      for (int x = 0; x < a.K; ++x) p += I[x] == j ? P[x] : 0.0f;
+    }
+    grad[j] = Elem<T>::from_f(w * (fast_exp2((Elem<T>::to_f(s[j]) - st.x) * c - st.y) - p));
+  }
+}
+
+// ------------------------------------------------------------------ a CTA a row
+__device__ __forceinline__ float2 block_join(float2 v, float c, float2* red) {
+  v = warp_join(v, c);
   __syncthreads();
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
   __syncthreads();
   v = red[0];
-  for (int w = 1; w < kDistillThreads / 32; ++w) v = join(v, red[w]);
+  for (int w = 1; w < kDistillWarps; ++w) v = join(v, red[w], c);
   return v;
 }
 
+// Columns [0, n) of a row: the 16-byte aligned middle by vectors, f(first column, pointer); the rest one by one, g(column).
+template <typename T, typename F, typename G>
+__device__ __forceinline__ void over_row(const T* s, int n, F f, G g) {
+  constexpr int V = 16 / sizeof(T), U = 4;
+  const int head = min(n, static_cast<int>((16 - (reinterpret_cast<uintptr_t>(s) & 15)) % 16 / sizeof(T)));
+  const int vecs = (n - head) / V, rest = n - vecs * V;
+  int i = threadIdx.x;
+  for (; i + (U - 1) * kDistillThreads < vecs; i += U * kDistillThreads) {
+    uint4 x[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) x[u] = *reinterpret_cast<const uint4*>(s + head + (i + u * kDistillThreads) * V);
+#pragma unroll
+    for (int u = 0; u < U; ++u) f(head + (i + u * kDistillThreads) * V, x[u]);
+  }
+  for (; i < vecs; i += kDistillThreads) f(head + i * V, *reinterpret_cast<const uint4*>(s + head + i * V));
+  for (int e = threadIdx.x; e < rest; e += kDistillThreads) g(e < head ? e : vecs * V + e);
+}
+
 template <typename T>
-__global__ void __launch_bounds__(kDistillThreads) distill_kernel(const DistillArgs a) {
+__global__ void __launch_bounds__(kDistillThreads, 2) distill_kernel(const DistillArgs a) {
+  constexpr int V = 16 / sizeof(T);
   extern __shared__ float sm[];
   float* P = sm;                                  // [K] teacher weights
   int* I = reinterpret_cast<int*>(sm + a.K);      // [K] columns; -1: not used
-  __shared__ float2 red[kDistillThreads / 32];
+  __shared__ uint32_t bits[kDistillBits];
+  __shared__ float2 red[kDistillWarps];
   const int tid = threadIdx.x;
   const float c = a.inv_tau * kLog2e;
   for (int64_t row = blockIdx.x; row < a.R; row += gridDim.x) {
     const T* s = static_cast<const T*>(a.scores) + row * a.score_stride;
-    int seen = a.n;
-    if (a.visible != nullptr) {
-      seen = a.visible[row];
-      if ((seen < 0 || seen > a.n) && tid == 0) raise_status(a.status, SPRUCE_STATUS_BAD_LENGTH);
-      seen = min(max(seen, 0), a.n);
-    }
+    const int seen = row_seen(a, row, tid == 0);
     __syncthreads();
+    for (int b = tid; b < kDistillBits; b += kDistillThreads) bits[b] = 0;
+    __syncthreads();
+    float2 t = make_float2(-INFINITY, 0.0f);
+    bool mine = false;
     for (int k = tid; k < a.K; k += kDistillThreads) {
-      const int64_t id = a.ids64 ? static_cast<const int64_t*>(a.ids)[row * a.id_stride + k]
-                                 : static_cast<const int32_t*>(a.ids)[row * a.id_stride + k];
-      if (id >= seen) raise_status(a.status, SPRUCE_STATUS_BAD_INDEX);
-      const bool use = id >= 0 && id < seen;
-      I[k] = use ? static_cast<int>(id) : -1;
-      P[k] = use ? load_as_float(a.teacher, a.teacher_dtype, row * a.teacher_stride + k) : -INFINITY;
+      int column;
+      float logit;
+      row_entry(a, row, k, seen, column, logit);
+      I[k] = column;
+      P[k] = logit;
+      if (column < 0) continue;
+      t = join(t, make_float2(logit, logit == -INFINITY ? 0.0f : 1.0f), c);
+      if (a.grad != nullptr) mine = mine || (atomicOr(&bits[(column >> 5) % kDistillBits], 1u << (column & 31)) >> (column & 31) & 1);
     }
-    // Teacher: maximum and sum.
-    float m = -INFINITY, l = 0.0f;
-    for (int k = tid; k < a.K; k += kDistillThreads) m = fmaxf(m, P[k]);
-    float tm = block_join(m, 0.0f, red).x;
-    const float tref = tm == -INFINITY ? 0.0f : tm;
-    for (int k = tid; k < a.K; k += kDistillThreads) l += I[k] < 0 ? 0.0f : exp2f((P[k] - tref) * c);
-    const float tsum = block_join(0.0f, l, red).y;
-    // Student.
-    float2 st;
+    const bool twice = __syncthreads_or(mine);
+    t = block_join(t, c, red);
+    const float tref = t.x == -INFINITY ? 0.0f : t.x, tsum = t.y;
+    float2 st;  // maximum of the scores, log2 of the sum over it
     if (a.stats_in != nullptr) {
       st = make_float2(a.stats_in[2 * row], a.stats_in[2 * row + 1]);
     } else {
-      m = -INFINITY;
-      for (int j = tid; j < seen; j += kDistillThreads) m = fmaxf(m, Elem<T>::to_f(s[j]));
-      const float top = block_join(m, 0.0f, red).x, ref = top == -INFINITY ? 0.0f : top;
-      l = 0.0f;
-      for (int j = tid; j < seen; j += kDistillThreads) l += exp2f((Elem<T>::to_f(s[j]) - ref) * c);
-      const float sum = block_join(0.0f, l, red).y;
-      st = make_float2(ref, log2f(sum));  // -inf: nothing to see
+      float m = -INFINITY, l = 0.0f;
+      auto more = [&](float top) {  // the running maximum moves
+        if (top > m) {
+          l *= fast_exp2((m - top) * c);
+          m = top;
+        }
+      };
+      over_row<T>(s, seen,
+                  [&](int, const uint4& y) {
+                    float x[V];
+                    unpack16<T>(y, x);
+                    float top = x[0];
+#pragma unroll
+                    for (int e = 1; e < V; ++e) top = fmaxf(top, x[e]);
+                    more(top);
+                    const float ref = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+                    for (int e = 0; e < V; ++e) l += fast_exp2((x[e] - ref) * c);
+                  },
+                  [&](int j) {
+                    const float x = Elem<T>::to_f(s[j]);
+                    more(x);
+                    l += fast_exp2((x - (m == -INFINITY ? 0.0f : m)) * c);
+                  });
+      const float2 all = block_join(make_float2(m, l), c, red);
+      st = make_float2(all.x == -INFINITY ? 0.0f : all.x, log2f(all.y));
     }
     const bool empty = st.y == -INFINITY || tsum == 0.0f;
-    l = 0.0f;
+    const float tlog = log2f(tsum), inv = 1.0f / tsum;
+    float loss = 0.0f;
     for (int k = tid; k < a.K; k += kDistillThreads) {
       if (I[k] < 0 || empty) continue;
-      const float e = (P[k] - tref) * c, p = exp2f(e) / tsum;
-      if (a.loss != nullptr && p != 0.0f)
-        l += p * ((e - log2f(tsum)) - ((Elem<T>::to_f(s[I[k]]) - st.x) * c - st.y));
+      const float e = (P[k] - tref) * c, p = fast_exp2(e) * inv;
+      if (a.loss != nullptr && p != 0.0f) loss += p * ((e - tlog) - ((Elem<T>::to_f(s[I[k]]) - st.x) * c - st.y));
       P[k] = p;
     }
     if (a.loss != nullptr) {
-      const float loss = block_join(0.0f, l, red).y * kLn2;
+      loss = block_join(make_float2(0.0f, loss), c, red).y * kLn2;
       if (tid == 0) {
         a.loss[row] = empty ? 0.0f : loss;
         if (a.stats != nullptr) {
@@ -103,28 +307,72 @@ __global__ void __launch_bounds__(kDistillThreads) distill_kernel(const DistillA
     if (a.grad == nullptr) continue;
     T* grad = static_cast<T*>(a.grad) + row * a.grad_stride;
     const float w = a.weight[row * a.weight_stride] * a.inv_tau;
-    for (int j = tid; j < a.n; j += kDistillThreads)
-      grad[j] = Elem<T>::from_f(j < seen && !empty ? w * exp2f((Elem<T>::to_f(s[j]) - st.x) * c - st.y) : 0.0f);
+    const bool same = ((reinterpret_cast<uintptr_t>(s) ^ reinterpret_cast<uintptr_t>(grad)) & 15) == 0;
+    if (empty) {
+      for (int j = tid; j < a.n; j += kDistillThreads) grad[j] = Elem<T>::from_f(0.0f);
+      continue;
+    }
+    auto value = [&](float x) { return w * fast_exp2((x - st.x) * c - st.y); };
+    over_row<T>(s, seen,
+                [&](int j, const uint4& y) {
+                  float x[V];
+                  unpack16<T>(y, x);
+#pragma unroll
+                  for (int e = 0; e < V; ++e) x[e] = value(x[e]);
+                  if (same) {
+                    __stcs(reinterpret_cast<uint4*>(grad + j), pack16<T>(x));
+                  } else {
+#pragma unroll
+                    for (int e = 0; e < V; ++e) grad[j + e] = Elem<T>::from_f(x[e]);
+                  }
+                },
+                [&](int j) { grad[j] = Elem<T>::from_f(value(Elem<T>::to_f(s[j]))); });
+    for (int j = seen + tid; j < a.n; j += kDistillThreads) grad[j] = Elem<T>::from_f(0.0f);
     __syncthreads();
     for (int k = tid; k < a.K; k += kDistillThreads) {
       const int j = I[k];
-      if (j < 0 || empty) continue;
-      float p = 0.0f;
-      for (int x = 0; x < a.K; ++x) p += I[x] == j ? P[x] : 0.0f;
-      grad[j] = Elem<T>::from_f(w * (exp2f((Elem<T>::to_f(s[j]) - st.x) * c - st.y) - p));
+      if (j < 0) continue;
+      float p = P[k];
+      if (twice) {
+        p = 0.0f;
+        for (int x = 0; x < a.K; ++x) p += I[x] == j ? P[x] : 0.0f;
+      }
+      grad[j] = Elem<T>::from_f(w * (fast_exp2((Elem<T>::to_f(s[j]) - st.x) * c - st.y) - p));
     }
   }
 }
 
-cudaError_t launch_distill(const DistillArgs& a, int dtype, cudaStream_t stream) {
-  const int smem = a.K * 8;
-  const int G = static_cast<int>(std::min<int64_t>(a.R, 1 << 20));
-  switch (dtype) {
-    case SPRUCE_DTYPE_F32: distill_kernel<float><<<G, kDistillThreads, smem, stream>>>(a); break;
-    case SPRUCE_DTYPE_BF16: distill_kernel<__nv_bfloat16><<<G, kDistillThreads, smem, stream>>>(a); break;
-    default: distill_kernel<__half><<<G, kDistillThreads, smem, stream>>>(a); break;
-  }
+template <typename T>
+static cudaError_t launch_rows(const DistillArgs& a, cudaStream_t stream) {
+  constexpr int V = 16 / sizeof(T);
+  const int smem = kRowWarps * (2 * a.K + kRowBits) * 4;
+  const unsigned G = static_cast<unsigned>((a.R + kRowWarps - 1) / kRowWarps);
+  auto aligned = [](const void* p, int64_t stride) {
+    return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && stride % V == 0;
+  };
+  const bool in = aligned(a.scores, a.score_stride), out = a.grad != nullptr && aligned(a.grad, a.grad_stride);
+  const int vecs = (a.n + 32 * V - 1) / (32 * V);
+  if (vecs <= 1) distill_rows_kernel<T, 1><<<G, 32 * kRowWarps, smem, stream>>>(a, in, out);
+  else if (vecs <= 2) distill_rows_kernel<T, 2><<<G, 32 * kRowWarps, smem, stream>>>(a, in, out);
+  else if (vecs <= 4) distill_rows_kernel<T, 4><<<G, 32 * kRowWarps, smem, stream>>>(a, in, out);
+  else if (vecs <= 8) distill_rows_kernel<T, 8><<<G, 32 * kRowWarps, smem, stream>>>(a, in, out);
+  else distill_rows_kernel<T, 64 / V><<<G, 32 * kRowWarps, smem, stream>>>(a, in, out);
   return cudaGetLastError();
+}
+
+template <typename T>
+static cudaError_t launch(const DistillArgs& a, cudaStream_t stream) {
+  if (a.n <= kRowMost && a.K <= kRowEntries && a.R < (int64_t(1) << 33)) return launch_rows<T>(a, stream);
+  distill_kernel<T><<<static_cast<unsigned>(std::min<int64_t>(a.R, 1 << 20)), kDistillThreads, a.K * 8, stream>>>(a);
+  return cudaGetLastError();
+}
+
+cudaError_t launch_distill(const DistillArgs& a, int dtype, cudaStream_t stream) {
+  switch (dtype) {
+    case SPRUCE_DTYPE_F32: return launch<float>(a, stream);
+    case SPRUCE_DTYPE_BF16: return launch<__nv_bfloat16>(a, stream);
+    default: return launch<__half>(a, stream);
+  }
 }
 
 }  // namespace spruce
