@@ -15,8 +15,8 @@
 namespace spruce {
 
 constexpr int kDistillThreads = 512, kDistillWarps = kDistillThreads / 32;
-constexpr int kRowWarps = 8;            // rows of a CTA of the warp kernel
-constexpr int kRowMost = 2048, kRowEntries = 512;  // columns and teacher entries that it takes
+constexpr int kRowWarps = 4;            // rows of a CTA of the warp kernel
+constexpr int kRowMost = 2048, kRowEntries = 256;  // columns and teacher entries that it takes
 constexpr int kRowBits = 64, kDistillBits = 1024;  // words of the bitmaps; columns share bits modulo their size
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
@@ -56,14 +56,23 @@ __device__ __forceinline__ int row_seen(const DistillArgs& a, int64_t row, bool 
   if (report && (seen < 0 || seen > a.n)) raise_status(a.status, SPRUCE_STATUS_BAD_LENGTH);
   return min(max(seen, 0), a.n);
 }
-// A teacher entry: its column (-1: padding) and logit (-inf).
-__device__ __forceinline__ void row_entry(const DistillArgs& a, int64_t row, int k, int seen, int& column, float& logit) {
-  const int64_t id = a.ids64 ? static_cast<const int64_t*>(a.ids)[row * a.id_stride + k]
-                             : static_cast<const int32_t*>(a.ids)[row * a.id_stride + k];
-  if (id >= seen) raise_status(a.status, SPRUCE_STATUS_BAD_INDEX);
-  const bool use = id >= 0 && id < seen;
-  column = use ? static_cast<int>(id) : -1;
-  logit = use ? load_as_float(a.teacher, a.teacher_dtype, row * a.teacher_stride + k) : -INFINITY;
+// A teacher entry as it stands, and its column (-1: padding) and logit (-inf).
+struct Entry {
+  int64_t id;
+  float logit;
+};
+__device__ __forceinline__ Entry row_entry(const DistillArgs& a, int64_t row, int k) {
+  Entry e;
+  e.id = a.ids64 ? static_cast<const int64_t*>(a.ids)[row * a.id_stride + k]
+                 : static_cast<const int32_t*>(a.ids)[row * a.id_stride + k];
+  e.logit = load_as_float(a.teacher, a.teacher_dtype, row * a.teacher_stride + k);
+  return e;
+}
+__device__ __forceinline__ void use_entry(const DistillArgs& a, const Entry& e, int seen, int& column, float& logit) {
+  if (e.id >= seen) raise_status(a.status, SPRUCE_STATUS_BAD_INDEX);
+  const bool use = e.id >= 0 && e.id < seen;
+  column = use ? static_cast<int>(e.id) : -1;
+  logit = use ? e.logit : -INFINITY;
 }
 template <typename T>
 __device__ __forceinline__ void unpack16(const uint4& v, float (&x)[16 / sizeof(T)]) {
@@ -87,20 +96,28 @@ __global__ void __launch_bounds__(32 * kRowWarps) distill_rows_kernel(const Dist
   constexpr int V = 16 / sizeof(T);
   extern __shared__ float sm[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  float* P = sm + warp * (2 * a.K + kRowBits);     // [K] teacher weights
+  float* P = sm + warp * (3 * a.K + kRowBits);     // [K] teacher weights
   int* I = reinterpret_cast<int*>(P + a.K);        // [K] columns
-  uint32_t* bits = reinterpret_cast<uint32_t*>(I + a.K);
+  float* S = P + 2 * a.K;                          // [K] scores there
+  uint32_t* bits = reinterpret_cast<uint32_t*>(S + a.K);
   const int64_t row = (int64_t)blockIdx.x * kRowWarps + warp;
   if (row >= a.R) return;
   const float c = a.inv_tau * kLog2e;
   const T* s = static_cast<const T*>(a.scores) + row * a.score_stride;
+  // What does not hang on the visible columns is on its way first: the kernel is bound by the latency of its loads.
+  Entry early{-1, 0.0f};
+  if (lane < a.K) early = row_entry(a, row, lane);
+  float w = 0.0f;
+  if (a.grad != nullptr) w = a.weight[row * a.weight_stride] * a.inv_tau;
+  float2 st;
+  if (a.stats_in != nullptr) st = make_float2(a.stats_in[2 * row], a.stats_in[2 * row + 1]);
   const int seen = row_seen(a, row, lane == 0);
   float v[NV][V];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int col = (32 * i + lane) * V;
     if (vec_in && col + V <= seen) {
-      unpack16<T>(__ldcs(reinterpret_cast<const uint4*>(s + col)), v[i]);
+      unpack16<T>(*reinterpret_cast<const uint4*>(s + col), v[i]);
     } else {
 #pragma unroll
       for (int e = 0; e < V; ++e) v[i][e] = col + e < seen ? Elem<T>::to_f(s[col + e]) : -INFINITY;
@@ -114,9 +131,10 @@ __global__ void __launch_bounds__(32 * kRowWarps) distill_rows_kernel(const Dist
   for (int k = lane; k < a.K; k += 32) {
     int column;
     float logit;
-    row_entry(a, row, k, seen, column, logit);
+    use_entry(a, k < 32 ? early : row_entry(a, row, k), seen, column, logit);
     I[k] = column;
     P[k] = logit;
+    S[k] = column < 0 ? 0.0f : Elem<T>::to_f(s[column]);
     tm = fmaxf(tm, logit);
     if (a.grad != nullptr && column >= 0)
       twice = twice || (atomicOr(&bits[(column >> 5) % kRowBits], 1u << (column & 31)) >> (column & 31) & 1);
@@ -128,10 +146,7 @@ __global__ void __launch_bounds__(32 * kRowWarps) distill_rows_kernel(const Dist
   for (int k = lane; k < a.K; k += 32) tsum += I[k] < 0 ? 0.0f : fast_exp2((P[k] - tref) * c);
   tsum = warp_sum(tsum);
   // Student.
-  float2 st;
-  if (a.stats_in != nullptr) {
-    st = make_float2(a.stats_in[2 * row], a.stats_in[2 * row + 1]);
-  } else {
+  if (a.stats_in == nullptr) {
     float m = -INFINITY, l = 0.0f;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
@@ -151,7 +166,7 @@ __global__ void __launch_bounds__(32 * kRowWarps) distill_rows_kernel(const Dist
   for (int k = lane; k < a.K; k += 32) {
     if (I[k] < 0 || empty) continue;
     const float e = (P[k] - tref) * c, p = fast_exp2(e) * inv;
-    if (a.loss != nullptr && p != 0.0f) loss += p * ((e - tlog) - ((Elem<T>::to_f(s[I[k]]) - st.x) * c - st.y));
+    if (a.loss != nullptr && p != 0.0f) loss += p * ((e - tlog) - ((S[k] - st.x) * c - st.y));
     P[k] = p;
   }
   if (a.loss != nullptr) {
@@ -166,7 +181,6 @@ __global__ void __launch_bounds__(32 * kRowWarps) distill_rows_kernel(const Dist
   }
   if (a.grad == nullptr) return;
   T* grad = static_cast<T*>(a.grad) + row * a.grad_stride;
-  const float w = a.weight[row * a.weight_stride] * a.inv_tau;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int col = (32 * i + lane) * V;
@@ -190,7 +204,7 @@ __global__ void __launch_bounds__(32 * kRowWarps) distill_rows_kernel(const Dist
       p = 0.0f;
       for (int x = 0; x < a.K; ++x) p += I[x] == j ? P[x] : 0.0f;
     }
-    grad[j] = Elem<T>::from_f(w * (fast_exp2((Elem<T>::to_f(s[j]) - st.x) * c - st.y) - p));
+    grad[j] = Elem<T>::from_f(w * (fast_exp2((S[k] - st.x) * c - st.y) - p));
   }
 }
 
@@ -223,8 +237,9 @@ __device__ __forceinline__ void over_row(const T* s, int n, F f, G g) {
   for (int e = threadIdx.x; e < rest; e += kDistillThreads) g(e < head ? e : vecs * V + e);
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kDistillThreads, 2) distill_kernel(const DistillArgs a) {
+// CTAS an SM: two with the gradient, four without.
+template <typename T, int CTAS>
+__global__ void __launch_bounds__(kDistillThreads, CTAS) distill_kernel(const DistillArgs a) {
   constexpr int V = 16 / sizeof(T);
   extern __shared__ float sm[];
   float* P = sm;                                  // [K] teacher weights
@@ -244,7 +259,7 @@ __global__ void __launch_bounds__(kDistillThreads, 2) distill_kernel(const Disti
     for (int k = tid; k < a.K; k += kDistillThreads) {
       int column;
       float logit;
-      row_entry(a, row, k, seen, column, logit);
+      use_entry(a, row_entry(a, row, k), seen, column, logit);
       I[k] = column;
       P[k] = logit;
       if (column < 0) continue;
@@ -345,7 +360,7 @@ __global__ void __launch_bounds__(kDistillThreads, 2) distill_kernel(const Disti
 template <typename T>
 static cudaError_t launch_rows(const DistillArgs& a, cudaStream_t stream) {
   constexpr int V = 16 / sizeof(T);
-  const int smem = kRowWarps * (2 * a.K + kRowBits) * 4;
+  const int smem = kRowWarps * (3 * a.K + kRowBits) * 4;
   const unsigned G = static_cast<unsigned>((a.R + kRowWarps - 1) / kRowWarps);
   auto aligned = [](const void* p, int64_t stride) {
     return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && stride % V == 0;
@@ -363,7 +378,11 @@ static cudaError_t launch_rows(const DistillArgs& a, cudaStream_t stream) {
 template <typename T>
 static cudaError_t launch(const DistillArgs& a, cudaStream_t stream) {
   if (a.n <= kRowMost && a.K <= kRowEntries && a.R < (int64_t(1) << 33)) return launch_rows<T>(a, stream);
-  distill_kernel<T><<<static_cast<unsigned>(std::min<int64_t>(a.R, 1 << 20)), kDistillThreads, a.K * 8, stream>>>(a);
+  const unsigned G = static_cast<unsigned>(std::min<int64_t>(a.R, 1 << 20));
+  if (a.grad == nullptr)
+    distill_kernel<T, 4><<<G, kDistillThreads, a.K * 8, stream>>>(a);
+  else
+    distill_kernel<T, 2><<<G, kDistillThreads, a.K * 8, stream>>>(a);
   return cudaGetLastError();
 }
 
