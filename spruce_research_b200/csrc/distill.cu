@@ -15,7 +15,7 @@
 namespace spruce {
 
 constexpr int kDistillThreads = 512, kDistillWarps = kDistillThreads / 32;
-constexpr int kRowWarps = 4;            // rows of a CTA of the warp kernel
+constexpr int kRowWarps = 2;            // rows of a CTA of the warp kernel
 constexpr int kRowMost = 2048, kRowEntries = 256;  // columns and teacher entries that it takes
 constexpr int kRowBits = 64, kDistillBits = 1024;  // words of the bitmaps; columns share bits modulo their size
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;

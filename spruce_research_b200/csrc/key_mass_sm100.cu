@@ -30,9 +30,9 @@ struct KeyMassLayout {
   static constexpr int TILE = NP * PANEL;
   static constexpr int OFF_K = 0;                       // [2 items][2 tiles]
   static constexpr int OFF_Q = OFF_K + 4 * TILE;
-  static constexpr int OFF_ROW = OFF_Q + QST * TILE;    // [LST]: 128 lse, 128 limits
-  static constexpr int OFF_SUM = OFF_ROW + LST * 1024;  // [2][256] sums handed over
-  static constexpr int OFF_PART = OFF_SUM + 2 * 1024;   // [8 CTAs][256] sums of a cluster
+  static constexpr int OFF_ROW = OFF_Q + QST * TILE;    // [LST]: 128 times -lse, 128 limits
+  static constexpr int OFF_SUM = OFF_ROW + LST * 1024;  // [4][256] sums handed over
+  static constexpr int OFF_PART = OFF_SUM + 4 * 1024;   // [8 CTAs][256] sums of a cluster
   static constexpr int OFF_BAR = OFF_PART + 8 * 1024;
   // k_full[2], k_empty[2], q_full[], q_empty[], l_full[], l_empty[], s_full[4], s_empty[4], drain
   static constexpr int NBAR = 4 + 2 * QST + 2 * LST + 8 + 1;
@@ -48,23 +48,42 @@ struct KeyMassItem {
   int tok0, steps;  // first token of this CTA's rows, and its row tiles
 };
 
-// The item at `at` of all; false where there is nothing to write.
-__device__ __forceinline__ bool key_mass_item(const KeyMassParams& p, int64_t at, int ntok, int rank, int parts, KeyMassItem& x) {
-  const int per = p.key_tiles * p.v.a.Hkv;
-  x.s = static_cast<int>(at / per);
-  const int rest = static_cast<int>(at % per);
-  x.g = rest % p.v.a.Hkv;
-  x.key0 = rest / p.v.a.Hkv * kKmKeys;
-  x.q = paged_seq(p.v, x.s);
-  x.keys = mass_keys(x.q);
-  if (x.q.qlen == 0 || x.key0 >= x.keys) return false;
-  // Tokens before the item's first key do not see it.
-  const int lo = min(max(x.key0 - x.q.first, 0), x.q.qlen);
-  const int tiles = (x.q.qlen - lo + ntok - 1) / ntok, each = (tiles + parts - 1) / parts;
-  x.tok0 = lo + rank * each * ntok;
-  x.steps = max(0, min(each, tiles - rank * each));
-  return true;
-}
+// Walks a CTA's items: those of its number, and every `stride` further.
+struct KeyMassWalk {
+  int s, rest, per, ds, dr;  // sequence, item in it, items of a sequence; the step
+  __device__ __forceinline__ KeyMassWalk(const KeyMassParams& p, int first, int stride) {
+    per = p.key_tiles * p.v.a.Hkv;
+    s = first / per;
+    rest = first - s * per;
+    ds = stride / per;
+    dr = stride - ds * per;
+  }
+  __device__ __forceinline__ bool more(const KeyMassParams& p) const { return s < p.v.a.S; }
+  __device__ __forceinline__ void next() {
+    s += ds;
+    rest += dr;
+    if (rest >= per) {
+      rest -= per;
+      ++s;
+    }
+  }
+  // False where there is nothing to write.
+  __device__ __forceinline__ bool item(const KeyMassParams& p, int ntok, int rank, int parts, KeyMassItem& x) const {
+    x.s = s;
+    const int tile = rest / p.v.a.Hkv;
+    x.g = rest - tile * p.v.a.Hkv;
+    x.key0 = tile * kKmKeys;
+    x.q = paged_seq(p.v, s);
+    x.keys = mass_keys(x.q);
+    if (x.q.qlen == 0 || x.key0 >= x.keys) return false;
+    // Tokens before the item's first key do not see it.
+    const int lo = min(max(x.key0 - x.q.first, 0), x.q.qlen);
+    const int tiles = (x.q.qlen - lo + ntok - 1) / ntok, each = (tiles + parts - 1) / parts;
+    x.tok0 = lo + rank * each * ntok;
+    x.steps = max(0, min(each, tiles - rank * each));
+    return true;
+  }
+};
 
 // All threads of the cluster's CTAs.
 __device__ __forceinline__ void cluster_sync() {
@@ -74,7 +93,7 @@ __device__ __forceinline__ void cluster_sync() {
 template <typename T, int D>
 __global__ void __launch_bounds__(kKmThreads, 1)
     key_mass_sm100_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ CUtensorMap tmk,
-                          const __grid_constant__ KeyMassParams p, int box, int ntok, int parts, int64_t items) {
+                          const __grid_constant__ KeyMassParams p, int box, int ntok, int parts) {
   using L = KeyMassLayout<D>;
   constexpr int QST = L::QST, LST = L::LST;
   extern __shared__ uint8_t smem_raw[];
@@ -93,7 +112,7 @@ __global__ void __launch_bounds__(kKmThreads, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::OFF_MISC);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::OFF_MISC + 4);
   const int rank = blockIdx.x % parts;
-  const int64_t first = blockIdx.x / parts, stride = gridDim.x / parts;
+  const int first = blockIdx.x / parts, stride = gridDim.x / parts;
   const int rows = ntok * p.v.rep;     // of a row tile that a box fills
 
   if (warp == kKmLoad) {
@@ -137,33 +156,47 @@ __global__ void __launch_bounds__(kKmThreads, 1)
     // ------------------------------------------------------------ K and Q
     const bool leader = elect_one();
     const int boxes = kKmKeys / box;  // at most 16
-    int kb = 0, kn = 0, st = 0, qn = 0;
+    int kn = 0, st = 0, qn = 0;
     bool ok = true;
-    for (int64_t at = first; ok && at < items; at += stride) {
-      if (!key_mass_item(p, at, ntok, rank, parts, x) || x.steps == 0) continue;
-      const int32_t* table = p.v.a.block_table + x.s * p.v.a.table_stride;
-      const int key = x.key0 + lane * box;
-      int page = static_cast<int>(p.v.a.num_pages);  // reads zeros
-      if (lane < boxes && key < x.keys) {
-        page = paged_page(p.v, table, key / p.v.a.page_size);
-        if (page < 0) page = static_cast<int>(p.v.a.num_pages);
-      }
-      if (kn >= 2 && !(ok = __all_sync(0xffffffffu, mbar_wait(&k_empty[kb], ((kn >> 1) - 1) & 1, status, abort_flag)))) break;
-      if (leader) mbar_arrive_expect_tx(&k_full[kb], 2 * L::TILE);
-      __syncwarp();
-      for (int b = 0; b < boxes; ++b) {
-        const int pb = __shfl_sync(0xffffffffu, page, b);
-        const int r = b * box;  // of the item's keys
-        if (leader)
-#pragma unroll
-          for (int pp = 0; pp < L::NP; ++pp)
-            tma_load_4d(smem + L::OFF_K + (2 * kb + (r >> 7)) * L::TILE + pp * L::PANEL + (r & 127) * 128, &tmk, &k_full[kb],
-                        pp * 64, (x.key0 + r) % p.v.a.page_size, x.g, pb);
+    KeyMassItem y;
+    // The keys of the next item that has some; called an item ahead of its rows, so that they are there in time.
+    auto load_keys = [&](KeyMassWalk& w) {
+      for (; w.more(p); w.next()) {
+        if (!w.item(p, ntok, rank, parts, y) || y.steps == 0) continue;
+        const int key = y.key0 + lane * box;
+        int page = static_cast<int>(p.v.a.num_pages);  // reads zeros
+        if (lane < boxes && key < y.keys) {
+          page = paged_page(p.v, p.v.a.block_table + y.s * p.v.a.table_stride, key / p.v.a.page_size);
+          if (page < 0) page = static_cast<int>(p.v.a.num_pages);
+        }
+        const int kb = kn & 1;
+        if (kn >= 2 && !(ok = __all_sync(0xffffffffu, mbar_wait(&k_empty[kb], ((kn >> 1) - 1) & 1, status, abort_flag)))) return;
+        if (leader) mbar_arrive_expect_tx(&k_full[kb], 2 * L::TILE);
         __syncwarp();
+        int row = y.key0 % p.v.a.page_size;  // of the next box in its page
+        for (int b = 0; b < boxes; ++b) {
+          const int pb = __shfl_sync(0xffffffffu, page, b);
+          const int r = b * box;  // of the item's keys
+          if (leader)
+#pragma unroll
+            for (int pp = 0; pp < L::NP; ++pp)
+              tma_load_4d(smem + L::OFF_K + (2 * kb + (r >> 7)) * L::TILE + pp * L::PANEL + (r & 127) * 128, &tmk, &k_full[kb],
+                          pp * 64, row, y.g, pb);
+          __syncwarp();
+          row += box;
+          if (row == p.v.a.page_size) row = 0;
+        }
+        ++kn;
+        w.next();
+        return;
       }
-      kb ^= 1;
-      ++kn;
-      for (int i = 0; i < x.steps; ++i) {
+    };
+    KeyMassWalk ahead(p, first, stride);
+    load_keys(ahead);
+    for (KeyMassWalk at(p, first, stride); ok && at.more(p); at.next()) {
+      if (!at.item(p, ntok, rank, parts, x) || x.steps == 0) continue;
+      load_keys(ahead);
+      for (int i = 0; ok && i < x.steps; ++i) {
         if (qn >= QST && !(ok = __all_sync(0xffffffffu, mbar_wait(&q_empty[st], ((qn / QST) - 1) & 1, status, abort_flag)))) break;
         if (leader) {
           mbar_arrive_expect_tx(&q_full[st], L::NP * rows * 128);
@@ -185,8 +218,8 @@ __global__ void __launch_bounds__(kKmThreads, 1)
     // ------------------------------------------------------------ lse and limits of the rows
     int ln = 0;
     bool ok = true;
-    for (int64_t at = first; ok && at < items; at += stride) {
-      if (!key_mass_item(p, at, ntok, rank, parts, x)) continue;
+    for (KeyMassWalk at(p, first, stride); ok && at.more(p); at.next()) {
+      if (!at.item(p, ntok, rank, parts, x)) continue;
       for (int i = 0; i < x.steps; ++i, ++ln) {
         const int st = ln % LST, tok = x.tok0 + i * ntok;
         float v[4];
@@ -206,7 +239,7 @@ __global__ void __launch_bounds__(kKmThreads, 1)
         float* dst = reinterpret_cast<float*>(smem + L::OFF_ROW + st * 1024);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          dst[lane + 32 * k] = v[k];
+          dst[lane + 32 * k] = -v[k];
           reinterpret_cast<int*>(dst)[128 + lane + 32 * k] = lim[k];
         }
         mbar_arrive(&l_full[st]);
@@ -227,8 +260,8 @@ __global__ void __launch_bounds__(kKmThreads, 1)
     };
     int kn = 0, qn = 0;
     bool ok = true;
-    for (int64_t at = first; ok && at < items; at += stride) {
-      if (!key_mass_item(p, at, ntok, rank, parts, x) || x.steps == 0) continue;
+    for (KeyMassWalk at(p, first, stride); ok && at.more(p); at.next()) {
+      if (!at.item(p, ntok, rank, parts, x) || x.steps == 0) continue;
       if (!(ok = wait(&k_full[kn & 1], (kn >> 1) & 1))) break;
       for (int i = 0; i < x.steps; ++i, ++qn) {
         const int st = qn % QST;
@@ -271,26 +304,35 @@ __global__ void __launch_bounds__(kKmThreads, 1)
     int qn = 0, done = 0;
     bool ok = true;
     // After a wait that ran out the warps still meet at the barriers.
-    for (int64_t at = first; at < items; at += stride) {
-      if (!key_mass_item(p, at, ntok, rank, parts, x)) continue;
+    for (KeyMassWalk at(p, first, stride); at.more(p); at.next()) {
+      if (!at.item(p, ntok, rank, parts, x)) continue;
       // Where the sum goes, and the old weight, fetched while the rows stream by.
-      int page = -1;
+      float* dst = nullptr;
       float old = 0.0f;
-      const int pos = x.key0 + key, slot = pos % p.v.a.page_size;
+      const int pos = x.key0 + key;
       if (half == 0 && rank == 0 && pos < x.keys) {
-        page = paged_page(p.v, p.v.a.block_table + x.s * p.v.a.table_stride, pos / p.v.a.page_size);
-        if (page >= 0 && pos < x.q.first && p.decay != 0.0f)
-          old = p.decay * p.mass[page * p.ms[0] + x.g * p.ms[1] + slot * p.ms[2]];
+        const int pi = pos / p.v.a.page_size, slot = pos - pi * p.v.a.page_size;
+        const int page = paged_page(p.v, p.v.a.block_table + x.s * p.v.a.table_stride, pi);
+        if (page >= 0) {
+          dst = p.out + page * p.os[0] + x.g * p.os[1] + slot * p.os[2];
+          if (pos < x.q.first && p.decay != 0.0f) old = p.decay * p.mass[page * p.ms[0] + x.g * p.ms[1] + slot * p.ms[2]];
+        }
       }
+      const int steps = x.steps;
+      // Row tiles [open0, open1): all tokens are the sequence's and see all the item's keys.
+      const int open0 = (max(0, x.key0 + kKmKeys - 1 - x.q.first - x.tok0) + ntok - 1) / ntok;
+      const int open1 = (x.q.qlen - x.tok0) / ntok;
+      const int left = (x.q.qlen - x.tok0) * p.v.rep - half * 64;  // rows from this half of the first tile on
       uint64_t sum2[2] = {f2_pack(0.0f, 0.0f), f2_pack(0.0f, 0.0f)};
-      auto rows_of = [&](const float (&s)[64], const float* lse, auto masked_c) {
+      // Sixteen rows; those of the other tiles have limits.
+      auto rows_of = [&](const float* s, const float* lse, auto masked_c) {
         constexpr bool masked = decltype(masked_c)::value;
 #pragma unroll
-        for (int k = 0; k < 16; ++k) {
+        for (int k = 0; k < 4; ++k) {
           const float4 v = *reinterpret_cast<const float4*>(lse + 4 * k);
           float x0, x1, x2, x3;
-          f2_unpack(f2_fma(f2_pack(s[4 * k], s[4 * k + 1]), sl2x2, f2_pack(-v.x, -v.y)), x0, x1);
-          f2_unpack(f2_fma(f2_pack(s[4 * k + 2], s[4 * k + 3]), sl2x2, f2_pack(-v.z, -v.w)), x2, x3);
+          f2_unpack(f2_fma(f2_pack(s[4 * k], s[4 * k + 1]), sl2x2, f2_pack(v.x, v.y)), x0, x1);
+          f2_unpack(f2_fma(f2_pack(s[4 * k + 2], s[4 * k + 3]), sl2x2, f2_pack(v.z, v.w)), x2, x3);
           float e0 = fast_exp2(x0), e1 = fast_exp2(x1), e2 = fast_exp2(x2), e3 = fast_exp2(x3);
           if constexpr (masked) {
             const int4 lim = *reinterpret_cast<const int4*>(lse + 128 + 4 * k);
@@ -303,24 +345,32 @@ __global__ void __launch_bounds__(kKmThreads, 1)
           sum2[1] = f2_add(sum2[1], f2_pack(e2, e3));
         }
       };
-      for (int i = 0; ok && i < x.steps; ++i, ++qn) {
+      for (int i = 0; ok && i < steps; ++i, ++qn) {
         const uint32_t buf = qn & 1;
         ok = __all_sync(0xffffffffu, mbar_wait(&l_full[qn % LST], (qn / LST) & 1, status, abort_flag) &&
                                          mbar_wait(&s_full[2 * t + buf], (qn >> 1) & 1, status, abort_flag));
         if (!ok) break;
         tc_fence_after();
-        float s[64];
-        tmem_ld32(tS + buf * 128, *reinterpret_cast<float(*)[32]>(s));
-        tmem_ld32(tS + buf * 128 + 32, *reinterpret_cast<float(*)[32]>(s + 32));
-        tmem_wait_ld();
-        tc_fence_before();
-        mbar_arrive(&s_empty[2 * t + buf]);
         const float* lse = reinterpret_cast<const float*>(smem + L::OFF_ROW + (qn % LST) * 1024) + half * 64;
-        // All tokens of the tile are the sequence's and see all the item's keys, or its rows have limits.
-        if (x.q.first + x.tok0 + i * ntok >= x.key0 + kKmKeys - 1 && x.tok0 + (i + 1) * ntok <= x.q.qlen)
-          rows_of(s, lse, std::false_type{});
-        else
-          rows_of(s, lse, std::true_type{});
+        const int there = min(left - i * rows, rows - half * 64);  // rows of this half
+        const bool open = i >= open0 && i < open1;
+#pragma unroll
+        for (int r = 0; r < 64; r += 32) {  // 64 scores at once would not fit the registers of five warps a scheduler
+          float s[32];
+          tmem_ld32(tS + buf * 128 + r, s);
+          tmem_wait_ld();
+          if (r == 32) {
+            tc_fence_before();
+            mbar_arrive(&s_empty[2 * t + buf]);
+          }
+          if (open) {
+            rows_of(s, lse + r, std::false_type{});
+            rows_of(s + 16, lse + r + 16, std::false_type{});
+          } else {
+            if (r < there) rows_of(s, lse + r, std::true_type{});
+            if (r + 16 < there) rows_of(s + 16, lse + r + 16, std::true_type{});
+          }
+        }
         __syncwarp();
         if (lane == 0) mbar_arrive(&l_empty[qn % LST]);
       }
@@ -328,12 +378,20 @@ __global__ void __launch_bounds__(kKmThreads, 1)
       f2_unpack(sum2[0], a0, a1);
       f2_unpack(sum2[1], a2, a3);
       float sum = (a0 + a1) + (a2 + a3);
-      // Two buffers: what is handed over now is read before the barrier of the item after the next.
-      float* const mine = given + (done & 1) * 256;
-      if (half == 1) mine[key] = sum;
-      named_barrier_sync(1 + t, 256);
-      if (half == 0) sum += mine[key];
-      float* const dst = page >= 0 ? p.out + page * p.os[0] + x.g * p.os[1] + slot * p.os[2] : nullptr;
+      // The second half hands its sum over and goes on.  It is never four items ahead: the scores of a step wait for both halves to
+      // have taken those two steps before, and where an item has no step it waits itself.
+      float* const mine = given + (done & 3) * 256;
+      const uint32_t bar = 1 + t * 4 + (done & 3);
+      if (half == 1) {
+        mine[key] = sum;
+        if (steps > 0 && ok)
+          asm volatile("bar.arrive %0, 256;" ::"r"(bar) : "memory");
+        else
+          named_barrier_sync(bar, 256);
+      } else {
+        named_barrier_sync(bar, 256);
+        sum += mine[key];
+      }
       if (parts == 1) {
         if (dst != nullptr) *dst = sum + old;
       } else if (half == 0) {  // the only item: to the cluster's first CTA
@@ -396,6 +454,7 @@ static cudaError_t launch_rows(const KeyMassArgs& a, int dtype, cudaStream_t str
   if (e != cudaSuccess) return e;
   const KeyMassParams p = key_mass_params(a, kKmKeys);
   const int64_t items = (int64_t)a.a.S * p.key_tiles * a.a.Hkv;
+  if ((int64_t)p.key_tiles * a.a.Hkv > (1 << 30)) return cudaErrorInvalidValue;
   const int sms = sm_count();
   // CTAs of an item: as many as leave one item each, and a row tile each of the longest sequence allowed.
   int parts = 1;
@@ -411,7 +470,7 @@ static cudaError_t launch_rows(const KeyMassArgs& a, int dtype, cudaStream_t str
   cfg.stream = stream;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kern, mq, mk, p, box, ntok, parts, items);
+  return cudaLaunchKernelEx(&cfg, kern, mq, mk, p, box, ntok, parts);
 }
 
 cudaError_t launch_key_mass_sm100(const KeyMassArgs& a, int dtype, cudaStream_t stream) {
