@@ -7,8 +7,10 @@
 // tokens as fit 128 rows, each a TMA box of (token, head of the group) rows.  Items go to the CTAs round robin; where a
 // cluster of CTAs can be had for each, it shares the item's rows and its first CTA adds the sums up in their order.
 //
-// Warps: 0-3 the first 64 rows of tile 0 (thread = key = TMEM lane), 4-7 the others, 8-15 likewise of tile 1, 16 issues the
-// MMAs and owns TMEM, 17 loads K (an item ahead) and Q, 18 brings the rows' lse and limits.  Each S^T_t has two buffers.
+// Warps: 0-3 the first 64 rows of tile 0 (thread = key = TMEM lane), 4-7 the others, 8-15 likewise of tile 1, 16 and 17 issue
+// the MMAs of a tile each (a check of a barrier waits behind the MMAs that its warp has queued: one warp's checks would leave the
+// tensor core idle), 16 owns TMEM, 18 loads K (an item ahead) and Q, 19 works the items out and brings the rows' lse and limits.  Each S^T_t has two
+// buffers.
 //
 // Every wait is bounded (common.cuh).
 #include <algorithm>
@@ -19,7 +21,7 @@
 
 namespace spruce {
 
-constexpr int kKmThreads = 608, kKmMma = 16, kKmLoad = 17, kKmLse = 18;
+constexpr int kKmThreads = 640, kKmMma = 16, kKmMma1 = 17, kKmLoad = 18, kKmLse = 19;
 constexpr int kKmKeys = 256;
 
 template <int D>
@@ -32,10 +34,12 @@ struct KeyMassLayout {
   static constexpr int OFF_Q = OFF_K + 4 * TILE;
   static constexpr int OFF_ROW = OFF_Q + QST * TILE;    // [LST]: 128 times -lse, 128 limits
   static constexpr int OFF_SUM = OFF_ROW + LST * 1024;  // [4][256] sums handed over
-  static constexpr int OFF_PART = OFF_SUM + 4 * 1024;   // [8 CTAs][256] sums of a cluster
+  static constexpr int OFF_ITEM = OFF_SUM + 4 * 1024;   // [4] what the softmax warps need of an item
+  static constexpr int OFF_PART = OFF_ITEM + 4 * 64;   // [8 CTAs][256] sums of a cluster
   static constexpr int OFF_BAR = OFF_PART + 8 * 1024;
-  // k_full[2], k_empty[2], q_full[], q_empty[], l_full[], l_empty[], s_full[4], s_empty[4], drain
-  static constexpr int NBAR = 4 + 2 * QST + 2 * LST + 8 + 1;
+  // k_full[2], k_empty[2], q_full[], q_empty[], l_full[], l_empty[], s_full[4], s_empty[4], drain[2], i_full[4], i_empty[4],
+  // g_full[2][4]
+  static constexpr int NBAR = 4 + 2 * QST + 2 * LST + 8 + 2 + 8 + 8;
   static constexpr int OFF_MISC = OFF_BAR + NBAR * 8;
   static constexpr int BYTES = 1024 + OFF_MISC + 16;
   static_assert(BYTES <= 227 * 1024, "shared memory of a CTA");
@@ -47,6 +51,14 @@ struct KeyMassItem {
   int s, g, key0, keys;  // keys: of the sequence, that its new tokens see
   int tok0, steps;  // first token of this CTA's rows, and its row tiles
 };
+
+// An item as the softmax warps take it; steps < 0 after the last.
+struct KeyMassTask {
+  int s, g, key0, keys, first, steps;
+  int open0, open1;  // row tiles whose tokens are all the sequence's and see all the item's keys
+  int left;          // query rows from this CTA's first on
+};
+static_assert(sizeof(KeyMassTask) <= 64, "fits its slot");
 
 // Walks a CTA's items: those of its number, and every `stride` further.
 struct KeyMassWalk {
@@ -101,14 +113,17 @@ __global__ void __launch_bounds__(kKmThreads, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint32_t* const status = p.v.a.status;
   uint64_t* k_full = reinterpret_cast<uint64_t*>(smem + L::OFF_BAR);
-  uint64_t* k_empty = k_full + 2;
+  uint64_t* k_empty = k_full + 2;      // 2 arrivals: a tile's MMAs each
   uint64_t* q_full = k_empty + 2;
-  uint64_t* q_empty = q_full + QST;
+  uint64_t* q_empty = q_full + QST;    // likewise
   uint64_t* l_full = q_empty + QST;    // 32 arrivals
   uint64_t* l_empty = l_full + LST;    // 16: a lane of each softmax warp
   uint64_t* s_full = l_empty + LST;    // [tile * 2 + buffer]
   uint64_t* s_empty = s_full + 4;      // 256 arrivals
-  uint64_t* drain = s_empty + 4;
+  uint64_t* drain = s_empty + 4;       // [tile]
+  uint64_t* i_full = drain + 2;
+  uint64_t* i_empty = i_full + 4;      // 16: a lane of each softmax warp
+  uint64_t* g_full = i_empty + 4;      // [tile * 4 + item % 4], 128 arrivals: the second half's sums are there
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::OFF_MISC);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::OFF_MISC + 4);
   const int rank = blockIdx.x % parts;
@@ -118,7 +133,15 @@ __global__ void __launch_bounds__(kKmThreads, 1)
   if (warp == kKmLoad) {
     if (lane == 0) {
       *abort_flag = 0;
-      for (int i = 0; i < 4 + 2 * QST; ++i) mbar_init(&k_full[i], 1);  // and k_empty, q_full, q_empty
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(&k_full[i], 1);
+        mbar_init(&k_empty[i], 2);
+        mbar_init(&drain[i], 1);
+      }
+      for (int i = 0; i < QST; ++i) {
+        mbar_init(&q_full[i], 1);
+        mbar_init(&q_empty[i], 2);
+      }
       for (int i = 0; i < LST; ++i) {
         mbar_init(&l_full[i], 32);
         mbar_init(&l_empty[i], 16);
@@ -126,8 +149,11 @@ __global__ void __launch_bounds__(kKmThreads, 1)
       for (int i = 0; i < 4; ++i) {
         mbar_init(&s_full[i], 1);
         mbar_init(&s_empty[i], 256);
+        mbar_init(&i_full[i], 1);
+        mbar_init(&i_empty[i], 16);
+        mbar_init(&g_full[i], 128);
+        mbar_init(&g_full[4 + i], 128);
       }
-      mbar_init(drain, 1);
       fence_barrier_init();
       prefetch_tmap(&tmq);
       prefetch_tmap(&tmk);
@@ -195,7 +221,6 @@ __global__ void __launch_bounds__(kKmThreads, 1)
     load_keys(ahead);
     for (KeyMassWalk at(p, first, stride); ok && at.more(p); at.next()) {
       if (!at.item(p, ntok, rank, parts, x) || x.steps == 0) continue;
-      load_keys(ahead);
       for (int i = 0; ok && i < x.steps; ++i) {
         if (qn >= QST && !(ok = __all_sync(0xffffffffu, mbar_wait(&q_empty[st], ((qn / QST) - 1) & 1, status, abort_flag)))) break;
         if (leader) {
@@ -208,6 +233,9 @@ __global__ void __launch_bounds__(kKmThreads, 1)
         __syncwarp();
         ++qn;
         if (++st == QST) st = 0;
+        // The next item's keys, whose place the last item leaves: after the rows that this item starts with, or the tensor core
+        // would wait for those at every item.
+        if (i == min(QST, x.steps) - 1) load_keys(ahead);
       }
     }
     // No copy may be in flight when the CTA exits.
@@ -216,11 +244,31 @@ __global__ void __launch_bounds__(kKmThreads, 1)
     __syncwarp();
   } else if (warp == kKmLse) {
     // ------------------------------------------------------------ lse and limits of the rows
-    int ln = 0;
+    int ln = 0, in = 0;
     bool ok = true;
+    auto tell = [&](const KeyMassTask& y) {
+      if (in >= 4 && !(ok = __all_sync(0xffffffffu, mbar_wait(&i_empty[in & 3], ((in >> 2) - 1) & 1, status, abort_flag)))) return;
+      if (lane == 0) {
+        *reinterpret_cast<KeyMassTask*>(smem + L::OFF_ITEM + (in & 3) * 64) = y;
+        mbar_arrive(&i_full[in & 3]);
+      }
+      __syncwarp();
+      ++in;
+    };
+    KeyMassTask y{};
     for (KeyMassWalk at(p, first, stride); ok && at.more(p); at.next()) {
       if (!at.item(p, ntok, rank, parts, x)) continue;
-      for (int i = 0; i < x.steps; ++i, ++ln) {
+      y.s = x.s;
+      y.g = x.g;
+      y.key0 = x.key0;
+      y.keys = x.keys;
+      y.first = x.q.first;
+      y.steps = x.steps;
+      y.open0 = (max(0, x.key0 + kKmKeys - 1 - x.q.first - x.tok0) + ntok - 1) / ntok;
+      y.open1 = (x.q.qlen - x.tok0) / ntok;
+      y.left = (x.q.qlen - x.tok0) * p.v.rep;
+      tell(y);
+      for (int i = 0; ok && i < x.steps; ++i, ++ln) {
         const int st = ln % LST, tok = x.tok0 + i * ntok;
         float v[4];
         int lim[4];
@@ -245,12 +293,15 @@ __global__ void __launch_bounds__(kKmThreads, 1)
         mbar_arrive(&l_full[st]);
       }
     }
-  } else if (warp == kKmMma) {
-    // ------------------------------------------------------------ MMA issuer
+    y.steps = -1;
+    if (ok) tell(y);
+  } else if (warp == kKmMma || warp == kKmMma1) {
+    // ------------------------------------------------------------ MMA issuers, one a tile
     const bool leader = elect_one();
+    const int t = warp - kKmMma;
     constexpr uint32_t idesc = idesc_f16(UmmaFormat<T>::value, 0, 0, 128, 128);
     const uint64_t dq0 = smem_desc(smem_u32(smem + L::OFF_Q), 16, 1024);
-    const uint64_t dk0 = smem_desc(smem_u32(smem + L::OFF_K), 16, 1024);
+    const uint64_t dk0 = smem_desc(smem_u32(smem + L::OFF_K + t * L::TILE), 16, 1024);
     auto commit = [&](uint64_t* bar) {
       if (leader) umma_commit(bar);
       __syncwarp();
@@ -266,32 +317,25 @@ __global__ void __launch_bounds__(kKmThreads, 1)
       for (int i = 0; i < x.steps; ++i, ++qn) {
         const int st = qn % QST;
         const uint32_t buf = qn & 1;
-        // A check of a barrier waits behind this warp's queued MMAs: all that a step needs is checked before its MMAs.
-        ok = wait(&q_full[st], (qn / QST) & 1);
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-          if (ok && qn >= 2) ok = wait(&s_empty[2 * t + buf], ((qn >> 1) - 1) & 1);
+        ok = wait(&q_full[st], (qn / QST) & 1) && (qn < 2 || wait(&s_empty[2 * t + buf], ((qn >> 1) - 1) & 1));
         if (!ok) break;
         tc_fence_after();
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-#pragma unroll
-          for (int ks = 0; ks < D / 16; ++ks) {
-            const uint32_t off = ((ks >> 2) * L::PANEL + (ks & 3) * 32) >> 4;
-            if (leader)
-              umma_f16_ss(tmem + (2 * t + buf) * 128, dk0 + (((2 * (kn & 1) + t) * L::TILE) >> 4) + off,
-                          dq0 + ((st * L::TILE) >> 4) + off, idesc, ks > 0 ? 1u : 0u);
-            __syncwarp();
-          }
-          commit(&s_full[2 * t + buf]);
+        for (int ks = 0; ks < D / 16; ++ks) {
+          const uint32_t off = ((ks >> 2) * L::PANEL + (ks & 3) * 32) >> 4;
+          if (leader)
+            umma_f16_ss(tmem + (2 * t + buf) * 128, dk0 + ((2 * (kn & 1) * L::TILE) >> 4) + off,
+                        dq0 + ((st * L::TILE) >> 4) + off, idesc, ks > 0 ? 1u : 0u);
+          __syncwarp();
         }
+        commit(&s_full[2 * t + buf]);
         commit(&q_empty[st]);
       }
       if (ok) commit(&k_empty[kn & 1]);
       ++kn;
     }
-    commit(drain);  // no MMA may be in flight when TMEM is released
-    mbar_wait(drain, 0, status, nullptr);
+    commit(&drain[t]);  // no MMA may be in flight when TMEM is released
+    mbar_wait(&drain[t], 0, status, nullptr);
     __syncwarp();
   } else {
     // ------------------------------------------------------------ weights and sums
@@ -301,28 +345,33 @@ __global__ void __launch_bounds__(kKmThreads, 1)
     float* const given = reinterpret_cast<float*>(smem + L::OFF_SUM);
     const float sl2 = p.v.scale_log2;
     const uint64_t sl2x2 = f2_pack(sl2, sl2);
-    int qn = 0, done = 0;
+    int qn = 0;
     bool ok = true;
-    // After a wait that ran out the warps still meet at the barriers.
-    for (KeyMassWalk at(p, first, stride); at.more(p); at.next()) {
-      if (!at.item(p, ntok, rank, parts, x)) continue;
-      // Where the sum goes, and the old weight, fetched while the rows stream by.
+    for (int done = 0; ok; ++done) {
+      ok = __all_sync(0xffffffffu, mbar_wait(&i_full[done & 3], (done >> 2) & 1, status, abort_flag));
+      if (!ok) break;
+      const KeyMassTask* const y = reinterpret_cast<const KeyMassTask*>(smem + L::OFF_ITEM + (done & 3) * 64);
+      const int steps = y->steps;
+      if (steps < 0) break;
+      const int open0 = y->open0, open1 = y->open1, left = y->left - half * 64;
+      // Where the sum goes, and the old weight, fetched while the rows stream by: the page first, what hangs on it a step later.
       float* dst = nullptr;
       float old = 0.0f;
-      const int pos = x.key0 + key;
-      if (half == 0 && rank == 0 && pos < x.keys) {
-        const int pi = pos / p.v.a.page_size, slot = pos - pi * p.v.a.page_size;
-        const int page = paged_page(p.v, p.v.a.block_table + x.s * p.v.a.table_stride, pi);
-        if (page >= 0) {
-          dst = p.out + page * p.os[0] + x.g * p.os[1] + slot * p.os[2];
-          if (pos < x.q.first && p.decay != 0.0f) old = p.decay * p.mass[page * p.ms[0] + x.g * p.ms[1] + slot * p.ms[2]];
+      const int pos = y->key0 + key;
+      const bool writes = half == 0 && rank == 0 && pos < y->keys;
+      const int pi = pos / p.v.a.page_size;
+      int page = -1;
+      if (writes) page = p.v.a.block_table[y->s * p.v.a.table_stride + pi];
+      auto place = [&] {
+        if (!writes) return;
+        if (page < 0 || page >= p.v.a.num_pages) {
+          raise_status(status, SPRUCE_STATUS_BAD_PAGE);
+          return;
         }
-      }
-      const int steps = x.steps;
-      // Row tiles [open0, open1): all tokens are the sequence's and see all the item's keys.
-      const int open0 = (max(0, x.key0 + kKmKeys - 1 - x.q.first - x.tok0) + ntok - 1) / ntok;
-      const int open1 = (x.q.qlen - x.tok0) / ntok;
-      const int left = (x.q.qlen - x.tok0) * p.v.rep - half * 64;  // rows from this half of the first tile on
+        const int slot = pos - pi * p.v.a.page_size;
+        dst = p.out + page * p.os[0] + y->g * p.os[1] + slot * p.os[2];
+        if (pos < y->first && p.decay != 0.0f) old = p.mass[page * p.ms[0] + y->g * p.ms[1] + slot * p.ms[2]];
+      };
       uint64_t sum2[2] = {f2_pack(0.0f, 0.0f), f2_pack(0.0f, 0.0f)};
       // Sixteen rows; those of the other tiles have limits.
       auto rows_of = [&](const float* s, const float* lse, auto masked_c) {
@@ -373,25 +422,25 @@ __global__ void __launch_bounds__(kKmThreads, 1)
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&l_empty[qn % LST]);
+        if (i == 0) place();
       }
+      if (steps == 0) place();
       float a0, a1, a2, a3;
       f2_unpack(sum2[0], a0, a1);
       f2_unpack(sum2[1], a2, a3);
       float sum = (a0 + a1) + (a2 + a3);
-      // The second half hands its sum over and goes on.  It is never four items ahead: the scores of a step wait for both halves to
-      // have taken those two steps before, and where an item has no step it waits itself.
+      // The second half hands its sum over and goes on; its place is free again when all are done with the item.
       float* const mine = given + (done & 3) * 256;
-      const uint32_t bar = 1 + t * 4 + (done & 3);
       if (half == 1) {
         mine[key] = sum;
-        if (steps > 0 && ok)
-          asm volatile("bar.arrive %0, 256;" ::"r"(bar) : "memory");
-        else
-          named_barrier_sync(bar, 256);
+        mbar_arrive(&g_full[t * 4 + (done & 3)]);
       } else {
-        named_barrier_sync(bar, 256);
+        ok = __all_sync(0xffffffffu, mbar_wait(&g_full[t * 4 + (done & 3)], (done >> 2) & 1, status, abort_flag)) && ok;
         sum += mine[key];
       }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&i_empty[done & 3]);
+      old *= p.decay;
       if (parts == 1) {
         if (dst != nullptr) *dst = sum + old;
       } else if (half == 0) {  // the only item: to the cluster's first CTA
@@ -403,7 +452,6 @@ __global__ void __launch_bounds__(kKmThreads, 1)
         to = dst;
         old_part = old;
       }
-      ++done;
     }
   }
 
