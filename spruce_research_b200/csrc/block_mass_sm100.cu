@@ -146,6 +146,8 @@ __global__ void __launch_bounds__(kBmThreads, 1)
     tmem_relinquish();
   }
   tc_fence_before();
+  let_next_kernel_start();
+  wait_for_earlier_kernels();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
@@ -362,6 +364,8 @@ __global__ void __launch_bounds__(kBmThreads, 1)
 
 // Heads added in their order, rows scaled to a mean, zeros past the diagonal.
 __global__ void __launch_bounds__(256) block_mass_join_kernel(const BlockParams p) {
+  let_next_kernel_start();
+  wait_for_earlier_kernels();
   const int i = blockIdx.x % p.qb, bg = blockIdx.x / p.qb;
   const float share = 1.0f / static_cast<float>(min(64, p.a.T - i * 64) * p.rep);
   const float* part = p.part + (((int64_t)bg * p.tiles + i / 2) * p.rep * 2 + (i & 1)) * p.kbp;
@@ -421,10 +425,8 @@ static cudaError_t launch_block(const BlockMassArgs& a, CUtensorMapDataType dt, 
   const int G = std::min(p.units, sm_count());
   p.blocks = a.workspace;
   p.part = a.workspace + (int64_t)G * 256 * p.kbp;
-  kern<<<G, kBmThreads, L::BYTES, stream>>>(mq, mk, p);
-  if ((e = cudaGetLastError()) != cudaSuccess) return e;
-  block_mass_join_kernel<<<a.B * a.Hkv * p.qb, 256, 0, stream>>>(p);
-  return cudaGetLastError();
+  e = launch_early(kern, G, kBmThreads, L::BYTES, stream, mq, mk, p);
+  return e != cudaSuccess ? e : launch_early(block_mass_join_kernel, a.B * a.Hkv * p.qb, 256, 0, stream, p);
 }
 
 cudaError_t launch_block_mass_sm100(const BlockMassArgs& a, int dtype, cudaStream_t stream) {

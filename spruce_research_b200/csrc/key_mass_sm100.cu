@@ -170,6 +170,8 @@ __global__ void __launch_bounds__(kKmThreads, 1)
   }
   fence_proxy_async_smem();
   tc_fence_before();
+  let_next_kernel_start();
+  wait_for_earlier_kernels();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
@@ -508,16 +510,18 @@ static cudaError_t launch_rows(const KeyMassArgs& a, int dtype, cudaStream_t str
   int parts = 1;
   while (parts < 8 && items * parts * 2 <= sms && 2 * parts * ntok <= a.a.max_q) parts *= 2;
   cudaLaunchConfig_t cfg{};
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = parts;
-  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cudaLaunchAttribute attr[2]{};
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = parts;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.gridDim = dim3(static_cast<unsigned>(parts * std::min<int64_t>(items, sms / parts)));
   cfg.blockDim = dim3(kKmThreads);
   cfg.dynamicSmemBytes = L::BYTES;
   cfg.stream = stream;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
   return cudaLaunchKernelEx(&cfg, kern, mq, mk, p, box, ntok, parts);
 }
 
