@@ -861,7 +861,8 @@ def _tma_ok(t: torch.Tensor) -> torch.Tensor:
 
 def _row_major(t: torch.Tensor, rows: int) -> torch.Tensor:
     """[..., n] as [rows, n] with a unit last stride."""
-    t = t.reshape(rows, t.shape[-1])
+    if t.dim() != 2:
+        t = t.reshape(rows, t.shape[-1])
     return t if t.stride(1) == 1 or t.shape[1] <= 1 else t.contiguous()
 
 
@@ -882,11 +883,11 @@ def _distill(scores, ids, teacher, visible, temperature, status, *, loss=False, 
     if visible is not None:
         if visible.dtype != torch.int32 or visible.shape != lead:
             raise ValueError(f"visible must be int32 {tuple(lead)}, got {visible.dtype} {tuple(visible.shape)}")
-        visible = visible.reshape(R).contiguous()
+        visible = visible.contiguous() if len(lead) == 1 else visible.reshape(R).contiguous()
     if weight is not None:
         if weight.dtype != torch.float32 or weight.shape != lead:
             raise ValueError(f"the rows' weights must be float32 {tuple(lead)}, got {weight.dtype} {tuple(weight.shape)}")
-        weight = weight.reshape(R)
+        weight = weight if len(lead) == 1 else weight.reshape(R)
     x, i, t = _row_major(scores, R), _row_major(ids, R), _row_major(teacher, R)
     out = torch.empty(lead, device=x.device, dtype=torch.float32) if loss else None
     made = torch.empty((R, 2), device=x.device, dtype=torch.float32) if want_stats else None

@@ -6,12 +6,15 @@ and values in pages; every later chunk or token is appended with its head norms 
 over the pages.
 
 ``PagedKVCache`` owns the pages of every layer and the sequences' page tables (host), ``PagedStep`` is one forward's
-batch (device), ``PagedSparseLayer`` runs one layer of it.
+batch (device), ``PagedSparseLayer`` runs one layer of it.  A cache that keeps the attention weight of its keys
+(``track_mass``) can be cut to a budget: ``PagedKVCache.evict`` keeps each head's heaviest.
 
     python -m spruce_research_b200.paged          # a small layer: prompts, then decode steps, with their times
+    python -m spruce_research_b200.paged 2048     # the same, then cut to 2048 tokens a sequence and decoded further
 """
 from __future__ import annotations
 
+import sys
 from dataclasses import dataclass
 
 import torch
@@ -31,17 +34,20 @@ class PagedStep:
     max_q_len: int
     max_kv_len: int
     tokens: int
+    positions: torch.Tensor | None = None   # int64 [tokens] in their sequences, where an eviction left these ahead of the slots
+    max_position: int = 0                    # positions end before this
 
 
 class PagedKVCache:
     """Pages of ``page_size`` tokens for ``num_layers`` layers: ``k`` and ``v`` [layers, pages, Hkv, page_size, D].
 
     A page id names the same page of every layer.  Heads lie outside the tokens of a page, so that one head's page
-    is one contiguous block.
+    is one contiguous block.  With ``track_mass``, ``mass`` float32 [layers, pages, Hkv, page_size] holds the attention weight
+    that each key has received, which layers add to and :meth:`evict` goes by.
     """
 
     def __init__(self, num_layers: int, num_pages: int, page_size: int, kv_heads: int, head_dim: int,
-                 dtype: torch.dtype = torch.bfloat16, device="cuda"):
+                 dtype: torch.dtype = torch.bfloat16, device="cuda", track_mass: bool = False):
         if page_size < 16 or page_size % 16:
             raise ValueError(f"page_size must be a multiple of 16, got {page_size}")
         if min(num_layers, num_pages, kv_heads, head_dim) < 1:
@@ -49,10 +55,12 @@ class PagedKVCache:
         shape = (num_layers, num_pages, kv_heads, page_size, head_dim)
         self.k = torch.empty(shape, dtype=dtype, device=device)
         self.v = torch.empty(shape, dtype=dtype, device=device)
+        self.mass = torch.zeros(shape[:4], dtype=torch.float32, device=device) if track_mass else None
         self.page_size = page_size
         self._free = list(range(num_pages - 1, -1, -1))
         self._pages: dict = {}
         self._length: dict = {}
+        self._evicted: dict = {}   # tokens that evictions took, and the slots that the last one left
 
     @property
     def free_pages(self) -> int:
@@ -62,16 +70,23 @@ class PagedKVCache:
         """Tokens the sequence holds (0 for one the cache does not know)."""
         return self._length.get(seq_id, 0)
 
+    def position(self, seq_id) -> int:
+        """Position of the sequence's next token: its length and what evictions took from it."""
+        return self.length(seq_id) + self._evicted.get(seq_id, (0, 0))[0]
+
     def drop(self, seq_id) -> None:
         """Return a sequence's pages.  Kernels of its last step may still run: the next step's follow them."""
         self._free.extend(reversed(self._pages.pop(seq_id, [])))
         self._length.pop(seq_id, None)
+        self._evicted.pop(seq_id, None)
 
     def truncate(self, seq_id, length: int) -> None:
         """Keep a sequence's first ``length`` tokens: drafts that were rejected, or a step whose forward did not run."""
         held = self.length(seq_id)
         if not 0 <= length <= held:
             raise ValueError(f"a sequence of {held} tokens cannot be cut to {length}")
+        if length < self._evicted.get(seq_id, (0, 0))[1]:
+            raise ValueError(f"the first {self._evicted[seq_id][1]} slots are an eviction's: each head holds other tokens there")
         if seq_id in self._pages:
             pages, keep = self._pages[seq_id], -(-length // self.page_size)
             self._free.extend(reversed(pages[keep:]))
@@ -96,20 +111,59 @@ class PagedKVCache:
         for (s, _), m, count in zip(new_tokens, lengths, need):
             self._pages.setdefault(s, []).extend(self._free.pop() for _ in range(count))
             self._length[s] = m
-        width = max([len(self._pages[s]) for s, _ in new_tokens], default=0)
-        S = len(new_tokens)
+        dev = self._describe([s for s, _ in new_tokens], [n for _, n in new_tokens], lengths)
+        ends = [self.position(s) for s, _ in new_tokens]
+        positions = None
+        if any(self._evicted.get(s, (0, 0))[0] for s, _ in new_tokens):
+            positions = torch.cat([torch.arange(end - n, end) for end, (_, n) in zip(ends, new_tokens)]).to(self.k.device)
+        return PagedStep([s for s, _ in new_tokens], *dev, max((n for _, n in new_tokens), default=0), max(lengths, default=0),
+                         sum(n for _, n in new_tokens), positions, max(ends, default=0))
+
+    def _describe(self, seq_ids, counts, lengths):
+        """Page table, offsets of ``counts`` and lengths of sequences, on the device."""
+        width = max([len(self._pages[s]) for s in seq_ids], default=0)
+        S = len(seq_ids)
         # One host tensor and one copy: table, offsets, lengths.
         host = torch.zeros(S * width + 2 * S + 1, dtype=torch.int32)
         table, cu, kv = host[:S * width].view(S, width), host[S * width:S * width + S + 1], host[S * width + S + 1:]
-        for i, (s, n) in enumerate(new_tokens):
+        for i, (s, n) in enumerate(zip(seq_ids, counts)):
             pages = self._pages[s]
             table[i, :len(pages)] = torch.tensor(pages, dtype=torch.int32)
             cu[i + 1] = cu[i] + n
             kv[i] = lengths[i]
         dev = host.to(self.k.device)
-        return PagedStep([s for s, _ in new_tokens], dev[:S * width].view(S, width), dev[S * width:S * width + S + 1],
-                         dev[S * width + S + 1:], max((n for _, n in new_tokens), default=0), max(lengths, default=0),
-                         int(cu[-1]))
+        return dev[:S * width].view(S, width), dev[S * width:S * width + S + 1], dev[S * width + S + 1:]
+
+    def evict(self, seq_ids, keep: int, *, sinks: int = 0, recent: int = 0) -> list:
+        """Cut sequences to ``keep`` tokens in every layer and return the pages that this empties.
+
+        Each KV head keeps its first ``sinks`` slots, its last ``recent`` ones and of those between the keys of the largest mass;
+        they move, in their order, to the first slots.  Sequences of at most ``keep`` tokens stay as they are.  New tokens go on at
+        :meth:`position`.  Steps described before do not hold any more.  Returns the sequences that were cut.
+        """
+        if self.mass is None:
+            raise ValueError("this cache was made without track_mass")
+        keep, sinks, recent = int(keep), int(sinks), int(recent)
+        if keep < 1 or sinks < 0 or recent < 0 or sinks + recent > keep:
+            raise ValueError(f"cannot keep {sinks} first and {recent} last of {keep} tokens")
+        seq_ids = list(seq_ids)
+        if len(set(seq_ids)) < len(seq_ids):
+            raise ValueError("a sequence appears twice in one eviction")
+        cut = [s for s in seq_ids if self.length(s) > keep]
+        if not cut:
+            return cut
+        lengths = [self.length(s) for s in cut]
+        table, _, lens = self._describe(cut, [0] * len(cut), lengths)
+        for k, v, mass in zip(self.k, self.v, self.mass):
+            native.paged_evict(k, v, mass, table, lens, keep, sinks=sinks, recent=recent, max_kv_len=max(lengths))
+        left = -(-keep // self.page_size)
+        for s, n in zip(cut, lengths):
+            pages = self._pages[s]
+            self._free.extend(reversed(pages[left:]))
+            del pages[left:]
+            self._length[s] = keep
+            self._evicted[s] = (self._evicted.get(s, (0, 0))[0] + n - keep, keep)
+        return cut
 
 
 class PagedSparseLayer:
@@ -117,14 +171,24 @@ class PagedSparseLayer:
 
     Takes the projections before norms and rotation, packed ``q [N, Hq, D]``, ``k`` / ``v`` [N, Hkv, D].  ``rope`` is a
     :func:`rope.rope_table` of the longest sequence (None: no rotation); ``q_weight`` / ``k_weight`` are head norms (None: no norm).
+
+    Where the cache keeps its keys' weights, each step multiplies the old ones of its sequences by ``decay`` and adds
+    what its queries give; a sparse prefill sets them by its last ``observe`` queries, which attend to the whole prompt for it.
     """
 
     def __init__(self, cache: PagedKVCache, layer_idx: int, rope: torch.Tensor | None, *,
                  prefill: SparsePrefillLayer | None = None, q_weight: torch.Tensor | None = None,
-                 k_weight: torch.Tensor | None = None, eps: float = 1e-6, interleaved: bool = False):
+                 k_weight: torch.Tensor | None = None, eps: float = 1e-6, interleaved: bool = False,
+                 decay: float = 1.0, observe: int = 64):
         if not 0 <= layer_idx < cache.k.shape[0]:
             raise ValueError(f"layer_idx {layer_idx} is outside the cache's {cache.k.shape[0]} layers")
+        if not 0 <= decay <= 1:
+            raise ValueError(f"decay must be in [0, 1], got {decay}")
+        if observe < 1:
+            raise ValueError(f"observe must be positive, got {observe}")
         self.k_cache, self.v_cache = cache.k[layer_idx], cache.v[layer_idx]
+        self.mass = None if cache.mass is None else cache.mass[layer_idx]
+        self.decay, self.observe = decay, observe
         self.rope, self.sparse = rope, prefill
         self.rotation = dict(q_weight=q_weight, k_weight=k_weight, eps=eps, interleaved=interleaved)
 
@@ -133,9 +197,21 @@ class PagedSparseLayer:
         rows = [x.shape[0] for x in tensors]
         if min(rows) < step.tokens or not spare and max(rows) > step.tokens:
             raise ValueError(f"the step has {step.tokens} tokens, q, k and v have {rows}")
-        if self.rope is not None and step.max_kv_len > self.rope.shape[0]:
-            raise ValueError(f"sequences of {step.max_kv_len} tokens need a rotation table of as many positions, got "
+        most = max(step.max_kv_len, step.max_position)
+        if self.rope is not None and most > self.rope.shape[0]:
+            raise ValueError(f"sequences of {most} tokens need a rotation table of as many positions, got "
                              f"{self.rope.shape[0]}")
+
+    def _attend(self, q, step: PagedStep, cu_q, max_q_len: int, decay: float, out=None) -> torch.Tensor:
+        """Attention of ``q`` over the cache; where the cache keeps weights, what ``q`` gives is added."""
+        batch = (step.block_table, cu_q, step.kv_lens)
+        bounds = dict(max_q_len=max_q_len, max_kv_len=step.max_kv_len)
+        if self.mass is None:
+            return native.paged_attention(q, self.k_cache, self.v_cache, *batch, out=out, **bounds)
+        lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
+        out = native.paged_attention(q, self.k_cache, self.v_cache, *batch, out=out, lse=lse, **bounds)
+        native.paged_key_mass(q, self.k_cache, self.mass, *batch, lse, decay=decay, **bounds)
+        return out
 
     def extend(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, step: PagedStep,
                out: torch.Tensor | None = None) -> torch.Tensor:
@@ -144,10 +220,12 @@ class PagedSparseLayer:
         N may exceed the step's tokens; the rows past them are not written.
         """
         self._check((q, k, v), step, spare=True)
+        positions = step.positions
+        if positions is not None and positions.shape[0] < k.shape[0]:  # rows past the step's tokens are left out
+            positions = torch.nn.functional.pad(positions, (0, k.shape[0] - positions.shape[0]))
         q = native.paged_append(k, v, self.k_cache, self.v_cache, step.block_table, step.cu_q, step.kv_lens, q=q,
-                                rope=self.rope, **self.rotation)
-        return native.paged_attention(q, self.k_cache, self.v_cache, step.block_table, step.cu_q, step.kv_lens,
-                                      max_q_len=step.max_q_len, max_kv_len=step.max_kv_len, out=out)
+                                rope=self.rope, positions=positions, **self.rotation)
+        return self._attend(q, step, step.cu_q, step.max_q_len, self.decay, out)
 
     def prefill(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, step: PagedStep):
         """Block-sparse prefill of one whole prompt; its keys and values go to the cache.
@@ -165,17 +243,22 @@ class PagedSparseLayer:
         native.paged_append(kr[0].transpose(0, 1), v, self.k_cache, self.v_cache, step.block_table, step.cu_q,
                             step.kv_lens)
         out, selected = self.sparse(qr, kr, vs)
+        if self.mass is not None:
+            last = min(self.observe, step.tokens)
+            self._attend(qr[0, :, -last:].transpose(0, 1), step, torch.arange(0, 2 * last, last, device=q.device, dtype=torch.int32),
+                         last, 0.0)
         return out[0], selected
 
 
-def main(prompt_tokens: int = 8192, sequences: int = 4, decode_steps: int = 32) -> None:
-    """Prompts through the sparse prefill, then decode steps of all of them, on one 28-query / 4-KV-head layer."""
+def main(prompt_tokens: int = 8192, sequences: int = 4, decode_steps: int = 32, budget: int = 0) -> None:
+    """Prompts through the sparse prefill, then decode steps of all of them, on one 28-query / 4-KV-head layer; with a
+    ``budget``, the cache keeps its keys' weights, is cut to so many tokens a sequence and decodes on."""
     from .rope import rope_table
     from .synthetic import k_for_density, make_gate_weights
 
     Hq, Hkv, D, page = 28, 4, 128, 64
-    total = prompt_tokens + decode_steps
-    cache = PagedKVCache(1, sequences * -(-total // page), page, Hkv, D)
+    total = prompt_tokens + (2 if budget else 1) * decode_steps
+    cache = PagedKVCache(1, sequences * -(-total // page), page, Hkv, D, track_mass=budget > 0)
     wq, wk = make_gate_weights(1, D, D, seed=2, device="cuda")
     sparse = SparsePrefillLayer(wq[0], wk[0], max(2, k_for_density(-(-prompt_tokens // 64), 0.10)))
     layer = PagedSparseLayer(cache, 0, rope_table(D, total, 1e6), prefill=sparse)
@@ -193,15 +276,24 @@ def main(prompt_tokens: int = 8192, sequences: int = 4, decode_steps: int = 32) 
         b.synchronize()
         return a.elapsed_time(b)
 
+    def decode():
+        for _ in range(decode_steps):
+            qkv, step = project(sequences), cache.step([(s, 1) for s in range(sequences)])
+            ms = timed(lambda: layer.extend(*qkv, step))
+        print(f"decode: {sequences} sequences at {step.max_kv_len} tokens, {1e3 * ms:.1f} us for the last step")
+
     for s in range(sequences):
         qkv, step = project(prompt_tokens), cache.step([(s, prompt_tokens)])
         ms = timed(lambda: layer.prefill(*qkv, step))
         print(f"prompt {s}: {prompt_tokens} tokens, {sparse.k_selected} blocks a row, {ms:.3f} ms")
-    for i in range(decode_steps):
-        qkv, step = project(sequences), cache.step([(s, 1) for s in range(sequences)])
-        ms = timed(lambda: layer.extend(*qkv, step))
-    print(f"decode: {sequences} sequences at {step.max_kv_len} tokens, {1e3 * ms:.1f} us for the last step")
+    decode()
+    if budget > 0:
+        before = cache.free_pages
+        ms = timed(lambda: cache.evict(range(sequences), budget, sinks=min(64, budget // 8), recent=budget // 4))
+        print(f"eviction: {sequences} sequences cut to {budget} tokens, {cache.free_pages - before} pages returned, "
+              f"{1e3 * ms:.1f} us")
+        decode()
 
 
 if __name__ == "__main__":
-    main()
+    main(budget=int(sys.argv[1]) if len(sys.argv) > 1 else 0)
