@@ -5,8 +5,8 @@
 //
 // Bound by HBM: the scores are read once (twice by a separate backward pass) and the gradient written once.  Rows of up to 2048
 // columns (a gate's) take a warp each, which holds the row in registers between the sums and the gradient.  Longer ones (a
-// vocabulary's) take a CTA each, which keeps a running maximum and sum; its gradient pass reads the row again, from L2 when both
-// run in one call: two CTAs an SM, so that their rows stay there.  The teacher's columns are written again after the others,
+// vocabulary's) take a CTA each, which keeps a running maximum and sum; its gradient pass reads the row again, mostly from L2 when
+// both run in one call.  The teacher's columns are written again after the others,
 // so that each element is rounded once.  A column named twice is found by a bitmap; only rows that have one search for it.
 #include <algorithm>
 
@@ -14,8 +14,8 @@
 
 namespace spruce {
 
-constexpr int kDistillThreads = 512, kDistillWarps = kDistillThreads / 32;
 constexpr int kRowWarps = 2;            // rows of a CTA of the warp kernel
+constexpr int kShortRow = 24 << 10;    // bytes of the rows that the smallest CTAs take
 constexpr int kRowMost = 2048, kRowEntries = 256;  // columns and teacher entries that it takes
 constexpr int kRowBits = 64, kDistillBits = 1024;  // words of the bitmaps; columns share bits modulo their size
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
@@ -209,54 +209,55 @@ __global__ void __launch_bounds__(32 * kRowWarps) distill_rows_kernel(const Dist
 }
 
 // ------------------------------------------------------------------ a CTA a row
+template <int THREADS>
 __device__ __forceinline__ float2 block_join(float2 v, float c, float2* red) {
   v = warp_join(v, c);
   __syncthreads();
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
   __syncthreads();
   v = red[0];
-  for (int w = 1; w < kDistillWarps; ++w) v = join(v, red[w], c);
+  for (int w = 1; w < THREADS / 32; ++w) v = join(v, red[w], c);
   return v;
 }
 
 // Columns [0, n) of a row: the 16-byte aligned middle by vectors, f(first column, pointer); the rest one by one, g(column).
-template <typename T, typename F, typename G>
+template <typename T, int THREADS, typename F, typename G>
 __device__ __forceinline__ void over_row(const T* s, int n, F f, G g) {
   constexpr int V = 16 / sizeof(T), U = 4;
   const int head = min(n, static_cast<int>((16 - (reinterpret_cast<uintptr_t>(s) & 15)) % 16 / sizeof(T)));
   const int vecs = (n - head) / V, rest = n - vecs * V;
   int i = threadIdx.x;
-  for (; i + (U - 1) * kDistillThreads < vecs; i += U * kDistillThreads) {
+  for (; i + (U - 1) * THREADS < vecs; i += U * THREADS) {
     uint4 x[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) x[u] = *reinterpret_cast<const uint4*>(s + head + (i + u * kDistillThreads) * V);
+    for (int u = 0; u < U; ++u) x[u] = *reinterpret_cast<const uint4*>(s + head + (i + u * THREADS) * V);
 #pragma unroll
-    for (int u = 0; u < U; ++u) f(head + (i + u * kDistillThreads) * V, x[u]);
+    for (int u = 0; u < U; ++u) f(head + (i + u * THREADS) * V, x[u]);
   }
-  for (; i < vecs; i += kDistillThreads) f(head + i * V, *reinterpret_cast<const uint4*>(s + head + i * V));
-  for (int e = threadIdx.x; e < rest; e += kDistillThreads) g(e < head ? e : vecs * V + e);
+  for (; i < vecs; i += THREADS) f(head + i * V, *reinterpret_cast<const uint4*>(s + head + i * V));
+  for (int e = threadIdx.x; e < rest; e += THREADS) g(e < head ? e : vecs * V + e);
 }
 
-// CTAS an SM: two with the gradient, four without.
-template <typename T, int CTAS>
-__global__ void __launch_bounds__(kDistillThreads, CTAS) distill_kernel(const DistillArgs a) {
+// CTAS an SM.
+template <typename T, int THREADS, int CTAS>
+__global__ void __launch_bounds__(THREADS, CTAS) distill_kernel(const DistillArgs a) {
   constexpr int V = 16 / sizeof(T);
   extern __shared__ float sm[];
   float* P = sm;                                  // [K] teacher weights
   int* I = reinterpret_cast<int*>(sm + a.K);      // [K] columns; -1: not used
   __shared__ uint32_t bits[kDistillBits];
-  __shared__ float2 red[kDistillWarps];
+  __shared__ float2 red[THREADS / 32];
   const int tid = threadIdx.x;
   const float c = a.inv_tau * kLog2e;
   for (int64_t row = blockIdx.x; row < a.R; row += gridDim.x) {
     const T* s = static_cast<const T*>(a.scores) + row * a.score_stride;
     const int seen = row_seen(a, row, tid == 0);
     __syncthreads();
-    for (int b = tid; b < kDistillBits; b += kDistillThreads) bits[b] = 0;
+    for (int b = tid; b < kDistillBits; b += THREADS) bits[b] = 0;
     __syncthreads();
     float2 t = make_float2(-INFINITY, 0.0f);
     bool mine = false;
-    for (int k = tid; k < a.K; k += kDistillThreads) {
+    for (int k = tid; k < a.K; k += THREADS) {
       int column;
       float logit;
       use_entry(a, row_entry(a, row, k), seen, column, logit);
@@ -267,7 +268,7 @@ __global__ void __launch_bounds__(kDistillThreads, CTAS) distill_kernel(const Di
       if (a.grad != nullptr) mine = mine || (atomicOr(&bits[(column >> 5) % kDistillBits], 1u << (column & 31)) >> (column & 31) & 1);
     }
     const bool twice = __syncthreads_or(mine);
-    t = block_join(t, c, red);
+    t = block_join<THREADS>(t, c, red);
     const float tref = t.x == -INFINITY ? 0.0f : t.x, tsum = t.y;
     float2 st;  // maximum of the scores, log2 of the sum over it
     if (a.stats_in != nullptr) {
@@ -280,7 +281,7 @@ __global__ void __launch_bounds__(kDistillThreads, CTAS) distill_kernel(const Di
           m = top;
         }
       };
-      over_row<T>(s, seen,
+      over_row<T, THREADS>(s, seen,
                   [&](int, const uint4& y) {
                     float x[V];
                     unpack16<T>(y, x);
@@ -297,20 +298,20 @@ __global__ void __launch_bounds__(kDistillThreads, CTAS) distill_kernel(const Di
                     more(x);
                     l += fast_exp2((x - (m == -INFINITY ? 0.0f : m)) * c);
                   });
-      const float2 all = block_join(make_float2(m, l), c, red);
+      const float2 all = block_join<THREADS>(make_float2(m, l), c, red);
       st = make_float2(all.x == -INFINITY ? 0.0f : all.x, log2f(all.y));
     }
     const bool empty = st.y == -INFINITY || tsum == 0.0f;
     const float tlog = log2f(tsum), inv = 1.0f / tsum;
     float loss = 0.0f;
-    for (int k = tid; k < a.K; k += kDistillThreads) {
+    for (int k = tid; k < a.K; k += THREADS) {
       if (I[k] < 0 || empty) continue;
       const float e = (P[k] - tref) * c, p = fast_exp2(e) * inv;
       if (a.loss != nullptr && p != 0.0f) loss += p * ((e - tlog) - ((Elem<T>::to_f(s[I[k]]) - st.x) * c - st.y));
       P[k] = p;
     }
     if (a.loss != nullptr) {
-      loss = block_join(make_float2(0.0f, loss), c, red).y * kLn2;
+      loss = block_join<THREADS>(make_float2(0.0f, loss), c, red).y * kLn2;
       if (tid == 0) {
         a.loss[row] = empty ? 0.0f : loss;
         if (a.stats != nullptr) {
@@ -324,11 +325,11 @@ __global__ void __launch_bounds__(kDistillThreads, CTAS) distill_kernel(const Di
     const float w = a.weight[row * a.weight_stride] * a.inv_tau;
     const bool same = ((reinterpret_cast<uintptr_t>(s) ^ reinterpret_cast<uintptr_t>(grad)) & 15) == 0;
     if (empty) {
-      for (int j = tid; j < a.n; j += kDistillThreads) grad[j] = Elem<T>::from_f(0.0f);
+      for (int j = tid; j < a.n; j += THREADS) grad[j] = Elem<T>::from_f(0.0f);
       continue;
     }
     auto value = [&](float x) { return w * fast_exp2((x - st.x) * c - st.y); };
-    over_row<T>(s, seen,
+    over_row<T, THREADS>(s, seen,
                 [&](int j, const uint4& y) {
                   float x[V];
                   unpack16<T>(y, x);
@@ -342,9 +343,9 @@ __global__ void __launch_bounds__(kDistillThreads, CTAS) distill_kernel(const Di
                   }
                 },
                 [&](int j) { grad[j] = Elem<T>::from_f(value(Elem<T>::to_f(s[j]))); });
-    for (int j = seen + tid; j < a.n; j += kDistillThreads) grad[j] = Elem<T>::from_f(0.0f);
+    for (int j = seen + tid; j < a.n; j += THREADS) grad[j] = Elem<T>::from_f(0.0f);
     __syncthreads();
-    for (int k = tid; k < a.K; k += kDistillThreads) {
+    for (int k = tid; k < a.K; k += THREADS) {
       const int j = I[k];
       if (j < 0) continue;
       float p = P[k];
@@ -377,12 +378,23 @@ static cudaError_t launch_rows(const DistillArgs& a, cudaStream_t stream) {
 
 template <typename T>
 static cudaError_t launch(const DistillArgs& a, cudaStream_t stream) {
-  if (a.n <= kRowMost && a.K <= kRowEntries && a.R < (int64_t(1) << 33)) return launch_rows<T>(a, stream);
+  constexpr int V = 16 / sizeof(T);
+  const bool whole = (reinterpret_cast<uintptr_t>(a.scores) & 15u) == 0 && a.score_stride % V == 0 &&
+                     (a.grad == nullptr || ((reinterpret_cast<uintptr_t>(a.grad) & 15u) == 0 && a.grad_stride % V == 0));
+  // The warp kernel takes rows that are not 16-byte aligned element by element: long ones are better off with the other, which
+  // takes their middle by vectors (15879 rows of 1316 columns in bf16: 130 us there).
+  if (a.n <= (whole ? kRowMost : kRowMost / 2) && a.K <= kRowEntries && a.R < (int64_t(1) << 31)) return launch_rows<T>(a, stream);
   const unsigned G = static_cast<unsigned>(std::min<int64_t>(a.R, 1 << 20));
-  if (a.grad == nullptr)
-    distill_kernel<T, 4><<<G, kDistillThreads, a.K * 8, stream>>>(a);
+  // Short rows in small CTAs, whose barriers hold up fewer threads (49305 rows of 6352 columns in bf16, loss and gradient: 1274 /
+  // 610 / 359 us with 512 / 256 / 128 threads; 3000 of 16000 in fp32: 79 us with 256, 103 with 128; 4096 of 131072 in bf16: 554 us
+  // with 256, 574 with 512).  Fewer rows than SMs get more threads each.
+  const int64_t bytes = (int64_t)a.n * sizeof(T);
+  if (a.R < sm_count())
+    distill_kernel<T, 512, 2><<<G, 512, a.K * 8, stream>>>(a);
+  else if (bytes <= kShortRow)
+    distill_kernel<T, 128, 10><<<G, 128, a.K * 8, stream>>>(a);
   else
-    distill_kernel<T, 2><<<G, kDistillThreads, a.K * 8, stream>>>(a);
+    distill_kernel<T, 256, 5><<<G, 256, a.K * 8, stream>>>(a);
   return cudaGetLastError();
 }
 

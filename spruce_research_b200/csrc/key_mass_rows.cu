@@ -1,4 +1,4 @@
-// Softmax weight of cached keys under few query rows (bf16 / fp16): decode and drafts, bound by the HBM read of K.
+// Softmax weight of cached keys under few query rows: decode and drafts, bound by the HBM read of K.
 //
 // The formula is mass.cu's.  A warp takes 16 keys at a time as the A operand of m16n8k16 MMAs and the query rows of the
 // (sequence, KV head), 8 or 16 or more of them, as B.  A dot product may take its dims in any order, so both operands are
@@ -141,6 +141,105 @@ __global__ void __launch_bounds__(kKrThreads, kKrPerSm<D, NT>) key_mass_rows_ker
   }
 }
 
+// ------------------------------------------------------------------ fp32
+// Eight lanes a key, each with D / 8 dims of it; the query rows come from shared memory.  Eight rows' partial dots are summed over the
+// lanes by a transposing butterfly (7 shuffles), which leaves row c with lane c.
+template <int D, int NT>
+__global__ void __launch_bounds__(kKrThreads, 2) key_mass_rows_f32_kernel(const KeyMassParams p) {
+  constexpr int R = 8 * NT, CH = D / 32;
+  using Walk = PagedWalk<R, kKrTile>;
+  __shared__ __align__(16) float Q[R][D];
+  __shared__ int64_t scratch[33];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, kr = lane >> 3, c = lane & 7;
+  let_next_kernel_start();
+  wait_for_earlier_kernels();
+  Walk walk;
+  if (!paged_run<R, kKrTile, kKrThreads>(p.v, walk, scratch)) return;
+  PagedPiece x;
+  while (walk.next(p.v, x)) {
+    const int rows = x.q.qlen * p.v.rep;
+    const PagedRows row_at(p.v, x.q.q0, 0, x.g);
+    __syncthreads();
+    for (int e = threadIdx.x; e < R * (D / 4); e += kKrThreads) {
+      const int r = e / (D / 4), d = e % (D / 4) * 4;
+      float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if (r < rows) v = *reinterpret_cast<const float4*>(static_cast<const float*>(p.v.a.q) + row_at.offset(r, p.v.a.qn, p.v.a.qh) + d);
+      *reinterpret_cast<float4*>(&Q[r][d]) = v;
+    }
+    __syncthreads();
+    if (x.keys == 0) continue;
+    float lse[NT];   // of row 8 t + c
+    int last[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      lse[t] = INFINITY;
+      last[t] = -1;
+      if (8 * t + c < rows) {
+        lse[t] = mass_row_lse(p.lse[row_at.offset(8 * t + c, p.ln, p.lh)]);
+        last[t] = x.q.first + row_at.token(8 * t + c);
+      }
+    }
+    const int32_t* table = p.v.a.block_table + x.s * p.v.a.table_stride;
+    const float* kc = static_cast<const float*>(p.v.a.kc) + x.g * p.v.a.ks[1] + c * 4;
+    for (int tile = x.t0 + warp; tile < x.t1; tile += kKrWarps) {
+      const int key0 = tile * kKrTile, pi = key0 / p.v.a.page_size, slot = key0 - pi * p.v.a.page_size;
+      const int page = paged_page(p.v, table, pi);  // sixteen keys lie in one page
+      if (page < 0) continue;
+      float4 k[4][CH];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < CH; ++j) {
+          k[i][j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          if (key0 + 4 * i + kr < x.keys)
+            k[i][j] = __ldcs(reinterpret_cast<const float4*>(kc + page * p.v.a.ks[0] + (slot + 4 * i + kr) * p.v.a.ks[2] + j * 32));
+        }
+      float old = 0.0f;  // of key 4 c + kr, which lanes c < 4 write
+      const int mine = key0 + 4 * c + kr;
+      if (c < 4 && mine < x.q.first && p.decay != 0.0f)
+        old = p.decay * p.mass[page * p.ms[0] + x.g * p.ms[1] + (slot + 4 * c + kr) * p.ms[2]];
+      float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        float s[4][8];
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[i][r] = 0.0f;
+#pragma unroll
+          for (int j = 0; j < CH; ++j) {
+            const float4 q = *reinterpret_cast<const float4*>(&Q[8 * t + r][j * 32 + c * 4]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              s[i][r] = fmaf(q.x, k[i][j].x, fmaf(q.y, k[i][j].y, fmaf(q.z, k[i][j].z, fmaf(q.w, k[i][j].w, s[i][r]))));
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+#pragma unroll
+          for (int o = 4; o > 0; o >>= 1) {
+            const bool up = c & o;
+#pragma unroll
+            for (int r = 0; r < o; ++r) {
+              const float send = up ? s[i][r] : s[i][r + o], keep = up ? s[i][r + o] : s[i][r];
+              s[i][r] = keep + __shfl_xor_sync(0xffffffffu, send, o);
+            }
+          }
+          const float e = exp2f(s[i][0] * p.v.scale_log2 - lse[t]);
+          sum[i] += key0 + 4 * i + kr <= last[t] ? e : 0.0f;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1) sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], o);
+      if (c < 4 && mine < x.keys)
+        p.out[page * p.os[0] + x.g * p.os[1] + (slot + 4 * c + kr) * p.os[2]] =
+            (c == 0 ? sum[0] : (c == 1 ? sum[1] : (c == 2 ? sum[2] : sum[3]))) + old;
+    }
+  }
+}
+
 template <typename T, int D, int NT>
 static cudaError_t launch(const KeyMassArgs& a, cudaStream_t stream) {
   KeyMassParams p = key_mass_params(a, kKrTile);
@@ -158,7 +257,21 @@ static cudaError_t launch_tiles(const KeyMassArgs& a, cudaStream_t stream) {
   return launch<T, D, 4>(a, stream);
 }
 
+template <int D, int NT>
+static cudaError_t launch_f32(const KeyMassArgs& a, cudaStream_t stream) {
+  KeyMassParams p = key_mass_params(a, kKrTile);
+  p.v = paged_params(a.a, 8 * NT, 1, 4);
+  const int64_t tiles = (int64_t)a.a.S * p.key_tiles * a.a.Hkv;
+  const int64_t ctas = std::min<int64_t>((tiles + kKrWarps - 1) / kKrWarps, sm_count() * 2);
+  return launch_early(key_mass_rows_f32_kernel<D, NT>, static_cast<int>(std::max<int64_t>(1, ctas)), kKrThreads, 0, stream, p);
+}
+
 cudaError_t launch_key_mass_rows(const KeyMassArgs& a, int dtype, cudaStream_t stream) {
+  if (dtype == SPRUCE_DTYPE_F32) {
+    const bool eight = (int64_t)a.a.max_q * (a.a.Hq / a.a.Hkv) <= 8;
+    if (a.a.D == 128) return eight ? launch_f32<128, 1>(a, stream) : launch_f32<128, 2>(a, stream);
+    return eight ? launch_f32<64, 1>(a, stream) : launch_f32<64, 2>(a, stream);
+  }
   if (dtype == SPRUCE_DTYPE_BF16)
     return a.a.D == 128 ? launch_tiles<__nv_bfloat16, 128>(a, stream) : launch_tiles<__nv_bfloat16, 64>(a, stream);
   return a.a.D == 128 ? launch_tiles<__half, 128>(a, stream) : launch_tiles<__half, 64>(a, stream);

@@ -14,7 +14,7 @@
 
 namespace spruce {
 
-constexpr int kTileKeys = 64, kTileThreads = 256;
+constexpr int kTileKeys = 64, kTileRows = 64, kTileThreads = 256;
 
 // Four elements of a row as floats.
 template <typename T>
@@ -53,9 +53,9 @@ __device__ __forceinline__ void tile_scores(const float* A, int ra, const float*
 
 // ------------------------------------------------------------------ key mass
 // One (sequence, KV head, 64 keys) at a time; R query rows a step.
-template <typename T, int D, int R>
+template <typename T, int D>
 __global__ void __launch_bounds__(kTileThreads) key_mass_tile_kernel(const KeyMassParams p) {
-  constexpr int P = D + 4, N = R / 16;
+  constexpr int R = kTileRows, P = D + 4, N = R / 16;
   extern __shared__ float sm[];
   float* Ks = sm;                      // [64][P]
   float* Qs = Ks + kTileKeys * P;      // [R][P]
@@ -121,10 +121,10 @@ __global__ void __launch_bounds__(kTileThreads) key_mass_tile_kernel(const KeyMa
   }
 }
 
-template <typename T, int D, int R>
+template <typename T, int D>
 static cudaError_t launch_tile(const KeyMassArgs& a, int sms, cudaStream_t stream) {
-  constexpr int smem = sizeof(float) * ((kTileKeys + R) * (D + 4) + 2 * R);
-  auto kern = key_mass_tile_kernel<T, D, R>;
+  constexpr int R = kTileRows, smem = sizeof(float) * ((kTileKeys + R) * (D + 4) + 2 * R);
+  auto kern = key_mass_tile_kernel<T, D>;
   static std::atomic<uint64_t> done{0};
   cudaError_t e = allow_smem(reinterpret_cast<const void*>(kern), smem, done);
   if (e != cudaSuccess) return e;
@@ -136,24 +136,20 @@ static cudaError_t launch_tile(const KeyMassArgs& a, int sms, cudaStream_t strea
 
 template <typename T>
 static cudaError_t launch_key_mass_t(const KeyMassArgs& a, int sms, cudaStream_t stream) {
-  const bool few = (int64_t)a.a.max_q * (a.a.Hq / a.a.Hkv) <= 16;
-  if (a.a.D == 128) return few ? launch_tile<T, 128, 16>(a, sms, stream) : launch_tile<T, 128, 64>(a, sms, stream);
-  return few ? launch_tile<T, 64, 16>(a, sms, stream) : launch_tile<T, 64, 64>(a, sms, stream);
+  return a.a.D == 128 ? launch_tile<T, 128>(a, sms, stream) : launch_tile<T, 64>(a, sms, stream);
 }
 
+// fp32 rows by the lanes of a warp where they are few (16 sequences of 2000 to 8000 tokens, 7 rows: 135 us by tiles of 64 rows);
+// 16 bits on the tensor cores, but where a group has more heads than a row tile has rows.
 cudaError_t launch_key_mass(const KeyMassArgs& a, int dtype, cudaStream_t stream) {
   const int sms = sm_count();
   if (key_mass_params(a, kTileKeys).key_tiles == 0) return cudaSuccess;
   const int rep = a.a.Hq / a.a.Hkv;
-  if (dtype != SPRUCE_DTYPE_F32) {
-    if ((int64_t)a.a.max_q * rep <= kKmFewRows) return launch_key_mass_rows(a, dtype, stream);
-    if (rep <= 128) return launch_key_mass_sm100(a, dtype, stream);
-  }
-  switch (dtype) {
-    case SPRUCE_DTYPE_F32: return launch_key_mass_t<float>(a, sms, stream);
-    case SPRUCE_DTYPE_BF16: return launch_key_mass_t<__nv_bfloat16>(a, sms, stream);
-    default: return launch_key_mass_t<__half>(a, sms, stream);
-  }
+  const int64_t rows = (int64_t)a.a.max_q * rep;
+  if (rows <= (dtype == SPRUCE_DTYPE_F32 ? kKmFewRowsF32 : kKmFewRows)) return launch_key_mass_rows(a, dtype, stream);
+  if (dtype == SPRUCE_DTYPE_F32) return launch_key_mass_t<float>(a, sms, stream);
+  if (rep <= 128) return launch_key_mass_sm100(a, dtype, stream);
+  return dtype == SPRUCE_DTYPE_BF16 ? launch_key_mass_t<__nv_bfloat16>(a, sms, stream) : launch_key_mass_t<__half>(a, sms, stream);
 }
 
 // ------------------------------------------------------------------ block mass

@@ -34,9 +34,9 @@ inline KeyMassParams key_mass_params(const KeyMassArgs& a, int tile) {
 }
 
 // Key mass of more than kKmFewRows query rows a sequence and KV head, in 16 bits (key_mass_sm100.cu).
-constexpr int kKmFewRows = 32;
+constexpr int kKmFewRows = 32, kKmFewRowsF32 = 16;
 cudaError_t launch_key_mass_sm100(const KeyMassArgs& a, int dtype, cudaStream_t stream);
-// At most that many, in 16 bits (key_mass_rows.cu).
+// At most that many (key_mass_rows.cu).
 cudaError_t launch_key_mass_rows(const KeyMassArgs& a, int dtype, cudaStream_t stream);
 
 // Block mass in 16 bits (block_mass_sm100.cu).
