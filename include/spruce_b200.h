@@ -525,7 +525,8 @@ SPRUCE_API int spruce_paged_attention_lse(const spruce_paged_attention_lse_args 
  * for every slot j of a sequence that has new tokens; slots of the new tokens themselves start from 0, whatever mass
  * holds there, and with decay = 0 no old value is read.  Sequences without new tokens, and all other slots, are left as they are.
  * lse is spruce_paged_attention_lse's; a row whose lse is -inf gives nothing.  mass and mass_out are fp32 [num_pages,
- * Hkv, page_size] by strides (page, head, row) and may be one.  Bounds, pages and alignment are spruce_paged_attention's:
+ * Hkv, page_size] by strides (page, head, row) and may be one; no page may belong to two sequences of the call (both would
+ * write its weights).  Bounds, pages and alignment are spruce_paged_attention's:
  * queries past max_q_len give none, and slots that only they see, those past max_kv_len and those of a bad page are left as
  * they are.  A key that holds an infinity or a NaN may get any weight; it does not reach other keys.  Each sum is formed in a
  * fixed order.

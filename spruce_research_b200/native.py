@@ -722,7 +722,8 @@ def paged_key_mass(q: torch.Tensor, k_cache: torch.Tensor, mass: torch.Tensor, b
     ``mass'[j] = decay * mass[j] + sum over queries i that see j and heads h of j's group of exp(scale q_ih.k_j - lse_ih)``
     for each slot of a sequence with new tokens; the new tokens' own slots start from 0.  With ``decay`` 0 nothing old
     is read.  The batch is described as for :func:`paged_attention`, whose ``lse`` [N, Hq] this takes.  ``out`` (``mass`` itself
-    by default) receives the sums; slots of no such sequence are left as they are.
+    by default) receives the sums; slots of no such sequence are left as they are.  No page may belong to two sequences of
+    the call: both would write its weights.
     """
     out = mass if out is None else out
     device = q.get_device()

@@ -183,3 +183,54 @@ def test_the_same_cache_is_cut_twice_then_replayed_in_a_graph():
     assert torch.equal(kept, kept2) and torch.equal(lens, lens2)
     assert all(torch.equal(a, b) for a, b in zip(want, (to.k, to.v, to.mass)))
     assert native.paged_evict(c.k, c.v, c.mass, c.table[:0], c.kv[:0], 10, max_kv_len=5)[0].shape == (0, 2, 5)
+
+
+@pytest.mark.parametrize("into", [False, True])
+def test_pieces_of_more_slots_than_shared_memory_holds(into):
+    """A million slots of one head: the weights past those that a CTA keeps are read again."""
+    n, keep, page = 1_000_003, 5001, 64
+    g = torch.Generator(device="cuda").manual_seed(1)
+    pages = -(-n // page)
+    table = torch.randperm(pages, generator=torch.Generator().manual_seed(1)).int()[None].cuda()
+    k = torch.randn(pages, 1, page, 8, generator=g, device="cuda", dtype=torch.bfloat16)
+    v, mass = k + 1, torch.rand(pages, 1, page, generator=g, device="cuda").mul_(4096).floor_()      # many ties
+    kv = torch.tensor([n], device="cuda", dtype=torch.int32)
+    flat = [x[:, 0][table[0].long()].reshape(pages * page, -1)[:n] for x in (k, v, mass[..., None])]
+    w = flat[2][:, 0].clone()
+    w[:3], w[n - 100:] = math.inf, math.inf
+    want = torch.sort(w, descending=True, stable=True).indices[:keep].sort().values
+    to = (torch.zeros(100, 1, page, 8, device="cuda", dtype=torch.bfloat16), torch.zeros(100, 1, page, 8, device="cuda", dtype=torch.bfloat16),
+          torch.zeros(100, 1, page, device="cuda"), torch.arange(100, device="cuda", dtype=torch.int32)[None])
+    kept, lens = native.paged_evict(k, v, mass, table, kv, keep, sinks=3, recent=100, max_kv_len=n, into=to if into else None)
+    assert lens.item() == keep and torch.equal(kept[0, 0].long(), want)
+    j = torch.arange(keep, device="cuda")
+    at = (to[3] if into else table)[0].long()[j // page]
+    for x, y in zip(to[:3] if into else (k, v, mass), flat):
+        assert torch.equal(x[at, 0, j % page].reshape(keep, -1), y[want])
+
+
+def test_heads_that_several_ctas_share_replay_in_a_graph():
+    c = Cache([40000, 9000], 2, 64, 64, torch.bfloat16)
+    to = Cache([3000, 3000], 2, 64, 64, torch.bfloat16, seed=3)
+    kw = dict(sinks=1, recent=9, max_kv_len=40000, into=(to.k, to.v, to.mass, to.table))
+    kept, lens = native.paged_evict(c.k, c.v, c.mass, c.table, c.kv, 3000, **kw)
+    want = [x.clone() for x in (to.k, to.v, to.mass)]
+    for s, heads in enumerate(c.want(3000, 1, 9)):
+        for h, slots in enumerate(heads):
+            assert kept[s, h].tolist() == slots
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        kept2, lens2 = native.paged_evict(c.k, c.v, c.mass, c.table, c.kv, 3000, **kw)
+    for x in (to.k, to.v, to.mass):
+        x.zero_()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        graph.replay()
+    side.synchronize()
+    assert torch.equal(kept, kept2) and torch.equal(lens, lens2)
+    j = torch.arange(3000, device="cuda")
+    for s in range(2):
+        at = to.table[s].long()[j // 64]
+        for x, y in zip((to.k, to.v, to.mass), want):
+            assert torch.equal(x[at, :, j % 64], y[at, :, j % 64])

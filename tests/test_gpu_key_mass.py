@@ -116,6 +116,19 @@ def test_weights_of_ragged_batches(dtype, heads, qlens, kvs, page):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("heads", [(130, 1, 64), (256, 2, 128), (65, 1, 64)])
+def test_groups_of_more_heads_than_a_row_tile_has_rows(dtype, heads):
+    check(Batch([3, 0, 1], [200, 9, 70], *heads, 32, dtype), decay=0.5)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_a_prompt_of_its_own_keys(dtype):
+    """Few keys under many rows: a cluster shares an item, and the diagonal crosses every row tile."""
+    check(Batch([1500], [1500], 8, 1, 128, 64, dtype), decay=0.0)
+    check(Batch([700], [1300], 4, 2, 64, 16, dtype), decay=1.0)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("decay", [0.0, 0.75, 1.0])
 @pytest.mark.parametrize("in_place", [True, False])
 @pytest.mark.parametrize("q", [1, 40])
