@@ -8,15 +8,17 @@
 // keys are through, 2^(b - total) is summed over the 64 rows of a query block: 32 a round by a transposing butterfly, 31
 // shuffles for 32 sums of a warp.  Heads are added by a second kernel in their order, so nothing depends on timing.
 //
-// Warps: 0-3 the first 64 keys of tile 0 (thread = row = TMEM lane), 4-7 the others, 8-15 likewise of tile 1, 16 issues the
-// MMAs and owns TMEM, 17 loads Q and K.  Four warps a scheduler hide each other's latencies (two of 128 keys a row: 4.72 ms
-// where these take 4.58).  Each S_t has two buffers, which fill TMEM: the tensor core runs a tile ahead of the exponentials, which bound the kernel
+// Warps: 0-3 the first 64 keys of tile 0 (thread = row = TMEM lane), 4-7 the others, 8-15 likewise of tile 1, 16 and 17
+// issue the MMAs of a tile each (a check of a barrier waits behind the MMAs that its warp has queued; one issuer for both: 4.55 ms
+// where two take 4.45), 16 owns TMEM, 18 loads Q and K.  Four softmax warps a scheduler hide each other's latencies (two of 128
+// keys a row: 4.72 ms where these took 4.58).  Each S_t has two buffers, which fill TMEM: the tensor core runs a tile ahead of the exponentials, which bound the kernel
 // (16 a clock and SM, against 32 scores a clock of the MMAs at d = 128).  Part of them runs on the FMA pipe instead, as a
-// polynomial of degree 4 with a relative error of 2.7e-6: an eighth (none, 1/8, 1/4, 3/8: 4.65, 4.58, 4.58, 4.78 ms; the
+// polynomial of degree 4 with a relative error of 2.7e-6: a quarter (none, 1/8, 1/4, 3/8: 4.62, 4.53, 4.48, 4.78 ms; the
 // issue slots bound what the exponentials leave).  Exponentials over an old maximum, without a pass for the block's own,
 // measured 1.5% slower: the branch for a row that outgrows it keeps blocks from overlapping.
 //
-// On a B200, 28 query / 4 KV heads of 128 in bf16: 32768 tokens 4.58 ms, 840 TFLOP/s; the exponentials' pipe 78% busy.
+// On a B200, 28 query / 4 KV heads of 128 in bf16: 32768 tokens 4.48 ms, 859 TFLOP/s (the exponentials alone would take 2.9 ms
+// with a quarter on the FMA pipe or 3.2 without, the MMAs 2.4).
 //
 // Units go to the CTAs longest first, back and forth over them.
 //
@@ -29,9 +31,9 @@
 
 namespace spruce {
 
-constexpr int kBmThreads = 576, kBmMma = 16, kBmLoad = 17;
+constexpr int kBmThreads = 608, kBmMma = 16, kBmMma1 = 17, kBmLoad = 18;
 constexpr int kBmKeys = 128;
-constexpr int kBmMufu = 7;  // of 8 pairs of exponentials; the others by polynomial
+constexpr int kBmMufu = 6;  // of 8 pairs of exponentials; the others by polynomial
 
 template <int D>
 struct BlockLayout {
@@ -44,8 +46,8 @@ struct BlockLayout {
   static constexpr int OFF_SUM = OFF_K + KST * TILE;     // [8 pairs of warps][2][32] floats: sums handed to the other warp of a block
   static constexpr int OFF_ML = OFF_SUM + 8 * 2 * 32 * 4;  // [2][2 tiles][2 halves][128] maxima and sums
   static constexpr int OFF_BAR = OFF_ML + 2 * 512 * 8;
-  // k_full[], k_empty[], q_full, q_empty, s_full[2][2], s_empty[2][2], drain
-  static constexpr int NBAR = 2 * KST + 2 + 4 + 4 + 1;
+  // k_full[], k_empty[], q_full, q_empty, s_full[2][2], s_empty[2][2], drain[2]
+  static constexpr int NBAR = 2 * KST + 2 + 4 + 4 + 2;
   static constexpr int OFF_MISC = OFF_BAR + NBAR * 8;
   static constexpr int BYTES = 1024 + OFF_MISC + 16;
   static_assert(BYTES <= 227 * 1024, "shared memory of a CTA");
@@ -130,12 +132,18 @@ __global__ void __launch_bounds__(kBmThreads, 1)
   if (warp == kBmLoad) {
     if (lane == 0) {
       *abort_flag = 0;
-      for (int s = 0; s < 2 * KST + 2; ++s) mbar_init(&k_full[s], 1);  // and k_empty, q_full, q_empty
+      for (int s = 0; s < KST; ++s) {
+        mbar_init(&k_full[s], 1);
+        mbar_init(&k_empty[s], 2);
+      }
+      mbar_init(q_full, 1);
+      mbar_init(q_empty, 2);
       for (int s = 0; s < 4; ++s) {
         mbar_init(&s_full[s], 1);
         mbar_init(&s_empty[s], 256);
       }
-      mbar_init(drain, 1);
+      mbar_init(&drain[0], 1);
+      mbar_init(&drain[1], 1);
       fence_barrier_init();
       prefetch_tmap(&tmq);
       prefetch_tmap(&tmk);
@@ -192,11 +200,12 @@ __global__ void __launch_bounds__(kBmThreads, 1)
     }
     for (int k = max(0, loaded - KST); k < loaded; ++k) mbar_wait(&k_full[k % KST], (k / KST) & 1, status, nullptr);
     __syncwarp();
-  } else if (warp == kBmMma) {
-    // ------------------------------------------------------------ MMA issuer
+  } else if (warp == kBmMma || warp == kBmMma1) {
+    // ------------------------------------------------------------ MMA issuers, one a tile
     const bool leader = elect_one();
+    const int t = warp - kBmMma;
     constexpr uint32_t idesc = idesc_f16(UmmaFormat<T>::value, 0, 0, 128, 128);
-    const uint64_t dq0 = smem_desc(smem_u32(smem + L::OFF_Q), 16, 1024);
+    const uint64_t dq0 = smem_desc(smem_u32(smem + L::OFF_Q + t * L::TILE), 16, 1024);
     const uint64_t dk0 = smem_desc(smem_u32(smem + L::OFF_K), 16, 1024);
     auto commit = [&](uint64_t* bar) {
       if (leader) umma_commit(bar);
@@ -206,34 +215,29 @@ __global__ void __launch_bounds__(kBmThreads, 1)
       return __all_sync(0xffffffffu, mbar_wait(bar, parity, status, abort_flag));
     };
     int st = 0;
-    uint32_t turn = 0, issued[2] = {0, 0};
+    uint32_t turn = 0, issued = 0;
     bool ok = true;
     for (int r = 0; ok && block_unit(p, r, u); ++r) {
       if (!(ok = wait(q_full, r & 1))) break;
       const int n = max(u.keys[0], u.keys[1]);
-      for (int j = 0; ok && j < n; ++j) {
-        // A check of a barrier waits behind this warp's queued MMAs: all that a step needs is checked before its MMAs.
+      for (int j = 0; j < n; ++j) {
         ok = wait(&k_full[st], turn);
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-          if (ok && j < u.keys[t] && issued[t] >= 2)
-            ok = wait(&s_empty[2 * t + (issued[t] & 1)], ((issued[t] >> 1) - 1) & 1);
-        if (!ok) break;
-        tc_fence_after();
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          if (j >= u.keys[t]) continue;
-          const uint32_t buf = issued[t]++ & 1;
+        if (ok && j < u.keys[t]) {
+          const uint32_t buf = issued & 1;
+          if (issued >= 2) ok = wait(&s_empty[2 * t + buf], ((issued >> 1) - 1) & 1);
+          if (!ok) break;
+          ++issued;
+          tc_fence_after();
 #pragma unroll
           for (int ks = 0; ks < D / 16; ++ks) {
             const uint32_t off = ((ks >> 2) * L::PANEL + (ks & 3) * 32) >> 4;
             if (leader)
-              umma_f16_ss(tmem + (2 * t + buf) * 128, dq0 + ((t * L::TILE) >> 4) + off, dk0 + ((st * L::TILE) >> 4) + off,
-                          idesc, ks > 0 ? 1u : 0u);
+              umma_f16_ss(tmem + (2 * t + buf) * 128, dq0 + off, dk0 + ((st * L::TILE) >> 4) + off, idesc, ks > 0 ? 1u : 0u);
             __syncwarp();
           }
           commit(&s_full[2 * t + buf]);
         }
+        if (!ok) break;
         commit(&k_empty[st]);
         if (++st == KST) {
           st = 0;
@@ -242,8 +246,8 @@ __global__ void __launch_bounds__(kBmThreads, 1)
       }
       if (ok) commit(q_empty);
     }
-    commit(drain);  // no MMA may be in flight when TMEM is released
-    mbar_wait(drain, 0, status, nullptr);
+    commit(&drain[t]);  // no MMA may be in flight when TMEM is released
+    mbar_wait(&drain[t], 0, status, nullptr);
     __syncwarp();
   } else {
     // ------------------------------------------------------------ softmax and sums

@@ -19,7 +19,7 @@
 
 namespace spruce {
 
-constexpr int kKrThreads = 256, kKrWarps = kKrThreads / 32;
+constexpr int kKrThreads = 128, kKrWarps = kKrThreads / 32;
 constexpr int kKrTile = 16;
 
 template <typename T>
@@ -34,8 +34,9 @@ __device__ __forceinline__ void kr_mma(float (&c)[4], uint32_t a0, uint32_t a1, 
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// CTAs an SM: three where the fragments of the query rows leave registers for it.
-template <int D, int NT> constexpr int kKrPerSm = D * NT <= 128 ? 3 : 2;
+// CTAs an SM: as many as the fragments of the query rows leave registers for.
+template <int D, int NT> constexpr int kKrPerSm = D * NT <= 128 ? 6 : (D * NT == 512 ? 3 : 4);
+constexpr int kKrPerSmF32 = 4;
 
 // NT: tiles of 8 query rows.
 template <typename T, int D, int NT>
@@ -145,7 +146,7 @@ __global__ void __launch_bounds__(kKrThreads, kKrPerSm<D, NT>) key_mass_rows_ker
 // Eight lanes a key, each with D / 8 dims of it; the query rows come from shared memory.  Eight rows' partial dots are summed over the
 // lanes by a transposing butterfly (7 shuffles), which leaves row c with lane c.
 template <int D, int NT>
-__global__ void __launch_bounds__(kKrThreads, 2) key_mass_rows_f32_kernel(const KeyMassParams p) {
+__global__ void __launch_bounds__(kKrThreads, kKrPerSmF32) key_mass_rows_f32_kernel(const KeyMassParams p) {
   constexpr int R = 8 * NT, CH = D / 32;
   using Walk = PagedWalk<R, kKrTile>;
   __shared__ __align__(16) float Q[R][D];
@@ -262,7 +263,7 @@ static cudaError_t launch_f32(const KeyMassArgs& a, cudaStream_t stream) {
   KeyMassParams p = key_mass_params(a, kKrTile);
   p.v = paged_params(a.a, 8 * NT, 1, 4);
   const int64_t tiles = (int64_t)a.a.S * p.key_tiles * a.a.Hkv;
-  const int64_t ctas = std::min<int64_t>((tiles + kKrWarps - 1) / kKrWarps, sm_count() * 2);
+  const int64_t ctas = std::min<int64_t>((tiles + kKrWarps - 1) / kKrWarps, sm_count() * kKrPerSmF32);
   return launch_early(key_mass_rows_f32_kernel<D, NT>, static_cast<int>(std::max<int64_t>(1, ctas)), kKrThreads, 0, stream, p);
 }
 
