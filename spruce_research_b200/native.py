@@ -864,7 +864,7 @@ def _row_major(t: torch.Tensor, rows: int) -> torch.Tensor:
     """[..., n] as [rows, n] with a unit last stride."""
     if t.dim() != 2:
         t = t.reshape(rows, t.shape[-1])
-    return t if t.stride(1) == 1 or t.shape[1] <= 1 else t.contiguous()
+    return t if t.stride(1) == 1 else t.contiguous()
 
 
 def _distill(scores, ids, teacher, visible, temperature, status, *, loss=False, stats=None, want_stats=False,
@@ -874,29 +874,35 @@ def _distill(scores, ids, teacher, visible, temperature, status, *, loss=False, 
     if not (device == ids.get_device() == teacher.get_device()
             and _on_one_device(device, visible, stats, weight, status)):
         _refuse_devices(scores, ids, teacher, visible, stats, weight, status)
-    if scores.dim() < 1 or ids.dim() != scores.dim() or ids.shape[:-1] != scores.shape[:-1] or teacher.shape != ids.shape:
-        raise ValueError(f"expected scores [..., n], ids [..., K] and teacher [..., K], got {tuple(scores.shape)}, "
-                         f"{tuple(ids.shape)}, {tuple(teacher.shape)}")
-    if ids.dtype not in (torch.int32, torch.int64):
+    shape, ids_shape = scores.shape, ids.shape
+    lead = shape[:-1]
+    if len(shape) < 1 or len(ids_shape) != len(shape) or ids_shape[:-1] != lead or teacher.shape != ids_shape:
+        raise ValueError(f"expected scores [..., n], ids [..., K] and teacher [..., K], got {tuple(shape)}, "
+                         f"{tuple(ids_shape)}, {tuple(teacher.shape)}")
+    ids64 = ids.dtype is torch.int64
+    if not ids64 and ids.dtype is not torch.int32:
         raise ValueError(f"ids must be int32 or int64, got {ids.dtype}")
-    lead, n, K = scores.shape[:-1], scores.shape[-1], ids.shape[-1]
-    R = math.prod(lead)
+    n, K = shape[-1], ids_shape[-1]
+    flat = len(lead) == 1
+    R = lead[0] if flat else math.prod(lead)
     if visible is not None:
-        if visible.dtype != torch.int32 or visible.shape != lead:
+        if visible.dtype is not torch.int32 or visible.shape != lead:
             raise ValueError(f"visible must be int32 {tuple(lead)}, got {visible.dtype} {tuple(visible.shape)}")
-        visible = visible.contiguous() if len(lead) == 1 else visible.reshape(R).contiguous()
+        visible = visible.contiguous() if flat else visible.reshape(R).contiguous()
+    step = 0
     if weight is not None:
-        if weight.dtype != torch.float32 or weight.shape != lead:
+        if weight.dtype is not torch.float32 or weight.shape != lead:
             raise ValueError(f"the rows' weights must be float32 {tuple(lead)}, got {weight.dtype} {tuple(weight.shape)}")
-        weight = weight if len(lead) == 1 else weight.reshape(R)
+        weight = weight if flat else weight.reshape(R)
+        step = weight.stride(0)
     x, i, t = _row_major(scores, R), _row_major(ids, R), _row_major(teacher, R)
-    out = torch.empty(lead, device=x.device, dtype=torch.float32) if loss else None
-    made = torch.empty((R, 2), device=x.device, dtype=torch.float32) if want_stats else None
-    grad = torch.empty(scores.shape, device=x.device, dtype=x.dtype) if weight is not None else None
+    out = scores.new_empty(lead, dtype=torch.float32) if loss else None
+    made = scores.new_empty((R, 2), dtype=torch.float32) if want_stats else None
+    grad = scores.new_empty(shape) if weight is not None else None
     args = _lib.TOPK_DISTILL_ARGS.pack(
         x.data_ptr(), i.data_ptr(), t.data_ptr(), _ptr(visible), _ptr(out), _ptr(made), _ptr(stats), _ptr(weight),
-        _ptr(grad), _status_ptr(status), _lib.stream_on(device), x.stride(0), i.stride(0), t.stride(0),
-        weight.stride(0) if weight is not None else 0, n, _dt(x), _dt(t), i.dtype == torch.int64, R, n, K, temperature)
+        _ptr(grad), _status_ptr(status), _lib.stream_on(device), x.stride(0), i.stride(0), t.stride(0), step, n, _dt(x), _dt(t),
+        ids64, R, n, K, temperature)
     _lib.launch(_lib.load().spruce_topk_distill, args, device)
     return out, made, grad
 
