@@ -780,12 +780,14 @@ def paged_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, mass: torch.Tensor
         raise ValueError(f"the caches of `into` must be [pages, {Hkv}, {page_size}, {D}], got {tuple(to_shape)}")
     if not k_cache.dtype == v_cache.dtype == k_out.dtype == v_out.dtype:
         raise ValueError("the caches must share a dtype")
-    if any(x.stride(3) != 1 for x in (k_cache, v_cache, k_out, v_out)):
+    ks, vs = k_cache.stride(), v_cache.stride()
+    kos, vos = (ks, vs) if into is None else (k_out.stride(), v_out.stride())
+    if not ks[3] == vs[3] == kos[3] == vos[3] == 1:
         raise ValueError("the caches need a unit last stride")
     _check_mass(mass, shape, "mass")
     _check_mass(mass_out, to_shape, "the mass of `into`")
     S = kv_lens.numel()
-    for table in (block_table, out_table):
+    for table in (block_table,) if into is None else (block_table, out_table):
         if table.dtype != torch.int32 or table.dim() != 2 or table.shape[0] != S:
             raise ValueError(f"a block table must be int32 [{S}, pages], got {table.dtype} {tuple(table.shape)}")
         if table.shape[1] > 1 and table.stride(1) != 1:
@@ -796,16 +798,21 @@ def paged_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, mass: torch.Tensor
     if keep < 0 or max_kv_len < 0:
         raise ValueError("keep and max_kv_len must not be negative")
     kept = kv_lens.new_empty((S, Hkv, min(keep, max_kv_len)))
-    lens = torch.empty_like(kv_lens)
+    lens = kv_lens.new_empty(S)
     args = _lib.PAGED_EVICT_ARGS.pack(
         k_cache.data_ptr(), v_cache.data_ptr(), mass.data_ptr(), k_out.data_ptr(), v_out.data_ptr(),
         mass_out.data_ptr(), block_table.data_ptr(), out_table.data_ptr(), kv_lens.data_ptr(), kept.data_ptr(),
-        lens.data_ptr(), _status_ptr(status), _lib.stream_on(device), *k_cache.stride()[:3], *v_cache.stride()[:3],
-        *mass.stride(), *k_out.stride()[:3], *v_out.stride()[:3], *mass_out.stride(), _dt(k_cache), S, Hkv, D, pages,
+        lens.data_ptr(), _status_ptr(status), _lib.stream_on(device), *ks[:3], *vs[:3],
+        *mass.stride(), *kos[:3], *vos[:3], *mass_out.stride(), _dt(k_cache), S, Hkv, D, pages,
         page_size, block_table.stride(0), block_table.shape[1], to_shape[0], out_table.stride(0), out_table.shape[1],
         max_kv_len, kept.shape[2], keep, sinks, recent)
     _lib.launch(_lib.load().spruce_paged_evict, args, device)
     return kept, lens
+
+
+@functools.lru_cache(maxsize=256)
+def _block_mass_workspace_bytes(B: int, Hq: int, Hkv: int, T: int, D: int, dtype: int) -> int:
+    return int(_lib.load().spruce_block_mass_workspace_bytes(B, Hq, Hkv, T, D, dtype))
 
 
 def block_mass(q: torch.Tensor, k: torch.Tensor, *, scale: float | None = None, out: torch.Tensor | None = None,
@@ -818,46 +825,48 @@ def block_mass(q: torch.Tensor, k: torch.Tensor, *, scale: float | None = None, 
     device = q.get_device()
     if not (device == k.get_device() and _on_one_device(device, out, workspace, status)):
         _refuse_devices(q, k, out, workspace, status)
-    if q.dim() != 4 or k.dim() != 4:
+    shape, ks = q.shape, k.shape
+    if len(shape) != 4 or len(ks) != 4:
         raise ValueError("q and k must be [B, H, T, D]")
-    B, Hq, T, D = q.shape
-    Hkv = k.shape[1]
+    B, Hq, T, D = shape
+    Hkv = ks[1]
     if q.dtype != k.dtype:
         raise ValueError("q and k must share a dtype")
-    if k.shape[0] != B or k.shape[2] != T or k.shape[3] != D:
-        raise ValueError(f"k must be [{B}, Hkv, {T}, {D}], got {tuple(k.shape)}")
+    if ks[0] != B or ks[2] != T or ks[3] != D:
+        raise ValueError(f"k must be [{B}, Hkv, {T}, {D}], got {tuple(ks)}")
     dt, qb = _dt(q), (T + BLOCK - 1) // BLOCK
-    q, k = _tma_ok(q), _tma_ok(k)
+    q, q_strides = _tma_ok(q)
+    k, k_strides = _tma_ok(k)
     if out is None:
-        out = torch.empty((B, Hkv, qb, qb), device=q.device, dtype=torch.float32)
+        out = q.new_empty((B, Hkv, qb, qb), dtype=torch.float32)
     elif tuple(out.shape) != (B, Hkv, qb, qb) or out.dtype != torch.float32 or not out.is_contiguous():
         raise ValueError(f"out must be contiguous float32 {(B, Hkv, qb, qb)}")
     if workspace is None:
-        nbytes = _lib.load().spruce_block_mass_workspace_bytes(B, Hq, Hkv, T, D, dt)
+        nbytes = _block_mass_workspace_bytes(B, Hq, Hkv, T, D, dt)
         if nbytes < 0:
-            raise ValueError(f"bad block mass shape: q {tuple(q.shape)}, k {tuple(k.shape)}")
-        workspace = torch.empty(nbytes // 4, device=q.device, dtype=torch.float32)
+            raise ValueError(f"bad block mass shape: q {tuple(shape)}, k {tuple(ks)}")
+        workspace = q.new_empty(nbytes // 4, dtype=torch.float32)
     elif not workspace.is_contiguous():
         raise ValueError("workspace must be contiguous")
     else:
         nbytes = workspace.nbytes
     args = _lib.BLOCK_MASS_ARGS.pack(
         q.data_ptr(), k.data_ptr(), out.data_ptr(), workspace.data_ptr(), _status_ptr(status), _lib.stream_on(device),
-        *q.stride(), *k.stride(), dt, B, Hq, Hkv, T, D, nbytes, D ** -0.5 if scale is None else scale)
+        *q_strides, *k_strides, dt, B, Hq, Hkv, T, D, nbytes, D ** -0.5 if scale is None else scale)
     _lib.launch(_lib.load().spruce_block_mass, args, device)
     return out
 
 
-def _tma_ok(t: torch.Tensor) -> torch.Tensor:
-    """A view whose rows are 16-byte aligned and that steps forwards (a copy only if it is not)."""
+def _tma_ok(t: torch.Tensor) -> tuple[torch.Tensor, tuple]:
+    """[B, H, T, D] with 16-byte aligned rows that steps forwards (a copy only if it is not), and strides to say so."""
     vn = 16 // t.element_size()
-    if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(
-            n == 1 or (s > 0 and s % vn == 0) for n, s in zip(t.shape[:-1], t.stride()[:-1])):
-        if all(s % vn == 0 and s > 0 for s in t.stride()[:-1]):
-            return t
-        # A dimension of one element never steps: any stride will do.
-        return t.as_strided(t.shape, [s if n > 1 else t.shape[-1] for n, s in zip(t.shape[:-1], t.stride()[:-1])] + [1])
-    return t.clone(memory_format=torch.contiguous_format)
+    (b, h, n, d), (sb, sh, sn, sd) = t.shape, t.stride()
+    # A dimension of one element never steps: any stride will do.
+    sb, sh, sn = sb if b > 1 else d, sh if h > 1 else d, sn if n > 1 else d
+    if sd == 1 and t.data_ptr() % 16 == 0 and not (sb | sh | sn) % vn and min(sb, sh, sn) > 0:
+        return t, (sb, sh, sn, 1)
+    t = t.clone(memory_format=torch.contiguous_format)
+    return t, (h * n * d, n * d, d, 1)
 
 
 def _row_major(t: torch.Tensor, rows: int) -> torch.Tensor:
