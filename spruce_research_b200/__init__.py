@@ -11,6 +11,8 @@ Reference-named drop-ins:
   route_overrides          charged_route_density
 Per-layer pipeline: pipeline.SparsePrefillLayer; multi-GPU split: sharding.
 Serving: rope.rope_table, paged.PagedKVCache, paged.PagedSparseLayer (over native.qk_norm_rope,
-native.paged_append and native.paged_attention).
+native.paged_append and native.paged_attention); eviction by attention weight: paged.PagedKVCache.evict (over
+native.paged_key_mass and native.paged_evict).
+Teaching a gate: selector.train (over native.block_mass and selector.loss.topk_distill_loss).
 """
 __version__ = "0.1.0"

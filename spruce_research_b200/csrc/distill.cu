@@ -8,6 +8,10 @@
 // vocabulary's) take a CTA each, which keeps a running maximum and sum; its gradient pass reads the row again, mostly from L2 when
 // both run in one call.  The teacher's columns are written again after the others,
 // so that each element is rounded once.  A column named twice is found by a bitmap; only rows that have one search for it.
+//
+// On a B200: 4096 bf16 rows of 131072 columns, 64 entries each: forward 194 us (5.6 TB/s), backward 346 us (6.2 TB/s); 57344 fp32 rows
+// of 512, half of them visible, loss and gradient in one call: 61 us, bound by instruction issue (75%) and the latency of a
+// row's loads.  A warp that walks several rows and fetches the next one's entries ahead measured 68 to 90 us there.
 #include <algorithm>
 
 #include "mass_common.cuh"

@@ -8,7 +8,7 @@
 //
 // Work is split as the attention's: all key tiles of the batch laid end to end, cut into equal runs, one a CTA; its warps
 // take the run's tiles in turn.  A key belongs to one warp, so nothing is joined.  Bytes in flight come from the number of warps: a
-// tile each of 24 warps an SM measured 50 us where two or three tiles each of 16 took 59 and 63.  Loads are marked to leave
+// tile each of 24 warps an SM measured 50 us where two or three tiles each of 16 took 59 and 63 (CTAs of 128 or 256 threads alike).  Loads are marked to leave
 // the caches first (62 -> 54 us).
 //
 // On a B200, 64 sequences of 300 to 8192 tokens, 28 query / 4 KV heads of 128 in bf16: 50 us, 5.7 TB/s.
@@ -144,7 +144,8 @@ __global__ void __launch_bounds__(kKrThreads, kKrPerSm<D, NT>) key_mass_rows_ker
 
 // ------------------------------------------------------------------ fp32
 // Eight lanes a key, each with D / 8 dims of it; the query rows come from shared memory.  Eight rows' partial dots are summed over the
-// lanes by a transposing butterfly (7 shuffles), which leaves row c with lane c.
+// lanes by a transposing butterfly (7 shuffles), which leaves row c with lane c.  16 sequences of 2000 to 8000 tokens, 28 / 4 heads of
+// 128: 36 us, 4.5 TB/s.
 template <int D, int NT>
 __global__ void __launch_bounds__(kKrThreads, kKrPerSmF32) key_mass_rows_f32_kernel(const KeyMassParams p) {
   constexpr int R = 8 * NT, CH = D / 32;

@@ -12,6 +12,12 @@
 // tensor core idle), 16 owns TMEM, 18 loads K (an item ahead) and Q, 19 works the items out and brings the rows' lse and limits.  Each S^T_t has two
 // buffers.
 //
+// Bound by the softmax warps: 16 exponentials a clock and SM (2048 clocks a step of 256 keys x 128 rows) and their issue, which
+// took 2460 of a step's 2960 clocks; the MMAs take 1100 and K comes from HBM behind them.  All exponentials are the hardware's: a
+// polynomial on the FMA pipe takes NaN for a number, and a row's NaN stands in one column only.
+// On a B200, 28 query / 4 KV heads of 128 in bf16: 64 tokens over 131072 99 us (608 TFLOP/s); a ragged fp16 batch of 9
+// sequences of up to 3000 tokens and 300 new ones 16 us.
+//
 // Every wait is bounded (common.cuh).
 #include <algorithm>
 #include <type_traits>

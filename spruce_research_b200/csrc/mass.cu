@@ -8,6 +8,11 @@
 // pass over the keys is enough, and a key's sum belongs to one CTA: no atomics, the order is fixed.  The block mass goes
 // over the scores once as well: for every row and key block it keeps b = log2(sum of 2^s over the block), from which the
 // row's total and then every weight 2^(b - total) follow, one exponential a (row, block) more.
+//
+// 16-bit inputs have tensor-core kernels (key_mass_rows.cu, key_mass_sm100.cu, block_mass_sm100.cu); these serve fp32, and key
+// mass with more than 128 heads a group.  Bound by the FMA pipe and shared-memory reads (4 x 4 scores a thread: 8 wavefronts to 64
+// FMAs).  On a B200 in fp32, 28 / 4 heads of 128: 64 tokens over 16K 280 us (26 TFLOP/s), block mass of 4000 tokens 3.1 ms
+// (19 TFLOP/s).
 #include <algorithm>
 
 #include "mass_common.cuh"
