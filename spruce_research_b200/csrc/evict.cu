@@ -12,7 +12,8 @@
 // pages there is nothing to wait for: a warp takes 32 whole rows.
 //
 // On a B200 (4 KV heads of 128, bf16): one sequence of 131072 tokens cut to 16384 36 us, of which the selection, a chain of nine
-// cluster barriers, takes about 20; 64 sequences of 300 to 8192 tokens cut to 2048 101 us, 82 of them the copy (5.9 TB/s).
+// cluster barriers, takes about 20; 64 sequences of 300 to 8192 tokens cut to 2048 101 us, 82 of them the copy (5.9 TB/s).  In place
+// 87 and 174 us: rounds of short pieces of scattered rows.
 #include <algorithm>
 
 #include "mass_common.cuh"
@@ -69,6 +70,7 @@ __device__ __forceinline__ int evict_page(const int32_t* table, int index, int64
   return -1;
 }
 
+// 256 threads measured 41 us and 1024 as much as 512 for one long sequence, 110 and 105 against 101 us for 64 (with the copies).
 constexpr int kSelectThreads = 512, kSelectWarps = kSelectThreads / 32;
 constexpr int kSelectBins = 2048, kSelectMostCtas = 16;
 constexpr int kSelectCached = 48 * 1024;  // slots of a CTA whose weights fit in shared memory; longer pieces are read again
@@ -306,8 +308,8 @@ __global__ void __launch_bounds__(kSelectThreads, 2)
 
 // In place: a CTA takes a slice of the columns of all rows, so that the rows' order is its own affair.  A round is kMoveRows rows a
 // thread; the places of the next are looked up while this one's rows are on their way.
-constexpr int kMoveThreads = 256, kMoveRows = 8;
-constexpr int kMoveSlice = 32;  // bytes of a row that a CTA takes
+constexpr int kMoveThreads = 1024, kMoveRows = 4;
+constexpr int kMoveSlice = 32;  // bytes of a row that a CTA takes, twice that where there are more CTAs than the GPU holds
 
 template <typename V>
 __device__ __forceinline__ void move_rows(const EvictArgs& a, const PageDiv& pd, const EvictSeq& q, int s, int g, char* data,
@@ -461,7 +463,10 @@ cudaError_t launch_evict(const EvictArgs& a, cudaStream_t stream) {
   if (e != cudaSuccess || most == 0) return e;
   const int row = a.D * a.es;
   if (a.in_place) {
-    const int slice = row % kMoveSlice == 0 ? kMoveSlice : 16;
+    // 256 threads of 8 rows, 32 bytes: 110 us for one sequence of 131072 tokens cut to 16384, 272 for 64 cut to 2048; 1024 threads of
+    // 4 rows 87 and 213; 64 bytes 109 and 174.
+    int slice = row % kMoveSlice == 0 ? kMoveSlice : 16;
+    if (row % (2 * slice) == 0 && heads * (2 * (row / slice) + 1) > 2 * sm_count()) slice *= 2;
     return launch_early(evict_move_kernel, static_cast<int>(heads * (2 * (row / slice) + 1)), kMoveThreads, 0, stream, a, pd,
                         row / slice, slice / 16);
   }

@@ -167,6 +167,21 @@ def test_strided_weights_and_queries(q):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("q, kv", [(1, 90), (1, 9000), (60, 90), (300, 2500)])   # whole units and joined ones of each kernel
+def test_log_sums_into_columns_of_a_wider_tensor(dtype, q, kv):
+    """By strides, nothing beside them; rows of no sequence keep what they had."""
+    b = Batch([q, 0, 2], [kv, 7, 2], 8, 2, 64, 16, dtype)
+    lse = torch.empty(b.q.shape[:2], device="cuda")
+    out = b.call(lse=lse)
+    wide = torch.full((b.q.shape[0] + 3, 20), 7.0, device="cuda")
+    padded = torch.cat([b.q, b.q[:3]])
+    got = native.paged_attention(padded, b.kc, b.vc, b.table, b.cu, b.kv, max_q_len=max(q, 2), max_kv_len=kv,
+                                 out=torch.full_like(padded, 7.0), lse=wide[:, 4:12])
+    assert torch.equal(got[:-3], out) and (got[-3:] == 7).all()
+    assert torch.equal(wide[:-3, 4:12], lse) and (wide[-3:] == 7).all() and (wide[:, :4] == 7).all() and (wide[:, 12:] == 7).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("q", [1, 60])
 def test_rows_that_count_for_nothing_and_scores_that_are_not_finite(dtype, q):
     """An lse of -inf gives nothing.  What a masked place holds does not matter: rows past a sequence are NaN already, and a NaN key
