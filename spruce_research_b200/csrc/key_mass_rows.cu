@@ -7,9 +7,9 @@
 // whole 64-byte pieces of 8 keys.  Q's fragments stay in registers while the warp walks its keys.
 //
 // Work is split as the attention's: all key tiles of the batch laid end to end, cut into equal runs, one a CTA; its warps
-// take the run's tiles in turn.  A key belongs to one warp, so nothing is joined.  Bytes in flight come from the number of warps: a
-// tile each of 24 warps an SM measured 50 us where two or three tiles each of 16 took 59 and 63 (CTAs of 128 or 256 threads alike).  Loads are marked to leave
-// the caches first (62 -> 54 us).
+// take the run's tiles in turn.  A key belongs to one warp, so nothing is joined.  Bytes in flight come from the number of
+// warps: a tile each of 24 warps an SM measured 50 us where two or three tiles each of 16 took 59 and 63 (CTAs of 128 or
+// 256 threads alike).  Loads are marked to leave the caches first (62 -> 54 us).
 //
 // On a B200, 64 sequences of 300 to 8192 tokens, 28 query / 4 KV heads of 128 in bf16: 50 us, 5.7 TB/s.
 #include <algorithm>

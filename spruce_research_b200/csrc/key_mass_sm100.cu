@@ -7,10 +7,10 @@
 // tokens as fit 128 rows, each a TMA box of (token, head of the group) rows.  Items go to the CTAs round robin; where a
 // cluster of CTAs can be had for each, it shares the item's rows and its first CTA adds the sums up in their order.
 //
-// Warps: 0-3 the first 64 rows of tile 0 (thread = key = TMEM lane), 4-7 the others, 8-15 likewise of tile 1, 16 and 17 issue
-// the MMAs of a tile each (a check of a barrier waits behind the MMAs that its warp has queued: one warp's checks would leave the
-// tensor core idle), 16 owns TMEM, 18 loads K (an item ahead) and Q, 19 works the items out and brings the rows' lse and limits.  Each S^T_t has two
-// buffers.
+// Warps: 0-3 the first 64 rows of tile 0 (thread = key = TMEM lane), 4-7 the others, 8-15 likewise of tile 1, 16 and 17
+// issue the MMAs of a tile each (a check of a barrier waits behind the MMAs that its warp has queued: one warp's checks
+// would leave the tensor core idle), 16 owns TMEM, 18 loads K (an item ahead) and Q, 19 works the items out and brings the
+// rows' lse and limits.  Each S^T_t has two buffers.
 //
 // Bound by the softmax warps: 16 exponentials a clock and SM (2048 clocks a step of 256 keys x 128 rows) and their issue, which
 // took 2460 of a step's 2960 clocks; the MMAs take 1100 and K comes from HBM behind them.  All exponentials are the hardware's: a
