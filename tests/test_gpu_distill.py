@@ -258,3 +258,18 @@ def test_the_top_blocks_of_a_teacher():
     assert ids.tolist() == [[0, -1], [1, 0], [0, 2]] and ids.dtype == torch.int32
     p = torch.softmax(logits.masked_fill(ids < 0, -math.inf), -1)
     assert torch.allclose(p, torch.tensor([[1.0, 0.0], [0.75, 0.25], [4 / 7, 3 / 7]], device="cuda"))
+
+
+@pytest.mark.parametrize("n", [131072, 1000])
+def test_rows_past_the_32_bit_offset(n):
+    """The last rows of more than 2^32 scores give what they give by themselves."""
+    R = (1 << 32) // n + 20
+    few = make(12, n, 8, torch.bfloat16, seed=4)
+    scores = torch.zeros(R, n, device="cuda", dtype=torch.bfloat16)
+    ids = torch.full((R, 8), -1, device="cuda", dtype=torch.int32)
+    teacher, weight = torch.zeros(R, 8, device="cuda"), torch.ones(R, device="cuda")
+    scores[-12:], ids[-12:], teacher[-12:], weight[-12:] = few[0], few[1], few[2], few[4]
+    loss, grad = native.topk_distill(scores, ids, teacher, grad_weight=weight)
+    alone, alone_grad = native.topk_distill(*few[:3], grad_weight=few[4])
+    assert (loss[:-12] == 0).all() and (grad[-20:-12] == 0).all()
+    assert (loss[-12:] - alone).abs().max() <= 1e-5 and (grad[-12:].float() - alone_grad.float()).abs().max() <= 2.0 ** -8 * alone_grad.abs().max()

@@ -234,3 +234,31 @@ def test_heads_that_several_ctas_share_replay_in_a_graph():
         at = to.table[s].long()[j // 64]
         for x, y in zip((to.k, to.v, to.mass), want):
             assert torch.equal(x[at, :, j % 64], y[at, :, j % 64])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("q", [1, 40])
+def test_pages_past_the_32_bit_offset(dtype, q):
+    """The last pages of a cache of more than 2^32 elements: weights, and rows evicted into a small cache, as from a small one."""
+    Hkv, page, D, n = 4, 128, 128, 700
+    pages = (1 << 32) // (Hkv * page * D) + 40
+    g = torch.Generator(device="cuda").manual_seed(3)
+    ids = torch.tensor([pages - 1 - 3 * i for i in range(6)], dtype=torch.int32, device="cuda")
+    big = torch.empty(pages, Hkv, page, D, device="cuda", dtype=dtype)
+    small = torch.randn(6, Hkv, page, D, generator=g, device="cuda").to(dtype)
+    big[ids.long()] = small
+    x = torch.randn(q, 8, D, generator=g, device="cuda").to(dtype)
+    mass = torch.zeros(pages, Hkv, page, device="cuda")
+    near = torch.zeros(6, Hkv, page, device="cuda")
+    cu, kv = (torch.tensor(t, device="cuda", dtype=torch.int32) for t in ([0, q], [n]))
+    order = torch.arange(6, device="cuda", dtype=torch.int32)[None]
+    lse = torch.full((q, 8), 12.0, device="cuda")
+    kw = dict(max_q_len=q, max_kv_len=n, decay=0.0)
+    native.paged_key_mass(x, big, mass, ids[None], cu, kv, lse, **kw)
+    native.paged_key_mass(x, small, near, order, cu, kv, lse, **kw)
+    assert torch.equal(mass[ids.long()], near) and near.sum() > 0
+    out = [[torch.zeros(2, Hkv, page, D, device="cuda", dtype=dtype) for _ in range(2)]
+           + [torch.zeros(2, Hkv, page, device="cuda"), torch.arange(2, device="cuda", dtype=torch.int32)[None]] for _ in range(2)]
+    a = native.paged_evict(big, big, mass, ids[None], kv, 200, sinks=1, recent=20, max_kv_len=n, into=out[0])
+    b = native.paged_evict(small, small, near, order, kv, 200, sinks=1, recent=20, max_kv_len=n, into=out[1])
+    assert all(torch.equal(s, t) for s, t in zip((*a, *out[0]), (*b, *out[1]))) and out[0][0].any()
