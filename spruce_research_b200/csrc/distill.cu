@@ -10,7 +10,7 @@
 // so that each element is rounded once.  A column named twice is found by a bitmap; only rows that have one search for it.
 //
 // On a B200: 4096 bf16 rows of 131072 columns, 64 entries each: forward 194 us (5.6 TB/s), backward 346 us (6.2 TB/s); 57344 fp32 rows
-// of 512, half of them visible, loss and gradient in one call: 61 us, bound by instruction issue (75%) and the latency of a
+// of 512, half of them visible, loss and gradient in one call: 59 us, bound by instruction issue (75%) and the latency of a
 // row's loads.  A warp that walks several rows and fetches the next one's entries ahead measured 68 to 90 us there.
 #include <algorithm>
 
@@ -122,9 +122,12 @@ __global__ void __launch_bounds__(32 * kRowWarps) distill_rows_kernel(const Dist
     const int col = (32 * i + lane) * V;
     if (vec_in && col + V <= seen) {
       unpack16<T>(*reinterpret_cast<const uint4*>(s + col), v[i]);
-    } else {
+    } else if (32 * i * V < seen) {  // of the warp
 #pragma unroll
       for (int e = 0; e < V; ++e) v[i][e] = col + e < seen ? Elem<T>::to_f(s[col + e]) : -INFINITY;
+    } else {
+#pragma unroll
+      for (int e = 0; e < V; ++e) v[i][e] = -INFINITY;
     }
   }
   // Teacher.
@@ -160,17 +163,18 @@ __global__ void __launch_bounds__(32 * kRowWarps) distill_rows_kernel(const Dist
     const float ref = m == -INFINITY ? 0.0f : m;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
+      if (32 * i * V < seen)
 #pragma unroll
-      for (int e = 0; e < V; ++e) l += fast_exp2((v[i][e] - ref) * c);
-    st = make_float2(ref, log2f(warp_sum(l)));  // -inf: nothing to see
+        for (int e = 0; e < V; ++e) l += fast_exp2((v[i][e] - ref) * c);
+    st = make_float2(ref, __log2f(warp_sum(l)));  // -inf: nothing to see
   }
   const bool empty = st.y == -INFINITY || tsum == 0.0f;
-  const float tlog = log2f(tsum), inv = 1.0f / tsum;
+  const float tlog = __log2f(tsum);
   float loss = 0.0f;
   for (int k = lane; k < a.K; k += 32) {
     if (I[k] < 0 || empty) continue;
-    const float e = (P[k] - tref) * c, p = fast_exp2(e) * inv;
-    if (a.loss != nullptr && p != 0.0f) loss += p * ((e - tlog) - ((S[k] - st.x) * c - st.y));
+    const float e = (P[k] - tref) * c - tlog, p = fast_exp2(e);
+    if (a.loss != nullptr && p != 0.0f) loss += p * (e - ((S[k] - st.x) * c - st.y));
     P[k] = p;
   }
   if (a.loss != nullptr) {
@@ -189,10 +193,15 @@ __global__ void __launch_bounds__(32 * kRowWarps) distill_rows_kernel(const Dist
   for (int i = 0; i < NV; ++i) {
     const int col = (32 * i + lane) * V;
     float g[V];
+    if (32 * i * V < seen && !empty) {  // of the warp
 #pragma unroll
-    for (int e = 0; e < V; ++e) g[e] = col + e < seen && !empty ? w * fast_exp2((v[i][e] - st.x) * c - st.y) : 0.0f;
+      for (int e = 0; e < V; ++e) g[e] = col + e < seen ? w * fast_exp2((v[i][e] - st.x) * c - st.y) : 0.0f;
+    } else {
+#pragma unroll
+      for (int e = 0; e < V; ++e) g[e] = 0.0f;
+    }
     if (vec_out && col + V <= a.n) {
-      __stcs(reinterpret_cast<uint4*>(grad + col), pack16<T>(g));
+      *reinterpret_cast<uint4*>(grad + col) = pack16<T>(g);  // not a streaming store: the teacher's columns follow (61.4 -> 59.4 us)
     } else {
 #pragma unroll
       for (int e = 0; e < V; ++e)
