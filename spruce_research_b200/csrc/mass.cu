@@ -219,7 +219,7 @@ __global__ void __launch_bounds__(kTileThreads) block_mass_tile_kernel(const Blo
 #pragma unroll
           for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
           const float up = fmaxf(m[y], top), at = up == -INFINITY ? 0.0f : up;
-          l[y] = l[y] * exp2f(m[y] - at) + sum * exp2f(ref - at);
+          l[y] = l[y] * exp2f(m[y] - at) + sum * exp2f(top - at);  // top, not ref: nothing times 2^(0 - at) may be no number
           m[y] = up;
           if (kk == 0) blocks[j * 64 + 4 * rr + y] = ref + log2f(sum);
         }

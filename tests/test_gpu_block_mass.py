@@ -143,3 +143,54 @@ def test_a_graph_and_another_stream():
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(out, want) and torch.equal(other, want)
+
+
+def want_without(q, k, gone):
+    """`want`, the keys `gone` [T] having a score of -inf in every row; a row that sees no others gives nothing."""
+    B, Hq, T, D = q.shape
+    Hkv, qb = k.shape[1], -(-T // 64)
+    rep = Hq // Hkv
+    out, bound = (torch.zeros(B, Hkv, qb, qb, device="cuda", dtype=torch.float64) for _ in range(2))
+    of = (torch.arange(T, device="cuda")[:, None] // 64 == torch.arange(qb, device="cuda")).double()
+    hidden = torch.ones(T, T, device="cuda", dtype=torch.bool).triu(1) | gone
+    for b in range(B):
+        for h in range(Hq):
+            x, y = q[b, h].double(), k[b, h // rep].double().masked_fill(gone[:, None], 0.0)
+            z = (x @ y.T * D ** -0.5).masked_fill(hidden, -math.inf)
+            S = (x.abs() @ y.abs().T * D ** -0.5).masked_fill(hidden, 0.0).amax(-1, keepdim=True)
+            total = torch.logsumexp(z, -1, keepdim=True)
+            p = torch.exp(z - total).masked_fill(hidden, 0.0)
+            err = p * (4 * D * 2.0 ** -24 * S + 8 * 2.0 ** -24 * (S + total.abs() + 10) + 2 * E[q.dtype]
+                       + (qb + 64 + 64 * rep) * 2.0 ** -24).masked_fill(hidden.all(-1, keepdim=True), 0.0)
+            out[b, h // rep] += of.T @ p @ of
+            bound[b, h // rep] += of.T @ err @ of
+    n = of.sum(0)[:, None] * rep
+    return out / n, bound / n + 2.0 ** -120
+
+
+def check_without(q, k, gone):
+    status = torch.zeros(1, device="cuda", dtype=torch.int32)
+    got = native.block_mass(q, k, status=status)
+    w, bound = want_without(q, k, gone)
+    assert status.item() == 0
+    assert ((got - w).abs() <= bound).all(), ((got - w).abs() / bound).max()
+    return got
+
+
+@pytest.mark.parametrize("dtype", [torch.float32])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("far", [0.0, -200.0])
+@pytest.mark.parametrize("overflow", [False, True])
+@pytest.mark.parametrize("dead", [(0,), (1,), (0, 1, 2, 3), (2, 3, 5), (0, 4)])
+def test_blocks_whose_scores_are_all_minus_infinity(dtype, D, far, overflow, dead):
+    """Whole blocks of -inf, by an infinite key or a product past fp32, ahead of scores near 0 and near -200: they weigh nothing."""
+    if overflow and dtype == torch.float16:
+        pytest.skip("products of fp16 do not leave fp32")
+    q, k = make(1, 4, 2, 500, D, dtype, scale=0.5)
+    q, k = q.clone(), k.clone()
+    q[..., 0], k[..., 0] = 16.0, far * D ** 0.5 / 16
+    q[..., 1], k[..., 1] = 1e30 if overflow else 1.0, 0.0
+    gone = torch.isin(torch.arange(500, device="cuda") // 64, torch.tensor(dead, device="cuda"))
+    k[:, :, gone, 1] = -1e30 if overflow else -math.inf
+    got = check_without(q, k, gone)
+    assert (got[..., list(dead)] == 0).all()
