@@ -332,7 +332,8 @@ __global__ void __launch_bounds__(kBmThreads, 1)
       const bool in = u.tile[t] / p.rep * 128 + row < p.a.T;
       const float top = fmaxf(m, other.x), ref = top == -INFINITY ? 0.0f : top;
       const float all = l * fast_exp2(m - ref) + other.y * fast_exp2(other.x - ref);
-      const float total = top == -INFINITY && all == all ? INFINITY : ref + __log2f(all);
+      // Rows past the prompt weigh nothing, though zero times an infinite key makes their scores NaN.
+      const float total = !in || (top == -INFINITY && all == all) ? INFINITY : ref + __log2f(all);
       // Weights of this warp's 32 rows, summed, and those of the other warp of the query block.
       float* const out = p.part + (((int64_t)u.bg * p.tiles * p.rep + u.tile[t]) * 2 + ((warp >> 1) & 1)) * p.kbp +
                          half * (p.kbp / 2);

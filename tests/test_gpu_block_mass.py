@@ -194,3 +194,15 @@ def test_blocks_whose_scores_are_all_minus_infinity(dtype, D, far, overflow, dea
     k[:, :, gone, 1] = -1e30 if overflow else -math.inf
     got = check_without(q, k, gone)
     assert (got[..., list(dead)] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("T, dead", [(1, 0), (65, 0), (65, 64), (130, 129), (300, 100), (300, 0), (300, 299), (1000, 500)])
+def test_a_key_of_minus_infinity_in_a_prompt_that_ends_inside_a_block(dtype, D, T, dead):
+    """The rows of a tile past the prompt are zeros, and zero times an infinite key is not a number: it stays there."""
+    q, k = make(2, 4, 2, T, D, dtype)
+    q, k = q.clone(), k.clone()
+    q[..., 0], k[..., 0] = 1.0, 0.0
+    k[:, :, dead, 0] = -math.inf
+    check_without(q, k, torch.arange(T, device="cuda") == dead)
