@@ -303,7 +303,9 @@ __global__ void __launch_bounds__(kBmThreads, 1)
         float a0, a1, a2, a3;
         f2_unpack(sum2[0], a0, a1);
         f2_unpack(sum2[1], a2, a3);
-        const float sum = (a0 + a1) + (a2 + a3);
+        // A block of -inf throughout weighs nothing: the polynomial does not go below 2^-125, which is not little to a row whose
+        // total turns out far below.
+        const float sum = top == -INFINITY ? 0.0f : (a0 + a1) + (a2 + a3);
         l = fmaf(l, fast_exp2(m - ref), sum);
         m = up;
         mine[(int64_t)j * 512] = ref + __log2f(sum);

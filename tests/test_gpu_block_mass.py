@@ -177,7 +177,7 @@ def check_without(q, k, gone):
     return got
 
 
-@pytest.mark.parametrize("dtype", [torch.float32])
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("D", [64, 128])
 @pytest.mark.parametrize("far", [0.0, -200.0])
 @pytest.mark.parametrize("overflow", [False, True])
