@@ -1180,11 +1180,12 @@ int spruce_topk_distill(const spruce_topk_distill_args* args) {
     return fail(SPRUCE_ERR_INVALID, "temperature must be positive and finite, got %g", x.tau);
   if (x.R == 0) return SPRUCE_OK;
   if ((x.scores == nullptr && x.n > 0) || ((x.ids == nullptr || x.teacher == nullptr) && x.K > 0) ||
-      (x.loss == nullptr && x.grad == nullptr) || (x.grad != nullptr && x.weight == nullptr) ||
-      (x.stats_in != nullptr && x.grad == nullptr))
+      (x.loss == nullptr && x.grad == nullptr && x.n > 0) || (x.grad != nullptr && x.weight == nullptr) ||
+      (x.stats_in != nullptr && x.grad == nullptr && x.n > 0))
     return fail(SPRUCE_ERR_INVALID, "null pointer");
   if (x.stats_in != nullptr && (x.loss != nullptr || x.stats != nullptr))
     return fail(SPRUCE_ERR_INVALID, "stats_in is for the gradient alone");
+  if (x.n == 0 && x.loss == nullptr) return SPRUCE_OK;  // a gradient without columns, whose address may be null
   spruce::DistillArgs a{};
   a.scores = x.scores;
   a.score_stride = x.score_stride;

@@ -273,3 +273,14 @@ def test_rows_past_the_32_bit_offset(n):
     alone, alone_grad = native.topk_distill(*few[:3], grad_weight=few[4])
     assert (loss[:-12] == 0).all() and (grad[-20:-12] == 0).all()
     assert (loss[-12:] - alone).abs().max() <= 1e-5 and (grad[-12:].float() - alone_grad.float()).abs().max() <= 2.0 ** -8 * alone_grad.abs().max()
+
+
+@pytest.mark.parametrize("lead", [(3,), (2, 3), (0,)])
+def test_rows_without_columns_have_an_empty_gradient(lead):
+    scores = torch.zeros(*lead, 0, device="cuda", requires_grad=True)
+    ids, teacher = torch.zeros(*lead, 2, device="cuda", dtype=torch.int32), torch.zeros(*lead, 2, device="cuda")
+    loss = topk_distill_loss(scores, ids, teacher)
+    loss.sum().backward()
+    assert loss.shape == lead and (loss == 0).all() and scores.grad.shape == scores.shape
+    loss, grad = native.topk_distill(scores.detach(), ids, teacher, grad_weight=torch.ones(lead, device="cuda"))
+    assert (loss == 0).all() and grad.shape == scores.shape

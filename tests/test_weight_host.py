@@ -187,6 +187,13 @@ def test_empty_calls_do_nothing():
     assert lib.spruce_block_mass_workspace_bytes(1, 28, 4, 131072, 96, 1) == -1
 
 
+def test_a_gradient_without_columns_is_an_empty_call():
+    """An empty tensor's address is null."""
+    struct, good = GOOD["topk_distill"]
+    for change in (dict(n=0, loss=0, stats_in=256, weight=256), dict(n=0, scores=0, loss=0, weight=256)):
+        assert _lib.load().spruce_topk_distill(_pack(struct, _fields("topk_distill"), **(good | change))) == _lib.OK
+
+
 # ------------------------------------------------------------------ the cache
 def _tracked(monkeypatch, pages=12, page=16, layers=2):
     cut = []
