@@ -550,7 +550,7 @@ SPRUCE_API int spruce_paged_key_mass(const spruce_paged_key_mass_args *args);
  * the lowest slot; NaN counts as the largest); where keep < sinks + recent, sinks go first.  The kept rows of K, V and mass move, in
  * their order, to slots 0 .. keep - 1 of the pages that out_table names, in the caches *_out.  Shorter sequences keep all.
  * In place (the outputs are the inputs, out_table is block_table), or into pages that no sequence of the call reads.  In
- * place, no page may belong to two sequences of the call.  Slots past the kept ones are left as they are.
+ * place, K and V are two arrays and no page may belong to two sequences of the call.  Slots past the kept ones are left as they are.
  * kept int32 [S, Hkv, width] receives the old slots, -1 past the kept ones; width >= min(keep, max_kv_len).  new_lens int32
  * [S] receives the new lengths and may not be kv_lens.  A sequence longer than max_kv_len or its table is left as it is (kept
  * -1, its length unchanged) and raises SPRUCE_STATUS_BAD_LENGTH; masses and rows of a bad page count as 0 and

@@ -1059,16 +1059,18 @@ int spruce_paged_evict(const spruce_paged_evict_args* args) {
     ok = ok && x.kc_strides[i] % vn == 0 && x.vc_strides[i] % vn == 0 && x.k_out_strides[i] % vn == 0 &&
          x.v_out_strides[i] % vn == 0;
   if (!ok) return fail(SPRUCE_ERR_UNSUPPORTED, "the caches need 16-byte aligned rows");
-  const bool in_place = x.k_out == x.k_cache;
+  // With the same table an output that is an input has to be its own, and all the others theirs; with another table the pages are
+  // the caller's promise.
+  const bool in_place = most > 0 && x.out_table == x.block_table &&
+                        (x.k_out == x.k_cache || x.v_out == x.v_cache || x.k_out == x.v_cache || x.v_out == x.k_cache ||
+                         x.mass_out == x.mass);
   if (in_place) {
-    bool same = x.v_out == x.v_cache && x.mass_out == x.mass && x.out_table == x.block_table &&
+    bool same = x.k_out == x.k_cache && x.v_out == x.v_cache && x.mass_out == x.mass && x.k_out != x.v_out &&
                 x.out_table_stride == x.table_stride && x.out_pages == x.num_pages;
     for (int i = 0; i < 3; ++i)
       same = same && x.kc_strides[i] == x.k_out_strides[i] && x.vc_strides[i] == x.v_out_strides[i] &&
              x.mass_strides[i] == x.mass_out_strides[i];
-    // The keys alone may lie in the same cache: then the other pages are the caller's promise.
-    if (!same && x.out_table == x.block_table)
-      return fail(SPRUCE_ERR_INVALID, "in place, every output has to be its input");
+    if (!same) return fail(SPRUCE_ERR_INVALID, "in place, every output has to be its input, K and V apart");
   }
   spruce::EvictArgs a{};
   a.k = x.k_cache;
@@ -1104,7 +1106,7 @@ int spruce_paged_evict(const spruce_paged_evict_args* args) {
   a.recent = (int)(x.recent < cap ? x.recent : cap);
   a.num_pages = x.num_pages;
   a.to_pages = x.out_pages;
-  a.in_place = in_place && x.out_table == x.block_table;
+  a.in_place = in_place;
   a.status = x.status;
   return cuda_status(spruce::launch_evict(a, as_stream(x.stream)), "eviction launch");
 }

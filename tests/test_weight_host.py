@@ -175,6 +175,17 @@ def test_c_entries_refuse_before_any_device_work(name, change, words):
     assert getattr(lib, f"spruce_{name}")(None) == _lib.ERR_INVALID
 
 
+@pytest.mark.parametrize("change", [dict(k_out=1024), dict(k_out=1024, v_out=1024), dict(k_out=1024, mass_out=1024),
+                                    dict(k_out=1024, v_out=256, mass_out=1024), dict(v_cache=256, v_out=256),
+                                    dict(k_out=512, v_out=256)])
+def test_an_eviction_that_is_partly_in_place_is_refused(change):
+    """Rows of one array would be written over before they are read, or moved twice."""
+    struct, good = GOOD["paged_evict"]
+    lib = _lib.load()
+    assert lib.spruce_paged_evict(_pack(struct, _fields("paged_evict"), **(good | change))) == _lib.ERR_INVALID
+    assert "in place" in lib.spruce_last_error().decode()
+
+
 def test_empty_calls_do_nothing():
     lib = _lib.load()
     for name, change in (("paged_key_mass", dict(N=0)), ("paged_key_mass", dict(S=0)), ("paged_evict", dict(S=0)),
