@@ -243,7 +243,7 @@ class PagedSparseLayer:
         native.paged_append(kr[0].transpose(0, 1), v, self.k_cache, self.v_cache, step.block_table, step.cu_q,
                             step.kv_lens)
         out, selected = self.sparse(qr, kr, vs)
-        if self.mass is not None:
+        if self.mass is not None and step.tokens:
             last = min(self.observe, step.tokens)
             self._attend(qr[0, :, -last:].transpose(0, 1), step, torch.arange(0, 2 * last, last, device=q.device, dtype=torch.int32),
                          last, 0.0)

@@ -280,6 +280,19 @@ def test_a_layer_adds_weights_only_where_its_cache_keeps_them(monkeypatch):
         layer.extend(torch.zeros(59, 2, 64), torch.zeros(59, 2, 64), torch.zeros(59, 2, 64), step)
 
 
+def test_an_empty_prompt_has_no_queries_to_observe(monkeypatch):
+    c, _ = _tracked(monkeypatch)
+    calls = []
+    for name in ("paged_append", "paged_attention", "paged_key_mass", "qk_norm_rope"):
+        def call(*args, called=name, **kw):
+            calls.append(called)
+            return args[:2] if called == "qk_norm_rope" else args[0]
+        monkeypatch.setattr(native, name, call)
+    layer = PagedSparseLayer(c, 0, None, prefill=lambda q, k, v: (q, None))
+    x = torch.zeros(0, 2, 64)
+    assert layer.prefill(x, x, x, c.step([("a", 0)]))[0].shape == (2, 0, 64) and calls == ["qk_norm_rope", "paged_append"]
+
+
 # ------------------------------------------------------------------ the gate
 @pytest.mark.parametrize("P", [1, 3])
 def test_training_scores_are_the_gates_formula(P):
