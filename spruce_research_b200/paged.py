@@ -36,6 +36,9 @@ class PagedStep:
     tokens: int
     positions: torch.Tensor | None = None   # int64 [tokens] in their sequences, where an eviction left these ahead of the slots
     max_position: int = 0                    # positions end before this
+    counts: list | None = None               # each sequence's new tokens, and its length with them
+    lengths: list | None = None
+    serial: int = 0                          # of the cache's steps
 
 
 class PagedKVCache:
@@ -61,6 +64,8 @@ class PagedKVCache:
         self._pages: dict = {}
         self._length: dict = {}
         self._evicted: dict = {}   # tokens that evictions took, and the slots that the last one left
+        self._last: dict = {}      # each sequence's last step, while no eviction has moved its tokens
+        self._steps = 0
 
     @property
     def free_pages(self) -> int:
@@ -79,9 +84,14 @@ class PagedKVCache:
         self._free.extend(reversed(self._pages.pop(seq_id, [])))
         self._length.pop(seq_id, None)
         self._evicted.pop(seq_id, None)
+        self._last.pop(seq_id, None)
 
     def truncate(self, seq_id, length: int) -> None:
-        """Keep a sequence's first ``length`` tokens: drafts that were rejected, or a step whose forward did not run."""
+        """Keep a sequence's first ``length`` tokens: drafts that were rejected, or a step whose forward did not run.
+
+        The weight that the other tokens gave to keys before them stays in ``mass``, and the old ones have faded once for their step:
+        drafts go through :meth:`PagedSparseLayer.draft`, which gives none until they are accepted.
+        """
         held = self.length(seq_id)
         if not 0 <= length <= held:
             raise ValueError(f"a sequence of {held} tokens cannot be cut to {length}")
@@ -111,13 +121,27 @@ class PagedKVCache:
         for (s, _), m, count in zip(new_tokens, lengths, need):
             self._pages.setdefault(s, []).extend(self._free.pop() for _ in range(count))
             self._length[s] = m
+        self._steps += 1
+        self._last.update((s, self._steps) for s, _ in new_tokens)
         dev = self._describe([s for s, _ in new_tokens], [n for _, n in new_tokens], lengths)
         ends = [self.position(s) for s, _ in new_tokens]
         positions = None
         if any(self._evicted.get(s, (0, 0))[0] for s, _ in new_tokens):
             positions = torch.cat([torch.arange(end - n, end) for end, (_, n) in zip(ends, new_tokens)]).to(self.k.device)
         return PagedStep([s for s, _ in new_tokens], *dev, max((n for _, n in new_tokens), default=0), max(lengths, default=0),
-                         sum(n for _, n in new_tokens), positions, max(ends, default=0))
+                         sum(n for _, n in new_tokens), positions, max(ends, default=0), [n for _, n in new_tokens], lengths,
+                         self._steps)
+
+    def accepted(self, step: PagedStep) -> list:
+        """How many of a step's new tokens each of its sequences still holds, before anything but :meth:`truncate` and :meth:`drop`."""
+        if step.counts is None:
+            raise ValueError("this step was not described by a cache")
+        kept = []
+        for s, n, length in zip(step.seq_ids, step.counts, step.lengths):
+            if s in self._length and self._last.get(s) != step.serial:
+                raise ValueError(f"sequence {s!r} has gone on or lost tokens to an eviction since this step")
+            kept.append(max(0, n - length + self.length(s)))
+        return kept
 
     def _describe(self, seq_ids, counts, lengths):
         """Page table, offsets of ``counts`` and lengths of sequences, on the device."""
@@ -163,6 +187,7 @@ class PagedKVCache:
             del pages[left:]
             self._length[s] = keep
             self._evicted[s] = (self._evicted.get(s, (0, 0))[0] + n - keep, keep)
+            self._last.pop(s, None)
         return cut
 
 
@@ -174,6 +199,7 @@ class PagedSparseLayer:
 
     Where the cache keeps its keys' weights, each step multiplies the old ones of its sequences by ``decay`` and adds
     what its queries give; a sparse prefill sets them by its last ``observe`` queries, which attend to the whole prompt for it.
+    Tokens that may be taken back go through :meth:`draft` and :meth:`accept`.
     """
 
     def __init__(self, cache: PagedKVCache, layer_idx: int, rope: torch.Tensor | None, *,
@@ -186,6 +212,7 @@ class PagedSparseLayer:
             raise ValueError(f"decay must be in [0, 1], got {decay}")
         if observe < 1:
             raise ValueError(f"observe must be positive, got {observe}")
+        self.cache = cache
         self.k_cache, self.v_cache = cache.k[layer_idx], cache.v[layer_idx]
         self.mass = None if cache.mass is None else cache.mass[layer_idx]
         self.decay, self.observe = decay, observe
@@ -202,16 +229,29 @@ class PagedSparseLayer:
             raise ValueError(f"sequences of {most} tokens need a rotation table of as many positions, got "
                              f"{self.rope.shape[0]}")
 
-    def _attend(self, q, step: PagedStep, cu_q, max_q_len: int, decay: float, out=None) -> torch.Tensor:
-        """Attention of ``q`` over the cache; where the cache keeps weights, what ``q`` gives is added."""
-        batch = (step.block_table, cu_q, step.kv_lens)
-        bounds = dict(max_q_len=max_q_len, max_kv_len=step.max_kv_len)
-        if self.mass is None:
-            return native.paged_attention(q, self.k_cache, self.v_cache, *batch, out=out, **bounds)
-        lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
-        out = native.paged_attention(q, self.k_cache, self.v_cache, *batch, out=out, lse=lse, **bounds)
-        native.paged_key_mass(q, self.k_cache, self.mass, *batch, lse, decay=decay, **bounds)
-        return out
+    def _attend(self, q, step: PagedStep, cu_q, max_q_len: int, out=None):
+        """Attention of ``q`` over the cache and, where the cache keeps weights, the rows' log-sums: ``(out, lse)``."""
+        lse = None if self.mass is None else torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
+        out = native.paged_attention(q, self.k_cache, self.v_cache, step.block_table, cu_q, step.kv_lens, out=out,
+                                     max_q_len=max_q_len, max_kv_len=step.max_kv_len, lse=lse)
+        return out, lse
+
+    def _weigh(self, q, lse, step: PagedStep, cu_q, kv_lens, max_q_len: int, decay: float) -> None:
+        """Add the weight that ``q`` gives, if the cache keeps any."""
+        if self.mass is not None:
+            native.paged_key_mass(q, self.k_cache, self.mass, step.block_table, cu_q, kv_lens, lse, decay=decay,
+                                  max_q_len=max_q_len, max_kv_len=step.max_kv_len)
+
+    def _extend(self, q, k, v, step: PagedStep, out):
+        """Append and attend: ``(out, rotated q, lse)``."""
+        self._check((q, k, v), step, spare=True)
+        positions = step.positions
+        if positions is not None and positions.shape[0] < k.shape[0]:  # rows past the step's tokens are left out
+            positions = torch.nn.functional.pad(positions, (0, k.shape[0] - positions.shape[0]))
+        q = native.paged_append(k, v, self.k_cache, self.v_cache, step.block_table, step.cu_q, step.kv_lens, q=q,
+                                rope=self.rope, positions=positions, **self.rotation)
+        out, lse = self._attend(q, step, step.cu_q, step.max_q_len, out)
+        return out, q, lse
 
     def extend(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, step: PagedStep,
                out: torch.Tensor | None = None) -> torch.Tensor:
@@ -219,13 +259,44 @@ class PagedSparseLayer:
 
         N may exceed the step's tokens; the rows past them are not written.
         """
-        self._check((q, k, v), step, spare=True)
-        positions = step.positions
-        if positions is not None and positions.shape[0] < k.shape[0]:  # rows past the step's tokens are left out
-            positions = torch.nn.functional.pad(positions, (0, k.shape[0] - positions.shape[0]))
-        q = native.paged_append(k, v, self.k_cache, self.v_cache, step.block_table, step.cu_q, step.kv_lens, q=q,
-                                rope=self.rope, positions=positions, **self.rotation)
-        return self._attend(q, step, step.cu_q, step.max_q_len, self.decay, out)
+        out, q, lse = self._extend(q, k, v, step, out)
+        self._weigh(q, lse, step, step.cu_q, step.kv_lens, step.max_q_len, self.decay)
+        return out
+
+    def draft(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, step: PagedStep,
+              out: torch.Tensor | None = None):
+        """:meth:`extend` by tokens that may be taken back: ``(out, seen)``.
+
+        The cache's weights stay as they are until :meth:`accept` gets ``seen``.
+        """
+        out, q, lse = self._extend(q, k, v, step, out)
+        return out, (q, lse)
+
+    def accept(self, seen, step: PagedStep) -> None:
+        """Add the weight of those of a drafted step's tokens that the cache still holds, as a step of these alone does.
+
+        Once a step and layer, after :meth:`PagedKVCache.truncate` and before the sequences' next step or eviction.  A sequence that
+        keeps none of the step's tokens keeps its weights.
+        """
+        counts = self.cache.accepted(step)
+        most = max(counts, default=0)
+        if self.mass is None or most == 0:
+            return
+        (q, lse), cu_q, kv_lens = seen, step.cu_q, step.kv_lens
+        if counts != step.counts:
+            n, S = sum(counts), len(counts)
+            # One host tensor and one copy: the tokens kept, their offsets, what the lengths lose.
+            host, at = torch.zeros(n + 2 * S + 1, dtype=torch.int32), 0
+            rows, cu, less = host[:n], host[n:n + S + 1], host[n + S + 1:]
+            for i, (kept, count) in enumerate(zip(counts, step.counts)):
+                first = int(cu[i])
+                rows[first:first + kept] = torch.arange(at, at + kept)
+                cu[i + 1], less[i] = first + kept, count - kept
+                at += count
+            dev = host.to(q.device)
+            q, lse = q.index_select(0, dev[:n]), lse.index_select(0, dev[:n])
+            cu_q, kv_lens = dev[n:n + S + 1], kv_lens - dev[n + S + 1:]
+        self._weigh(q, lse, step, cu_q, kv_lens, most, self.decay)
 
     def prefill(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, step: PagedStep):
         """Block-sparse prefill of one whole prompt; its keys and values go to the cache.
@@ -245,8 +316,10 @@ class PagedSparseLayer:
         out, selected = self.sparse(qr, kr, vs)
         if self.mass is not None and step.tokens:
             last = min(self.observe, step.tokens)
-            self._attend(qr[0, :, -last:].transpose(0, 1), step, torch.arange(0, 2 * last, last, device=q.device, dtype=torch.int32),
-                         last, 0.0)
+            cu_q = torch.arange(0, 2 * last, last, device=q.device, dtype=torch.int32)
+            rows = qr[0, :, -last:].transpose(0, 1)
+            _, lse = self._attend(rows, step, cu_q, last)
+            self._weigh(rows, lse, step, cu_q, step.kv_lens, last, 0.0)
         return out[0], selected
 
 

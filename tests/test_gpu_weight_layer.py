@@ -151,3 +151,42 @@ def test_a_layers_teacher_and_the_training_command():
     assert torch.equal(teacher[:, :, 6].exp().round(decimals=5), mass[:, :, 6].topk(3, -1).values.round(decimals=5))
     losses = train.main(tokens=512, steps=2, top=4)
     assert len(losses) == 2 and all(math.isfinite(x) for x in losses)
+
+
+@pytest.mark.parametrize("Hq,Hkv,D,page", [(28, 4, 128, 64), (4, 2, 64, 16)])
+def test_rejected_drafts_leave_no_weight(Hq, Hkv, D, page):
+    """Draft, truncate, accept, twice, against the same tokens without the rejected ones.  The keys are the same; the log-sums may come
+    from kernels of other row counts, each good to 1e-4, twice that for every weight, which fading does not enlarge."""
+    g = torch.Generator(device="cuda").manual_seed(8)
+    table = rope_table(D, 1024, 1e6)
+    caches = [PagedKVCache(1, 120, page, Hkv, D, track_mass=True) for _ in range(2)]
+    layers = [PagedSparseLayer(c, 0, table, decay=0.75) for c in caches]
+    split = lambda y: (y[:, :Hq], y[:, Hq:Hq + Hkv], y[:, Hq + Hkv:])  # noqa: E731
+
+    def tokens(n):
+        return torch.randn(n, Hq + 2 * Hkv, D, generator=g, device="cuda", dtype=torch.bfloat16)
+
+    held = {"a": 300, "b": 77, "c": 40}
+    x = tokens(sum(held.values()))
+    for c, layer in zip(caches, layers):
+        layer.extend(*split(x), c.step(list(held.items())))
+    before = rows(caches[0], caches[0].mass, 0, "c", 40).clone()
+    for drafts, good in (((5, 9, 3), (2, 9, 0)), ((12, 1, 4), (7, 0, 0))):
+        parts = [tokens(n) for n in drafts]
+        step = caches[0].step(list(zip("abc", drafts)))
+        out, seen = layers[0].draft(*split(torch.cat(parts)), step)
+        for s, n, kept in zip("abc", drafts, good):
+            caches[0].truncate(s, caches[0].length(s) - n + kept)
+        layers[0].accept(seen, step)
+        kept = [(s, n) for s, n in zip("abc", good) if n]
+        want = layers[1].extend(*split(torch.cat([p[:n] for p, n in zip(parts, good)])), caches[1].step(kept))
+        got = torch.cat([o[:n] for o, n in zip(out.split(drafts), good)])
+        assert (got.double() - want.double()).abs().max() <= 2e-2
+    assert torch.equal(rows(caches[0], caches[0].mass, 0, "c", 40), before)
+    x = tokens(3)
+    for c, layer in zip(caches, layers):
+        layer.extend(*split(x), c.step([("a", 1), ("b", 1), ("c", 1)]))
+    for s, n in {"a": 310, "b": 87, "c": 41}.items():
+        assert caches[0].length(s) == caches[1].length(s) == n
+        a, b = (rows(c, c.mass, 0, s, n) for c in caches)
+        assert torch.allclose(a, b, rtol=2e-4, atol=1e-6) and a.sum() > Hq

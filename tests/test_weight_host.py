@@ -293,6 +293,61 @@ def test_an_empty_prompt_has_no_queries_to_observe(monkeypatch):
     assert layer.prefill(x, x, x, c.step([("a", 0)]))[0].shape == (2, 0, 64) and calls == ["qk_norm_rope", "paged_append"]
 
 
+def test_drafts_weigh_when_they_are_accepted(monkeypatch):
+    c, _ = _tracked(monkeypatch)
+    calls = []
+    for name in ("paged_append", "paged_attention", "paged_key_mass"):
+        def call(*args, called=name, **kw):
+            calls.append((called, args, kw))
+            return kw["q"] if called == "paged_append" else args[0]
+        monkeypatch.setattr(native, name, call)
+    layer = PagedSparseLayer(c, 1, None, decay=0.5)
+    c.step([("a", 30), ("b", 20), ("c", 5), ("d", 9)])
+
+    def drafted():
+        step = c.step([("a", 4), ("b", 3), ("c", 2), ("d", 2)])
+        x = torch.randn(13, 2, 64)                                                  # a buffer of a fixed size
+        out, seen = layer.draft(x, x, x, step)
+        assert [n for n, _, _ in calls] == ["paged_append", "paged_attention"] and torch.equal(out, x)
+        seen[1][:] = torch.arange(26.0).view(13, 2)
+        del calls[:]
+        return x, seen, step
+
+    x, seen, step = drafted()
+    c.truncate("a", 31)
+    c.truncate("c", 4)                                                              # less than before the step
+    c.drop("d")
+    assert c.accepted(step) == [1, 3, 0, 0]
+    layer.accept(seen, step)
+    (name, (q, k, mass, table, cu, kv, lse), kw), = calls
+    assert name == "paged_key_mass" and k is layer.k_cache and mass is layer.mass and table is step.block_table
+    assert torch.equal(q, x[[0, 4, 5, 6]]) and torch.equal(lse, seen[1][[0, 4, 5, 6]])
+    assert cu.tolist() == [0, 1, 4, 4, 4] and kv.tolist() == [31, 23, 5, 9] and cu.dtype == kv.dtype == I32
+    assert kw == dict(decay=0.5, max_q_len=3, max_kv_len=step.max_kv_len)
+    del calls[:]
+    x, seen, step = drafted()
+    layer.accept(seen, step)                                                        # all of them
+    (name, args, kw), = calls
+    assert args[0] is seen[0] and args[4] is step.cu_q and args[5] is step.kv_lens and kw["max_q_len"] == 4
+    del calls[:]
+    x, seen, step = drafted()
+    for s, n in zip("abcd", (35, 26, 6, 2)):
+        c.truncate(s, n)
+    layer.accept(seen, step)                                                        # none
+    assert not calls
+    c.step([("a", 1)])
+    with pytest.raises(ValueError, match="'a' has gone on"):
+        layer.accept(seen, step)
+    x, seen, step = drafted()
+    c.evict(["b"], 20)
+    with pytest.raises(ValueError, match="'b' has gone on"):
+        layer.accept(seen, step)
+    plain = PagedSparseLayer(PagedKVCache(1, 4, 16, 2, 64, torch.float32, "cpu"), 0, None)
+    step = plain.cache.step([("a", 2)])
+    out, seen = plain.draft(x[:2], x[:2], x[:2], step)
+    assert seen[1] is None and plain.accept(seen, step) is None and [n for n, _, _ in calls][-1] == "paged_attention"
+
+
 # ------------------------------------------------------------------ the gate
 @pytest.mark.parametrize("P", [1, 3])
 def test_training_scores_are_the_gates_formula(P):
