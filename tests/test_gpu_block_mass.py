@@ -206,3 +206,14 @@ def test_a_key_of_minus_infinity_in_a_prompt_that_ends_inside_a_block(dtype, D, 
     q[..., 0], k[..., 0] = 1.0, 0.0
     k[:, :, dead, 0] = -math.inf
     check_without(q, k, torch.arange(T, device="cuda") == dead)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("B, Hq, Hkv, T, D", [
+    (3, 28, 4, 1100, 128),   # 384 units of mixed lengths on 148 CTAs, 216 items of the fp32 kernel
+    (40, 12, 4, 300, 64),    # 800 units, the first 160 of a single tile: CTAs that take two such in a row; 800 items
+    (5, 8, 2, 2100, 64),     # 340 units of up to 17 key tiles, 330 items
+])
+def test_ctas_that_take_several_units(dtype, B, Hq, Hkv, T, D):
+    got = check(*make(B, Hq, Hkv, T, D, dtype, seed=T))
+    assert (got.sum(-1) - 1).abs().max() < 1e-4

@@ -262,3 +262,33 @@ def test_pages_past_the_32_bit_offset(dtype, q):
     a = native.paged_evict(big, big, mass, ids[None], kv, 200, sinks=1, recent=20, max_kv_len=n, into=out[0])
     b = native.paged_evict(small, small, near, order, kv, 200, sinks=1, recent=20, max_kv_len=n, into=out[1])
     assert all(torch.equal(s, t) for s, t in zip((*a, *out[0]), (*b, *out[1]))) and out[0][0].any()
+
+
+@pytest.mark.parametrize("dtype, D", [(torch.bfloat16, 128), (torch.float16, 128), (torch.float32, 64), (torch.float32, 128)])
+@pytest.mark.parametrize("keep", [40, 250, 699])
+def test_many_heads_in_place(dtype, D, keep):
+    """More CTAs of slices than the GPU holds at a time, so that each takes 64 bytes of a row; ragged lengths, moves of many and few slots."""
+    lens = [700, 33, 251, 640, 1, 0, 412, 699, 250, 700]
+    heads, row = 3 * len(lens), D * torch.empty(0, dtype=dtype).element_size()
+    assert heads * (2 * (row // 32) + 1) > 2 * torch.cuda.get_device_properties(0).multi_processor_count
+    c = Cache(lens, 3, D, 16, dtype, seed=keep)
+    c.mass[c.table[0, 0].long(), :, 0] = 0.0       # its slot goes, so almost every row of the first sequence moves by one
+    c.check(keep, 0, 1)
+
+
+def test_long_heads_of_one_cta_each():
+    """So many heads that none gets a second CTA, and more slots than a CTA's shared memory holds: the rest is read again."""
+    lens, keep, heads = [49200, 50003], 2000, 40
+    c = Cache(lens, heads, 8, 64, torch.bfloat16, weights=lambda m: (m * 64).floor())      # many ties
+    assert 2 * heads * 2 > torch.cuda.get_device_properties(0).multi_processor_count
+    before = [[c.rows(x, s).clone() for x in (c.k, c.v, c.mass)] for s in range(2)]
+    kept, new = native.paged_evict(c.k, c.v, c.mass, c.table, c.kv, keep, sinks=3, recent=100, max_kv_len=max(lens))
+    assert new.tolist() == [keep, keep]
+    for s, n in enumerate(lens):
+        w = before[s][2].clone()
+        w[:3], w[n - 100:] = math.inf, math.inf
+        want = torch.sort(w, dim=0, descending=True, stable=True).indices[:keep].sort(0).values
+        assert torch.equal(kept[s].long(), want.T)
+        for x, y in zip((c.k, c.v, c.mass), before[s]):
+            at = want if y.dim() == 2 else want[..., None].expand(-1, -1, y.shape[2])
+            assert torch.equal(c.rows(x, s, keep), y.gather(0, at))
