@@ -10,16 +10,17 @@
 //
 // Warps: 0-3 the first 64 keys of tile 0 (thread = row = TMEM lane), 4-7 the others, 8-15 likewise of tile 1, 16 and 17
 // issue the MMAs of a tile each (a check of a barrier waits behind the MMAs that its warp has queued; one issuer for both:
-// 4.55 ms where two take 4.45), 16 owns TMEM, 18 loads Q and K.  Four softmax warps a scheduler hide each other's latencies
+// 4.55 ms where two take 4.48), 16 owns TMEM, 18 loads Q and K.  Four softmax warps a scheduler hide each other's latencies
 // (two of 128 keys a row: 4.72 ms where these took 4.58).  Each S_t has two buffers, which fill TMEM: the tensor core runs
 // a tile ahead of the exponentials, which bound the kernel (16 a clock and SM, against 32 scores a clock of the MMAs at d =
 // 128).  Part of them runs on the FMA pipe instead, as a polynomial of degree 4 with a relative error of 2.7e-6: a quarter
-// (none, 1/8, 1/4, 3/8: 4.62, 4.53, 4.48, 4.78 ms; the issue slots bound what the exponentials leave).  Exponentials over
+// (none, 1/8, 1/4, 3/8: 4.62, 4.53, 4.48, 4.78 ms; then the exponentials' pipe is 72% busy and issue 63%: neither is full, what
+// is left is the latency of a block's chain of maximum, exponentials and sum).  Exponentials over
 // an old maximum, without a pass for the block's own, measured 1.5% slower: the branch for a row that outgrows it keeps
 // blocks from overlapping.
 //
-// On a B200, 28 query / 4 KV heads of 128 in bf16: 32768 tokens 4.48 ms, 859 TFLOP/s (the exponentials alone would take 2.4
-// ms with a quarter on the FMA pipe or 3.2 without, the MMAs 2.4).
+// On a B200, 28 query / 4 KV heads of 128 in bf16: 32768 tokens 4.5 to 4.7 ms, 825 to 850 TFLOP/s (the exponentials alone would
+// take 2.4 ms with a quarter on the FMA pipe or 3.2 without, the MMAs 2.4); 131072 tokens 76 ms.
 //
 // Units go to the CTAs longest first, back and forth over them.
 //

@@ -11,9 +11,9 @@
 // never touch each other, so a (sequence, head) is spread over many CTAs that need not wait for one another.  Into other
 // pages there is nothing to wait for: a warp takes 32 whole rows.
 //
-// On a B200 (4 KV heads of 128, bf16): one sequence of 131072 tokens cut to 16384 36 us, of which the selection, a chain of nine
-// cluster barriers, takes about 20; 64 sequences of 300 to 8192 tokens cut to 2048 101 us, 82 of them the copy (5.9 TB/s).  In place
-// 87 and 174 us: rounds of short pieces of scattered rows.
+// On a B200 (4 KV heads of 128, bf16): one sequence of 131072 tokens cut to 16384 36 us, of which the selection, a chain of twelve
+// cluster barriers (three a pass, three around them), takes about 20; 64 sequences of 300 to 8192 tokens cut to 2048 101 us, 82 of them the copy (5.9 TB/s).  In place
+// 84 to 87 and 172 to 175 us: rounds of short pieces of scattered rows.
 #include <algorithm>
 
 #include "mass_common.cuh"

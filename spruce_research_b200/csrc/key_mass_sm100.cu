@@ -14,8 +14,8 @@
 //
 // Bound by the softmax warps: 16 exponentials a clock and SM (2048 clocks a step of 256 keys x 128 rows) and their issue, which
 // took 2460 of a step's 2960 clocks; the MMAs take 1100 and K comes from HBM behind them.  All exponentials are the hardware's: a
-// polynomial on the FMA pipe takes NaN for a number, and a row's NaN stands in one column only.
-// On a B200, 28 query / 4 KV heads of 128 in bf16: 64 tokens over 131072 99 us (608 TFLOP/s); a ragged fp16 batch of 9
+// polynomial on the FMA pipe, which takes NaN for a number, would need the steps with a NaN lse set apart, and was not built.
+// On a B200, 28 query / 4 KV heads of 128 in bf16: 64 tokens over 131072 99 to 104 us (577 to 608 TFLOP/s); a ragged fp16 batch of 9
 // sequences of up to 3000 tokens and 300 new ones 16 us.
 //
 // Every wait is bounded (common.cuh).

@@ -144,8 +144,11 @@ static cudaError_t launch_key_mass_t(const KeyMassArgs& a, int sms, cudaStream_t
   return a.a.D == 128 ? launch_tile<T, 128>(a, sms, stream) : launch_tile<T, 64>(a, sms, stream);
 }
 
-// fp32 rows by the lanes of a warp where they are few (16 sequences of 2000 to 8000 tokens, 7 rows: 135 us by tiles of 64 rows);
-// 16 bits on the tensor cores, but where a group has more heads than a row tile has rows.
+// fp32 rows by the lanes of a warp where they are few: 16 sequences of 2000 to 8000 tokens, 28 / 4 heads of 128: 7 rows 36 us, by tiles
+// of 64 rows 223, 14 rows 52 and 226; one of 131000 54 and 336, 79 and 345.
+// 16 bits by warp MMAs where rows are few, which read K at full rate: 64 sequences of 300 to 8191 tokens, 7 / 14 / 28 rows 50 / 59 / 76
+// us, on tcgen05 100 / 95 / 97; one of 131000 28 / 32 / 41 and 44 / 44 / 46.  With one KV head and 24 or 32 rows the two are even on one
+// long sequence (16.0 and 15.4, 16.4 and 15.3) and 25 to 37 us on 64.  Groups of more heads than a row tile has rows take the tiles.
 cudaError_t launch_key_mass(const KeyMassArgs& a, int dtype, cudaStream_t stream) {
   const int sms = sm_count();
   if (key_mass_params(a, kTileKeys).key_tiles == 0) return cudaSuccess;
