@@ -528,8 +528,8 @@ SPRUCE_API int spruce_paged_attention_lse(const spruce_paged_attention_lse_args 
  * Hkv, page_size] by strides (page, head, row) and may be one; no page may belong to two sequences of the call (both would
  * write its weights).  Bounds, pages and alignment are spruce_paged_attention's:
  * queries past max_q_len give none, and slots that only they see, those past max_kv_len and those of a bad page are left as
- * they are.  A key that holds an infinity or a NaN may get any weight; it does not reach other keys.  Each sum is formed in a
- * fixed order.
+ * they are.  A score of -inf adds nothing; a key with a score of NaN or +inf may get any weight, and no other key does by it.  Each
+ * sum is formed in a fixed order.
  */
 typedef struct {
   const void *q, *k_cache;

@@ -256,3 +256,26 @@ def test_weights_replay_in_a_graph_and_on_another_stream(q):
     torch.cuda.synchronize()
     named = want != 3.0
     assert torch.equal(mass[named], want[named]) and torch.equal(got, lse)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("heads", [(7, 1, 64), (28, 4, 128), (10, 2, 64), (40, 1, 64), (65, 1, 64), (4, 4, 128)])
+@pytest.mark.parametrize("q", [1, 5, 40, 300])
+def test_keys_whose_scores_are_minus_infinity_get_nothing(dtype, heads, q):
+    """Zero rows that fill a tile up make no number with an infinite key, wherever in the tiles and the prompt it stands."""
+    Hq, Hkv, D = heads
+    b = Batch([q, q], [700 + q, 300 + q], Hq, Hkv, D, 16, dtype)
+    b.q[..., 0] = 1.0
+    b.kc[..., 0] = 0.0
+    dead = torch.tensor([0, 3, 64, 127, 128, 200, 255, 290], device="cuda")
+    for s in range(2):
+        b.kc[b.table[s].long()[dead // 16], :, dead % 16, 0] = -math.inf
+    batch, kw = (b.table, b.cu, b.kv), dict(max_q_len=q, max_kv_len=700 + q)
+    lse, mass = torch.empty(2 * q, Hq, device="cuda"), torch.zeros(b.kc.shape[:3], device="cuda")
+    native.paged_attention(b.q, b.kc, b.vc, *batch, lse=lse, **kw)
+    native.paged_key_mass(b.q, b.kc, mass, *batch, lse, decay=0.0, **kw)
+    for s, n in enumerate((700 + q, 300 + q)):
+        j = torch.arange(n, device="cuda")
+        got = mass[b.table[s].long()[j // 16], :, j % 16]
+        # Each row gives 1 in all: its weights are good to 2 E, as its lse is, and the sum of q rep of them over n keys.
+        assert (got[dead] == 0).all() and (got.sum(0).double() / (q * Hq // Hkv) - 1).abs().max() <= 1e-3
