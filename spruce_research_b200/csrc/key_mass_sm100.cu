@@ -17,7 +17,7 @@
 // polynomial on the FMA pipe, which takes NaN for a number, would need the steps with a NaN lse set apart, and was not built.
 // Where a tile is filled up with zero rows (groups of 7 heads: 2 of 128), its last 32 are summed one by one: 95 -> 97 us, so that a
 // key at -inf gets 0.
-// On a B200, 28 query / 4 KV heads of 128 in bf16: 64 tokens over 131072 99 to 104 us (577 to 608 TFLOP/s); a ragged fp16 batch of 9
+// On a B200, 28 query / 4 KV heads of 128 in bf16: 64 tokens over 131072 97 to 105 us (570 to 620 TFLOP/s); a ragged fp16 batch of 9
 // sequences of up to 3000 tokens and 300 new ones 16 us.
 //
 // Every wait is bounded (common.cuh).
