@@ -12,7 +12,7 @@
 // issue the MMAs of a tile each (a check of a barrier waits behind the MMAs that its warp has queued; one issuer for both:
 // 4.55 ms where two take 4.48), 16 owns TMEM, 18 loads Q and K.  Four softmax warps a scheduler hide each other's latencies
 // (two of 128 keys a row: 4.72 ms where these took 4.58).  Each S_t has two buffers, which fill TMEM: the tensor core runs
-// a tile ahead of the exponentials, which bound the kernel (16 a clock and SM, against 32 scores a clock of the MMAs at d =
+// a tile ahead of the exponentials, which are slower (16 a clock and SM, against 32 scores a clock of the MMAs at d =
 // 128).  Part of them runs on the FMA pipe instead, as a polynomial of degree 4 with a relative error of 2.7e-6: a quarter
 // (none, 1/8, 1/4, 3/8: 4.62, 4.53, 4.48, 4.78 ms; then the exponentials' pipe is 72% busy and issue 63%: neither is full, what
 // is left is the latency of a block's chain of maximum, exponentials and sum).  Exponentials over

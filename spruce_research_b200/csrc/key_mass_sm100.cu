@@ -15,8 +15,8 @@
 // Bound by the softmax warps: 16 exponentials a clock and SM (2048 clocks a step of 256 keys x 128 rows) and their issue, which
 // took 2460 of a step's 2960 clocks; the MMAs take 1100 and K comes from HBM behind them.  All exponentials are the hardware's: a
 // polynomial on the FMA pipe, which takes NaN for a number, would need the steps with a NaN lse set apart, and was not built.
-// Where a tile is filled up with zero rows (groups of 7 heads: 2 of 128), its last 32 are summed one by one: 95 -> 97 us, so that a
-// key at -inf gets 0.
+// Where a tile is filled up with zero rows (groups of 7 heads: 2 of 128), its last 32 go by their limits: 95 -> 97 us, so that a key
+// at -inf gets 0.
 // On a B200, 28 query / 4 KV heads of 128 in bf16: 64 tokens over 131072 97 to 105 us (570 to 620 TFLOP/s); a ragged fp16 batch of 9
 // sequences of up to 3000 tokens and 300 new ones 16 us.
 //
